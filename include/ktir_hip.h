@@ -41,6 +41,8 @@ extern "C" {
 #define KTIR_I64 5
 #define KTIR_I8 6
 #define KTIR_I16 7
+#define KTIR_E4M3 8 /* 8-bit float, 4 exponent and 3 mantissa bits, no infinities (codes of an 8-bit cache) */
+#define KTIR_F64 9  /* frequencies of rotary positions */
 
 /* ---- fused-program opcodes ----
  * A program is a straight-line list of instructions over 8 virtual registers
@@ -477,6 +479,126 @@ typedef struct ktir_pattn {
   int32_t splits, waves;
 } ktir_pattn_t;
 int ktir_launch_paged_attention(const ktir_pattn_t* d);
+
+/* ==== operators of a served model's layer: rotary positions, a key / value
+ * cache in 8 bits, attention over it.  No counterpart in the reference, whose
+ * caches hold 16 bits and whose rotation reads tables of cosines.
+ *
+ * Streams: `stream` of a descriptor is 0 (the library's stream, ordered with
+ * every other entry point), KTIR_STREAM_NULL (the device's null stream) or a
+ * hipStream_t of the library's device.  A launch allocates nothing, waits for
+ * nothing and copies nothing, so it may be captured into a graph; what it reads
+ * from device memory (positions, lengths, tables) it reads when it runs.
+ * Lengths, tables and offsets in device memory that are out of range are not
+ * followed: the launch stays inside the arrays that its descriptor names and
+ * sets the device error word (ktir_check_error_flag: KTIR_E_INDEX). */
+#define KTIR_STREAM_NULL 1
+
+/* A tensor [tokens, heads, columns], column stride 1; strides in elements. */
+typedef struct ktir_rows3 {
+  uint64_t ptr;
+  int64_t tok, head;
+} ktir_rows3_t;
+
+/* ---- rotary positions ----
+ * For every token t with pos[t] >= 0, head h and pair i < rot / 2:
+ *   a = inverse ? -pos[t] freq[i] : pos[t] freq[i],  c = amplitude cos a,  s = amplitude sin a
+ *   (x, y) = the pair's values: columns i and i + rot / 2, or 2 i and 2 i + 1 (interleaved)
+ *   out = (x c - y s, y c + x s)
+ * and columns from rot on are copied.  The angle is reduced in 64 bits, c, s and
+ * the products are f32, and the result is rounded once.  `inverse` is the rotation
+ * back: the gradient's way through the operator.  Rows of tokens with
+ * pos < 0 are left as they were.  Two tensors (queries and keys) share one
+ * launch; heads2 = 0: one.  An output may be its input itself, and must
+ * otherwise not overlap it.  dtype: KTIR_F16, KTIR_BF16 or KTIR_F32. */
+typedef struct ktir_rope {
+  int64_t tokens, heads, heads2, columns, rot;
+  ktir_rows3_t in, out, in2, out2;
+  uint64_t pos;                        /* [tokens], KTIR_I32 or KTIR_I64 */
+  uint64_t freq;                       /* const double* [rot / 2], radians per position */
+  uint64_t stream;
+  double amplitude;
+  int32_t pos_dtype, dtype, interleaved, inverse;
+} ktir_rope_t;
+int ktir_launch_rope(const ktir_rope_t* d);
+
+/* ---- a paged key / value cache in 8 bits ----
+ * Code c of page p, row r, head h, column x stands for c * scale[p, h].  Codes
+ * are KTIR_I8 or KTIR_E4M3, both caches [pages, page, heads, columns] with
+ * column stride 1, rows on 16-byte bounds; scales are f32 and not negative.
+ * `page` (tokens) is a power of two from 16 to 256, `columns` a multiple of 16
+ * up to 256. */
+typedef struct ktir_kv8 {
+  uint64_t k, v, k_scale, v_scale;
+  int64_t pages, page, heads, columns;
+  int64_t k_page, k_tok, k_head, v_page, v_tok, v_head;            /* strides of the codes (elements = bytes) */
+  int64_t ks_page, ks_head, vs_page, vs_head;                      /* strides of the scales (elements) */
+  int32_t dtype, pad;
+} ktir_kv8_t;
+
+/* A batch: sequence s has the new tokens q_start[s] .. q_start[s + 1] of
+ * `tokens`, the last ones of its kv_len[s] cached tokens, whose token t lies in
+ * row t % page of page table[s * table_row + t / page] (int32, `width` entries a
+ * sequence; entries past the last token's are not read).  New token i of
+ * sequence s is at position kv_len[s] - (q_start[s + 1] - q_start[s]) + i.
+ * Tokens outside every sequence pad the batch. */
+typedef struct ktir_kv8_batch {
+  uint64_t table, q_start, kv_len;     /* const int32_t* */
+  int64_t seqs, tokens, table_row, width;
+} ktir_kv8_batch_t;
+
+/* ---- append: the batch's new keys and values into the cache ----
+ * For every page that new tokens fall in, and every head, with the new values x
+ * of that page and head (K and V alike; top = 127 or 448):
+ *   scale' = max(max |x| / top, 2^-100), and the page's scale before, if older tokens
+ *            of the sequence lie in the page, where that is more
+ *   code   = rint(x / scale') or the nearest e4m3 value, within +- top (x times 1 / scale')
+ * and where scale' is more than the scale before, the older tokens' codes are
+ * rounded again: code times (scale before / scale').  A page that receives a
+ * value that is not finite reads as NaN from then on (scale' = NaN, new codes 0).
+ * Tokens at negative positions are not stored.  A page that two sequences of a
+ * call both write keeps the codes and the scale of either.
+ * k, v: [tokens, heads, columns], KTIR_F16 or KTIR_BF16. */
+typedef struct ktir_kv8_append {
+  ktir_kv8_t cache;
+  ktir_kv8_batch_t batch;
+  ktir_rows3_t k, v;
+  uint64_t stream;
+  int32_t dtype, pad;
+} ktir_kv8_append_t;
+int ktir_launch_kv8_append(const ktir_kv8_append_t* d);
+
+/* ---- attention over the cache ----
+ * For every new token at position p of a sequence and every query head g, which
+ * reads KV head g / (q_heads / heads):
+ *   s_j = scale * (q . k_j), over tokens j with 0 <= j < kv_len, and with `causal`
+ *         j <= p, and with window > 0 j > p - window
+ *   out = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m),  lse = m + ln sum_j exp(s_j - m)
+ * A row that no token is left for gets 0 and -inf; padding rows are left as
+ * they were.  Products of q and codes are exact, sums f32, probabilities enter
+ * the second product as ktir_kv8_attn.hip says; the result is rounded once to dtype
+ * (KTIR_F16 or KTIR_BF16, of q and out).  Codes of tokens past kv_len are not
+ * looked at; an e4m3 NaN code of a value makes the rows of its sequence NaN.
+ * max_q and max_k bound the new and the cached tokens of every sequence: what
+ * a sequence has beyond is left out, with the device error word set.
+ * `splits` workgroups share a sequence's tokens.  ktir_kv8_attention_plan sets
+ * it (host only) and says how many bytes of workspace `ws` must then hold;
+ * launches that may run at the same time need a workspace each.  0: no
+ * workspace, as 1. */
+typedef struct ktir_kv8_attn {
+  ktir_kv8_t cache;
+  ktir_kv8_batch_t batch;
+  ktir_rows3_t q, out;
+  uint64_t lse;                        /* float* or 0; strides lse_tok, lse_head */
+  int64_t lse_tok, lse_head;
+  int64_t q_heads, max_q, max_k, window;
+  uint64_t ws, stream;
+  int64_t ws_bytes;
+  float scale;
+  int32_t dtype, causal, splits;
+} ktir_kv8_attn_t;
+int ktir_kv8_attention_plan(ktir_kv8_attn_t* d);      /* sets splits and ws_bytes */
+int ktir_launch_kv8_attention(const ktir_kv8_attn_t* d);
 
 #ifdef __cplusplus
 }

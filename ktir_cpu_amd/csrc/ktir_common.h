@@ -9,7 +9,8 @@ namespace ktir {
 // Status plumbing shared by every translation unit (defined in ktir_runtime.hip).
 int set_error(int code, const char* fmt, ...);
 hipStream_t stream();
-int* device_error_flag();   // device int: 1 = negative indirect index seen
+int* device_error_flag();   // device int: 1 = negative indirect index seen, 2 = length or table entry out of range
+int device();               // the library's device, -1 before ktir_init
 int rmw_scratch_setup(int device);   // ktir_init: per-device scratch of the allocation-free RMW
 
 #define KTIR_HIP_CHECK(expr)                                                        \

@@ -69,6 +69,7 @@ int set_error(int code, const char* fmt, ...) {
 
 hipStream_t stream() { return g_stream; }
 int* device_error_flag() { return g_err_flag; }
+int device() { return g_device; }
 
 }  // namespace ktir
 
@@ -277,7 +278,9 @@ extern "C" int ktir_check_error_flag(void) {
   KTIR_HIP_CHECK(hipStreamSynchronize(g_stream));
   volatile int* flag = g_err_flag;
   if (flag && *flag) {
+    const int what = *flag;
     *flag = 0;
+    if (what == 2) return set_error(KTIR_E_INDEX, "a length, an offset or a page of the batch is outside its bounds");
     return set_error(KTIR_E_INDEX, "indirect index is negative");
   }
   return KTIR_OK;

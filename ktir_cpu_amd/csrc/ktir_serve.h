@@ -1,0 +1,87 @@
+// What the serving operators share (rotary positions, the 8-bit key / value
+// cache, attention over it): the stream and device of a launch, the checks of a
+// cache and a batch, and how a kernel finds its sequence.
+#pragma once
+#include "ktir_common.h"
+
+namespace ktir {
+
+constexpr int OUT_OF_RANGE = 2;      // what a kernel leaves in the device error word
+
+// the library's device is current while this lives
+class OnDevice {
+ public:
+  OnDevice() {
+    ok_ = hipGetDevice(&before_) == hipSuccess && (before_ == device() || hipSetDevice(device()) == hipSuccess);
+  }
+  ~OnDevice() {
+    if (ok_ && before_ != device()) (void)hipSetDevice(before_);
+  }
+  OnDevice(const OnDevice&) = delete;
+  OnDevice& operator=(const OnDevice&) = delete;
+  bool ok() const { return ok_; }
+
+ private:
+  int before_ = 0;
+  bool ok_ = false;
+};
+
+inline hipStream_t stream_of(uint64_t s) {
+  return s == 0 ? stream() : s == KTIR_STREAM_NULL ? (hipStream_t) nullptr : (hipStream_t)s;
+}
+
+// the checks of ktir_kv8.hip, for both operators on the cache
+int check_kv8(const char* what, const ktir_kv8_t& c, bool written);
+int check_batch(const char* what, const ktir_kv8_batch_t& b, const ktir_kv8_t& c);
+int check_rows3(const char* what, const ktir_rows3_t& r, int64_t tokens, int64_t heads, int64_t columns, bool written);
+int ready(const char* what);         // whether ktir_init has run
+
+// the first byte behind a [tokens, heads, columns] tensor of `bytes` an element
+inline uint64_t end_of(const ktir_rows3_t& r, int64_t tokens, int64_t heads, int64_t columns, int bytes) {
+  return r.ptr + ((uint64_t)(tokens - 1) * r.tok + (uint64_t)(heads - 1) * r.head + columns) * bytes;
+}
+
+__device__ __forceinline__ const KTIR_G(int32_t)* ints(uint64_t p) { return (const KTIR_G(int32_t)*)p; }
+
+// A sequence of the batch: its first new token, how many are new, how many are
+// cached with them, and how many of those its table has pages for.  Offsets and
+// lengths that are out of range are cut to the batch and the table.
+struct Seq {
+  int64_t start;
+  int32_t n_new, n_kv, n_held;
+};
+
+__device__ __forceinline__ Seq seq_of(const ktir_kv8_batch_t& b, int64_t page, int64_t s, int* err) {
+  const int64_t a = ints(b.q_start)[s], e = ints(b.q_start)[s + 1], n = ints(b.kv_len)[s];
+  const int64_t start = a < 0 ? 0 : a < b.tokens ? a : b.tokens, end = e < start ? start : e < b.tokens ? e : b.tokens;
+  const int64_t kv = n < 0 ? 0 : n, held = kv < b.width * page ? kv : b.width * page;
+  if (start != a || end != e || held != n) *err = OUT_OF_RANGE;
+  return {start, (int32_t)(end - start), (int32_t)kv, (int32_t)held};
+}
+
+// The sequence that slot `w` of a launch belongs to, and its number in it, where
+// sequence s has the slots from floor(q_start[s] / per) + extra * s on (so every
+// sequence has at least floor(n / per) + extra of them): the last s whose first
+// slot is not after w, with nth < 0 if there is none.  All lanes of a wavefront
+// search together, 64 sequences a step.
+__device__ __forceinline__ int64_t seq_of_slot(const ktir_kv8_batch_t& b, int64_t per, int64_t extra, int64_t w, int64_t* nth) {
+  const int l = threadIdx.x & 63;
+  int64_t s = 0, first = INT64_MAX;
+  for (int64_t base = 0; base < b.seqs; base += 64) {
+    int64_t at = INT64_MAX;
+    if (base + l < b.seqs) {
+      const int64_t q = ints(b.q_start)[base + l];
+      at = (q < 0 ? 0 : q) / per + extra * (base + l);
+    }
+    const uint64_t below = __ballot(at <= w);
+    if (!below) break;
+    const int last = 63 - __builtin_clzll(below);
+    s = base + last;
+    first = (int64_t)__shfl((long long)at, last);
+    if (last < 63) break;
+  }
+  *nth = w - first;
+  return s;
+}
+
+}  // namespace ktir

@@ -43,6 +43,8 @@ DTYPE_CODE = {"f16": K["KTIR_F16"], "bf16": K["KTIR_BF16"], "f32": K["KTIR_F32"]
               "i32": K["KTIR_I32"], "index": K["KTIR_I32"], "i64": K["KTIR_I64"], "i8": K["KTIR_I8"],
               "i16": K["KTIR_I16"]}
 ELEM_BYTES = {"f16": 2, "bf16": 2, "f32": 4, "i1": 1, "i32": 4, "index": 4, "i64": 8, "i8": 1, "i16": 2}
+# types that only the serving operators take (no KTIR function has them)
+SERVING_CODE = {**DTYPE_CODE, "e4m3": K["KTIR_E4M3"], "f64": K["KTIR_F64"]}
 # numpy storage dtype of each KTIR dtype in device memory (bf16 as raw bits)
 STORAGE = {"f16": np.float16, "bf16": np.uint16, "f32": np.float32, "i1": np.bool_, "i32": np.int32,
            "index": np.int32, "i64": np.int64, "i8": np.int8, "i16": np.int16}
@@ -138,71 +140,131 @@ class PATTN(C.Structure):
                 ("splits", C.c_int32), ("waves", C.c_int32)]
 
 
+class Rows3(C.Structure):
+    _fields_ = [("ptr", C.c_uint64), ("tok", C.c_int64), ("head", C.c_int64)]
+
+
+class Rope(C.Structure):
+    _fields_ = [("tokens", C.c_int64), ("heads", C.c_int64), ("heads2", C.c_int64), ("columns", C.c_int64),
+                ("rot", C.c_int64), ("in_", Rows3), ("out", Rows3), ("in2", Rows3), ("out2", Rows3),
+                ("pos", C.c_uint64), ("freq", C.c_uint64), ("stream", C.c_uint64), ("amplitude", C.c_double),
+                ("pos_dtype", C.c_int32), ("dtype", C.c_int32), ("interleaved", C.c_int32), ("inverse", C.c_int32)]
+
+
+class KV8(C.Structure):
+    _fields_ = [(n, C.c_uint64) for n in ("k", "v", "k_scale", "v_scale")] + \
+               [(n, C.c_int64) for n in ("pages", "page", "heads", "columns", "k_page", "k_tok", "k_head", "v_page",
+                                         "v_tok", "v_head", "ks_page", "ks_head", "vs_page", "vs_head")] + \
+               [("dtype", C.c_int32), ("pad", C.c_int32)]
+
+
+class KV8Batch(C.Structure):
+    _fields_ = [(n, C.c_uint64) for n in ("table", "q_start", "kv_len")] + \
+               [(n, C.c_int64) for n in ("seqs", "tokens", "table_row", "width")]
+
+
+class KV8Append(C.Structure):
+    _fields_ = [("cache", KV8), ("batch", KV8Batch), ("k", Rows3), ("v", Rows3), ("stream", C.c_uint64),
+                ("dtype", C.c_int32), ("pad", C.c_int32)]
+
+
+class KV8Attn(C.Structure):
+    _fields_ = [("cache", KV8), ("batch", KV8Batch), ("q", Rows3), ("out", Rows3), ("lse", C.c_uint64)] + \
+               [(n, C.c_int64) for n in ("lse_tok", "lse_head", "q_heads", "max_q", "max_k", "window")] + \
+               [("ws", C.c_uint64), ("stream", C.c_uint64), ("ws_bytes", C.c_int64), ("scale", C.c_float),
+                ("dtype", C.c_int32), ("causal", C.c_int32), ("splits", C.c_int32)]
+
+
 class KTIRDeviceError(RuntimeError):
     pass
 
 
+_opened = None
 _lib = None
+_device = None
 _lock = threading.Lock()
+
+
+def opened():
+    """The HIP library with its entry points declared, no device touched: what
+    host-only queries need."""
+    global _opened
+    with _lock:
+        if _opened is None:
+            _opened = _open()
+        return _opened
 
 
 def lib():
     """Load the HIP library and initialise device 0 (raises when unavailable)."""
-    global _lib
-    with _lock:
-        if _lib is not None:
-            return _lib
-        if not os.path.exists(LIB_PATH):
-            raise RuntimeError(f"{LIB_PATH} is not built: run `python -m ktir_cpu_amd.build` "
-                               "(the KTIR GPU backend has no CPU fallback)")
-        L = C.CDLL(LIB_PATH)
-        L.ktir_last_error.restype = C.c_char_p
-        for name in ("ktir_init", "ktir_malloc", "ktir_free", "ktir_memcpy_h2d", "ktir_memcpy_d2h",
-                     "ktir_memcpy_d2d", "ktir_memset", "ktir_sync", "ktir_check_error_flag",
-                     "ktir_launch_program", "ktir_scatter_winners", "ktir_iat_offsets",
-                     "ktir_launch_matmul", "ktir_event_create", "ktir_event_record",
-                     "ktir_event_elapsed_ms", "ktir_event_destroy", "ktir_device_info",
-                     "ktir_launch_row_rmw", "ktir_launch_attention", "ktir_rmw_variant", "ktir_shutdown", "ktir_set_row_grid_limit",
-                     "ktir_launch_row_rmw_noalloc", "ktir_launch_paged_attention",
-                     "ktir_upload_list", "ktir_download_list"):
-            getattr(L, name).restype = C.c_int
-        L.ktir_malloc.argtypes = [C.c_uint64, C.POINTER(C.c_uint64)]
-        L.ktir_free.argtypes = [C.c_uint64]
-        L.ktir_memcpy_h2d.argtypes = [C.c_uint64, C.c_void_p, C.c_uint64]
-        L.ktir_memcpy_d2h.argtypes = [C.c_void_p, C.c_uint64, C.c_uint64]
-        u64s, ptrs = C.POINTER(C.c_uint64), C.POINTER(C.c_void_p)
-        L.ktir_upload_list.argtypes = [C.c_int, u64s, ptrs, u64s]
-        L.ktir_download_list.argtypes = [C.c_int, ptrs, u64s, u64s]
-        L.ktir_memcpy_d2d.argtypes = [C.c_uint64, C.c_uint64, C.c_uint64]
-        L.ktir_memset.argtypes = [C.c_uint64, C.c_int, C.c_uint64]
-        L.ktir_launch_program.argtypes = [C.POINTER(Prog)]
-        L.ktir_scatter_winners.argtypes = [C.POINTER(Leaf), C.c_int64, C.c_int64, C.c_uint64]
-        L.ktir_iat_offsets.argtypes = [C.POINTER(IAT)]
-        L.ktir_launch_matmul.argtypes = [C.POINTER(MM)]
-        L.ktir_launch_row_rmw.argtypes = [C.POINTER(RMW)]
-        L.ktir_rmw_variant.argtypes = [C.POINTER(RMW)]
-        L.ktir_launch_row_rmw_noalloc.argtypes = [C.POINTER(RMW)]
-        L.ktir_set_row_grid_limit.argtypes = [C.c_int64]
-        L.ktir_launch_attention.argtypes = [C.POINTER(ATTN)]
-        L.ktir_launch_paged_attention.argtypes = [C.POINTER(PATTN)]
-        L.ktir_event_create.argtypes = [C.POINTER(C.c_uint64)]
-        L.ktir_event_record.argtypes = [C.c_uint64]
-        L.ktir_event_elapsed_ms.argtypes = [C.c_uint64, C.c_uint64, C.POINTER(C.c_float)]
-        L.ktir_event_destroy.argtypes = [C.c_uint64]
-        L.ktir_device_info.argtypes = [C.POINTER(C.c_int), C.POINTER(C.c_int), C.POINTER(C.c_int64),
-                                       C.c_char_p, C.c_int]
-        rc = L.ktir_init(int(os.environ.get("KTIR_DEVICE", "0")))
-        if rc != 0:
-            raise RuntimeError("KTIR GPU backend: no usable HIP device: "
-                               + L.ktir_last_error().decode(errors="replace"))
-        _lib = L
+    global _lib, _device
+    if _lib is not None:
         return _lib
+    L = opened()
+    with _lock:
+        if _lib is None:
+            device = device_index()
+            rc = L.ktir_init(device)
+            if rc != 0:
+                raise RuntimeError("KTIR GPU backend: no usable HIP device: "
+                                   + L.ktir_last_error().decode(errors="replace"))
+            _lib, _device = L, device
+        return _lib
+
+
+def _open():
+    """dlopen and the entry points' types."""
+    if not os.path.exists(LIB_PATH):
+        raise RuntimeError(f"{LIB_PATH} is not built: run `python -m ktir_cpu_amd.build` "
+                           "(the KTIR GPU backend has no CPU fallback)")
+    L = C.CDLL(LIB_PATH)
+    L.ktir_last_error.restype = C.c_char_p
+    for name in ("ktir_init", "ktir_malloc", "ktir_free", "ktir_memcpy_h2d", "ktir_memcpy_d2h",
+                 "ktir_memcpy_d2d", "ktir_memset", "ktir_sync", "ktir_check_error_flag",
+                 "ktir_launch_program", "ktir_scatter_winners", "ktir_iat_offsets",
+                 "ktir_launch_matmul", "ktir_event_create", "ktir_event_record",
+                 "ktir_event_elapsed_ms", "ktir_event_destroy", "ktir_device_info",
+                 "ktir_launch_row_rmw", "ktir_launch_attention", "ktir_rmw_variant", "ktir_shutdown", "ktir_set_row_grid_limit",
+                 "ktir_launch_row_rmw_noalloc", "ktir_launch_paged_attention",
+                 "ktir_upload_list", "ktir_download_list", "ktir_launch_rope", "ktir_launch_kv8_append",
+                 "ktir_kv8_attention_plan", "ktir_launch_kv8_attention"):
+        getattr(L, name).restype = C.c_int
+    L.ktir_malloc.argtypes = [C.c_uint64, C.POINTER(C.c_uint64)]
+    L.ktir_free.argtypes = [C.c_uint64]
+    L.ktir_memcpy_h2d.argtypes = [C.c_uint64, C.c_void_p, C.c_uint64]
+    L.ktir_memcpy_d2h.argtypes = [C.c_void_p, C.c_uint64, C.c_uint64]
+    u64s, ptrs = C.POINTER(C.c_uint64), C.POINTER(C.c_void_p)
+    L.ktir_upload_list.argtypes = [C.c_int, u64s, ptrs, u64s]
+    L.ktir_download_list.argtypes = [C.c_int, ptrs, u64s, u64s]
+    L.ktir_memcpy_d2d.argtypes = [C.c_uint64, C.c_uint64, C.c_uint64]
+    L.ktir_memset.argtypes = [C.c_uint64, C.c_int, C.c_uint64]
+    L.ktir_launch_program.argtypes = [C.POINTER(Prog)]
+    L.ktir_scatter_winners.argtypes = [C.POINTER(Leaf), C.c_int64, C.c_int64, C.c_uint64]
+    L.ktir_iat_offsets.argtypes = [C.POINTER(IAT)]
+    L.ktir_launch_matmul.argtypes = [C.POINTER(MM)]
+    L.ktir_launch_row_rmw.argtypes = [C.POINTER(RMW)]
+    L.ktir_rmw_variant.argtypes = [C.POINTER(RMW)]
+    L.ktir_launch_row_rmw_noalloc.argtypes = [C.POINTER(RMW)]
+    L.ktir_set_row_grid_limit.argtypes = [C.c_int64]
+    L.ktir_launch_attention.argtypes = [C.POINTER(ATTN)]
+    L.ktir_launch_paged_attention.argtypes = [C.POINTER(PATTN)]
+    L.ktir_event_create.argtypes = [C.POINTER(C.c_uint64)]
+    L.ktir_event_record.argtypes = [C.c_uint64]
+    L.ktir_event_elapsed_ms.argtypes = [C.c_uint64, C.c_uint64, C.POINTER(C.c_float)]
+    L.ktir_event_destroy.argtypes = [C.c_uint64]
+    L.ktir_device_info.argtypes = [C.POINTER(C.c_int), C.POINTER(C.c_int), C.POINTER(C.c_int64),
+                                   C.c_char_p, C.c_int]
+    L.ktir_launch_rope.argtypes = [C.POINTER(Rope)]
+    L.ktir_launch_kv8_append.argtypes = [C.POINTER(KV8Append)]
+    L.ktir_kv8_attention_plan.argtypes = [C.POINTER(KV8Attn)]
+    L.ktir_launch_kv8_attention.argtypes = [C.POINTER(KV8Attn)]
+    return L
 
 
 def check(rc: int, what: str = ""):
     if rc == 0:
         return
-    msg = lib().ktir_last_error().decode(errors="replace")
+    msg = opened().ktir_last_error().decode(errors="replace")
     if what:
         msg = f"{what}: {msg}"
     if rc == K["KTIR_E_INDEX"]:
@@ -217,6 +279,11 @@ def check(rc: int, what: str = ""):
 def set_row_grid_limit(max_workgroups: int):
     """Bound the workgroups of row-program launches (0: no bound)."""
     check(lib().ktir_set_row_grid_limit(int(max_workgroups)), "ktir_set_row_grid_limit")
+
+
+def device_index() -> int:
+    """The HIP device that the library runs on, or will."""
+    return int(os.environ.get("KTIR_DEVICE", "0")) if _device is None else _device
 
 
 def device_info() -> dict:
