@@ -527,7 +527,7 @@ int ktir_launch_rope(const ktir_rope_t* d);
  * are KTIR_I8 or KTIR_E4M3, both caches [pages, page, heads, columns] with
  * column stride 1, rows on 16-byte bounds; scales are f32 and not negative.
  * `page` (tokens) is a power of two from 16 to 256, `columns` a multiple of 16
- * up to 256. */
+ * up to 256; tokens of a page lie at most 2^22 bytes apart. */
 typedef struct ktir_kv8 {
   uint64_t k, v, k_scale, v_scale;
   int64_t pages, page, heads, columns;
@@ -581,10 +581,10 @@ int ktir_launch_kv8_append(const ktir_kv8_append_t* d);
  * looked at; an e4m3 NaN code of a value makes the rows of its sequence NaN.
  * max_q and max_k bound the new and the cached tokens of every sequence: what
  * a sequence has beyond is left out, with the device error word set.
- * `splits` workgroups share a sequence's tokens.  ktir_kv8_attention_plan sets
- * it (host only) and says how many bytes of workspace `ws` must then hold;
- * launches that may run at the same time need a workspace each.  0: no
- * workspace, as 1. */
+ * `splits` workgroups share a sequence's cached tokens.  ktir_kv8_attention_plan
+ * sets it and ws_bytes (host only), the bytes of workspace that `ws` must then
+ * have, on a 16-byte bound; launches that may run at the same time need a
+ * workspace each.  splits 0 or 1: no workspace. */
 typedef struct ktir_kv8_attn {
   ktir_kv8_t cache;
   ktir_kv8_batch_t batch;

@@ -36,6 +36,7 @@ static int check_codes(const char* what, uint64_t ptr, int64_t page, int64_t tok
   if (!ptr) return set_error(KTIR_E_ARG, "%s: a cache is missing", what);
   if (page < 0 || tok < 0 || head < 0 || page > FAR || tok > FAR || head > FAR)
     return set_error(KTIR_E_ARG, "%s: cache strides %lld, %lld, %lld", what, (long long)page, (long long)tok, (long long)head);
+  if (tok > (1 << 22)) return set_error(KTIR_E_UNSUPPORTED, "%s: tokens of a page lie %lld bytes apart", what, (long long)tok);
   if ((ptr | page | tok | head) & 15) return set_error(KTIR_E_UNSUPPORTED, "%s: cache rows lie off 16-byte bounds", what);
   if (!written) return KTIR_OK;
   int64_t n[3] = {c.pages, c.page, c.heads}, st[3] = {page, tok, head};
@@ -117,7 +118,7 @@ __global__ __launch_bounds__(64) void kv8_append_plain(const ktir_kv8_append_t d
   const int64_t head = blockIdx.y >> 1;
   const bool is_v = blockIdx.y & 1;
   int64_t nth;
-  const int64_t s = seq_of_slot(d.batch, c.page, 2, blockIdx.x, &nth);
+  const int64_t s = seq_of_slot(d.batch, 1, c.page, 2, blockIdx.x, &nth);
   const Seq q = seq_of(d.batch, c.page, s, err);
   const int64_t pos0 = (int64_t)q.n_kv - q.n_new, from = pos0 < 0 ? 0 : pos0;      // the first position that is stored
   const int64_t p = from / c.page + nth;                                         // the page's number in the sequence

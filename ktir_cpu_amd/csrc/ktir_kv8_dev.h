@@ -1,0 +1,117 @@
+// Device helpers of the attention kernels over an 8-bit cache.
+//
+// Keys' codes become f16 operands, which hold both code types exactly, and so do
+// queries of either type, each row times a power of two; so every product of a
+// score is exact and their sum is the matrix instruction's f32.
+//
+// The scales stay out of the operands: with t_j = log2(e) scale kscale q . k_j and
+// page scales kscale, vscale,
+//   w_j = 2^(t_j + log2 vscale - b) = vscale p_j 2^-b   enters the product with V's codes,
+//   l = 2^-16 sum w_j / vscale,  out = 2^-16 (sum w_j code_j) / l,  lse = (b + 16 + log2 l) ln 2,
+// one addition per page and one multiply-add per weight (2^-16 keeps l finite
+// for 2^28 keys whose vscale is the least, 2^-100).  b follows the row's largest exponent.
+#pragma once
+#include "ktir_attn_common.h"
+#include "ktir_serve.h"
+
+namespace ktir {
+
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x3_t __attribute__((ext_vector_type(3), aligned(4)));
+
+constexpr float B_LAG = 8.f;                     // b is changed when an exponent passes it by more
+constexpr float B_NONE = -1e38f;                 // b of a row that has seen no key
+constexpr float L_UNIT = 0x1p-16f;
+constexpr float LEAST_V = 0x1p-100f;             // the least vscale that w is computed with (codes of smaller ones count 0)
+
+template <bool BF16>
+__device__ __forceinline__ f32x4_t mfma16(const uint4& a, const uint4& b, f32x4_t c) {
+  if constexpr (BF16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+  else return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, b), c, 0, 0, 0);
+}
+
+// bytes `lo` of x and `hi` of y as the low bytes of two halves, zeros above
+template <int LO, int HI>
+__device__ __forceinline__ uint32_t bytes2(uint32_t x, uint32_t y) {
+  return __builtin_amdgcn_perm(y, x, 0x0c000c00u | (uint32_t)(4 + HI) << 16 | (uint32_t)LO);
+}
+
+// such a pair of i8 codes as f16: 0x6400 + (c + 128) is 1152 + c
+__device__ __forceinline__ uint32_t i8_half2(uint32_t w) {
+  const f16x2_t v = __builtin_bit_cast(f16x2_t, w ^ 0x64806480u), off = {(_Float16)-1152.f, (_Float16)-1152.f};
+  return __builtin_bit_cast(uint32_t, v + off);
+}
+
+// codes 2 k, 2 k + 1 of a word
+template <int CODE, int K>
+__device__ __forceinline__ uint32_t word_half2(uint32_t w) {
+  if constexpr (CODE == KTIR_I8) return i8_half2(bytes2<2 * K, 2 * K + 1>(w, w));
+  else return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, K == 1));
+}
+
+// eight codes in a row
+template <int CODE>
+__device__ __forceinline__ uint4 row_half8(uint32_t w0, uint32_t w1) {
+  return make_uint4(word_half2<CODE, 0>(w0), word_half2<CODE, 1>(w0), word_half2<CODE, 0>(w1), word_half2<CODE, 1>(w1));
+}
+
+// two words, four codes each, as four bf16 pairs (x's code, y's code)
+template <int CODE>
+__device__ __forceinline__ void cross_bf2(uint32_t x, uint32_t y, uint32_t (&out)[4]) {
+  if constexpr (CODE == KTIR_I8) {
+#pragma unroll
+    for (int n = 0; n < 4; ++n) out[n] = cvt2<true>((float)(int8_t)(x >> (8 * n)), (float)(int8_t)(y >> (8 * n)));
+  } else {
+    const uint32_t a = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, 1.0f, false)),
+                   b = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(y, 1.0f, false)),
+                   c = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, 1.0f, true)),
+                   e = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(y, 1.0f, true));
+    out[0] = __builtin_amdgcn_perm(b, a, 0x05040100u);
+    out[1] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+    out[2] = __builtin_amdgcn_perm(e, c, 0x05040100u);
+    out[3] = __builtin_amdgcn_perm(e, c, 0x07060302u);
+  }
+}
+
+// The rows of one tile of a launch: query head h * grp + r % grp of token
+// i = r / grp of sequence s, r from row0 on; what they see of the keys.
+struct Tile {
+  int64_t s;
+  Seq q;
+  int row0, rows;        // of the tile, rows 0: nothing to do
+  int keys;              // cached tokens that count
+  int lo, hi;            // tokens that some row of the tile sees
+};
+
+// tokens [lo, hi) that row r of tile t sees
+__device__ __forceinline__ void seen(const ktir_kv8_attn_t& d, const Tile& t, int r, int grp, int* lo, int* hi) {
+  const int64_t pos = (int64_t)t.q.n_kv - t.q.n_new + r / grp;
+  *hi = d.causal && pos + 1 < t.keys ? (pos < 0 ? 0 : (int)(pos + 1)) : t.keys;
+  *lo = d.window && pos - d.window + 1 > 0 ? (int)(pos - d.window + 1) : 0;
+}
+
+// tile `slot` of a launch with tiles of TM rows: a sequence each where that holds
+// max_q tokens, otherwise found by the batch's offsets
+__device__ __forceinline__ Tile tile_of(const ktir_kv8_attn_t& d, int64_t slot, int TM, int grp, int* err) {
+  Tile t;
+  int64_t nth = 0;
+  t.s = d.max_q * grp > TM ? seq_of_slot(d.batch, grp, TM, 1, slot, &nth) : slot;
+  t.rows = 0;
+  if (nth < 0) return t;
+  t.q = seq_of(d.batch, d.cache.page, t.s, err);
+  t.keys = t.q.n_held;
+  if (t.keys > d.max_k || t.q.n_new > d.max_q) *err = OUT_OF_RANGE;
+  if (t.keys > d.max_k) t.keys = (int)d.max_k;
+  const int64_t n = (t.q.n_new < d.max_q ? t.q.n_new : d.max_q) * grp, left = n - nth * TM;
+  if (left <= 0) return t;
+  t.row0 = (int)(nth * TM);
+  t.rows = left < TM ? (int)left : TM;
+  int x;
+  seen(d, t, t.row0, grp, &t.lo, &x);
+  seen(d, t, t.row0 + t.rows - 1, grp, &x, &t.hi);
+  return t;
+}
+
+}  // namespace ktir

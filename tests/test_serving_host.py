@@ -247,6 +247,16 @@ def test_attention_refused():
             attention(**kw)
     refused(attention(out=far(23, (7, 4, 64), "<f2", strides=(512, 64, 2))), match="overlap")
     refused(attention(lse=far(25, (7, 4), "<f4", strides=(4, 4))), match="overlap")
+    with pytest.raises(ValueError, match="workspace"):
+        attention(max_k=1 << 16, workspace=far(24, (8,), "|u1"))
+    with pytest.raises(ValueError, match="workspace"):
+        attention(max_k=1 << 16, workspace=Fake((1 << 28,), "|u1", ptr=(1 << 34) + 4))
+    op = attention(max_k=1 << 16)
+    assert op.desc.splits > 1 and op.workspace_bytes > 0
+    for name, value in (("ws", 0), ("ws", (1 << 34) + 8), ("ws_bytes", op.workspace_bytes - 4), ("splits", op.desc.splits + 1)):
+        op = attention(max_k=1 << 16)
+        setattr(op.desc, name, value)
+        refused(op, match="workspace")
     for name, value, code in (("dtype", rt.K["KTIR_F32"], "KTIR_E_UNSUPPORTED"), ("q_heads", 0, "KTIR_E_ARG"),
                               ("splits", -1, "KTIR_E_ARG"), ("scale", math.inf, "KTIR_E_ARG"), ("lse", 2, "KTIR_E_ARG")):
         op = attention()
