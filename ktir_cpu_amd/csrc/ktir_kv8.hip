@@ -90,79 +90,195 @@ int check_batch(const char* what, const ktir_kv8_batch_t& b, const ktir_kv8_t& c
 
 // ---- append ----------------------------------------------------------------
 
-// one code of x / scale
-template <int CODE>
-__device__ __forceinline__ uint8_t code_of(float x) {
-  if constexpr (CODE == KTIR_I8) {
-    const float r = __builtin_rintf(x);
-    return (uint8_t)(int8_t)(int)__builtin_fminf(__builtin_fmaxf(r, -127.f), 127.f);
-  } else {
-    const float r = __builtin_fminf(__builtin_fmaxf(x, -448.f), 448.f);
-    return (uint8_t)(__builtin_amdgcn_cvt_pk_fp8_f32(r, r, 0, false) & 0xff);
-  }
-}
-
-template <int CODE>
-__device__ __forceinline__ float value_of(uint8_t c) {
-  if constexpr (CODE == KTIR_I8) return (float)(int8_t)c;
-  else return __builtin_amdgcn_cvt_f32_fp8(c, 0);
-}
+typedef uint32_t u4_t __attribute__((ext_vector_type(4)));
 
 template <int CODE>
 constexpr float TOP = CODE == KTIR_I8 ? 127.f : 448.f;
 
-// one wavefront per page slot, head, and K or V
+// four values over their scale as codes
 template <int CODE>
-__global__ __launch_bounds__(64) void kv8_append_plain(const ktir_kv8_append_t d, int* err) {
+__device__ __forceinline__ uint32_t codes4(const float* x) {
+  if constexpr (CODE == KTIR_I8) {
+    uint32_t w = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int c = (int)__builtin_amdgcn_fmed3f(__builtin_rintf(x[i]), -127.f, 127.f);
+      w |= (uint32_t)(c & 0xff) << (8 * i);
+    }
+    return w;
+  } else {
+    float y[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[i] = __builtin_amdgcn_fmed3f(x[i], -448.f, 448.f);
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], w, true);
+  }
+}
+
+template <int CODE>
+__device__ __forceinline__ void values4(uint32_t w, float* x) {
+  if constexpr (CODE == KTIR_I8) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = (float)(int8_t)(w >> (8 * i));
+  } else {
+    x[0] = __builtin_amdgcn_cvt_f32_fp8(w, 0);
+    x[1] = __builtin_amdgcn_cvt_f32_fp8(w, 1);
+    x[2] = __builtin_amdgcn_cvt_f32_fp8(w, 2);
+    x[3] = __builtin_amdgcn_cvt_f32_fp8(w, 3);
+  }
+}
+
+// 16 new values: packed as they are, and as f32 times `f`
+struct New16 {
+  uint32_t w[8];
+};
+
+__device__ __forceinline__ New16 new16(uint64_t ptr, int64_t e, bool wide) {
+  New16 r;
+  const KTIR_G(uint16_t)* p = (const KTIR_G(uint16_t)*)ptr + e;
+  if (wide) {
+    const u4_t a = ((const KTIR_G(u4_t)*)p)[0], b = ((const KTIR_G(u4_t)*)p)[1];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r.w[i] = a[i], r.w[4 + i] = b[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r.w[i] = p[2 * i] | (uint32_t)p[2 * i + 1] << 16;
+  }
+  return r;
+}
+
+template <bool BF16>
+__device__ __forceinline__ u4_t codes16(const New16& x, float f, int code) {
+  u4_t o;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float v[4];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const uint32_t w = x.w[2 * i + k];
+      if constexpr (BF16) {
+        v[2 * k] = __uint_as_float(w << 16) * f;
+        v[2 * k + 1] = __uint_as_float(w & 0xffff0000u) * f;
+      } else {
+        v[2 * k] = (float)__builtin_bit_cast(_Float16, (uint16_t)w) * f;
+        v[2 * k + 1] = (float)__builtin_bit_cast(_Float16, (uint16_t)(w >> 16)) * f;
+      }
+    }
+    o[i] = code == KTIR_I8 ? codes4<KTIR_I8>(v) : codes4<KTIR_E4M3>(v);
+  }
+  return o;
+}
+
+// the largest of 16 packed absolute values: of both types the bits grow with the value, and past infinity for NaN
+__device__ __forceinline__ uint32_t top16(const New16& x, uint32_t top) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t a = x.w[i] & 0x7fffu, b = (x.w[i] >> 16) & 0x7fffu;
+    top = top > a ? top : a;
+    top = top > b ? top : b;
+  }
+  return top;
+}
+
+constexpr int APPEND_KEPT = 4;       // units of 16 values that a thread keeps between the two passes
+
+// W wavefronts (1 or 4) per page that new tokens fall in, head, and K or V: a thread
+// takes units of 16 columns of a row.  The new values are read once, into
+// registers, up to 64 W APPEND_KEPT units; units past those (pages of 256 rows of 256
+// columns) are read again, from the cache.
+template <int CODE, bool BF16, int W>
+__global__ __launch_bounds__(256) void kv8_append(const ktir_kv8_append_t d, int* err) {
+  __shared__ uint32_t tops[4];
   const ktir_kv8_t& c = d.cache;
-  const int64_t head = blockIdx.y >> 1;
-  const bool is_v = blockIdx.y & 1;
+  const int wave = uni((int)(threadIdx.x >> 6)), tid = W == 1 ? (int)(threadIdx.x & 63) : (int)threadIdx.x;
+  const int hv = W == 1 ? (int)blockIdx.y * 4 + wave : (int)blockIdx.y;
+  if (hv >= 2 * c.heads) return;
+  const int64_t head = hv >> 1;
+  const bool is_v = hv & 1;
   int64_t nth;
   const int64_t s = seq_of_slot(d.batch, 1, c.page, 2, blockIdx.x, &nth);
+  if (nth < 0) return;
   const Seq q = seq_of(d.batch, c.page, s, err);
+  const int shift = __builtin_ctz((uint32_t)c.page);
   const int64_t pos0 = (int64_t)q.n_kv - q.n_new, from = pos0 < 0 ? 0 : pos0;      // the first position that is stored
-  const int64_t p = from / c.page + nth;                                         // the page's number in the sequence
-  const int64_t lo = p * c.page < from ? from : p * c.page, hi = (p + 1) * c.page < q.n_held ? (p + 1) * c.page : q.n_held;
-  if (nth < 0 || lo >= hi) return;
+  const int64_t p = (from >> shift) + nth;                                       // the page's number in the sequence
+  const int64_t lo = p << shift < from ? from : p << shift, hi = (p + 1) << shift < q.n_held ? (p + 1) << shift : q.n_held;
+  if (lo >= hi) return;
   const int64_t at = ints(d.batch.table)[s * d.batch.table_row + p];
+
+  const ktir_rows3_t& in = is_v ? d.v : d.k;
+  const int G = (int)c.columns >> 4, per = 64 * W / G, r = tid / G, col = (tid - r * G) * 16;     // rows a pass; this thread's
+  const int n = (int)(hi - lo), r0 = (int)(lo & (c.page - 1));
+  const bool wide = !((in.ptr | (uint64_t)in.tok * 2 | (uint64_t)in.head * 2) & 15), mine = r < per;
+  const int64_t e0 = (q.start + lo - pos0) * in.tok + head * in.head + col;
+  New16 x[APPEND_KEPT];
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < APPEND_KEPT; ++i)
+    if (mine && i * per + r < n) x[i] = new16(in.ptr, e0 + (i * per + r) * in.tok, wide);
+#pragma unroll
+  for (int i = 0; i < APPEND_KEPT; ++i)
+    if (mine && i * per + r < n) top = top16(x[i], top);
+  for (int row = APPEND_KEPT * per + r; mine && row < n; row += per) top = top16(new16(in.ptr, e0 + row * in.tok, wide), top);
   if (at < 0 || at >= c.pages) {
     *err = OUT_OF_RANGE;
     return;
   }
-  const ktir_rows3_t& in = is_v ? d.v : d.k;
-  const uint64_t codes = (is_v ? c.v + at * c.v_page + head * c.v_head : c.k + at * c.k_page + head * c.k_head);
-  const int64_t tok = is_v ? c.v_tok : c.k_tok;
+  KTIR_G(uint8_t)* codes = (KTIR_G(uint8_t)*)(is_v ? c.v + at * c.v_page + head * c.v_head : c.k + at * c.k_page + head * c.k_head) + col;
+  const int tok = (int)(is_v ? c.v_tok : c.k_tok);
   KTIR_G(float)* scale = is_v ? (KTIR_G(float)*)c.v_scale + at * c.vs_page + head * c.vs_head
                               : (KTIR_G(float)*)c.k_scale + at * c.ks_page + head * c.ks_head;
-  const int l = threadIdx.x, n = (int)(hi - lo), r0 = (int)(lo - p * c.page), D = (int)c.columns;
-  const int64_t e0 = (q.start + lo - pos0) * in.tok + head * in.head;
-  float top = 0.f;
-  bool bad = false;
-  for (int i = l; i < n * D; i += 64) {
-    const float x = __builtin_fabsf(load_elem(in.ptr, e0 + (i / D) * in.tok + i % D, d.dtype));
-    bad |= !(x < __builtin_inff());
-    top = __builtin_fmaxf(top, x);
-  }
-  for (int o = 32; o; o >>= 1) top = __builtin_fmaxf(top, __shfl_xor(top, o));
-  bad = __any(bad);
   const float before = r0 ? *scale : 0.f;
-  float now = __builtin_fmaxf(top / TOP<CODE>, LEAST_SCALE);
+#pragma unroll
+  for (int o = 32; o; o >>= 1) {
+    const uint32_t y = __shfl_xor(top, o);
+    top = top > y ? top : y;
+  }
+  if constexpr (W > 1) {
+    if ((threadIdx.x & 63) == 0) tops[wave] = top;
+    __syncthreads();                       // also: every wavefront has read the scale before it changes
+#pragma unroll
+    for (int i = 0; i < W; ++i) top = top > tops[i] ? top : tops[i];
+  }
+  const float most = BF16 ? __uint_as_float(top << 16) : (float)__builtin_bit_cast(_Float16, (uint16_t)top);
+  float now = __builtin_fmaxf(most / TOP<CODE>, LEAST_SCALE);
   if (!(now >= before)) now = before;                     // a page that was NaN stays so
-  if (bad) now = __builtin_nanf("");
+  if (!(most < __builtin_inff())) now = __builtin_nanf("");
   const bool nan = !(now < __builtin_inff());
   const float inv = 1.f / now;
-  if (r0 && now > before) {
+  if (now > before && mine) {              // older rows rounded to the new scale
     const float ratio = before * inv;
-    for (int i = l; i < r0 * D; i += 64) {
-      KTIR_G(uint8_t)* w = (KTIR_G(uint8_t)*)codes + (i / D) * tok + i % D;
-      *w = code_of<CODE>(value_of<CODE>(*w) * ratio);
+    for (int row = r; row < r0; row += per) {
+      KTIR_G(u4_t)* w = (KTIR_G(u4_t)*)(codes + row * tok);
+      u4_t y = *w;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float v[4];
+        values4<CODE>(y[i], v);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] *= ratio;
+        y[i] = codes4<CODE>(v);
+      }
+      *w = y;
     }
   }
-  for (int i = l; i < n * D; i += 64) {
-    const float x = load_elem(in.ptr, e0 + (i / D) * in.tok + i % D, d.dtype);
-    ((KTIR_G(uint8_t)*)codes)[(r0 + i / D) * tok + i % D] = nan ? 0 : code_of<CODE>(x * inv);
-  }
-  if (l == 0) *scale = now;
+  const u4_t none = {0, 0, 0, 0};
+#pragma unroll
+  for (int i = 0; i < APPEND_KEPT; ++i)
+    if (mine && i * per + r < n) *(KTIR_G(u4_t)*)(codes + (r0 + i * per + r) * tok) = nan ? none : codes16<BF16>(x[i], inv, CODE);
+  for (int row = APPEND_KEPT * per + r; mine && row < n; row += per)
+    *(KTIR_G(u4_t)*)(codes + (r0 + row) * tok) = nan ? none : codes16<BF16>(new16(in.ptr, e0 + row * in.tok, wide), inv, CODE);
+  if (tid == 0) *scale = now;
+}
+
+template <int CODE, bool BF16>
+static void append_go(const ktir_kv8_append_t& d, int64_t slots, hipStream_t st) {
+  // a page's units fit into one wavefront's registers: four pages or heads share a workgroup
+  const int64_t hv = 2 * d.cache.heads;
+  if (d.cache.page * (d.cache.columns / 16) <= 64 * APPEND_KEPT)
+    hipLaunchKernelGGL((kv8_append<CODE, BF16, 1>), dim3((unsigned)slots, (unsigned)((hv + 3) / 4)), dim3(256), 0, st, d, device_error_flag());
+  else
+    hipLaunchKernelGGL((kv8_append<CODE, BF16, 4>), dim3((unsigned)slots, (unsigned)hv), dim3(256), 0, st, d, device_error_flag());
 }
 
 }  // namespace ktir
@@ -185,9 +301,9 @@ extern "C" int ktir_launch_kv8_append(const ktir_kv8_append_t* d) {
   // a sequence's n new tokens touch at most floor(n / page) + 2 pages
   const int64_t slots = d->batch.tokens / d->cache.page + 2 * d->batch.seqs;
   if (slots > INT32_MAX || d->cache.heads > 32767) return set_error(KTIR_E_UNSUPPORTED, "%s: %lld pages, %lld heads in one launch", ME, (long long)slots, (long long)d->cache.heads);
-  const dim3 grid((unsigned)slots, (unsigned)(2 * d->cache.heads));
-  if (d->cache.dtype == KTIR_I8) hipLaunchKernelGGL(kv8_append_plain<KTIR_I8>, grid, dim3(64), 0, stream_of(d->stream), *d, device_error_flag());
-  else hipLaunchKernelGGL(kv8_append_plain<KTIR_E4M3>, grid, dim3(64), 0, stream_of(d->stream), *d, device_error_flag());
+  const hipStream_t st = stream_of(d->stream);
+  if (d->cache.dtype == KTIR_I8) d->dtype == KTIR_BF16 ? append_go<KTIR_I8, true>(*d, slots, st) : append_go<KTIR_I8, false>(*d, slots, st);
+  else d->dtype == KTIR_BF16 ? append_go<KTIR_E4M3, true>(*d, slots, st) : append_go<KTIR_E4M3, false>(*d, slots, st);
   KTIR_HIP_CHECK(hipGetLastError());
   return KTIR_OK;
 }

@@ -1,9 +1,11 @@
 // Rotary positions: pairs of a head's columns rotated by an angle that grows
 // with the token's position, y = (x0 c - x1 s, x1 c + x0 s).
-#include <climits>
 #include "ktir_serve.h"
 
 namespace ktir {
+
+typedef uint32_t u4_t __attribute__((ext_vector_type(4)));
+typedef float f4_t __attribute__((ext_vector_type(4)));
 
 // cosine and sine of token t's pair i, times the amplitude.  The angle passes
 // 2^20 radians at far positions, where f32 holds it to a sixteenth: the product
@@ -22,27 +24,208 @@ __device__ __forceinline__ int64_t rope_pos(const ktir_rope_t& d, int64_t t) {
   return d.pos_dtype == KTIR_I64 ? ((const KTIR_G(int64_t)*)d.pos)[t] : (int64_t)ints(d.pos)[t];
 }
 
-__global__ __launch_bounds__(256) void rope_plain(const ktir_rope_t d) {
-  const int64_t half = d.rot / 2, per = half + (d.columns - d.rot), total = d.tokens * per;
-  for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < total; at += (int64_t)gridDim.x * 256) {
-    const int64_t t = at / per, i = at - t * per, pos = rope_pos(d, t);
-    if (pos < 0) continue;
-    float c = 1.f, s = 0.f;
-    if (i < half) rope_angle(d, pos, (int)i, &c, &s);
-    for (int64_t h = 0; h < d.heads + d.heads2; ++h) {
-      const ktir_rows3_t &in = h < d.heads ? d.in : d.in2, &out = h < d.heads ? d.out : d.out2;
-      const int64_t hh = h < d.heads ? h : h - d.heads, e = t * in.tok + hh * in.head, o = t * out.tok + hh * out.head;
-      if (i >= half) {
-        const int64_t x = d.rot + (i - half);
-        if (in.ptr != out.ptr) store_elem(out.ptr, o + x, d.dtype, load_elem(in.ptr, e + x, d.dtype));
-        continue;
-      }
-      const int64_t x0 = d.interleaved ? 2 * i : i, x1 = d.interleaved ? 2 * i + 1 : i + half;
-      const float a = load_elem(in.ptr, e + x0, d.dtype), b = load_elem(in.ptr, e + x1, d.dtype);
-      store_elem(out.ptr, o + x0, d.dtype, __fsub_rn(__fmul_rn(a, c), __fmul_rn(b, s)));
-      store_elem(out.ptr, o + x1, d.dtype, __fadd_rn(__fmul_rn(b, c), __fmul_rn(a, s)));
+// V pairs: 2 V values as f32, and back.  Half layout: V values at `a` and their V
+// partners at `b`; interleaved: 2 V values from `a` on (b = a + V).
+template <int DT, int V>
+struct RopeRaw {
+  uint32_t w[2][DT == KTIR_F32 ? V : (V + 1) / 2];
+};
+
+template <int DT, int V>
+__device__ __forceinline__ void rope_load(uint64_t ptr, int64_t a, int64_t b, RopeRaw<DT, V>& r) {
+  const int64_t e[2] = {a, b};
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    if constexpr (V == 1) {
+      if constexpr (DT == KTIR_F32) r.w[i][0] = ((const KTIR_G(uint32_t)*)ptr)[e[i]];
+      else r.w[i][0] = ((const KTIR_G(uint16_t)*)ptr)[e[i]];
+    } else {
+      const u4_t x = *(const KTIR_G(u4_t)*)(ptr + e[i] * (DT == KTIR_F32 ? 4 : 2));
+#pragma unroll
+      for (int k = 0; k < 4; ++k) r.w[i][k] = x[k];
     }
   }
+}
+
+template <int DT, int V>
+__device__ __forceinline__ void rope_store(uint64_t ptr, int64_t a, int64_t b, const RopeRaw<DT, V>& r, bool two) {
+  const int64_t e[2] = {a, b};
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    if (i && !two) break;
+    if constexpr (V == 1) {
+      if constexpr (DT == KTIR_F32) ((KTIR_G(uint32_t)*)ptr)[e[i]] = r.w[i][0];
+      else ((KTIR_G(uint16_t)*)ptr)[e[i]] = (uint16_t)r.w[i][0];
+    } else {
+      *(KTIR_G(u4_t)*)(ptr + e[i] * (DT == KTIR_F32 ? 4 : 2)) = u4_t{r.w[i][0], r.w[i][1], r.w[i][2], r.w[i][3]};
+    }
+  }
+}
+
+template <int DT>
+__device__ __forceinline__ float rope_get(const uint32_t* w, int k) {
+  if constexpr (DT == KTIR_F32) return __uint_as_float(w[k]);
+  else {
+    const uint32_t h = (w[k >> 1] >> (16 * (k & 1))) & 0xffffu;
+    if constexpr (DT == KTIR_BF16) return __uint_as_float(h << 16);
+    else return (float)__builtin_bit_cast(_Float16, (uint16_t)h);
+  }
+}
+
+template <int DT>
+__device__ __forceinline__ uint32_t rope_bits(float x) {
+  if constexpr (DT == KTIR_F32) return __float_as_uint(x);
+  else if constexpr (DT == KTIR_BF16) return __builtin_bit_cast(uint16_t, (__bf16)x);
+  else return __builtin_bit_cast(uint16_t, (_Float16)x);
+}
+
+// x0 c - x1 s and x1 c + x0 s of V pairs
+template <int DT, bool INTER, int V>
+__device__ __forceinline__ void rope_turn_raw(RopeRaw<DT, V>& r, const float* c, const float* s) {
+  float out[2][V];
+#pragma unroll
+  for (int k = 0; k < V; ++k) {
+    float x, y;
+    if constexpr (INTER && V > 1) {
+      x = rope_get<DT>(r.w[2 * k / V], 2 * k % V);
+      y = rope_get<DT>(r.w[(2 * k + 1) / V], (2 * k + 1) % V);
+    } else {
+      x = rope_get<DT>(r.w[0], k);
+      y = rope_get<DT>(r.w[1], k);
+    }
+    const float u = __fsub_rn(__fmul_rn(x, c[k]), __fmul_rn(y, s[k])), v = __fadd_rn(__fmul_rn(y, c[k]), __fmul_rn(x, s[k]));
+    if constexpr (INTER && V > 1) {
+      out[2 * k / V][2 * k % V] = u;
+      out[(2 * k + 1) / V][(2 * k + 1) % V] = v;
+    } else {
+      out[0][k] = u;
+      out[1][k] = v;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      if constexpr (DT == KTIR_F32) r.w[i][k] = rope_bits<DT>(out[i][k]);
+      else if constexpr (V == 1) r.w[i][0] = rope_bits<DT>(out[i][0]);
+      else if (!(k & 1)) r.w[i][k / 2] = rope_bits<DT>(out[i][k]) | rope_bits<DT>(out[i][k + 1]) << 16;
+    }
+}
+
+constexpr int ROPE_PAIRS = 2048;     // angles of a workgroup's tokens in LDS
+constexpr int ROPE_TOKENS = 8;
+
+// A unit of columns: V pairs, or 2 V of the columns behind rot, as two vectors.
+template <bool INTER, int V>
+__device__ __forceinline__ void rope_columns(int u, int pairs, int half, int rot, int* a, int* b) {
+  if (u < pairs) {
+    *a = INTER ? 2 * u * V : u * V;
+    *b = INTER ? *a + V : *a + half;
+  } else {
+    *a = rot + (u - pairs) * 2 * V;
+    *b = *a + V;
+  }
+}
+
+// A workgroup has `per` tokens and, with several in y, a part of the heads.  Its
+// threads first make the angles of the tokens together, then each takes one unit of
+// columns over rows (token, head), R rows' loads ahead of the first's stores.
+template <int DT, bool INTER, int V, int R>
+__global__ __launch_bounds__(256) void rope_turn(const ktir_rope_t d, int per) {
+  __shared__ __attribute__((aligned(16))) float cs[ROPE_PAIRS], sn[ROPE_PAIRS];
+  __shared__ int live[ROPE_TOKENS];
+  const int half = (int)(d.rot / 2), rot = (int)d.rot, columns = (int)d.columns, pairs = half / V;
+  const bool tail = d.in.ptr != d.out.ptr || (d.heads2 && d.in2.ptr != d.out2.ptr);
+  const int units = pairs + (tail ? (columns - rot + 2 * V - 1) / (2 * V) : 0);
+  const int64_t t0 = (int64_t)blockIdx.x * per;
+  const int tokens = (int)(d.tokens - t0 < per ? d.tokens - t0 : per), heads = (int)(d.heads + d.heads2);
+  const int wide = units < 256 ? units : 256, step = 256 / wide;      // columns side by side, rows side by side
+  const int tid = threadIdx.x, u0 = tid % wide, stride = step * (int)gridDim.y, total = tokens * heads;
+
+  for (int i = tid; i < tokens * half; i += 256) {
+    const int t = i / half;
+    const int64_t pos = rope_pos(d, t0 + t);
+    rope_angle(d, pos < 0 ? 0 : pos, i - t * half, &cs[i], &sn[i]);
+  }
+  for (int t = tid; t < tokens; t += 256) live[t] = rope_pos(d, t0 + t) >= 0;
+  __syncthreads();
+  if (tid >= wide * step) return;
+  for (int u = u0; u < units; u += wide) {
+    int a, b;
+    rope_columns<INTER, V>(u, pairs, half, rot, &a, &b);
+    const bool two = b < columns;            // the last unit behind rot may be half one
+    if (!two) b = a;
+    int row = (int)blockIdx.y * step + tid / wide, t = 0, h = row;
+    while (row < total) {
+      RopeRaw<DT, V> r[R];
+      int at[R];
+      int64_t to[R];
+      uint64_t ptr[R];
+#pragma unroll
+      for (int k = 0; k < R; ++k) {
+        while (h >= heads) {
+          h -= heads;
+          ++t;
+        }
+        const bool second = h >= d.heads, on = row < total && live[t < tokens ? t : 0];
+        const ktir_rows3_t &in = second ? d.in2 : d.in, &out = second ? d.out2 : d.out;
+        const int64_t hh = second ? h - d.heads : h;
+        to[k] = (t0 + t) * out.tok + hh * out.head;
+        ptr[k] = on && (u < pairs || in.ptr != out.ptr) ? out.ptr : 0;
+        at[k] = t * half + u * V;
+        if (ptr[k]) {
+          const int64_t e = (t0 + t) * in.tok + hh * in.head;
+          rope_load<DT, V>(in.ptr, e + a, e + b, r[k]);
+        }
+        row += stride;
+        h += stride;
+      }
+#pragma unroll
+      for (int k = 0; k < R; ++k) {
+        if (!ptr[k]) continue;
+        if (u < pairs) {
+          __attribute__((aligned(16))) float c[V], s[V];
+          if constexpr (V > 1) {                             // half and so every unit's angles: multiples of 4
+#pragma unroll
+            for (int i = 0; i < V; i += 4) {
+              *(f4_t*)(c + i) = *(const f4_t*)&cs[at[k] + i];
+              *(f4_t*)(s + i) = *(const f4_t*)&sn[at[k] + i];
+            }
+          } else {
+            c[0] = cs[at[k]];
+            s[0] = sn[at[k]];
+          }
+          rope_turn_raw<DT, INTER, V>(r[k], c, s);
+        }
+        rope_store<DT, V>(ptr[k], to[k] + a, to[k] + b, r[k], two);
+      }
+    }
+  }
+}
+
+// whether every vector of V values of a tensor starts on a 16-byte bound
+static bool wide_rows(const ktir_rows3_t& r, int64_t tokens, int64_t heads, int V) {
+  return !(r.ptr & 15) && (tokens == 1 || r.tok % V == 0) && (heads == 1 || r.head % V == 0);
+}
+
+template <int DT, int V>
+static void rope_go(const ktir_rope_t& d, hipStream_t st) {
+  const int64_t half = d.rot / 2, units = half / V + (d.columns - d.rot + 2 * V - 1) / (2 * V), heads = d.heads + d.heads2;
+  int64_t per = d.tokens / 1024;
+  per = per > ROPE_TOKENS ? ROPE_TOKENS : per < 1 ? 1 : per;
+  if (per * half > ROPE_PAIRS) per = ROPE_PAIRS / half;
+  const int64_t blocks = (d.tokens + per - 1) / per, step = 256 / (units < 256 ? units : 256);
+  constexpr int R = 2;
+  // few tokens: one row of units a thread
+  int64_t y = 1;
+  if (blocks < 512) {
+    y = (per * heads + step - 1) / step;
+    const int64_t most = (1024 + blocks - 1) / blocks;
+    y = y > most ? most : y;
+  }
+  const dim3 grid((unsigned)blocks, (unsigned)y);
+  if (d.interleaved) hipLaunchKernelGGL((rope_turn<DT, true, V, R>), grid, dim3(256), 0, st, d, (int)per);
+  else hipLaunchKernelGGL((rope_turn<DT, false, V, R>), grid, dim3(256), 0, st, d, (int)per);
 }
 
 static int check_pair(const ktir_rope_t& d, const ktir_rows3_t& in, const ktir_rows3_t& out, int64_t heads) {
@@ -62,7 +245,7 @@ using namespace ktir;
 
 extern "C" int ktir_launch_rope(const ktir_rope_t* d) {
   if (!d) return set_error(KTIR_E_ARG, "ktir_launch_rope: no descriptor");
-  if (d->tokens < 0 || d->heads < 1 || d->heads2 < 0 || d->columns < 1 || d->columns > 4096 || d->heads > 65536 || d->heads2 > 65536)
+  if (d->tokens < 0 || d->tokens > INT32_MAX || d->heads < 1 || d->heads2 < 0 || d->columns < 1 || d->columns > 4096 || d->heads > 65536 || d->heads2 > 65536)
     return set_error(KTIR_E_ARG, "ktir_launch_rope: %lld tokens, %lld and %lld heads of %lld columns", (long long)d->tokens,
                      (long long)d->heads, (long long)d->heads2, (long long)d->columns);
   if (d->rot < 2 || d->rot > d->columns || (d->rot & 1))
@@ -81,8 +264,16 @@ extern "C" int ktir_launch_rope(const ktir_rope_t* d) {
   if (rc != KTIR_OK) return rc;
   OnDevice on;
   if (!on.ok()) return set_error(KTIR_E_HIP, "ktir_launch_rope: no device");
-  const int64_t total = d->tokens * (d->rot / 2 + d->columns - d->rot), blocks = (total + 255) / 256;
-  hipLaunchKernelGGL(rope_plain, dim3((unsigned)(blocks < 65536 ? blocks : 65536)), dim3(256), 0, stream_of(d->stream), *d);
+  const int V = d->dtype == KTIR_F32 ? 4 : 8;
+  bool wide = (d->rot / 2) % V == 0 && (d->columns - d->rot) % V == 0 && wide_rows(d->in, d->tokens, d->heads, V) &&
+              wide_rows(d->out, d->tokens, d->heads, V);
+  if (d->heads2) wide = wide && wide_rows(d->in2, d->tokens, d->heads2, V) && wide_rows(d->out2, d->tokens, d->heads2, V);
+  const hipStream_t st = stream_of(d->stream);
+  switch (d->dtype) {
+    case KTIR_F32: wide ? rope_go<KTIR_F32, 4>(*d, st) : rope_go<KTIR_F32, 1>(*d, st); break;
+    case KTIR_F16: wide ? rope_go<KTIR_F16, 8>(*d, st) : rope_go<KTIR_F16, 1>(*d, st); break;
+    default: wide ? rope_go<KTIR_BF16, 8>(*d, st) : rope_go<KTIR_BF16, 1>(*d, st);
+  }
   KTIR_HIP_CHECK(hipGetLastError());
   return KTIR_OK;
 }
