@@ -23,10 +23,10 @@ ARCH = os.environ.get("KTIR_OFFLOAD_ARCH", "gfx950")
 HIPCC_FLAGS = ["-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}", "-ffp-contract=off",
                "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
                "-Wno-unused-result"]
-# per-source additions: the paged attention MFMA kernel keeps its
-# accumulators in VGPRs (MFMA C/D operands in the VGPR form), since it
-# rescales them with VALU multiplies between products
-FILE_FLAGS = {"ktir_pattn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
+# per-source additions: the paged attention MFMA kernels keep their
+# accumulators in VGPRs (MFMA C/D operands in the VGPR form), since they
+# rescale them with VALU multiplies between products
+FILE_FLAGS = {f: ["-mllvm", "-amdgpu-mfma-vgpr-form"] for f in ("ktir_pattn.hip", "ktir_kv8_rows.hip")}
 
 
 def _hipcc() -> str:

@@ -50,6 +50,7 @@ extern "C" int ktir_launch_kv8_attention(const ktir_kv8_attn_t* d) {
   KV8Shape s;
   kv8_rows_shape(*d, &s);
   const int64_t splits = d->splits < 1 ? 1 : d->splits, tiles = s.slots * d->cache.heads;
+  if (splits > 256) return set_error(KTIR_E_ARG, "%s: %lld splits, 256 at most", ME, (long long)splits);
   if (tiles > INT32_MAX / splits)
     return set_error(KTIR_E_UNSUPPORTED, "%s: %lld tiles in %lld splits", ME, (long long)tiles, (long long)splits);
   if (splits > 1 && (!d->ws || (d->ws & 15) || d->ws_bytes / 4 / s.part / tiles < splits))

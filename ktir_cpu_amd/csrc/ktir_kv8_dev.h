@@ -92,13 +92,12 @@ __device__ __forceinline__ void seen(const ktir_kv8_attn_t& d, const Tile& t, in
   *lo = d.window && pos - d.window + 1 > 0 ? (int)(pos - d.window + 1) : 0;
 }
 
-// tile `slot` of a launch with tiles of TM rows: a sequence each where that holds
+// tile `slot` of a launch with tiles of TM (a power of two) rows: a sequence each where that holds
 // max_q tokens, otherwise found by the batch's offsets
 __device__ __forceinline__ Tile tile_of(const ktir_kv8_attn_t& d, int64_t slot, int TM, int grp, int* err) {
-  Tile t;
+  Tile t = {};
   int64_t nth = 0;
-  t.s = d.max_q * grp > TM ? seq_of_slot(d.batch, grp, TM, 1, slot, &nth) : slot;
-  t.rows = 0;
+  t.s = d.max_q * grp > TM ? seq_of_slot(d.batch, grp, __builtin_ctz(TM), 1, slot, &nth) : slot;
   if (nth < 0) return t;
   t.q = seq_of(d.batch, d.cache.page, t.s, err);
   t.keys = t.q.n_held;
@@ -111,6 +110,20 @@ __device__ __forceinline__ Tile tile_of(const ktir_kv8_attn_t& d, int64_t slot, 
   int x;
   seen(d, t, t.row0, grp, &t.lo, &x);
   seen(d, t, t.row0 + t.rows - 1, grp, &x, &t.hi);
+  return t;
+}
+
+// a tile's fields in scalar registers: they are the same in every lane
+__device__ __forceinline__ Tile uni(Tile t) {
+  t.s = uni(t.s);
+  t.q.start = uni(t.q.start);
+  t.q.n_new = uni(t.q.n_new);
+  t.q.n_kv = uni(t.q.n_kv);
+  t.row0 = uni(t.row0);
+  t.rows = uni(t.rows);
+  t.keys = uni(t.keys);
+  t.lo = uni(t.lo);
+  t.hi = uni(t.hi);
   return t;
 }
 

@@ -23,14 +23,18 @@
 namespace ktir {
 
 constexpr int ROWS_WAVES = 4, ROWS_STEP = 32, ROWS_GROUPS = 64;
+constexpr int MOST_SPLITS = 256;      // of a tile's keys
 
 // what a split of a tile leaves in the workspace: TM rows of 64 J sums, then b and l of each row
 template <int J, int MT>
 constexpr int64_t PART = 16 * MT * (64 * J + 2);
 
 template <int J>
-struct KV8Step {
+struct KV8Keys {
   u32x4_t k[2][J];
+};
+template <int J>
+struct KV8Values {
   uint32_t v[8][J];
 };
 
@@ -44,34 +48,52 @@ __device__ __forceinline__ float lane_of(float x, int i) {
   return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), i));
 }
 
-__device__ __forceinline__ KV8Groups kv8_groups(const ktir_kv8_attn_t& d, const Tile& t, int64_t head, int key, int end, int shift,
-                                                int* err) {
-  KV8Groups g = {0, 0.f, 0.f, 1.f};
-  if (key < end) {
-    const int64_t at = ints(d.batch.table)[t.s * d.batch.table_row + (key >> shift)];
-    if (at < 0 || at >= d.cache.pages) *err = OUT_OF_RANGE;
-    else g.page = (int)at;
-    g.ks = ((const KTIR_G(float)*)d.cache.k_scale)[g.page * d.cache.ks_page + head * d.cache.ks_head];
-    float vs = ((const KTIR_G(float)*)d.cache.v_scale)[g.page * d.cache.vs_page + head * d.cache.vs_head];
-    vs = vs < LEAST_V ? LEAST_V : vs;
-    g.lv = __builtin_amdgcn_logf(vs);
-    g.iv = L_UNIT / vs;
+// the pages of the groups that start at `key` in this lane; groups from `end` on: page 0, which weighs nothing
+__device__ __forceinline__ int kv8_pages(const ktir_kv8_attn_t& d, const Tile& t, int key, int end, int shift) {
+  return key < end ? ints(d.batch.table)[t.s * d.batch.table_row + (key >> shift)] : 0;
+}
+
+__device__ __forceinline__ KV8Groups kv8_groups(const ktir_kv8_attn_t& d, int64_t head, int page, bool there, int* err) {
+  if ((uint32_t)page >= (uint64_t)d.cache.pages) {
+    *err = OUT_OF_RANGE;
+    page = 0;
+  }
+  KV8Groups g = {page, 0.f, 0.f, L_UNIT};
+  if (there) {
+    g.ks = ((const KTIR_G(float)*)d.cache.k_scale)[page * d.cache.ks_page + head * d.cache.ks_head];
+    g.lv = ((const KTIR_G(float)*)d.cache.v_scale)[page * d.cache.vs_page + head * d.cache.vs_head];
   }
   return g;
 }
 
+// vscale as its logarithm and inverse (not where it is loaded: that would wait for it)
+__device__ __forceinline__ void kv8_scales(KV8Groups& g, bool there) {
+  if (!there) return;
+  const float vs = g.lv < LEAST_V ? LEAST_V : g.lv;
+  g.lv = __builtin_amdgcn_logf(vs);
+  g.iv = L_UNIT / vs;
+}
+
 // the codes of 32 keys from `key` on; groups that the wavefront does not have read page 0
 template <int J>
-__device__ __forceinline__ void kv8_load(const ktir_kv8_t& c, const KV8Groups& g, int group, int key, int64_t head, int koff, int voff,
-                                         const int (&kpiece)[J], KV8Step<J>& o) {
+__device__ __forceinline__ void kv8_keys(const ktir_kv8_t& c, const KV8Groups& g, int group, int key, int64_t head, int koff,
+                                         const int (&kpiece)[J], KV8Keys<J>& o) {
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    const int64_t page = __builtin_amdgcn_readlane(g.page, group + h);
-    const int64_t row = (key + 16 * h) & (c.page - 1);
+    const int64_t page = __builtin_amdgcn_readlane(g.page, group + h), row = (key + 16 * h) & (c.page - 1);
     const KTIR_G(uint8_t)* kp = (const KTIR_G(uint8_t)*)c.k + page * c.k_page + row * c.k_tok + head * c.k_head;
-    const KTIR_G(uint8_t)* vp = (const KTIR_G(uint8_t)*)c.v + page * c.v_page + row * c.v_tok + head * c.v_head;
 #pragma unroll
     for (int j = 0; j < J; ++j) o.k[h][j] = *(const KTIR_G(u32x4_t)*)(kp + (uint32_t)(koff + kpiece[j]));
+  }
+}
+
+template <int J>
+__device__ __forceinline__ void kv8_values(const ktir_kv8_t& c, const KV8Groups& g, int group, int key, int64_t head, int voff,
+                                           KV8Values<J>& o) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int64_t page = __builtin_amdgcn_readlane(g.page, group + h), row = (key + 16 * h) & (c.page - 1);
+    const KTIR_G(uint8_t)* vp = (const KTIR_G(uint8_t)*)c.v + page * c.v_page + row * c.v_tok + head * c.v_head;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const KTIR_G(uint8_t)* p = vp + (uint32_t)(voff + i * (int)c.v_tok);
@@ -93,29 +115,37 @@ __device__ __forceinline__ void kv8_load(const ktir_kv8_t& c, const KV8Groups& g
 }
 
 template <int CODE, int J, int MT>
-__global__ __launch_bounds__(256) void kv8_attn_rows(const ktir_kv8_attn_t d, int* err) {
-  constexpr int TM = 16 * MT, N = 4 * J, PITCH = 64 * J + 4;
-  __shared__ __attribute__((aligned(16))) float o_sum[TM * PITCH];
-  __shared__ float w_b[ROWS_WAVES][TM], w_l[ROWS_WAVES][TM];
+__global__ __launch_bounds__(64 * ROWS_WAVES, MT == 1 ? 2 : 1) void kv8_attn_rows(const ktir_kv8_attn_t d, int splits, int part, uint32_t slots, int hw, int* err) {
+  constexpr int W = ROWS_WAVES, TM = 16 * MT, N = 4 * J, PITCH = 64 * J + 4;
+  __shared__ __attribute__((aligned(16))) float o_sum[W][TM * PITCH];
+  __shared__ float w_b[W][TM], w_l[W][TM];
   const ktir_kv8_t& c = d.cache;
   const int l = threadIdx.x & 63, wave = uni((int)(threadIdx.x >> 6)), g4 = l >> 4, c16 = l & 15;
-  const int grp = (int)(d.q_heads / c.heads), D = (int)c.columns, shift = __builtin_ctz((uint32_t)c.page);
-  const int splits = d.splits < 1 ? 1 : d.splits, split = (int)(blockIdx.x % splits);
-  const int64_t item = blockIdx.x / splits, head = item % c.heads, slot = item / c.heads;
-  const Tile t = tile_of(d, slot, TM, grp, err);
+  const int grp = (int)((uint32_t)d.q_heads / (uint32_t)c.heads), D = (int)c.columns, shift = __builtin_ctz((uint32_t)c.page);
+  // Workgroups go to the 8 XCDs in turn.  The heads of a tile's split follow one
+  // another on one XCD, so the rows of a page are read together; tiles and splits
+  // take the XCDs in turn, a split its tiles from another one on, as the last splits
+  // of many tiles are empty.
+  const uint32_t heads = (uint32_t)c.heads, sets = heads / hw, octet = blockIdx.x / 8, eighth = octet / sets, u = eighth * 8 + blockIdx.x % 8;
+  const uint32_t split = u / slots, turned = u - split * slots + split % slots, slot = turned < slots ? turned : turned - slots;
+  if (split >= (uint32_t)splits) return;
+  const int turn = wave / hw, TW = W / hw;                   // of the head's TW wavefronts
+  const int64_t head = (octet - eighth * sets) * hw + wave % hw, item = (int64_t)slot * heads + head;
+  const Tile t = uni(tile_of(d, slot, TM, grp, err));
   if (!t.rows) return;
 
   // this workgroup's keys, and this wavefront's
-  const int from = t.lo & ~(ROWS_STEP - 1), span = t.hi > from ? t.hi - from : 0;
-  constexpr int QUANT = ROWS_STEP * ROWS_WAVES;
-  const int part = ((span + splits - 1) / splits + QUANT - 1) / QUANT * QUANT, active = span ? (span + part - 1) / part : 1;
-  if (split >= active) return;
-  const int lo = uni(from + split * part + wave * (part / ROWS_WAVES)), end = uni(lo + part / ROWS_WAVES < t.hi ? lo + part / ROWS_WAVES : t.hi);
+  const int from = t.lo & ~(ROWS_STEP - 1), span = t.hi > from ? t.hi - from : 0, active = span ? (span + part - 1) / part : 1;
+  if ((int)split >= active) return;
+  // (steps of 32 keys go to the splits' wavefronts in turn, so what all read at one time lies close together)
+  const int stride = ROWS_STEP * TW * active, lo = from + ((int)split * TW + turn) * ROWS_STEP, mine = (l >> 1) * stride + 16 * (l & 1);
+  const int page0 = kv8_pages(d, t, lo + mine, t.hi, shift);
 
   // Q: this lane's row of each 16, pieces g4, g4 + 4, .. of 16 columns; times 2^k, so that the row's largest value has exponent 14
   uint4 qf[MT][J][2];
   float rs[MT];
   int see_lo[MT], see_hi[MT], kpiece[J];
+  uint32_t raw[MT][J][8];
 #pragma unroll
   for (int j = 0; j < J; ++j) kpiece[j] = (4 * j + g4) * 16 < D ? (4 * j + g4) * 16 : 0;
   const bool whole = !((d.q.ptr | (uint64_t)d.q.tok * 2 | (uint64_t)d.q.head * 2) & 15);
@@ -125,31 +155,40 @@ __global__ __launch_bounds__(256) void kv8_attn_rows(const ktir_kv8_attn_t d, in
     if (r >= t.row0 + t.rows) r = t.row0 + t.rows - 1;              // a row that is not stored
     seen(d, t, r, grp, &see_lo[m], &see_hi[m]);
     const int64_t e = (t.q.start + r / grp) * d.q.tok + (head * grp + r % grp) * d.q.head;
-    uint32_t raw[J][8];
-    uint32_t top = 0;
 #pragma unroll
     for (int j = 0; j < J; ++j) {
       const int x = (4 * j + g4) * 16;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) raw[j][i] = 0;
+      for (int i = 0; i < 8; ++i) raw[m][j][i] = 0;
       if (x < D) {
         const KTIR_G(uint16_t)* p = (const KTIR_G(uint16_t)*)d.q.ptr + e + x;
         if (whole) {
           const u32x4_t a = ((const KTIR_G(u32x4_t)*)p)[0], b = ((const KTIR_G(u32x4_t)*)p)[1];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) raw[j][i] = a[i], raw[j][4 + i] = b[i];
+          for (int i = 0; i < 4; ++i) raw[m][j][i] = a[i], raw[m][j][4 + i] = b[i];
         } else {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) raw[j][i] = p[2 * i] | (uint32_t)p[2 * i + 1] << 16;
+          for (int i = 0; i < 8; ++i) raw[m][j][i] = p[2 * i] | (uint32_t)p[2 * i + 1] << 16;
         }
       }
+    }
+  }
+  const int koff = c16 * (int)c.k_tok, vcol = c16 * 4 * J + 4 * J <= D ? c16 * 4 * J : 0, voff = 4 * g4 * (int)c.v_tok + vcol;
+  // the first keys' pages, scales and codes are on their way while Q is made ready
+  KV8Groups g = kv8_groups(d, head, page0, lo + mine < t.hi, err);
+  KV8Keys<J> k[2];
+  if (lo < t.hi) kv8_keys<J>(c, g, 0, lo, head, koff, kpiece, k[0]);
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int j = 0; j < J; ++j)
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const uint32_t a = raw[j][i] & 0x7fffu, b = (raw[j][i] >> 16) & 0x7fffu;
+        const uint32_t a = raw[m][j][i] & 0x7fffu, b = (raw[m][j][i] >> 16) & 0x7fffu;
         top = top > a ? top : a;
         top = top > b ? top : b;
       }
-    }
     const bool bf = d.dtype == KTIR_BF16;
     {
       uint32_t y = __shfl_xor(top, 16);
@@ -158,24 +197,24 @@ __global__ __launch_bounds__(256) void kv8_attn_rows(const ktir_kv8_attn_t d, in
       top = top > y ? top : y;
     }
     // f16 queries are operands as they are; bf16 ones take the power of two that brings the largest to 2^14
-    int k = 0;
+    int k2 = 0;
     if (bf && top) {
-      k = 14 - ((int)(top >> 7) - 127);
-      k = k > 120 ? 120 : k < -113 ? -113 : k;
+      k2 = 14 - ((int)(top >> 7) - 127);
+      k2 = k2 > 120 ? 120 : k2 < -113 ? -113 : k2;
     }
-    const float up = __uint_as_float((uint32_t)(127 + k) << 23);
-    rs[m] = __uint_as_float((uint32_t)(127 - k) << 23) * (d.scale * LOG2E);
+    const float up = __uint_as_float((uint32_t)(127 + k2) << 23);
+    rs[m] = __uint_as_float((uint32_t)(127 - k2) << 23) * (d.scale * LOG2E);
 #pragma unroll
     for (int j = 0; j < J; ++j) {
       if (bf) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const f32x2_t v = uncvt2<true>(raw[j][i]);
-          raw[j][i] = cvt2<false>(v.x * up, v.y * up);
+          const f32x2_t v = uncvt2<true>(raw[m][j][i]);
+          raw[m][j][i] = cvt2<false>(v.x * up, v.y * up);
         }
       }
-      qf[m][j][0] = make_uint4(raw[j][0], raw[j][1], raw[j][2], raw[j][3]);
-      qf[m][j][1] = make_uint4(raw[j][4], raw[j][5], raw[j][6], raw[j][7]);
+      qf[m][j][0] = make_uint4(raw[m][j][0], raw[m][j][1], raw[m][j][2], raw[m][j][3]);
+      qf[m][j][1] = make_uint4(raw[m][j][4], raw[m][j][5], raw[m][j][6], raw[m][j][7]);
     }
   }
   int lo_most, hi_least, x;
@@ -193,9 +232,8 @@ __global__ __launch_bounds__(256) void kv8_attn_rows(const ktir_kv8_attn_t d, in
 #pragma unroll
     for (int n = 0; n < N; ++n) acc[m][n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   }
-  const int koff = c16 * (int)c.k_tok, vcol = c16 * 4 * J + 4 * J <= D ? c16 * 4 * J : 0, voff = 4 * g4 * (int)c.v_tok + vcol;
 
-  auto step = [&](const KV8Step<J>& o, const KV8Groups& g, int group, int key) {
+  auto step = [&](const KV8Keys<J>& o, KV8Values<J>& ov, const KV8Groups& g, int group, int key) {
     f32x4_t s[MT][2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -259,17 +297,17 @@ __global__ __launch_bounds__(256) void kv8_attn_rows(const ktir_kv8_attn_t d, in
       wh[m] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
       wl[m] = make_uint4(lo_[0], lo_[1], lo_[2], lo_[3]);
     }
-    uint32_t v[8][J];
-    const bool tail = CODE == KTIR_E4M3 && key + ROWS_STEP > t.hi;
+    if (CODE == KTIR_E4M3 && key + ROWS_STEP > t.hi) {     // NaN codes of tokens that no row sees
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+      for (int i = 0; i < 8; ++i)
 #pragma unroll
-      for (int j = 0; j < J; ++j) v[i][j] = tail && key + 16 * (i >> 2) + 4 * g4 + (i & 3) >= t.hi ? 0u : o.v[i][j];
+        for (int j = 0; j < J; ++j) ov.v[i][j] = key + 16 * (i >> 2) + 4 * g4 + (i & 3) >= t.hi ? 0u : ov.v[i][j];
+    }
 #pragma unroll
     for (int j = 0; j < J; ++j) {
       uint32_t p[4][4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) cross_bf2<CODE>(v[2 * i][j], v[2 * i + 1][j], p[i]);
+      for (int i = 0; i < 4; ++i) cross_bf2<CODE>(ov.v[2 * i][j], ov.v[2 * i + 1][j], p[i]);
 #pragma unroll
       for (int n = 0; n < 4; ++n) {
         const uint4 a = make_uint4(p[0][n], p[1][n], p[2][n], p[3][n]);
@@ -282,22 +320,29 @@ __global__ __launch_bounds__(256) void kv8_attn_rows(const ktir_kv8_attn_t d, in
     }
   };
 
-  for (int base = lo; base < end; base += 16 * ROWS_GROUPS) {
-    const KV8Groups g = kv8_groups(d, t, head, base + 16 * l, end, shift, err);
-    const int n = (end - base + ROWS_STEP - 1) / ROWS_STEP, steps = n < ROWS_GROUPS / 2 ? n : ROWS_GROUPS / 2;
-    KV8Step<J> o[2];
-    kv8_load<J>(c, g, 0, base, head, koff, voff, kpiece, o[0]);
+  for (int64_t first = lo; first < t.hi; first += (int64_t)stride * (ROWS_GROUPS / 2)) {
+    const int base = (int)first;
+    const bool there = first + mine < t.hi;
+    if (base != lo) {
+      g = kv8_groups(d, head, there ? kv8_pages(d, t, base + mine, t.hi, shift) : 0, there, err);
+      kv8_keys<J>(c, g, 0, base, head, koff, kpiece, k[0]);
+    }
+    const int n = (t.hi - base + stride - 1) / stride, steps = n < ROWS_GROUPS / 2 ? n : ROWS_GROUPS / 2;
     for (int i = 0; i < steps; i += 2) {
-      if (i + 1 < steps) kv8_load<J>(c, g, 2 * i + 2, base + ROWS_STEP * (i + 1), head, koff, voff, kpiece, o[1]);
-      step(o[0], g, 2 * i, base + ROWS_STEP * i);
-      if (i + 1 < steps) {
-        if (i + 2 < steps) kv8_load<J>(c, g, 2 * i + 4, base + ROWS_STEP * (i + 2), head, koff, voff, kpiece, o[0]);
-        step(o[1], g, 2 * i + 2, base + ROWS_STEP * (i + 1));
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        if (i + x >= steps) break;
+        const int key = base + stride * (i + x), group = 2 * (i + x);
+        KV8Values<J> v;
+        kv8_values<J>(c, g, group, key, head, voff, v);
+        if (i + x + 1 < steps) kv8_keys<J>(c, g, group + 2, key + stride, head, koff, kpiece, k[1 - x]);
+        if (x == 0 && i == 0) kv8_scales(g, there);      // with the first codes already on their way
+        step(k[x], v, g, group, key);
       }
     }
   }
 
-  // the four wavefronts' sums, one after another
+  // the wavefronts' sums, each in a part of LDS, then added in their order
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
     sum[m] += __shfl_xor(sum[m], 16);
@@ -308,92 +353,126 @@ __global__ __launch_bounds__(256) void kv8_attn_rows(const ktir_kv8_attn_t d, in
     }
   }
   __syncthreads();
-  float top[MT], f[MT];
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
-    top[m] = w_b[0][16 * m + c16];
+    const int row = 16 * m + c16;
+    float top = b[m];
+    for (int w = wave % hw; w < W; w += hw) top = __builtin_fmaxf(top, w_b[w][row]);
+    const float f = __builtin_amdgcn_exp2f(b[m] - top);
+    if (row < t.rows) {
 #pragma unroll
-    for (int w = 1; w < ROWS_WAVES; ++w) top[m] = __builtin_fmaxf(top[m], w_b[w][16 * m + c16]);
-    f[m] = __builtin_amdgcn_exp2f(b[m] - top[m]);
-  }
-#pragma unroll 1
-  for (int w = 0; w < ROWS_WAVES; ++w) {
-    if (w == wave) {
+      for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float* p = o_sum + (16 * m + c16) * PITCH + (4 * g4 + i) * N;
-#pragma unroll
-          for (int n = 0; n < N; ++n) p[n] = (w ? p[n] : 0.f) + acc[m][n][i] * f[m];
-        }
-    }
-    __syncthreads();
-  }
-
-  // alone: the result; otherwise its part for kv8_attn_join
-  KTIR_G(float)* ws = (KTIR_G(float)*)d.ws + blockIdx.x * PART<J, MT>;
-  for (int at = threadIdx.x; at < TM; at += 256) {
-    float bt = w_b[0][at], lt = 0.f;
-    for (int w = 1; w < ROWS_WAVES; ++w) bt = __builtin_fmaxf(bt, w_b[w][at]);
-    for (int w = 0; w < ROWS_WAVES; ++w) lt += w_l[w][at] * __builtin_amdgcn_exp2f(w_b[w][at] - bt);
-    w_b[0][at] = bt;
-    w_l[0][at] = lt;
-    if (active > 1) {
-      ws[TM * 64 * J + at] = bt;
-      ws[TM * 64 * J + TM + at] = lt;
-    } else if (d.lse && at < t.rows) {
-      const int r = t.row0 + at;
-      int a, z;
-      seen(d, t, r, grp, &a, &z);
-      ((KTIR_G(float)*)d.lse)[(t.q.start + r / grp) * d.lse_tok + (head * grp + r % grp) * d.lse_head] =
-          a >= z ? -__builtin_inff() : (bt + 16.f + __builtin_amdgcn_logf(lt)) * 0.69314718055994530942f;
+        for (int n = 0; n < N; n += 4)
+          *(f32x4_t*)(o_sum[wave] + row * PITCH + (4 * g4 + i) * N + n) =
+              f32x4_t{acc[m][n][i] * f, acc[m][n + 1][i] * f, acc[m][n + 2][i] * f, acc[m][n + 3][i] * f};
     }
   }
   __syncthreads();
-  for (int at = threadIdx.x; at < t.rows * 16 * J; at += 256) {
+
+  // alone: the result; otherwise its part for kv8_attn_join
+  KTIR_G(float)* ws = (KTIR_G(float)*)d.ws + (item * splits + split) * PART<J, MT>;
+  for (int at = turn * 64 + l; at < t.rows * 16 * J; at += 64 * TW) {
     const int row = at / (16 * J), x4 = at % (16 * J) * 4;
-    const f32x4_t o = *(const f32x4_t*)(o_sum + row * PITCH + x4);
+    f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+    float top = B_NONE, lt = 0.f;
+    for (int w = wave % hw; w < W; w += hw) {
+      o += *(const f32x4_t*)(o_sum[w] + row * PITCH + x4);
+      top = __builtin_fmaxf(top, w_b[w][row]);
+    }
+    for (int w = wave % hw; w < W; w += hw) lt += w_l[w][row] * __builtin_amdgcn_exp2f(w_b[w][row] - top);
     if (active > 1) {
       *(KTIR_G(f32x4_t)*)(ws + row * 64 * J + x4) = o;
+      if (x4 == 0) {
+        ws[TM * 64 * J + row] = top;
+        ws[TM * 64 * J + TM + row] = lt;
+      }
       continue;
     }
-    if (x4 >= D) continue;
     const int r = t.row0 + row;
     int a, z;
     seen(d, t, r, grp, &a, &z);
-    const float inv = L_UNIT / w_l[0][row];
-    const int64_t e = (t.q.start + r / grp) * d.out.tok + (head * grp + r % grp) * d.out.head + x4;
+    const int64_t tok = t.q.start + r / grp, h = head * grp + r % grp, e = tok * d.out.tok + h * d.out.head + x4;
+    const float inv = L_UNIT / lt;
+    if (x4 < D) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) store_elem(d.out.ptr, e + i, d.dtype, a >= z ? 0.f : o[i] * inv);
+      for (int i = 0; i < 4; ++i) store_elem(d.out.ptr, e + i, d.dtype, a >= z ? 0.f : o[i] * inv);
+    }
+    if (d.lse && x4 == 0)
+      ((KTIR_G(float)*)d.lse)[tok * d.lse_tok + h * d.lse_head] =
+          a >= z ? -__builtin_inff() : (top + 16.f + __builtin_amdgcn_logf(lt)) * 0.69314718055994530942f;
   }
 }
 
-// The parts of a tile's splits, joined in their order: one wavefront per row, J columns a lane.
-template <int J, int MT>
-__global__ __launch_bounds__(256) void kv8_attn_join(const ktir_kv8_attn_t d, int* err) {
-  constexpr int TM = 16 * MT, QUANT = ROWS_STEP * ROWS_WAVES;
+// The parts of a tile's splits, joined: B wavefronts for each of R rows, which take
+// up to 16 splits each in turn, J columns a lane.  Bound: latency.  All parts are
+// read at once, before the sequence's length says which of them were written.
+constexpr int JOIN_EACH = 16;
+
+template <int J, int MT, int R, int B>
+__global__ __launch_bounds__(64 * R * B) void kv8_attn_join(const ktir_kv8_attn_t d, int splits, int part, int* err) {
+  constexpr int TM = 16 * MT, LOOK = B == 1 ? 1 : MOST_SPLITS / 64;
+  static_assert(B * JOIN_EACH <= 64 * LOOK, "a lane looks at the b and l of each split");
+  __shared__ float f[R][64 * LOOK], sums[B == 1 ? 1 : R * B][64 * J];
   const ktir_kv8_t& c = d.cache;
-  const int l = threadIdx.x & 63, grp = (int)(d.q_heads / c.heads), D = (int)c.columns, splits = d.splits;
-  const int64_t item = blockIdx.x, head = item % c.heads, slot = item / c.heads;
-  const Tile t = tile_of(d, slot, TM, grp, err);
-  const int row = uni((int)(blockIdx.y * 4 + (threadIdx.x >> 6)));
-  if (row >= t.rows) return;
-  const int from = t.lo & ~(ROWS_STEP - 1), span = t.hi > from ? t.hi - from : 0;
-  const int part = ((span + splits - 1) / splits + QUANT - 1) / QUANT * QUANT, active = span ? (span + part - 1) / part : 1;
-  if (active <= 1) return;
+  const int l = threadIdx.x & 63, wave = uni((int)(threadIdx.x >> 6)), grp = (int)((uint32_t)d.q_heads / (uint32_t)c.heads), D = (int)c.columns;
+  const uint32_t heads = (uint32_t)c.heads, slot = blockIdx.x / heads;
+  const int64_t item = blockIdx.x, head = blockIdx.x - slot * heads;
+  const int sub = wave / B, turn = wave % B, row = (int)blockIdx.y * R + sub;
   const KTIR_G(float)* ws = (const KTIR_G(float)*)d.ws + item * splits * PART<J, MT>;
-  float top = B_NONE;
-  for (int s = l; s < active; s += 64) top = __builtin_fmaxf(top, ws[s * PART<J, MT> + TM * 64 * J + row]);
-  for (int o = 32; o; o >>= 1) top = __builtin_fmaxf(top, __shfl_xor(top, o));
-  float acc[J] = {}, lt = 0.f;
-  for (int s = 0; s < active; ++s) {
-    const KTIR_G(float)* p = ws + s * PART<J, MT>;
-    const float f = __builtin_amdgcn_exp2f(p[TM * 64 * J + row] - top);
-    lt += p[TM * 64 * J + TM + row] * f;
+  float x[JOIN_EACH][J], b[LOOK], w[LOOK];
 #pragma unroll
-    for (int j = 0; j < J; ++j) acc[j] += p[row * 64 * J + 64 * j + l] * f;
+  for (int i = 0; i < LOOK; ++i) {
+    b[i] = B_NONE, w[i] = 0.f;
+    if (row < TM && l + 64 * i < splits) {
+      b[i] = ws[(l + 64 * i) * PART<J, MT> + TM * 64 * J + row];
+      w[i] = ws[(l + 64 * i) * PART<J, MT> + TM * 64 * J + TM + row];
+    }
   }
+#pragma unroll
+  for (int k = 0; k < JOIN_EACH; ++k)
+    if (row < TM && turn + B * k < splits) {
+#pragma unroll
+      for (int j = 0; j < J; ++j) x[k][j] = ws[(turn + B * k) * PART<J, MT> + row * 64 * J + 64 * j + l];
+    }
+  const Tile t = uni(tile_of(d, slot, TM, grp, err));
+  const int from = t.lo & ~(ROWS_STEP - 1), span = t.hi > from ? t.hi - from : 0, active = span ? (span + part - 1) / part : 1;
+  const bool on = row < t.rows && active > 1;
+  float top = B_NONE, lt = 0.f;
+#pragma unroll
+  for (int i = 0; i < LOOK; ++i)
+    if (l + 64 * i < active) top = __builtin_fmaxf(top, b[i]);
+  for (int o = 32; o; o >>= 1) top = __builtin_fmaxf(top, __shfl_xor(top, o));
+#pragma unroll
+  for (int i = 0; i < LOOK; ++i) {
+    if (l + 64 * i >= active) continue;
+    const float e = __builtin_amdgcn_exp2f(b[i] - top);
+    lt += w[i] * e;
+    if (turn == 0) f[sub][l + 64 * i] = e;
+  }
+  for (int o = 32; o; o >>= 1) lt += __shfl_xor(lt, o);
+  __syncthreads();
+  float acc[J] = {};
+  if (on) {
+#pragma unroll
+    for (int k = 0; k < JOIN_EACH; ++k)
+      if (turn + B * k < active) {
+#pragma unroll
+        for (int j = 0; j < J; ++j) acc[j] += x[k][j] * f[sub][turn + B * k];
+      }
+  }
+  if constexpr (B > 1) {
+#pragma unroll
+    for (int j = 0; j < J; ++j) sums[wave][64 * j + l] = acc[j];
+    __syncthreads();
+    if (turn == 0) {
+#pragma unroll
+      for (int i = 1; i < B; ++i)
+#pragma unroll
+        for (int j = 0; j < J; ++j) acc[j] += sums[wave + i][64 * j + l];
+    }
+  }
+  if (!on || turn) return;
   const int r = t.row0 + row;
   int a, z;
   seen(d, t, r, grp, &a, &z);
@@ -416,27 +495,51 @@ void kv8_rows_shape(const ktir_kv8_attn_t& d, KV8Shape* s) {
   const int64_t TM = 16 * s->MT;
   s->slots = d.max_q * grp > TM ? d.batch.tokens * grp / TM + d.batch.seqs : d.batch.seqs;
   s->part = TM * (64 * s->J + 2);
-  // splits: enough workgroups for 256 CUs, no fewer than 256 keys each
-  const int64_t items = s->slots * d.cache.heads, most = (d.max_k + 255) / 256;
-  int64_t n = items ? 1024 / items : 1;
+  // the most tokens that a tile's rows see, from a step's bound on
+  s->span = d.max_k;
+  const int64_t near = d.window + (TM - 1) / grp + 1;
+  if (d.window && near < s->span) s->span = near;
+  s->span += ROWS_STEP - 1;
+  // Splits and heads of a workgroup.  Up to 2^19 keys (times KV heads) a wavefront's
+  // four work on one head: one workgroup a CU is best for one sequence (65536
+  // tokens of 8 heads: 36.8 us, two a CU 42.5), four where lengths may differ (8
+  // sequences of up to 8192: 21.8, 28.6 with one), none under 128 keys.  More come from
+  // HBM, which gives 4.8 TB/s to 128-byte rows of one head each, 5.6 where four heads'
+  // rows are read together (copy patterns of 268 MB; 64 sequences of 2460 tokens: 76.8
+  // and 69.6 us).
+  const int64_t heads = d.cache.heads, keys = s->slots * heads * s->span;
+  const bool tiles = d.max_q * grp > TM, far = keys > (1 << 19) && !tiles;
+  s->HW = !far ? 1 : heads % 4 == 0 ? 4 : heads % 2 == 0 ? 2 : 1;
+  const int64_t sets = s->slots * heads / s->HW;
+  int64_t n = sets ? (!tiles && (far ? s->slots * heads >= 256 : s->slots > 1) ? 1024 : 256) / sets : 1;
+  if (far && s->slots > 1) {                          // sequences of other lengths than the longest
+    const int64_t even = s->span / 512 < 4 ? s->span / 512 : 4;
+    n = n < even ? even : n;
+  }
+  const int64_t most = (s->span + 127) / 128;
   n = n > most ? most : n;
-  s->splits = n < 1 ? 1 : n > 64 ? 64 : (int)n;
+  s->splits = n < 1 ? 1 : n > MOST_SPLITS ? MOST_SPLITS : (int)n;
 }
 
 template <int CODE, int J, int MT>
 static int launch(const ktir_kv8_attn_t& d, const KV8Shape& s) {
-  const int64_t items = s.slots * d.cache.heads, splits = d.splits < 1 ? 1 : d.splits;
+  constexpr int W = ROWS_WAVES;
+  const int64_t QUANT = ROWS_STEP * W / s.HW, items = s.slots * d.cache.heads, splits = d.splits < 1 ? 1 : d.splits;
+  const int part = (int)(((s.span + splits - 1) / splits + QUANT - 1) / QUANT * QUANT);
   const hipStream_t st = stream_of(d.stream);
-  hipLaunchKernelGGL((kv8_attn_rows<CODE, J, MT>), dim3((unsigned)(items * splits)), dim3(256), 0, st, d, device_error_flag());
-  if (splits > 1)
-    hipLaunchKernelGGL((kv8_attn_join<J, MT>), dim3((unsigned)items, 4 * MT), dim3(256), 0, st, d, device_error_flag());
+  hipLaunchKernelGGL((kv8_attn_rows<CODE, J, MT>), dim3((unsigned)((s.slots * splits + 7) / 8 * 8 * (d.cache.heads / s.HW))), dim3(64 * W), 0, st, d, (int)splits, part, (uint32_t)s.slots, s.HW, device_error_flag());
+  if (splits > 1) {
+    const int64_t rows = d.max_q * (d.q_heads / d.cache.heads), most = rows < 16 * MT ? rows : 16 * MT;
+    if (splits <= JOIN_EACH) hipLaunchKernelGGL((kv8_attn_join<J, MT, 4, 1>), dim3((unsigned)items, (unsigned)((most + 3) / 4)), dim3(256), 0, st, d, (int)splits, part, device_error_flag());
+    else hipLaunchKernelGGL((kv8_attn_join<J, MT, 1, 16>), dim3((unsigned)items, (unsigned)most), dim3(1024), 0, st, d, (int)splits, part, device_error_flag());
+  }
   KTIR_HIP_CHECK(hipGetLastError());
   return KTIR_OK;
 }
 
 template <int CODE, int J>
 static int launch_j(const ktir_kv8_attn_t& d, const KV8Shape& s) {
-  return s.MT == 1 ? launch<CODE, J, 1>(d, s) : launch<CODE, J, 2>(d, s);
+  return s.MT == 2 ? launch<CODE, J, 2>(d, s) : launch<CODE, J, 1>(d, s);
 }
 
 template <int CODE>

@@ -28,8 +28,8 @@ class OnDevice {
 
 // The shape that ktir_kv8_rows.hip gives an attention launch.
 struct KV8Shape {
-  int J, MT, splits;
-  int64_t slots, part;                 // tiles of rows for each KV head; floats of a split's part in the workspace
+  int J, MT, HW, splits;               // columns in 64s, rows in 16s, heads of a workgroup
+  int64_t slots, part, span;           // tiles of rows for each KV head; floats of a split's part in the workspace; most keys of a tile
 };
 void kv8_rows_shape(const ktir_kv8_attn_t& d, KV8Shape* s);
 int kv8_rows_launch(const ktir_kv8_attn_t& d, const KV8Shape& s);
@@ -68,18 +68,18 @@ __device__ __forceinline__ Seq seq_of(const ktir_kv8_batch_t& b, int64_t page, i
 }
 
 // The sequence that slot `w` of a launch belongs to, and its number in it, where
-// sequence s has the slots from floor(q_start[s] * mul / per) + extra * s on (so
-// every sequence has at least floor(n * mul / per) + extra of them): the last s whose first
+// sequence s has the slots from floor(q_start[s] * mul / 2^shift) + extra * s on (so
+// one of n tokens has at least floor(n * mul / 2^shift) + extra): the last s whose first
 // slot is not after w, with nth < 0 if there is none.  All lanes of a wavefront
 // search together, 64 sequences a step.
-__device__ __forceinline__ int64_t seq_of_slot(const ktir_kv8_batch_t& b, int64_t mul, int64_t per, int64_t extra, int64_t w, int64_t* nth) {
+__device__ __forceinline__ int64_t seq_of_slot(const ktir_kv8_batch_t& b, int64_t mul, int shift, int64_t extra, int64_t w, int64_t* nth) {
   const int l = threadIdx.x & 63;
   int64_t s = 0, first = INT64_MAX;
   for (int64_t base = 0; base < b.seqs; base += 64) {
     int64_t at = INT64_MAX;
     if (base + l < b.seqs) {
       const int64_t q = ints(b.q_start)[base + l];
-      at = (q < 0 ? 0 : q) * mul / per + extra * (base + l);
+      at = ((q < 0 ? 0 : q) * mul >> shift) + extra * (base + l);
     }
     const uint64_t below = __ballot(at <= w);
     if (!below) break;

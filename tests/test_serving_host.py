@@ -251,10 +251,10 @@ def test_attention_refused():
         attention(max_k=1 << 16, workspace=far(24, (8,), "|u1"))
     with pytest.raises(ValueError, match="workspace"):
         attention(max_k=1 << 16, workspace=Fake((1 << 28,), "|u1", ptr=(1 << 34) + 4))
-    op = attention(max_k=1 << 16)
+    op = attention(max_k=1 << 13)
     assert op.desc.splits > 1 and op.workspace_bytes > 0
-    for name, value in (("ws", 0), ("ws", (1 << 34) + 8), ("ws_bytes", op.workspace_bytes - 4), ("splits", op.desc.splits + 1)):
-        op = attention(max_k=1 << 16)
+    for name, value in (("ws", 0), ("ws", (1 << 34) + 8), ("ws_bytes", op.workspace_bytes - 4), ("splits", op.desc.splits * 2)):
+        op = attention(max_k=1 << 13)
         setattr(op.desc, name, value)
         refused(op, match="workspace")
     for name, value, code in (("dtype", rt.K["KTIR_F32"], "KTIR_E_UNSUPPORTED"), ("q_heads", 0, "KTIR_E_ARG"),
