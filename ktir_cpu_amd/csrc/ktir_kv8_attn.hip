@@ -11,7 +11,7 @@ static int check_attn(const char* what, const ktir_kv8_attn_t& d) {
   if (rc != KTIR_OK) return rc;
   if (d.q_heads < 1 || d.q_heads % d.cache.heads || d.q_heads > 65536)
     return set_error(KTIR_E_ARG, "%s: %lld query heads over %lld", what, (long long)d.q_heads, (long long)d.cache.heads);
-  if (d.max_q < 0 || d.max_k < 0 || d.max_k > INT32_MAX - 65536) return set_error(KTIR_E_ARG, "%s: bounds %lld and %lld", what, (long long)d.max_q, (long long)d.max_k);
+  if (d.max_q < 0 || d.max_k < 0 || d.max_k > (1 << 30)) return set_error(KTIR_E_ARG, "%s: bounds %lld and %lld", what, (long long)d.max_q, (long long)d.max_k);
   if (d.window < 0 || (d.window && !d.causal)) return set_error(KTIR_E_ARG, "%s: window %lld", what, (long long)d.window);
   if (!(d.scale - d.scale == 0.f)) return set_error(KTIR_E_ARG, "%s: scale is not finite", what);
   if (d.batch.tokens * (d.q_heads / d.cache.heads) > (1 << 30)) return set_error(KTIR_E_UNSUPPORTED, "%s: %lld rows of a KV head", what, (long long)(d.batch.tokens * (d.q_heads / d.cache.heads)));
@@ -29,7 +29,9 @@ extern "C" int ktir_kv8_attention_plan(ktir_kv8_attn_t* d) {
   const int rc = check_attn(ME, *d);
   if (rc != KTIR_OK) return rc;
   KV8Shape s;
+  int64_t slots;
   kv8_rows_shape(*d, &s);
+  if (kv8_tile_takes(*d, &slots)) s.splits = 1;
   d->splits = s.splits;
   d->ws_bytes = s.splits > 1 ? s.slots * d->cache.heads * s.splits * s.part * 4 : 0;
   return KTIR_OK;
@@ -60,5 +62,7 @@ extern "C" int ktir_launch_kv8_attention(const ktir_kv8_attn_t* d) {
   if (rc != KTIR_OK) return rc;
   OnDevice on;
   if (!on.ok()) return set_error(KTIR_E_HIP, "%s: no device", ME);
+  int64_t slots;
+  if (kv8_tile_takes(*d, &slots)) return kv8_tile_launch(*d, slots);
   return kv8_rows_launch(*d, s);
 }

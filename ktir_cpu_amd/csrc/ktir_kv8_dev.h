@@ -75,6 +75,33 @@ __device__ __forceinline__ void cross_bf2(uint32_t x, uint32_t y, uint32_t (&out
   }
 }
 
+// two words, four codes each, as four f16 pairs (x's code, y's code)
+template <int CODE>
+__device__ __forceinline__ void cross_half2(uint32_t x, uint32_t y, uint32_t (&out)[4]) {
+  if constexpr (CODE == KTIR_I8) {
+    out[0] = i8_half2(bytes2<0, 0>(x, y));
+    out[1] = i8_half2(bytes2<1, 1>(x, y));
+    out[2] = i8_half2(bytes2<2, 2>(x, y));
+    out[3] = i8_half2(bytes2<3, 3>(x, y));
+  } else {
+    const uint32_t a = word_half2<CODE, 0>(x), b = word_half2<CODE, 0>(y), c = word_half2<CODE, 1>(x), e = word_half2<CODE, 1>(y);
+    out[0] = __builtin_amdgcn_perm(b, a, 0x05040100u);
+    out[1] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+    out[2] = __builtin_amdgcn_perm(e, c, 0x05040100u);
+    out[3] = __builtin_amdgcn_perm(e, c, 0x07060302u);
+  }
+}
+
+// Where the groups of 16 keys of a wavefront's next steps lie, a group per lane.
+struct KV8Groups {
+  int page;             // of the cache
+  float ks, lv, iv;     // kscale, log2 vscale, 2^-16 / vscale
+};
+
+__device__ __forceinline__ float lane_of(float x, int i) {
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), i));
+}
+
 // The rows of one tile of a launch: query head h * grp + r % grp of token
 // i = r / grp of sequence s, r from row0 on; what they see of the keys.
 struct Tile {
@@ -111,6 +138,74 @@ __device__ __forceinline__ Tile tile_of(const ktir_kv8_attn_t& d, int64_t slot, 
   seen(d, t, t.row0, grp, &t.lo, &x);
   seen(d, t, t.row0 + t.rows - 1, grp, &x, &t.hi);
   return t;
+}
+
+// the page of the group that starts at `key`; from `end` on: page 0, which weighs nothing
+__device__ __forceinline__ int kv8_pages(const ktir_kv8_attn_t& d, const Tile& t, int key, int end, int shift) {
+  return key < end ? ints(d.batch.table)[t.s * d.batch.table_row + (key >> shift)] : 0;
+}
+
+__device__ __forceinline__ KV8Groups kv8_groups(const ktir_kv8_attn_t& d, int64_t head, int page, bool there, int* err) {
+  if ((uint32_t)page >= (uint64_t)d.cache.pages) {
+    *err = OUT_OF_RANGE;
+    page = 0;
+  }
+  KV8Groups g = {page, 0.f, 0.f, L_UNIT};
+  if (there) {
+    g.ks = ((const KTIR_G(float)*)d.cache.k_scale)[page * d.cache.ks_page + head * d.cache.ks_head];
+    g.lv = ((const KTIR_G(float)*)d.cache.v_scale)[page * d.cache.vs_page + head * d.cache.vs_head];
+  }
+  return g;
+}
+
+// vscale as its logarithm and inverse (not where it is loaded: that would wait for it)
+__device__ __forceinline__ void kv8_scales(KV8Groups& g, bool there) {
+  if (!there) return;
+  const float vs = g.lv < LEAST_V ? LEAST_V : g.lv;
+  g.lv = __builtin_amdgcn_logf(vs);
+  g.iv = vs != vs ? 1.f : L_UNIT / vs;      // NaN is in lv, and so in the weights of the rows that see the page alone
+}
+
+// 16 query values from element e on, packed
+__device__ __forceinline__ void q16(const ktir_kv8_attn_t& d, int64_t e, bool whole, uint32_t (&raw)[8]) {
+  const KTIR_G(uint16_t)* p = (const KTIR_G(uint16_t)*)d.q.ptr + e;
+  if (whole) {
+    const u32x4_t a = ((const KTIR_G(u32x4_t)*)p)[0], b = ((const KTIR_G(u32x4_t)*)p)[1];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) raw[i] = a[i], raw[4 + i] = b[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) raw[i] = p[2 * i] | (uint32_t)p[2 * i + 1] << 16;
+  }
+}
+
+// the largest of N packed pairs' absolute bits
+template <int N>
+__device__ __forceinline__ uint32_t top_bits(const uint32_t (&raw)[N], uint32_t top) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const uint32_t a = raw[i] & 0x7fffu, b = (raw[i] >> 16) & 0x7fffu;
+    top = top > a ? top : a;
+    top = top > b ? top : b;
+  }
+  return top;
+}
+
+// f16 queries are operands as they are; bf16 ones take the power of two 2^k that brings the row's largest to 2^14
+__device__ __forceinline__ int q_power(uint32_t top) {
+  if (!top) return 0;
+  const int k = 14 - ((int)(top >> 7) - 127);
+  return k > 120 ? 120 : k < -113 ? -113 : k;
+}
+__device__ __forceinline__ float power2(int k) { return __uint_as_float((uint32_t)(127 + k) << 23); }
+
+template <int N>
+__device__ __forceinline__ void q_scaled(uint32_t (&raw)[N], float up) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const f32x2_t v = uncvt2<true>(raw[i]);
+    raw[i] = cvt2<false>(v.x * up, v.y * up);
+  }
 }
 
 // a tile's fields in scalar registers: they are the same in every lane

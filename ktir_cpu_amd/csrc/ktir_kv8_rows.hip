@@ -38,42 +38,6 @@ struct KV8Values {
   uint32_t v[8][J];
 };
 
-// where a wavefront's next 64 groups of 16 keys lie, a group per lane
-struct KV8Groups {
-  int page;             // of the cache
-  float ks, lv, iv;     // kscale, log2 vscale, 2^-16 / vscale
-};
-
-__device__ __forceinline__ float lane_of(float x, int i) {
-  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), i));
-}
-
-// the pages of the groups that start at `key` in this lane; groups from `end` on: page 0, which weighs nothing
-__device__ __forceinline__ int kv8_pages(const ktir_kv8_attn_t& d, const Tile& t, int key, int end, int shift) {
-  return key < end ? ints(d.batch.table)[t.s * d.batch.table_row + (key >> shift)] : 0;
-}
-
-__device__ __forceinline__ KV8Groups kv8_groups(const ktir_kv8_attn_t& d, int64_t head, int page, bool there, int* err) {
-  if ((uint32_t)page >= (uint64_t)d.cache.pages) {
-    *err = OUT_OF_RANGE;
-    page = 0;
-  }
-  KV8Groups g = {page, 0.f, 0.f, L_UNIT};
-  if (there) {
-    g.ks = ((const KTIR_G(float)*)d.cache.k_scale)[page * d.cache.ks_page + head * d.cache.ks_head];
-    g.lv = ((const KTIR_G(float)*)d.cache.v_scale)[page * d.cache.vs_page + head * d.cache.vs_head];
-  }
-  return g;
-}
-
-// vscale as its logarithm and inverse (not where it is loaded: that would wait for it)
-__device__ __forceinline__ void kv8_scales(KV8Groups& g, bool there) {
-  if (!there) return;
-  const float vs = g.lv < LEAST_V ? LEAST_V : g.lv;
-  g.lv = __builtin_amdgcn_logf(vs);
-  g.iv = L_UNIT / vs;
-}
-
 // the codes of 32 keys from `key` on; groups that the wavefront does not have read page 0
 template <int J>
 __device__ __forceinline__ void kv8_keys(const ktir_kv8_t& c, const KV8Groups& g, int group, int key, int64_t head, int koff,
@@ -160,17 +124,7 @@ __global__ __launch_bounds__(64 * ROWS_WAVES, MT == 1 ? 2 : 1) void kv8_attn_row
       const int x = (4 * j + g4) * 16;
 #pragma unroll
       for (int i = 0; i < 8; ++i) raw[m][j][i] = 0;
-      if (x < D) {
-        const KTIR_G(uint16_t)* p = (const KTIR_G(uint16_t)*)d.q.ptr + e + x;
-        if (whole) {
-          const u32x4_t a = ((const KTIR_G(u32x4_t)*)p)[0], b = ((const KTIR_G(u32x4_t)*)p)[1];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) raw[m][j][i] = a[i], raw[m][j][4 + i] = b[i];
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) raw[m][j][i] = p[2 * i] | (uint32_t)p[2 * i + 1] << 16;
-        }
-      }
+      if (x < D) q16(d, e + x, whole, raw[m][j]);
     }
   }
   const int koff = c16 * (int)c.k_tok, vcol = c16 * 4 * J + 4 * J <= D ? c16 * 4 * J : 0, voff = 4 * g4 * (int)c.v_tok + vcol;
@@ -182,37 +136,16 @@ __global__ __launch_bounds__(64 * ROWS_WAVES, MT == 1 ? 2 : 1) void kv8_attn_row
   for (int m = 0; m < MT; ++m) {
     uint32_t top = 0;
 #pragma unroll
-    for (int j = 0; j < J; ++j)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const uint32_t a = raw[m][j][i] & 0x7fffu, b = (raw[m][j][i] >> 16) & 0x7fffu;
-        top = top > a ? top : a;
-        top = top > b ? top : b;
-      }
-    const bool bf = d.dtype == KTIR_BF16;
-    {
-      uint32_t y = __shfl_xor(top, 16);
-      top = top > y ? top : y;
-      y = __shfl_xor(top, 32);
-      top = top > y ? top : y;
-    }
-    // f16 queries are operands as they are; bf16 ones take the power of two that brings the largest to 2^14
-    int k2 = 0;
-    if (bf && top) {
-      k2 = 14 - ((int)(top >> 7) - 127);
-      k2 = k2 > 120 ? 120 : k2 < -113 ? -113 : k2;
-    }
-    const float up = __uint_as_float((uint32_t)(127 + k2) << 23);
-    rs[m] = __uint_as_float((uint32_t)(127 - k2) << 23) * (d.scale * LOG2E);
+    for (int j = 0; j < J; ++j) top = top_bits(raw[m][j], top);
+    uint32_t y = __shfl_xor(top, 16);
+    top = top > y ? top : y;
+    y = __shfl_xor(top, 32);
+    top = top > y ? top : y;
+    const int up = d.dtype == KTIR_BF16 ? q_power(top) : 0;
+    rs[m] = power2(-up) * (d.scale * LOG2E);
 #pragma unroll
     for (int j = 0; j < J; ++j) {
-      if (bf) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const f32x2_t v = uncvt2<true>(raw[m][j][i]);
-          raw[m][j][i] = cvt2<false>(v.x * up, v.y * up);
-        }
-      }
+      if (d.dtype == KTIR_BF16) q_scaled(raw[m][j], power2(up));
       qf[m][j][0] = make_uint4(raw[m][j][0], raw[m][j][1], raw[m][j][2], raw[m][j][3]);
       qf[m][j][1] = make_uint4(raw[m][j][4], raw[m][j][5], raw[m][j][6], raw[m][j][7]);
     }
@@ -256,20 +189,18 @@ __global__ __launch_bounds__(64 * ROWS_WAVES, MT == 1 ? 2 : 1) void kv8_attn_row
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
       // exponents of the weights; a key that the row does not see has none
-      float u[8], inv[8];
+      float u[8];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const float f = ks[h] * rs[m];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) u[4 * h + i] = __builtin_fmaf(s[m][h][i], f, lv[h]), inv[4 * h + i] = iv[h];
+        for (int i = 0; i < 4; ++i) u[4 * h + i] = __builtin_fmaf(s[m][h][i], f, lv[h]);
       }
       if (cut) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const int j = key + 16 * (i >> 2) + 4 * g4 + (i & 3);
-          const bool out = j < see_lo[m] || j >= see_hi[m];
-          u[i] = out ? -__builtin_inff() : u[i];
-          inv[i] = out ? 0.f : inv[i];
+          u[i] = j < see_lo[m] || j >= see_hi[m] ? -__builtin_inff() : u[i];
         }
       }
       float top = u[0];
@@ -288,8 +219,8 @@ __global__ __launch_bounds__(64 * ROWS_WAVES, MT == 1 ? 2 : 1) void kv8_attn_row
 #pragma unroll
       for (int i = 0; i < 8; i += 2) {
         const float a = __builtin_amdgcn_exp2f(u[i] - b[m]), e = __builtin_amdgcn_exp2f(u[i + 1] - b[m]);
-        sum[m] = __builtin_fmaf(a, inv[i], sum[m]);
-        sum[m] = __builtin_fmaf(e, inv[i + 1], sum[m]);
+        sum[m] = __builtin_fmaf(a, iv[i >> 2], sum[m]);
+        sum[m] = __builtin_fmaf(e, iv[i >> 2], sum[m]);
         hi[i / 2] = cvt2<true>(a, e);
         const f32x2_t back = uncvt2<true>(hi[i / 2]);
         lo_[i / 2] = cvt2<true>(a - back.x, e - back.y);

@@ -33,6 +33,8 @@ struct KV8Shape {
 };
 void kv8_rows_shape(const ktir_kv8_attn_t& d, KV8Shape* s);
 int kv8_rows_launch(const ktir_kv8_attn_t& d, const KV8Shape& s);
+bool kv8_tile_takes(const ktir_kv8_attn_t& d, int64_t* slots);       // whether ktir_kv8_tile.hip takes it instead
+int kv8_tile_launch(const ktir_kv8_attn_t& d, int64_t slots);
 
 inline hipStream_t stream_of(uint64_t s) {
   return s == 0 ? stream() : s == KTIR_STREAM_NULL ? (hipStream_t) nullptr : (hipStream_t)s;

@@ -74,9 +74,11 @@ def append(x, codes, scale, code, page, table, q_start, kv_len):
     return codes, scale
 
 
-def attention(q, k, v, k_scale, v_scale, table, q_start, kv_len, *, scale, causal=True, window=0, page=None):
-    """(out, lse, bound of out, bound of lse) in float64; rows of no sequence are NaN."""
+def attention(q, k, v, k_scale, v_scale, table, q_start, kv_len, *, scale, causal=True, window=0, heads=None):
+    """(out, lse, bound of out, bound of lse) in float64; rows of no sequence, and heads
+    other than `heads`, are NaN."""
     D, grp, page = q.shape[2], q.shape[1] // k.shape[2], k.shape[1]
+    heads = range(q.shape[1]) if heads is None else heads
     out = torch.full(q.shape, math.nan, dtype=torch.float64)
     lse = torch.full(q.shape[:2], math.nan, dtype=torch.float64)
     bound, lbound = torch.zeros_like(out), torch.zeros_like(lse)
@@ -85,13 +87,14 @@ def attention(q, k, v, k_scale, v_scale, table, q_start, kv_len, *, scale, causa
         held = table[s, :-(-kv // page)].long()
         kk, vv = ((c.view(torch.uint8)[held].view(c.dtype).double() * sc[held].double()[:, None, :, None])
                   .reshape(-1, k.shape[2], D)[:kv] for c, sc in ((k, k_scale), (v, v_scale)))
+        vs = v_scale[held].double().repeat_interleave(page, 0)[:kv]
         j = torch.arange(kv)
         for i in range(n):
             pos = kv - n + i
             seen = (j <= pos) if causal else (j >= 0)
             if window:
                 seen &= j > pos - window
-            for h in range(q.shape[1]):
+            for h in heads:
                 a, b = kk[seen, h // grp], vv[seen, h // grp]
                 row = q[start + i, h].double()
                 if not len(a):
@@ -106,7 +109,11 @@ def attention(q, k, v, k_scale, v_scale, table, q_start, kv_len, *, scale, causa
                 # a weight: its exponential twice that far off above and below the line, f16 (2^-11),
                 # and the f32 sums over the keys
                 rel = 2 * ds + 2.0 ** -11 + len(a) * 2.0 ** -23
-                bound[start + i, h] = (p @ b.abs()) * rel
+                # and a weight (times its page's scale) that is less than 2^-25 of the row's largest is
+                # held in steps of 2^-24 where the largest is at least 2^11: half a step is 2^-36 of it
+                unit = vs[seen, h // grp]
+                small = 2.0 ** -36 * (p * unit).max() * (b.abs() / unit.clamp(min=2.0 ** -100)[:, None]).sum(0)
+                bound[start + i, h] = (p @ b.abs()) * rel + small
                 lbound[start + i, h] = ds + len(a) * 2.0 ** -24 + abs(lse[start + i, h]) * 2.0 ** -22
     return out, lse, bound, lbound
 

@@ -169,8 +169,12 @@ def attend(serving, b, **kw):
     return out, lse
 
 
-def check(b, out, lse, **kw):
-    want, wl, bound, lb = S.attention(b.q, *b.cache(), *b.where(), scale=kw.pop("scale", b.D ** -0.5), **kw)
+def check(b, out, lse, heads=None, **kw):
+    """All query heads, or some of them."""
+    want, wl, bound, lb = S.attention(b.q, *b.cache(), *b.where(), scale=kw.pop("scale", b.D ** -0.5), heads=heads, **kw)
+    if heads is not None:
+        heads = list(heads)
+        want, wl, bound, lb, out, lse = want[:, heads], wl[:, heads], bound[:, heads], lb[:, heads], out[:, heads], lse[:, heads]
     inside = torch.zeros(b.tokens, dtype=torch.bool)
     inside[int(b.q_start[0]):int(b.q_start[-1])] = True
     S.close(out[inside.cuda()], want[inside], bound[inside], b.dt, "out")
@@ -195,6 +199,18 @@ ATTN = {
 def test_attention(serving, lens, hk, grp, D, page, code, dt):
     b = S.Batch(ATTN[lens], hk=hk, grp=grp, D=D, page=page, code=code, dt=dt, pad=2, front=1 if lens == "chunks" else 0, seed=len(lens))
     check(b, *attend(serving, b))
+
+
+@pytest.mark.parametrize("dt", ["f16", "bf16"])
+@pytest.mark.parametrize("code", ["i8", "e4m3"])
+@pytest.mark.parametrize("hk,grp,D,page,window", [(16, 4, 128, 16, 0), (8, 7, 80, 32, 60), (16, 2, 256, 64, 0), (32, 3, 48, 16, 1),
+                                                  (4, 16, 192, 128, 100), (16, 5, 64, 256, 0)])
+def test_attention_prompts(serving, hk, grp, D, page, window, code, dt):
+    """Enough rows for the kernel of many rows: prompts, chunks behind cached tokens, rows
+    that see nothing, sequences of one token or none among them."""
+    b = S.Batch([(130, 130), (90, 300), (1, 70), (0, 5), (33, 20), (64, 64), (70, 1100), (128, 129)], hk=hk, grp=grp, D=D, page=page,
+                code=code, dt=dt, pad=3, front=1, seed=D)
+    check(b, *attend(serving, b, window=window), window=window, heads=(0, grp, hk * grp - 1))
 
 
 @pytest.mark.parametrize("lens", ["decode", "chunks", "empty rows"])
