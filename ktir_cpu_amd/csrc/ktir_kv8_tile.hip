@@ -18,22 +18,17 @@
 
 namespace ktir {
 
-constexpr int TILE_KEYS = 64, TILE_WAVES = 4, TILE_GROUPS = 64;
+constexpr int TILE_KEYS = 64;
 constexpr float TILE_TOP = 11.f, TILE_LAG = 4.f;       // exponent of the largest weight when b changes, and by how much it may grow
-
-template <int CODE, int J, int RB>
-struct TileRaw {
-  u32x4_t k[J];          // J pieces of 16 codes of a key
-  uint32_t v[J > 2 ? J / 2 : 1][8];      // 4 columns of 8 keys, (J + 1) / 2 times
-};
 
 // chunk slots in LDS: 16 bytes, 8 of a K row's (of 8 J), 8 of a V column's 64 keys
 __device__ __forceinline__ int k_slot(int key, int chunk) { return chunk ^ (key & 7); }
 __device__ __forceinline__ int v_slot(int col, int chunk) { return chunk ^ (((col >> 2) ^ col) & 7); }
 
-template <int CODE, int J, int RB>
-__global__ __launch_bounds__(256, 1) void kv8_attn_tile(const ktir_kv8_attn_t d, uint32_t slots, int* err) {
-  constexpr int TM = 128 * RB, DP = 64 * J, VU = J > 2 ? J / 2 : 1;
+template <int CODE, int J, int RB, int W>
+__global__ __launch_bounds__(64 * W, W / 4) void kv8_attn_tile(const ktir_kv8_attn_t d, uint32_t slots, int* err) {
+  constexpr int TM = 32 * RB * W, DP = 64 * J, NT = 64 * W;
+  constexpr int KU = TILE_KEYS * 4 * J, VU = 16 * 16 * J, KP = (KU + NT - 1) / NT, VP = (VU + NT - 1) / NT;   // units of a step, a thread's
   static_assert(J == 1 || J == 2 || J == 4, "columns in 64s");
   __shared__ __attribute__((aligned(16))) uint16_t ks[2][TILE_KEYS * DP], vs[2][DP * TILE_KEYS];
   const ktir_kv8_t& c = d.cache;
@@ -48,7 +43,7 @@ __global__ __launch_bounds__(256, 1) void kv8_attn_tile(const ktir_kv8_attn_t d,
 
   // this lane's rows; the wavefront's bounds of keys
   const int w0 = t.row0 + wave * 32 * RB, wn = t.rows - wave * 32 * RB < 32 * RB ? t.rows - wave * 32 * RB : 32 * RB;
-  int see_lo[RB], see_hi[RB], lo_least = 0, lo_most = 0, hi_least = 0, hi_most = 0;
+  int see_lo[RB], see_hi[RB], lo_most = 0, hi_least = 0, other;
   uint4 qf[RB][4 * J];
   float rs[RB];
   const bool whole = !((d.q.ptr | (uint64_t)d.q.tok * 2 | (uint64_t)d.q.head * 2) & 15);
@@ -78,8 +73,8 @@ __global__ __launch_bounds__(256, 1) void kv8_attn_tile(const ktir_kv8_attn_t d,
     }
 #pragma unroll
     for (int s = 0; s < 4 * J; ++s) top = top_bits(raw[s], top);
-    const uint32_t other = __shfl_xor(top, 32);
-    top = top > other ? top : other;
+    const uint32_t half = __shfl_xor(top, 32);
+    top = top > half ? top : half;
     const int up = d.dtype == KTIR_BF16 ? q_power(top) : 0;
     rs[b] = power2(-up) * (d.scale * LOG2E);
 #pragma unroll
@@ -89,10 +84,10 @@ __global__ __launch_bounds__(256, 1) void kv8_attn_tile(const ktir_kv8_attn_t d,
     }
   }
   if (wn > 0) {
-    seen(d, t, w0, grp, &lo_least, &hi_least);
-    seen(d, t, w0 + wn - 1, grp, &lo_most, &hi_most);
+    seen(d, t, w0, grp, &other, &hi_least);
+    seen(d, t, w0 + wn - 1, grp, &lo_most, &other);
   }
-  lo_least = uni(lo_least), lo_most = uni(lo_most), hi_least = uni(hi_least), hi_most = uni(hi_most);
+  lo_most = uni(lo_most), hi_least = uni(hi_least);
 
   f32x16_t acc[RB][2 * J];
   float base[RB], sum[RB];
@@ -106,181 +101,238 @@ __global__ __launch_bounds__(256, 1) void kv8_attn_tile(const ktir_kv8_attn_t d,
       for (int i = 0; i < 16; ++i) acc[b][n][i] = 0.f;
   }
 
-  // this thread's share of a step: J pieces of 16 codes of keys (tid / (4 J) + 64 / J p), and 4 columns of the 8 keys of one V chunk
-  KV8Groups g = {0, 0.f, 0.f, L_UNIT};
-  TileRaw<CODE, J, RB> raw;
-  const int kkey = tid / (4 * J), kcol = tid % (4 * J) * 16;
-  auto fetch = [&](int key) {                     // the groups of the step at `key` are in lanes ((key - from) / 16) % 64 of g
-    const int group = ((key - from) >> 4) & (TILE_GROUPS - 1);
+  // a thread's share of a step: units of 16 codes of a key, and of 4 columns of 4 keys of V
+  const int steps = t.hi > from ? (t.hi - from + TILE_KEYS - 1) / TILE_KEYS : 0;
+  KV8Groups g = {0, 0.f, 0.f, L_UNIT}, before = g, next = g;    // the groups of the 16 steps that keys are fetched of, and the 16s around
+  int g_from = 0;                                               // the first of g's steps
+  u32x4_t kraw[KP];
+  uint32_t vraw[VP][4];
 #pragma unroll
-    for (int p = 0; p < J; ++p) {
-      const int r = kkey + 64 / J * p;
-      // keys of a wavefront's piece lie in one group of 16: 64 / (4 J) of them, from a multiple of that on
-      const int64_t page = __builtin_amdgcn_readlane(g.page, group + uni(r >> 4)), row = (key + r) & (c.page - 1);
-      if (kcol < D) raw.k[p] = *(const KTIR_G(u32x4_t)*)(c.k + page * c.k_page + row * c.k_tok + head * c.k_head + kcol);
+  for (int p = 0; p < KP; ++p) kraw[p] = u32x4_t{0, 0, 0, 0};         // columns behind D
+#pragma unroll
+  for (int p = 0; p < VP; ++p)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) vraw[p][i] = 0;
+  auto page_of = [&](int j, int group) {         // of step j, in the groups of the step or of the 16 before
+    const int at = 4 * (j & 15) + (group & 3), now = __builtin_amdgcn_readlane(g.page, at), old = __builtin_amdgcn_readlane(before.page, at);
+    return (int64_t)(j < g_from ? old : now);
+  };
+  // key of a K unit, first key of a V unit: one group of 16 a wavefront
+  auto k_key = [&](int p) { return (tid + NT * p) / (4 * J); };
+  auto v_key = [&](int p) {
+    const int half = (tid + NT * p) / (16 * J), chunk = half >> 1;
+    return 16 * (chunk >> 1) + 4 * (chunk & 1) + 8 * (half & 1);
+  };
+  auto fetch_k = [&](int j) {
+    const int key = from + TILE_KEYS * j;
+#pragma unroll
+    for (int p = 0; p < KP; ++p) {
+      const int r = k_key(p), col = (tid + NT * p) % (4 * J) * 16;
+      const int64_t page = page_of(j, uni(r >> 4)), row = (key + r) & (c.page - 1);
+      if (col < D && (KU % NT == 0 || tid < KU)) kraw[p] = *(const KTIR_G(u32x4_t)*)(c.k + page * c.k_page + row * c.k_tok + head * c.k_head + col);
     }
+  };
+  auto fetch_v = [&](int j) {
+    const int key = from + TILE_KEYS * j;
 #pragma unroll
-    for (int p = 0; p < VU; ++p) {
-      const int unit = tid + 256 * p, chunk = unit / (16 * J), col = unit % (16 * J) * 4;
-      const int first = (16 * (chunk >> 1) + 4 * (chunk & 1)) & (TILE_KEYS - 1);
-      // (a wavefront has one group, two with 64 columns)
-      const int64_t page = J == 1 ? __shfl(g.page, group + (first >> 4)) : __builtin_amdgcn_readlane(g.page, group + uni(first >> 4));
-      if (unit < 8 * 16 * J) {
-        const uint64_t at = c.v + page * c.v_page + head * c.v_head + col;
-        const int64_t row = (key + first) & (c.page - 1);
-        if (col < D) {
+    for (int p = 0; p < VP; ++p) {
+      const int first = v_key(p), col = (tid + NT * p) % (16 * J) * 4;
+      const int64_t page = page_of(j, uni(first >> 4)), row = (key + first) & (c.page - 1);
+      if (col < D && (VU % NT == 0 || tid < VU)) {
+        const uint64_t at = c.v + page * c.v_page + row * c.v_tok + head * c.v_head + col;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) raw.v[p][i] = *(const KTIR_G(uint32_t)*)(at + (row + (i & 3) + 8 * (i >> 2)) * c.v_tok);
-        }
+        for (int i = 0; i < 4; ++i) vraw[p][i] = *(const KTIR_G(uint32_t)*)(at + i * c.v_tok);
       }
     }
   };
-  auto put = [&](int key, uint16_t* kb, uint16_t* vb) {
+  auto put_k = [&](int j) {
+    uint16_t* kb = ks[j & 1];
 #pragma unroll
-    for (int p = 0; p < J; ++p) {
-      const int r = kkey + 64 / J * p, chunk = kcol / 8;
-      *(uint4*)(kb + r * DP + 8 * k_slot(r, chunk)) = row_half8<CODE>(raw.k[p].x, raw.k[p].y);
-      *(uint4*)(kb + r * DP + 8 * k_slot(r, chunk + 1)) = row_half8<CODE>(raw.k[p].z, raw.k[p].w);
+    for (int p = 0; p < KP; ++p) {
+      if (KU % NT && tid >= KU) break;
+      const int r = k_key(p), chunk = (tid + NT * p) % (4 * J) * 2;
+      *(uint4*)(kb + r * DP + 8 * k_slot(r, chunk)) = row_half8<CODE>(kraw[p].x, kraw[p].y);
+      *(uint4*)(kb + r * DP + 8 * k_slot(r, chunk + 1)) = row_half8<CODE>(kraw[p].z, kraw[p].w);
     }
+  };
+  auto put_v = [&](int j) {
+    uint16_t* vb = vs[j & 1];
 #pragma unroll
-    for (int p = 0; p < VU; ++p) {
-      const int unit = tid + 256 * p, chunk = unit / (16 * J), col = unit % (16 * J) * 4;
-      if (unit >= 8 * 16 * J) break;
-      if (CODE == KTIR_E4M3 && key + TILE_KEYS > t.hi) {            // NaN codes of tokens that no row sees
-        const int first = key + 16 * (chunk >> 1) + 4 * (chunk & 1);
+    for (int p = 0; p < VP; ++p) {
+      if (VU % NT && tid >= VU) break;
+      const int half = (tid + NT * p) / (16 * J), chunk = half >> 1, col = (tid + NT * p) % (16 * J) * 4;
+      if (CODE == KTIR_E4M3 && j == steps - 1) {                    // NaN codes of tokens that no row sees
+        const int first = from + TILE_KEYS * j + v_key(p);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) raw.v[p][i] = first + (i & 3) + 8 * (i >> 2) < t.hi ? raw.v[p][i] : 0u;
+        for (int i = 0; i < 4; ++i) vraw[p][i] = first + i < t.hi ? vraw[p][i] : 0u;
       }
-      uint32_t o[4][4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) cross_half2<CODE>(raw.v[p][2 * i], raw.v[p][2 * i + 1], o[i]);
+      uint32_t a[4], b[4];
+      cross_half2<CODE>(vraw[p][0], vraw[p][1], a);
+      cross_half2<CODE>(vraw[p][2], vraw[p][3], b);
 #pragma unroll
       for (int n = 0; n < 4; ++n)
-        *(uint4*)(vb + (col + n) * TILE_KEYS + 8 * v_slot(col + n, chunk)) = make_uint4(o[0][n], o[1][n], o[2][n], o[3][n]);
+        *(uint2*)(vb + (col + n) * TILE_KEYS + 8 * v_slot(col + n, chunk) + 4 * (half & 1)) = make_uint2(a[n], b[n]);
     }
   };
-  int g_from = from;
-  auto groups = [&](int key) {                    // of the 64 groups from `key` on
-    g_from = key;
-    const bool there = key + 16 * l < t.hi;
-    g = kv8_groups(d, head, kv8_pages(d, t, key + 16 * l, t.hi, shift), there, err);
-    kv8_scales(g, there);
+  f32x16_t s[RB][2];                              // scores of a step: K rows times Q
+  auto clear = [&]() {
+#pragma unroll
+    for (int b = 0; b < RB; ++b)
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[b][k][i] = 0.f;
   };
-
+  auto scores = [&](int j, int first, int n) {    // of columns 16 first .. 16 (first + n)
+    const uint16_t* kb = ks[j & 1];
 #pragma unroll
-  for (int p = 0; p < J; ++p) raw.k[p] = u32x4_t{0, 0, 0, 0};         // columns behind D
+    for (int x = first; x < first + n; ++x)
 #pragma unroll
-  for (int p = 0; p < VU; ++p)
+      for (int k = 0; k < 2; ++k) {
+        const uint4 a = *(const uint4*)(kb + (32 * k + r32) * DP + 8 * k_slot(32 * k + r32, 2 * x + h));
 #pragma unroll
-    for (int i = 0; i < 8; ++i) raw.v[p][i] = 0;
-  KV8Groups now = g;                              // the groups of the step that is computed
-  if (from < t.hi) {
-    groups(from);
-    now = g;
-    fetch(from);
-    put(from, ks[0], vs[0]);
-    if (from + TILE_KEYS < t.hi) fetch(from + TILE_KEYS);
-  }
-  __syncthreads();
-
-  int buf = 0;
-  for (int key = from; key < t.hi; key += TILE_KEYS, buf ^= 1) {
-    const int group = ((key - from) >> 4) & (TILE_GROUPS - 1);
-    if (key + TILE_KEYS < t.hi) {
-      put(key + TILE_KEYS, ks[buf ^ 1], vs[buf ^ 1]);
-      if (key + 2 * TILE_KEYS < t.hi) {
-        if (!(((key + 2 * TILE_KEYS - from) >> 4) & (TILE_GROUPS - 1))) {
-          now = g;
-          groups(key + 2 * TILE_KEYS);
-        }
-        fetch(key + 2 * TILE_KEYS);
+        for (int b = 0; b < RB; ++b) s[b][k] = mfma_at<false>(a, qf[b][x], s[b][k]);
       }
-    }
-    if (key < hi_most && key + TILE_KEYS > lo_least && wn > 0) {
-      const uint16_t *kb = ks[buf], *vb = vs[buf];
-      f32x16_t s[RB][2];
+  };
+  auto top_of = [&](const f32x16_t (&x)[2]) {
+    float top = x[0][0];
 #pragma unroll
-      for (int b = 0; b < RB; ++b)
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) top = __builtin_fmaxf(top, x[k][i]);
+    return top;
+  };
+  if (steps) {
+    const bool there = from + 16 * l < t.hi;
+    g = kv8_groups(d, head, kv8_pages(d, t, from + 16 * l, t.hi, shift), there, err);
+    kv8_scales(g, there);
+    fetch_k(0);
+    fetch_v(0);
+    put_k(0);
+    put_v(0);
+    fetch_k(steps > 1 ? 1 : 0);
+    put_k(1);
+    fetch_v(steps > 1 ? 1 : 0);
+    fetch_k(steps > 2 ? 2 : 0);
+    __syncthreads();
+    clear();
+    scores(0, 0, 4 * J);
+    __syncthreads();
+  }
+
+  for (int j = 0; j < steps; ++j) {
+    // the next 16 steps' groups: their pages four steps ahead of the first fetch, then the scales
+    const int f = j + 3, key = from + TILE_KEYS * j;
+    if ((f & 15) == 12 && f + 4 < steps + 3) next.page = kv8_pages(d, t, from + TILE_KEYS * (f + 4) + 16 * l, t.hi, shift);
+    if ((f & 15) == 14 && f + 2 < steps + 3) next = kv8_groups(d, head, next.page, from + TILE_KEYS * (f + 2) + 16 * l < t.hi, err);
+    if (!(f & 15) && f < steps + 3) {
+      before = g;
+      g = next;
+      g_from = f;
+      kv8_scales(g, from + TILE_KEYS * f + 16 * l < t.hi);
+    }
+    float gks[4], glv[4], giv[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int at = 4 * (j & 15) + i;
+      gks[i] = j < g_from ? lane_of(before.ks, at) : lane_of(g.ks, at);
+      glv[i] = j < g_from ? lane_of(before.lv, at) : lane_of(g.lv, at);
+      giv[i] = j < g_from ? lane_of(before.iv, at) : lane_of(g.iv, at);
+    }
+    // exponents of the weights, less b
+    const bool cut = key < lo_most || key + TILE_KEYS > hi_least;
+#pragma unroll
+    for (int b = 0; b < RB; ++b) {
+      auto hidden = [&](int k, int i) {
+        const int at = key + 32 * k + 8 * (i >> 2) + 4 * h + (i & 3);
+        return at < see_lo[b] || at >= see_hi[b];
+      };
+      if (__any(base[b] == B_NONE)) {              // rows that have seen no key: b from this step's, their sums are 0
+        float top = -__builtin_inff();
 #pragma unroll
         for (int k = 0; k < 2; ++k)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) s[b][k][i] = 0.f;
-#pragma unroll
-      for (int x = 0; x < 4 * J; ++x)
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const uint4 a = *(const uint4*)(kb + (32 * k + r32) * DP + 8 * k_slot(32 * k + r32, 2 * x + h));
-#pragma unroll
-          for (int b = 0; b < RB; ++b) s[b][k] = mfma_at<false>(a, qf[b][x], s[b][k]);
-        }
-      const bool old = key < g_from;
-      float gks[4], glv[4], giv[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        gks[i] = lane_of(old ? now.ks : g.ks, group + i);
-        glv[i] = lane_of(old ? now.lv : g.lv, group + i);
-        giv[i] = lane_of(old ? now.iv : g.iv, group + i);
+          for (int i = 0; i < 16; ++i)
+            top = __builtin_fmaxf(top, mask_ninf(__builtin_fmaf(s[b][k][i], gks[2 * k + (i >> 3)] * rs[b], glv[2 * k + (i >> 3)]), hidden(k, i)));
+        top = __builtin_fmaxf(top, other_half(top));
+        base[b] = base[b] == B_NONE && top > -__builtin_inff() ? top - TILE_TOP : base[b];
       }
-      uint4 w[RB][4];
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[b][k][i] = __builtin_fmaf(s[b][k][i], gks[2 * k + (i >> 3)] * rs[b], glv[2 * k + (i >> 3)] - base[b]);
+      if (cut) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) s[b][k][i] = mask_ninf(s[b][k][i], hidden(k, i));
+      }
+    }
+    float top[RB], most = -__builtin_inff();
+#pragma unroll
+    for (int b = 0; b < RB; ++b) {
+      top[b] = top_of(s[b]);
+      most = __builtin_fmaxf(most, top[b]);
+    }
+    if (__any(most > TILE_TOP + TILE_LAG)) {
 #pragma unroll
       for (int b = 0; b < RB; ++b) {
-        // exponents of the weights, less b
+        top[b] = __builtin_fmaxf(top[b], other_half(top[b]));
+        const float by = top[b] > TILE_TOP ? top[b] - TILE_TOP : 0.f, keep = __builtin_amdgcn_exp2f(-by);
+        base[b] += by;
+        sum[b] *= keep;
+#pragma unroll
+        for (int n = 0; n < 2 * J; ++n)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) acc[b][n][i] *= keep;
 #pragma unroll
         for (int k = 0; k < 2; ++k)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int gi = 2 * k + (i >> 3);
-            s[b][k][i] = __builtin_fmaf(s[b][k][i], gks[gi] * rs[b], glv[gi]);
-          }
-        const bool cut = key < lo_most || key + TILE_KEYS > hi_least;
-        if (cut) {
-#pragma unroll
-          for (int k = 0; k < 2; ++k)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const int j = key + 32 * k + 8 * (i >> 2) + 4 * h + (i & 3);
-              s[b][k][i] = mask_ninf(s[b][k][i], j < see_lo[b] || j >= see_hi[b]);
-            }
-        }
-        float top = s[b][0][0];
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) top = __builtin_fmaxf(top, s[b][k][i]);
-        if (__any(top > base[b] + (TILE_TOP + TILE_LAG))) {
-          top = __builtin_fmaxf(top, other_half(top));
-          const float to = __builtin_fmaxf(base[b], top - TILE_TOP), keep = __builtin_amdgcn_exp2f(base[b] - to);
-          base[b] = to;
-          sum[b] *= keep;
-#pragma unroll
-          for (int n = 0; n < 2 * J; ++n)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) acc[b][n][i] *= keep;
-        }
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float e = __builtin_amdgcn_exp2f(s[b][k][i] - base[b]);
-            sum[b] = __builtin_fmaf(e, giv[2 * k + (i >> 3)], sum[b]);
-            s[b][k][i] = e;
-          }
-#pragma unroll
-        for (int p = 0; p < 4; ++p) {
-          const f32x16_t& x = s[b][p >> 1];
-          const int i = 8 * (p & 1);
-          w[b][p] = make_uint4(cvt2<false>(x[i], x[i + 1]), cvt2<false>(x[i + 2], x[i + 3]), cvt2<false>(x[i + 4], x[i + 5]),
-                               cvt2<false>(x[i + 6], x[i + 7]));
-        }
+          for (int i = 0; i < 16; ++i) s[b][k][i] -= by;
       }
+    }
+    // the codes of steps j + 2 (K) and j + 1 (V) into LDS, those of j + 3 and j + 2 on their way, the scores of j + 1:
+    // beside W V of step j.  (Past the last step: what was fetched last, again.)
+    f32x16_t u[RB][2];
 #pragma unroll
-      for (int p = 0; p < 4; ++p)
+    for (int b = 0; b < RB; ++b)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) u[b][k] = s[b][k];
+    clear();
+    const uint16_t* vb = vs[j & 1];
+    uint4 w[RB], old[RB];
+#pragma unroll
+    for (int p = 0; p < 5; ++p) {
+      __builtin_amdgcn_sched_barrier(0);
+      if (p == 0) put_k(j + 2);
+      if (p == 1) put_v(j + 1);
+      if (p == 2) fetch_k(j + 3 < steps ? j + 3 : steps - 1);
+      if (p == 3) fetch_v(j + 2 < steps ? j + 2 : steps - 1);
+      if (p < 4) scores(j + 1, p * J, J);
+      if (p < 4) {
+#pragma unroll
+        for (int b = 0; b < RB; ++b) {
+          float e[8];
+          old[b] = w[b];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            e[i] = __builtin_amdgcn_exp2f(u[b][p >> 1][8 * (p & 1) + i]);
+            sum[b] = __builtin_fmaf(e[i], giv[p], sum[b]);
+          }
+          w[b] = make_uint4(cvt2<false>(e[0], e[1]), cvt2<false>(e[2], e[3]), cvt2<false>(e[4], e[5]), cvt2<false>(e[6], e[7]));
+        }
+      } else {
+#pragma unroll
+        for (int b = 0; b < RB; ++b) old[b] = w[b];
+      }
+      if (p > 0) {
 #pragma unroll
         for (int n = 0; n < 2 * J; ++n) {
-          const uint4 a = *(const uint4*)(vb + (32 * n + r32) * TILE_KEYS + 8 * v_slot(32 * n + r32, 2 * p + h));
+          const uint4 a = *(const uint4*)(vb + (32 * n + r32) * TILE_KEYS + 8 * v_slot(32 * n + r32, 2 * (p - 1) + h));
 #pragma unroll
-          for (int b = 0; b < RB; ++b) acc[b][n] = mfma_at<false>(a, w[b][p], acc[b][n]);
+          for (int b = 0; b < RB; ++b) acc[b][n] = mfma_at<false>(a, old[b], acc[b][n]);
         }
+      }
     }
     __syncthreads();
   }
@@ -323,9 +375,9 @@ template <int CODE>
 static void tile_go(const ktir_kv8_attn_t& d, int64_t slots, hipStream_t st) {
   const dim3 grid((unsigned)(slots * d.cache.heads));
   const int D = (int)d.cache.columns;
-  if (D <= 64) hipLaunchKernelGGL((kv8_attn_tile<CODE, 1, 2>), grid, dim3(256), 0, st, d, (uint32_t)slots, device_error_flag());
-  else if (D <= 128) hipLaunchKernelGGL((kv8_attn_tile<CODE, 2, 2>), grid, dim3(256), 0, st, d, (uint32_t)slots, device_error_flag());
-  else hipLaunchKernelGGL((kv8_attn_tile<CODE, 4, 1>), grid, dim3(256), 0, st, d, (uint32_t)slots, device_error_flag());
+  if (D <= 64) hipLaunchKernelGGL((kv8_attn_tile<CODE, 1, 1, 8>), grid, dim3(512), 0, st, d, (uint32_t)slots, device_error_flag());
+  else if (D <= 128) hipLaunchKernelGGL((kv8_attn_tile<CODE, 2, 1, 8>), grid, dim3(512), 0, st, d, (uint32_t)slots, device_error_flag());
+  else hipLaunchKernelGGL((kv8_attn_tile<CODE, 4, 1, 4>), grid, dim3(256), 0, st, d, (uint32_t)slots, device_error_flag());
 }
 
 // whether a launch takes this kernel, and its tiles of rows for each KV head
