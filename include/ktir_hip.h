@@ -550,11 +550,11 @@ typedef struct ktir_kv8_batch {
 /* ---- append: the batch's new keys and values into the cache ----
  * For every page that new tokens fall in, and every head, with the new values x
  * of that page and head (K and V alike; top = 127 or 448):
- *   scale' = max(max |x| / top, 2^-100), and the page's scale before, if older tokens
- *            of the sequence lie in the page, where that is more
- *   code   = rint(x / scale') or the nearest e4m3 value, within +- top (x times 1 / scale')
+ *   scale' = max(max |x| * (1 / top), 2^-100), and the page's scale before, if older
+ *            tokens of the sequence lie in the page, where that is more
+ *   code   = rint(x * (1 / scale')) or the nearest e4m3 value, within +- top
  * and where scale' is more than the scale before, the older tokens' codes are
- * rounded again: code times (scale before / scale').  A page that receives a
+ * rounded again: code * (scale before * (1 / scale')).  Every operation is one in f32.  A page that receives a
  * value that is not finite reads as NaN from then on (scale' = NaN, new codes 0).
  * Tokens at negative positions are not stored.  A page that two sequences of a
  * call both write keeps the codes and the scale of either.

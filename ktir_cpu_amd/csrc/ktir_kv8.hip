@@ -93,7 +93,7 @@ int check_batch(const char* what, const ktir_kv8_batch_t& b, const ktir_kv8_t& c
 typedef uint32_t u4_t __attribute__((ext_vector_type(4)));
 
 template <int CODE>
-constexpr float TOP = CODE == KTIR_I8 ? 127.f : 448.f;
+constexpr float PER_TOP = 1.f / (CODE == KTIR_I8 ? 127.f : 448.f);
 
 // four values over their scale as codes
 template <int CODE>
@@ -241,7 +241,7 @@ __global__ __launch_bounds__(256) void kv8_append(const ktir_kv8_append_t d, int
     for (int i = 0; i < W; ++i) top = top > tops[i] ? top : tops[i];
   }
   const float most = BF16 ? __uint_as_float(top << 16) : (float)__builtin_bit_cast(_Float16, (uint16_t)top);
-  float now = __builtin_fmaxf(most / TOP<CODE>, LEAST_SCALE);
+  float now = __builtin_fmaxf(most * PER_TOP<CODE>, LEAST_SCALE);
   if (!(now >= before)) now = before;                     // a page that was NaN stays so
   if (!(most < __builtin_inff())) now = __builtin_nanf("");
   const bool nan = !(now < __builtin_inff());

@@ -21,8 +21,10 @@ namespace ktir {
 constexpr int TILE_KEYS = 64;
 constexpr float TILE_TOP = 11.f, TILE_LAG = 4.f;       // exponent of the largest weight when b changes, and by how much it may grow
 
-// chunk slots in LDS: 16 bytes, 8 of a K row's (of 8 J), 8 of a V column's 64 keys
-__device__ __forceinline__ int k_slot(int key, int chunk) { return chunk ^ (key & 7); }
+// Slots of 16-byte chunks in LDS rows: a K row has 8 J (8 columns each), a V column 8 (the
+// keys of one lane's operand each).  Eight lanes that read or write together (one chunk
+// of 8 keys, 8 pieces of 16 columns of a key, one chunk of 8 columns) hit distinct banks.
+__device__ __forceinline__ int k_slot(int key, int chunk) { return chunk ^ (key & 7) ^ (chunk >> 3 & 1); }
 __device__ __forceinline__ int v_slot(int col, int chunk) { return chunk ^ (((col >> 2) ^ col) & 7); }
 
 template <int CODE, int J, int RB, int W>
@@ -107,38 +109,35 @@ __global__ __launch_bounds__(64 * W, W / 4) void kv8_attn_tile(const ktir_kv8_at
   int g_from = 0;                                               // the first of g's steps
   u32x4_t kraw[KP];
   uint32_t vraw[VP][4];
-#pragma unroll
-  for (int p = 0; p < KP; ++p) kraw[p] = u32x4_t{0, 0, 0, 0};         // columns behind D
-#pragma unroll
-  for (int p = 0; p < VP; ++p)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) vraw[p][i] = 0;
   auto page_of = [&](int j, int group) {         // of step j, in the groups of the step or of the 16 before
     const int at = 4 * (j & 15) + (group & 3), now = __builtin_amdgcn_readlane(g.page, at), old = __builtin_amdgcn_readlane(before.page, at);
     return (int64_t)(j < g_from ? old : now);
   };
   // key of a K unit, first key of a V unit: one group of 16 a wavefront
   auto k_key = [&](int p) { return (tid + NT * p) / (4 * J); };
-  auto v_key = [&](int p) {
-    const int half = (tid + NT * p) / (16 * J), chunk = half >> 1;
-    return 16 * (chunk >> 1) + 4 * (chunk & 1) + 8 * (half & 1);
-  };
+  // (a V unit is half a chunk of 4 columns: 8 column fours, both halves, the other fours, the chunks)
+  auto v_chunk = [&](int p) { return (tid + NT * p) / (32 * J); };
+  const int v_half = tid >> 3 & 1;
+  auto v_col = [&](int p) { return ((tid & 7) + 8 * ((tid + NT * p) / 16 % (2 * J))) * 4; };
+  auto v_key = [&](int p) { return 16 * (v_chunk(p) >> 1) + 4 * (v_chunk(p) & 1) + 8 * v_half; };
   auto fetch_k = [&](int j) {
     const int key = from + TILE_KEYS * j;
 #pragma unroll
     for (int p = 0; p < KP; ++p) {
-      const int r = k_key(p), col = (tid + NT * p) % (4 * J) * 16;
+      // (columns behind D: the first ones again, times zeros in Q)
+      const int r = k_key(p), at = (tid + NT * p) % (4 * J) * 16, col = at < D ? at : 0;
       const int64_t page = page_of(j, uni(r >> 4)), row = (key + r) & (c.page - 1);
-      if (col < D && (KU % NT == 0 || tid < KU)) kraw[p] = *(const KTIR_G(u32x4_t)*)(c.k + page * c.k_page + row * c.k_tok + head * c.k_head + col);
+      if (KU % NT == 0 || tid < KU) kraw[p] = *(const KTIR_G(u32x4_t)*)(c.k + page * c.k_page + row * c.k_tok + head * c.k_head + col);
     }
   };
   auto fetch_v = [&](int j) {
     const int key = from + TILE_KEYS * j;
 #pragma unroll
     for (int p = 0; p < VP; ++p) {
-      const int first = v_key(p), col = (tid + NT * p) % (16 * J) * 4;
+      // (columns behind D: the first ones again, not stored)
+      const int first = v_key(p), x = v_col(p), col = x < D ? x : 0;
       const int64_t page = page_of(j, uni(first >> 4)), row = (key + first) & (c.page - 1);
-      if (col < D && (VU % NT == 0 || tid < VU)) {
+      if (VU % NT == 0 || tid < VU) {
         const uint64_t at = c.v + page * c.v_page + row * c.v_tok + head * c.v_head + col;
 #pragma unroll
         for (int i = 0; i < 4; ++i) vraw[p][i] = *(const KTIR_G(uint32_t)*)(at + i * c.v_tok);
@@ -160,8 +159,8 @@ __global__ __launch_bounds__(64 * W, W / 4) void kv8_attn_tile(const ktir_kv8_at
 #pragma unroll
     for (int p = 0; p < VP; ++p) {
       if (VU % NT && tid >= VU) break;
-      const int half = (tid + NT * p) / (16 * J), chunk = half >> 1, col = (tid + NT * p) % (16 * J) * 4;
-      if (CODE == KTIR_E4M3 && j == steps - 1) {                    // NaN codes of tokens that no row sees
+      const int chunk = v_chunk(p), col = v_col(p);
+      if (CODE == KTIR_E4M3) {                    // NaN codes of tokens that no row sees
         const int first = from + TILE_KEYS * j + v_key(p);
 #pragma unroll
         for (int i = 0; i < 4; ++i) vraw[p][i] = first + i < t.hi ? vraw[p][i] : 0u;
@@ -171,7 +170,7 @@ __global__ __launch_bounds__(64 * W, W / 4) void kv8_attn_tile(const ktir_kv8_at
       cross_half2<CODE>(vraw[p][2], vraw[p][3], b);
 #pragma unroll
       for (int n = 0; n < 4; ++n)
-        *(uint2*)(vb + (col + n) * TILE_KEYS + 8 * v_slot(col + n, chunk) + 4 * (half & 1)) = make_uint2(a[n], b[n]);
+        *(uint2*)(vb + (col + n) * TILE_KEYS + 8 * v_slot(col + n, chunk) + 4 * v_half) = make_uint2(a[n], b[n]);
     }
   };
   f32x16_t s[RB][2];                              // scores of a step: K rows times Q
@@ -303,7 +302,7 @@ __global__ __launch_bounds__(64 * W, W / 4) void kv8_attn_tile(const ktir_kv8_at
     uint4 w[RB], old[RB];
 #pragma unroll
     for (int p = 0; p < 5; ++p) {
-      __builtin_amdgcn_sched_barrier(0);
+      if (p == 0 || p == 2 || p == 4) __builtin_amdgcn_sched_barrier(0);
       if (p == 0) put_k(j + 2);
       if (p == 1) put_v(j + 1);
       if (p == 2) fetch_k(j + 3 < steps ? j + 3 : steps - 1);
@@ -380,12 +379,15 @@ static void tile_go(const ktir_kv8_attn_t& d, int64_t slots, hipStream_t st) {
   else hipLaunchKernelGGL((kv8_attn_tile<CODE, 4, 1, 4>), grid, dim3(256), 0, st, d, (uint32_t)slots, device_error_flag());
 }
 
-// whether a launch takes this kernel, and its tiles of rows for each KV head
+// Whether a launch takes this kernel, and its tiles of rows for each KV head.  With fewer
+// than 128 workgroups the kernel of few rows, which spreads the keys as well, is faster:
+// 512 tokens after 3584 (72 tiles) 89 us there and 149 here, 1024 after 3072 (136) 154
+// and 152, 2048 alone (264) 124 and 87, 16 sequences of 64 after 1984 (128) 105 and 88.
 bool kv8_tile_takes(const ktir_kv8_attn_t& d, int64_t* slots) {
   const int64_t grp = d.q_heads / d.cache.heads, TM = d.cache.columns <= 128 ? 256 : 128;
   if (d.max_q * grp <= TM / 2) return false;
   *slots = d.max_q * grp > TM ? d.batch.tokens * grp / TM + d.batch.seqs : d.batch.seqs;
-  return *slots * d.cache.heads >= 160;
+  return *slots * d.cache.heads >= 128;
 }
 
 int kv8_tile_launch(const ktir_kv8_attn_t& d, int64_t slots) {

@@ -2,7 +2,6 @@
 operators, and how far an f32 kernel with 16-bit operands may be from them."""
 import math
 
-import numpy as np
 import torch
 
 TOP = {"i8": 127.0, "e4m3": 448.0}
@@ -59,7 +58,7 @@ def append(x, codes, scale, code, page, table, q_start, kv_len):
             for h in range(x.shape[1]):
                 v = new[:, h]
                 before = scale[at, h].clone() if r0 else torch.tensor(0.0)
-                now = torch.maximum(v.abs().max() / np.float32(TOP[code]), torch.tensor(2.0 ** -100))
+                now = torch.maximum(v.abs().max() * torch.tensor(1.0 / TOP[code]), torch.tensor(2.0 ** -100))
                 now = now if now >= before else before
                 if not torch.isfinite(v).all():
                     now = torch.tensor(math.nan)
