@@ -112,21 +112,21 @@ struct Tile {
   int lo, hi;            // tokens that some row of the tile sees
 };
 
-// tokens [lo, hi) that row r of tile t sees
-__device__ __forceinline__ void seen(const ktir_kv8_attn_t& d, const Tile& t, int r, int grp, int* lo, int* hi) {
-  const int64_t pos = (int64_t)t.q.n_kv - t.q.n_new + r / grp;
+// tokens [lo, hi) that new token i of tile t's sequence sees
+__device__ __forceinline__ void token_sees(const ktir_kv8_attn_t& d, const Tile& t, int i, int* lo, int* hi) {
+  const int64_t pos = (int64_t)t.q.n_kv - t.q.n_new + i;
   *hi = d.causal && pos + 1 < t.keys ? (pos < 0 ? 0 : (int)(pos + 1)) : t.keys;
   *lo = d.window && pos - d.window + 1 > 0 ? (int)(pos - d.window + 1) : 0;
 }
+__device__ __forceinline__ void seen(const ktir_kv8_attn_t& d, const Tile& t, int r, int grp, int* lo, int* hi) {
+  token_sees(d, t, (int)((uint32_t)r / (uint32_t)grp), lo, hi);
+}
 
-// tile `slot` of a launch with tiles of TM (a power of two) rows: a sequence each where that holds
-// max_q tokens, otherwise found by the batch's offsets
-__device__ __forceinline__ Tile tile_of(const ktir_kv8_attn_t& d, int64_t slot, int TM, int grp, int* err) {
+// tile `nth` (of TM rows) of sequence s
+__device__ __forceinline__ Tile tile_at(const ktir_kv8_attn_t& d, int64_t s, int64_t nth, int TM, int grp, int* err) {
   Tile t = {};
-  int64_t nth = 0;
-  t.s = d.max_q * grp > TM ? seq_of_slot(d.batch, grp, __builtin_ctz(TM), 1, slot, &nth) : slot;
-  if (nth < 0) return t;
-  t.q = seq_of(d.batch, d.cache.page, t.s, err);
+  t.s = s;
+  t.q = seq_of(d.batch, d.cache.page, s, err);
   t.keys = t.q.n_held;
   if (t.keys > d.max_k || t.q.n_new > d.max_q) *err = OUT_OF_RANGE;
   if (t.keys > d.max_k) t.keys = (int)d.max_k;
@@ -135,8 +135,55 @@ __device__ __forceinline__ Tile tile_of(const ktir_kv8_attn_t& d, int64_t slot, 
   t.row0 = (int)(nth * TM);
   t.rows = left < TM ? (int)left : TM;
   int x;
-  seen(d, t, t.row0, grp, &t.lo, &x);
-  seen(d, t, t.row0 + t.rows - 1, grp, &x, &t.hi);
+  if (nth == 0 && left <= TM) {              // the whole sequence: its first and last token
+    token_sees(d, t, 0, &t.lo, &x);
+    token_sees(d, t, (t.q.n_new < d.max_q ? t.q.n_new : (int)d.max_q) - 1, &x, &t.hi);
+  } else {
+    seen(d, t, t.row0, grp, &t.lo, &x);
+    seen(d, t, t.row0 + t.rows - 1, grp, &x, &t.hi);
+  }
+  return t;
+}
+
+// whether a launch has one tile a sequence: its max_q tokens fit in TM (a power of two) rows
+__host__ __device__ inline bool one_tile(const ktir_kv8_attn_t& d, int TM, int grp) { return d.max_q * grp <= TM; }
+
+// tile `slot` of a launch: a sequence each, or found by the batch's offsets
+__device__ __forceinline__ Tile tile_of(const ktir_kv8_attn_t& d, int64_t slot, int TM, int grp, int* err) {
+  if (one_tile(d, TM, grp)) return tile_at(d, slot, 0, TM, grp, err);
+  int64_t nth;
+  const int64_t s = seq_of_slot(d.batch, grp, __builtin_ctz(TM), 1, slot, &nth);
+  return nth < 0 ? Tile{} : tile_at(d, s, nth, TM, grp, err);
+}
+
+// a tile's fields in scalar registers: they are the same in every lane, or lane i's
+__device__ __forceinline__ Tile uni(Tile t) {
+  t.s = uni(t.s);
+  t.q.start = uni(t.q.start);
+  t.q.n_new = uni(t.q.n_new);
+  t.q.n_kv = uni(t.q.n_kv);
+  t.row0 = uni(t.row0);
+  t.rows = uni(t.rows);
+  t.keys = uni(t.keys);
+  t.lo = uni(t.lo);
+  t.hi = uni(t.hi);
+  return t;
+}
+__device__ __forceinline__ int64_t lane_of(int64_t x, int i) {
+  const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)x, i), hi = __builtin_amdgcn_readlane((uint32_t)((uint64_t)x >> 32), i);
+  return (int64_t)((uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ int lane_of(int x, int i) { return __builtin_amdgcn_readlane(x, i); }
+__device__ __forceinline__ Tile lane_of(Tile t, int i) {
+  t.s = lane_of(t.s, i);
+  t.q.start = lane_of(t.q.start, i);
+  t.q.n_new = lane_of(t.q.n_new, i);
+  t.q.n_kv = lane_of(t.q.n_kv, i);
+  t.row0 = lane_of(t.row0, i);
+  t.rows = lane_of(t.rows, i);
+  t.keys = lane_of(t.keys, i);
+  t.lo = lane_of(t.lo, i);
+  t.hi = lane_of(t.hi, i);
   return t;
 }
 
@@ -206,20 +253,6 @@ __device__ __forceinline__ void q_scaled(uint32_t (&raw)[N], float up) {
     const f32x2_t v = uncvt2<true>(raw[i]);
     raw[i] = cvt2<false>(v.x * up, v.y * up);
   }
-}
-
-// a tile's fields in scalar registers: they are the same in every lane
-__device__ __forceinline__ Tile uni(Tile t) {
-  t.s = uni(t.s);
-  t.q.start = uni(t.q.start);
-  t.q.n_new = uni(t.q.n_new);
-  t.q.n_kv = uni(t.q.n_kv);
-  t.row0 = uni(t.row0);
-  t.rows = uni(t.rows);
-  t.keys = uni(t.keys);
-  t.lo = uni(t.lo);
-  t.hi = uni(t.hi);
-  return t;
 }
 
 }  // namespace ktir

@@ -25,9 +25,15 @@ namespace ktir {
 constexpr int ROWS_WAVES = 4, ROWS_STEP = 32, ROWS_GROUPS = 64;
 constexpr int MOST_SPLITS = 256;      // of a tile's keys
 
-// what a split of a tile leaves in the workspace: TM rows of 64 J sums, then b and l of each row
-template <int J, int MT>
-constexpr int64_t PART = 16 * MT * (64 * J + 2);
+// what a split of a tile of `rows` rows leaves in the workspace: 64 J sums each, then b and l of each row
+template <int J>
+__host__ __device__ constexpr int64_t part_size(int rows) { return (int64_t)rows * (64 * J + 4); }
+
+// the parts of a tile's keys, of `part` each
+__device__ __forceinline__ int tile_parts(const Tile& t, int part) {
+  const int from = t.lo & ~(ROWS_STEP - 1);
+  return t.hi > from ? (int)((uint32_t)(t.hi - from + part - 1) / (uint32_t)part) : 1;
+}
 
 template <int J>
 struct KV8Keys {
@@ -79,39 +85,78 @@ __device__ __forceinline__ void kv8_values(const ktir_kv8_t& c, const KV8Groups&
 }
 
 template <int CODE, int J, int MT>
-__global__ __launch_bounds__(64 * ROWS_WAVES, MT == 1 ? 2 : 1) void kv8_attn_rows(const ktir_kv8_attn_t d, int splits, int part, uint32_t slots, int hw, int* err) {
+__global__ __launch_bounds__(64 * ROWS_WAVES, MT == 1 ? 2 : 1) void kv8_attn_rows(const ktir_kv8_attn_t d, int splits, int part, int part_rows, uint32_t slots, int hw, int* err) {
   constexpr int W = ROWS_WAVES, TM = 16 * MT, N = 4 * J, PITCH = 64 * J + 4;
   __shared__ __attribute__((aligned(16))) float o_sum[W][TM * PITCH];
   __shared__ float w_b[W][TM], w_l[W][TM];
   const ktir_kv8_t& c = d.cache;
   const int l = threadIdx.x & 63, wave = uni((int)(threadIdx.x >> 6)), g4 = l >> 4, c16 = l & 15;
   const int grp = (int)((uint32_t)d.q_heads / (uint32_t)c.heads), D = (int)c.columns, shift = __builtin_ctz((uint32_t)c.page);
-  // Workgroups go to the 8 XCDs in turn.  The heads of a tile's split follow one
-  // another on one XCD, so the rows of a page are read together; tiles and splits
-  // take the XCDs in turn, a split its tiles from another one on, as the last splits
-  // of many tiles are empty.
+  // Workgroups go to the 8 XCDs in turn.  The heads of a part follow one another on one
+  // XCD, so the rows of a page are read together; the parts that there are take the
+  // XCDs in turn.
   const uint32_t heads = (uint32_t)c.heads, sets = heads / hw, octet = blockIdx.x / 8, eighth = octet / sets, u = eighth * 8 + blockIdx.x % 8;
-  const uint32_t split = u / slots, turned = u - split * slots + split % slots, slot = turned < slots ? turned : turned - slots;
-  if (split >= (uint32_t)splits) return;
   const int turn = wave / hw, TW = W / hw;                   // of the head's TW wavefronts
-  const int64_t head = (octet - eighth * sets) * hw + wave % hw, item = (int64_t)slot * heads + head;
-  const Tile t = uni(tile_of(d, slot, TM, grp, err));
-  if (!t.rows) return;
-
-  // this workgroup's keys, and this wavefront's
-  const int from = t.lo & ~(ROWS_STEP - 1), span = t.hi > from ? t.hi - from : 0, active = span ? (span + part - 1) / part : 1;
-  if ((int)split >= active) return;
+  const int64_t head = (octet - eighth * sets) * hw + wave % hw;
+  Tile t;
+  int split, active, from;
+  uint32_t slot;
+  if (d.batch.seqs == 1 && one_tile(d, TM, grp)) {
+    slot = 0;
+    split = (int)u;
+    t = uni(tile_at(d, 0, 0, TM, grp, err));
+    if (!t.rows) return;
+    active = tile_parts(t, part);
+    if (split >= active) return;
+  } else if (one_tile(d, TM, grp)) {
+    // one tile a sequence, of as many parts as its keys fill: the u-th part of all, 64 sequences a look
+    t.rows = 0;
+    uint32_t before = 0;
+    for (int64_t base = 0; base < d.batch.seqs; base += 64) {
+      Tile x = {};
+      if (base + l < d.batch.seqs) x = tile_at(d, base + l, 0, TM, grp, err);
+      int n = x.rows ? tile_parts(x, part) : 0;
+      n = n < splits ? n : splits;
+      int upto = n;                                          // parts of the sequences up to this lane's
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const int y = __shfl_up(upto, o);
+        upto += l >= o ? y : 0;
+      }
+      const uint32_t all = (uint32_t)lane_of(upto, 63);
+      if (u < before + all) {
+        const int i = __builtin_ctzll(__ballot(u < before + (uint32_t)upto));
+        t = lane_of(x, i);
+        active = lane_of(n, i);
+        split = (int)(u - before) - (lane_of(upto, i) - active);
+        slot = (uint32_t)base + i;
+        break;
+      }
+      before += all;
+    }
+    if (!t.rows) return;
+  } else {
+    split = (int)(u / slots);
+    slot = u - split * slots;
+    if (split >= splits) return;
+    t = uni(tile_of(d, slot, TM, grp, err));
+    if (!t.rows) return;
+    active = tile_parts(t, part);
+    if (split >= active) return;
+  }
+  from = t.lo & ~(ROWS_STEP - 1);
+  const int64_t item = (int64_t)slot * heads + head;
   // (steps of 32 keys go to the splits' wavefronts in turn, so what all read at one time lies close together)
-  const int stride = ROWS_STEP * TW * active, lo = from + ((int)split * TW + turn) * ROWS_STEP, mine = (l >> 1) * stride + 16 * (l & 1);
+  const int stride = ROWS_STEP * TW * active, lo = from + (split * TW + turn) * ROWS_STEP, mine = (l >> 1) * stride + 16 * (l & 1);
   const int page0 = kv8_pages(d, t, lo + mine, t.hi, shift);
 
-  // Q: this lane's row of each 16, pieces g4, g4 + 4, .. of 16 columns; times 2^k, so that the row's largest value has exponent 14
+  // Q: this lane's row of each 16, pieces g4 J .. g4 J + J of 16 columns (so a load of K touches whole 128-byte lines); times 2^k, so that the row's largest value has exponent 14
   uint4 qf[MT][J][2];
   float rs[MT];
   int see_lo[MT], see_hi[MT], kpiece[J];
   uint32_t raw[MT][J][8];
 #pragma unroll
-  for (int j = 0; j < J; ++j) kpiece[j] = (4 * j + g4) * 16 < D ? (4 * j + g4) * 16 : 0;
+  for (int j = 0; j < J; ++j) kpiece[j] = (g4 * J + j) * 16 < D ? (g4 * J + j) * 16 : 0;
   const bool whole = !((d.q.ptr | (uint64_t)d.q.tok * 2 | (uint64_t)d.q.head * 2) & 15);
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
@@ -121,7 +166,7 @@ __global__ __launch_bounds__(64 * ROWS_WAVES, MT == 1 ? 2 : 1) void kv8_attn_row
     const int64_t e = (t.q.start + r / grp) * d.q.tok + (head * grp + r % grp) * d.q.head;
 #pragma unroll
     for (int j = 0; j < J; ++j) {
-      const int x = (4 * j + g4) * 16;
+      const int x = (g4 * J + j) * 16;
 #pragma unroll
       for (int i = 0; i < 8; ++i) raw[m][j][i] = 0;
       if (x < D) q16(d, e + x, whole, raw[m][j]);
@@ -302,7 +347,7 @@ __global__ __launch_bounds__(64 * ROWS_WAVES, MT == 1 ? 2 : 1) void kv8_attn_row
   __syncthreads();
 
   // alone: the result; otherwise its part for kv8_attn_join
-  KTIR_G(float)* ws = (KTIR_G(float)*)d.ws + (item * splits + split) * PART<J, MT>;
+  KTIR_G(float)* ws = (KTIR_G(float)*)d.ws + (item * splits + split) * part_size<J>(part_rows);
   for (int at = turn * 64 + l; at < t.rows * 16 * J; at += 64 * TW) {
     const int row = at / (16 * J), x4 = at % (16 * J) * 4;
     f32x4_t o = {0.f, 0.f, 0.f, 0.f};
@@ -315,8 +360,8 @@ __global__ __launch_bounds__(64 * ROWS_WAVES, MT == 1 ? 2 : 1) void kv8_attn_row
     if (active > 1) {
       *(KTIR_G(f32x4_t)*)(ws + row * 64 * J + x4) = o;
       if (x4 == 0) {
-        ws[TM * 64 * J + row] = top;
-        ws[TM * 64 * J + TM + row] = lt;
+        ws[part_rows * 64 * J + row] = top;
+        ws[part_rows * (64 * J + 1) + row] = lt;
       }
       continue;
     }
@@ -341,7 +386,7 @@ __global__ __launch_bounds__(64 * ROWS_WAVES, MT == 1 ? 2 : 1) void kv8_attn_row
 constexpr int JOIN_EACH = 16;
 
 template <int J, int MT, int R, int B>
-__global__ __launch_bounds__(64 * R * B) void kv8_attn_join(const ktir_kv8_attn_t d, int splits, int part, int* err) {
+__global__ __launch_bounds__(64 * R * B) void kv8_attn_join(const ktir_kv8_attn_t d, int splits, int part, int part_rows, int* err) {
   constexpr int TM = 16 * MT, LOOK = B == 1 ? 1 : MOST_SPLITS / 64;
   static_assert(B * JOIN_EACH <= 64 * LOOK, "a lane looks at the b and l of each split");
   __shared__ float f[R][64 * LOOK], sums[B == 1 ? 1 : R * B][64 * J];
@@ -350,24 +395,25 @@ __global__ __launch_bounds__(64 * R * B) void kv8_attn_join(const ktir_kv8_attn_
   const uint32_t heads = (uint32_t)c.heads, slot = blockIdx.x / heads;
   const int64_t item = blockIdx.x, head = blockIdx.x - slot * heads;
   const int sub = wave / B, turn = wave % B, row = (int)blockIdx.y * R + sub;
-  const KTIR_G(float)* ws = (const KTIR_G(float)*)d.ws + item * splits * PART<J, MT>;
+  const int64_t size = part_size<J>(part_rows);
+  const KTIR_G(float)* ws = (const KTIR_G(float)*)d.ws + item * splits * size;
   float x[JOIN_EACH][J], b[LOOK], w[LOOK];
 #pragma unroll
   for (int i = 0; i < LOOK; ++i) {
     b[i] = B_NONE, w[i] = 0.f;
-    if (row < TM && l + 64 * i < splits) {
-      b[i] = ws[(l + 64 * i) * PART<J, MT> + TM * 64 * J + row];
-      w[i] = ws[(l + 64 * i) * PART<J, MT> + TM * 64 * J + TM + row];
+    if (row < part_rows && l + 64 * i < splits) {
+      b[i] = ws[(l + 64 * i) * size + part_rows * 64 * J + row];
+      w[i] = ws[(l + 64 * i) * size + part_rows * (64 * J + 1) + row];
     }
   }
 #pragma unroll
   for (int k = 0; k < JOIN_EACH; ++k)
-    if (row < TM && turn + B * k < splits) {
+    if (row < part_rows && turn + B * k < splits) {
 #pragma unroll
-      for (int j = 0; j < J; ++j) x[k][j] = ws[(turn + B * k) * PART<J, MT> + row * 64 * J + 64 * j + l];
+      for (int j = 0; j < J; ++j) x[k][j] = ws[(turn + B * k) * size + row * 64 * J + 64 * j + l];
     }
   const Tile t = uni(tile_of(d, slot, TM, grp, err));
-  const int from = t.lo & ~(ROWS_STEP - 1), span = t.hi > from ? t.hi - from : 0, active = span ? (span + part - 1) / part : 1;
+  const int parts = tile_parts(t, part), active = parts < splits ? parts : splits;
   const bool on = row < t.rows && active > 1;
   float top = B_NONE, lt = 0.f;
 #pragma unroll
@@ -425,27 +471,32 @@ void kv8_rows_shape(const ktir_kv8_attn_t& d, KV8Shape* s) {
   s->MT = d.max_q * grp > 16 ? 2 : 1;
   const int64_t TM = 16 * s->MT;
   s->slots = d.max_q * grp > TM ? d.batch.tokens * grp / TM + d.batch.seqs : d.batch.seqs;
-  s->part = TM * (64 * s->J + 2);
+  s->rows = (int)(d.max_q * grp < TM ? d.max_q * grp : TM);
+  s->part = s->rows * (64 * s->J + 4);
   // the most tokens that a tile's rows see, from a step's bound on
   s->span = d.max_k;
   const int64_t near = d.window + (TM - 1) / grp + 1;
   if (d.window && near < s->span) s->span = near;
   s->span += ROWS_STEP - 1;
-  // Splits and heads of a workgroup.  Up to 2^19 keys (times KV heads) a wavefront's
-  // four work on one head: one workgroup a CU is best for one sequence (65536
-  // tokens of 8 heads: 36.8 us, two a CU 42.5), four where lengths may differ (8
-  // sequences of up to 8192: 21.8, 28.6 with one), none under 128 keys.  More come from
-  // HBM, which gives 4.8 TB/s to 128-byte rows of one head each, 5.6 where four heads'
-  // rows are read together (copy patterns of 268 MB; 64 sequences of 2460 tokens: 76.8
-  // and 69.6 us).
+  // Heads of a workgroup, parts of the keys.  Up to 2^19 keys (times KV heads) a wavefront's
+  // four work on one head, on parts of 128 keys or more: one workgroup a CU is best for one
+  // sequence (65536 tokens of 8 heads: 36.8 us, two a CU 42.5), four for several (8 of up
+  // to 8192: 20.5, 28.6 with one).  More come from HBM, which gives 4.8 TB/s to 128-byte
+  // rows of one head each, 5.6 where four heads' rows are read together (read patterns of
+  // 268 MB; 64 sequences of 2460 tokens: 77 and 68.6 us).  There one workgroup a CU is
+  // best for one sequence (131072 tokens: 59.5 us, two 62.6); several, whose lengths the
+  // host does not know, get four if all were the longest, with parts of 512 keys or more
+  // (64 of 64 to 8192 tokens: parts of 1056 keys 78 us, of 832 74, of 2080 100, of 416 95;
+  // 64 of 2460: parts of 640 68 us, of 256 81; 256 of up to 2048: of 544 88, of 1056 94).
   const int64_t heads = d.cache.heads, keys = s->slots * heads * s->span;
-  const bool tiles = d.max_q * grp > TM, far = keys > (1 << 19) && !tiles;
+  const bool tiles = !one_tile(d, (int)TM, (int)grp), far = keys > (1 << 19) && !tiles;
   s->HW = !far ? 1 : heads % 4 == 0 ? 4 : heads % 2 == 0 ? 2 : 1;
   const int64_t sets = s->slots * heads / s->HW;
-  int64_t n = sets ? (!tiles && (far ? s->slots * heads >= 256 : s->slots > 1) ? 1024 : 256) / sets : 1;
-  if (far && s->slots > 1) {                          // sequences of other lengths than the longest
-    const int64_t even = s->span / 512 < 4 ? s->span / 512 : 4;
-    n = n < even ? even : n;
+  int64_t n = sets ? (tiles || s->slots <= 1 ? 256 : 1024) / sets : 1;
+  if (far && s->slots > 1) {
+    const int64_t even = (s->span + 511) / 512;
+    n = n < 4 ? 4 : n;
+    n = n < even ? n : even;
   }
   const int64_t most = (s->span + 127) / 128;
   n = n > most ? most : n;
@@ -457,12 +508,13 @@ static int launch(const ktir_kv8_attn_t& d, const KV8Shape& s) {
   constexpr int W = ROWS_WAVES;
   const int64_t QUANT = ROWS_STEP * W / s.HW, items = s.slots * d.cache.heads, splits = d.splits < 1 ? 1 : d.splits;
   const int part = (int)(((s.span + splits - 1) / splits + QUANT - 1) / QUANT * QUANT);
+  // two workgroups a CU, evenly: where three fit, some CUs get three and others one (510 parts of 704 keys: 89 and 72 us)
+  constexpr int held = (int)(sizeof(float) * W * (16 * MT * (64 * J + 4) + 2 * 16 * MT)), spare = held < 55000 ? 55000 - held : 0;
   const hipStream_t st = stream_of(d.stream);
-  hipLaunchKernelGGL((kv8_attn_rows<CODE, J, MT>), dim3((unsigned)((s.slots * splits + 7) / 8 * 8 * (d.cache.heads / s.HW))), dim3(64 * W), 0, st, d, (int)splits, part, (uint32_t)s.slots, s.HW, device_error_flag());
+  hipLaunchKernelGGL((kv8_attn_rows<CODE, J, MT>), dim3((unsigned)((s.slots * splits + 7) / 8 * 8 * (d.cache.heads / s.HW))), dim3(64 * W), spare, st, d, (int)splits, part, s.rows, (uint32_t)s.slots, s.HW, device_error_flag());
   if (splits > 1) {
-    const int64_t rows = d.max_q * (d.q_heads / d.cache.heads), most = rows < 16 * MT ? rows : 16 * MT;
-    if (splits <= JOIN_EACH) hipLaunchKernelGGL((kv8_attn_join<J, MT, 4, 1>), dim3((unsigned)items, (unsigned)((most + 3) / 4)), dim3(256), 0, st, d, (int)splits, part, device_error_flag());
-    else hipLaunchKernelGGL((kv8_attn_join<J, MT, 1, 16>), dim3((unsigned)items, (unsigned)most), dim3(1024), 0, st, d, (int)splits, part, device_error_flag());
+    if (splits <= JOIN_EACH) hipLaunchKernelGGL((kv8_attn_join<J, MT, 4, 1>), dim3((unsigned)items, (unsigned)((s.rows + 3) / 4)), dim3(256), 0, st, d, (int)splits, part, s.rows, device_error_flag());
+    else hipLaunchKernelGGL((kv8_attn_join<J, MT, 1, 16>), dim3((unsigned)items, (unsigned)s.rows), dim3(1024), 0, st, d, (int)splits, part, s.rows, device_error_flag());
   }
   KTIR_HIP_CHECK(hipGetLastError());
   return KTIR_OK;

@@ -28,7 +28,7 @@ class OnDevice {
 
 // The shape that ktir_kv8_rows.hip gives an attention launch.
 struct KV8Shape {
-  int J, MT, HW, splits;               // columns in 64s, rows in 16s, heads of a workgroup
+  int J, MT, HW, rows, splits;         // columns in 64s, rows in 16s, heads of a workgroup, most rows of a tile
   int64_t slots, part, span;           // tiles of rows for each KV head; floats of a split's part in the workspace; most keys of a tile
 };
 void kv8_rows_shape(const ktir_kv8_attn_t& d, KV8Shape* s);
