@@ -11,8 +11,8 @@ static int check_attn(const char* what, const ktir_kv8_attn_t& d) {
   if (rc != KTIR_OK) return rc;
   if (d.q_heads < 1 || d.q_heads % d.cache.heads || d.q_heads > 65536)
     return set_error(KTIR_E_ARG, "%s: %lld query heads over %lld", what, (long long)d.q_heads, (long long)d.cache.heads);
-  if (d.max_q < 0 || d.max_k < 0 || d.max_k > (1 << 30)) return set_error(KTIR_E_ARG, "%s: bounds %lld and %lld", what, (long long)d.max_q, (long long)d.max_k);
-  if (d.window < 0 || (d.window && !d.causal)) return set_error(KTIR_E_ARG, "%s: window %lld", what, (long long)d.window);
+  if (d.max_q < 0 || d.max_q > INT32_MAX || d.max_k < 0 || d.max_k > (1 << 30)) return set_error(KTIR_E_ARG, "%s: bounds %lld and %lld", what, (long long)d.max_q, (long long)d.max_k);
+  if (d.window < 0 || d.window > INT32_MAX || (d.window && !d.causal)) return set_error(KTIR_E_ARG, "%s: window %lld", what, (long long)d.window);
   if (!(d.scale - d.scale == 0.f)) return set_error(KTIR_E_ARG, "%s: scale is not finite", what);
   if (d.batch.tokens * (d.q_heads / d.cache.heads) > (1 << 30)) return set_error(KTIR_E_UNSUPPORTED, "%s: %lld rows of a KV head", what, (long long)(d.batch.tokens * (d.q_heads / d.cache.heads)));
   if (d.splits < 0) return set_error(KTIR_E_ARG, "%s: %d splits", what, d.splits);

@@ -472,6 +472,7 @@ void kv8_rows_shape(const ktir_kv8_attn_t& d, KV8Shape* s) {
   const int64_t TM = 16 * s->MT;
   s->slots = d.max_q * grp > TM ? d.batch.tokens * grp / TM + d.batch.seqs : d.batch.seqs;
   s->rows = (int)(d.max_q * grp < TM ? d.max_q * grp : TM);
+  if (s->rows < 1) s->rows = 1;
   s->part = s->rows * (64 * s->J + 4);
   // the most tokens that a tile's rows see, from a step's bound on
   s->span = d.max_k;
@@ -488,13 +489,13 @@ void kv8_rows_shape(const ktir_kv8_attn_t& d, KV8Shape* s) {
   // host does not know, get four if all were the longest, with parts of 512 keys or more
   // (64 of 64 to 8192 tokens: parts of 1056 keys 78 us, of 832 74, of 2080 100, of 416 95;
   // 64 of 2460: parts of 640 68 us, of 256 81; 256 of up to 2048: of 544 88, of 1056 94).
-  const int64_t heads = d.cache.heads, keys = s->slots * heads * s->span;
+  const int64_t heads = d.cache.heads, longest = s->span - (ROWS_STEP - 1), keys = s->slots * heads * longest;
   const bool tiles = !one_tile(d, (int)TM, (int)grp), far = keys > (1 << 19) && !tiles;
   s->HW = !far ? 1 : heads % 4 == 0 ? 4 : heads % 2 == 0 ? 2 : 1;
   const int64_t sets = s->slots * heads / s->HW;
   int64_t n = sets ? (tiles || s->slots <= 1 ? 256 : 1024) / sets : 1;
   if (far && s->slots > 1) {
-    const int64_t even = (s->span + 511) / 512;
+    const int64_t even = longest / 512;
     n = n < 4 ? 4 : n;
     n = n < even ? n : even;
   }

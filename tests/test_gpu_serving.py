@@ -93,6 +93,23 @@ def test_rope_gradient(serving):
     S.close(got, want, bound + 1e-12, "f32")
 
 
+@pytest.mark.parametrize("tokens,heads,D,rot,dt,inter", [(9001, 2, 64, 64, "f16", False), (8195, 1, 16, 8, "bf16", True),
+                                                         (3, 2, 4096, 4096, "f16", False), (2, 1, 1001, 1000, "f32", True)])
+def test_rope_long(serving, tokens, heads, D, rot, dt, inter):
+    """Several tokens a workgroup, and rows of more units than it has threads."""
+    g = torch.Generator().manual_seed(D)
+    x = torch.randn((tokens, heads, D), generator=g).to(S.DT[dt])
+    pos = torch.arange(tokens, dtype=torch.int32) * 7
+    pos[tokens // 2] = -1
+    freq, _ = serving.rope_frequencies(rot)
+    out = torch.full_like(x, 5.0).cuda()
+    serving.Rope(x.cuda(), pos.cuda(), torch.from_numpy(freq).cuda(), out, interleaved=inter).run()
+    sync()
+    want, bound = S.rope(x, pos, freq, interleaved=inter)
+    want[tokens // 2] = 5.0
+    S.close(out, want, bound, dt)
+
+
 # ---- append ----------------------------------------------------------------------
 
 LENS = {
@@ -218,6 +235,102 @@ def test_attention_prompts(serving, hk, grp, D, page, window, code, dt):
 def test_attention_window(serving, lens, window):
     b = S.Batch(ATTN[lens], hk=2, grp=3, D=64, dt="bf16", pad=1, seed=window)
     check(b, *attend(serving, b, window=window), window=window)
+
+
+@pytest.mark.parametrize("hk,grp,D,dt,lens", [
+    (8, 4, 128, "bf16", [(1, 4096 - 61 * i) for i in range(40)] + [(0, 9), (1, 0), (1, 1)]),
+    (3, 5, 80, "f16", [(2, 3000), (3, 5000)] + [(1, 7 * i + 1) for i in range(70)]),
+    (2, 2, 256, "bf16", [(1, 9000 * i + 5) for i in range(8)]),
+    (6, 1, 192, "f16", [(4, 2500 * i + 9) for i in range(9)]), (8, 4, 64, "bf16", [(1, 70001)]), (4, 2, 128, "f16", [(3, 140000)])])
+@pytest.mark.parametrize("code", ["i8", "e4m3"])
+def test_attention_long(serving, code, hk, grp, D, dt, lens):
+    """More keys than one workgroup takes: parts of sequences of all lengths, four, two
+    or one head a workgroup, joined."""
+    b = S.Batch(lens, hk=hk, grp=grp, D=D, page=32, code=code, dt=dt, pad=1, seed=hk)
+    check(b, *attend(serving, b), heads=(0, hk * grp - 1))
+
+
+def test_attention_long_window(serving):
+    b = S.Batch([(1, 60000), (2, 70000), (1, 3), (5, 40000)] * 8, hk=4, grp=2, D=64, page=64, dt="bf16", seed=1)
+    check(b, *attend(serving, b, window=30001), window=30001, heads=(3, 7))
+
+
+def test_attention_of_shared_pages_and_far_ones(serving):
+    """Sequences that share a prefix's pages, a page twice in one table, and pages
+    whose offset passes 2^32 bytes in a cache of 5 GB."""
+    b = S.Batch([(2, 90), (1, 75), (3, 48)], hk=8, grp=2, D=128, dt="bf16")
+    pages = (5 << 30) // (16 * 8 * 128)
+    big = [torch.empty((pages, 16, 8, 128), dtype=torch.int8, device="cuda") for _ in range(2)]
+    scales = [torch.full((pages, 8), math.nan, device="cuda") for _ in range(2)]
+    at = torch.tensor([pages - 1 - 3 * i for i in range(b.pages)])
+    for x, y in zip(big + scales, b.cache()):
+        x[at.cuda()] = y.cuda()
+    b.table[1, :3] = b.table[0, :3]
+    b.table[2, 1] = b.table[2, 0]
+    where = [at.to(torch.int32)[b.table.long().clamp(min=0)].cuda(), b.q_start.cuda(), b.kv_len.cuda()]
+    out = torch.zeros_like(b.q).cuda()
+    cache = serving.KV8Cache(*big, *scales)
+    serving.KV8Attention(cache, b.q.cuda(), out, *where, **b.most).run()
+    sync()
+    want, _, bound, _ = S.attention(b.q, *b.cache(), *b.where(), scale=b.D ** -0.5)
+    S.close(out, want, bound, "bf16")
+    # appending there, to pages that no other sequence has
+    b = S.Batch([(2, 90), (1, 75), (3, 48)], hk=8, grp=2, D=128, dt="bf16")
+    where[0] = at.to(torch.int32)[b.table.long().clamp(min=0)].cuda()
+    serving.KV8Append(cache, *dev(b.new_k, b.new_v), *where).run()
+    sync()
+    for x, codes, scale, c2, s2 in ((b.new_k, b.k, b.k_scale, big[0], scales[0]), (b.new_v, b.v, b.v_scale, big[1], scales[1])):
+        wc, ws = S.append(x, codes, scale, "i8", 16, *b.where())
+        assert torch.equal(c2[at.cuda()].cpu(), wc) and torch.equal(s2[at.cuda()].cpu(), ws)
+
+
+def test_attention_of_an_empty_v(serving):
+    """A cache of zeros at the least scale, and of scale 0: the result is 0, the weights' sum is kept."""
+    for scale in (2.0 ** -100, 0.0):
+        b = S.Batch([(1, 5000), (40, 200)], hk=1, grp=4, D=64, dt="bf16")
+        b.v[:] = 0
+        b.v_scale[:] = scale
+        check(b, *attend(serving, b))
+
+
+def test_two_launches_at_once_and_a_shared_workspace(serving):
+    """Two launches that split keys, each with its workspace, on two streams; then both one
+    after another in one workspace."""
+    bs = [S.Batch([(1, 20000), (1, 9000)], hk=2, grp=4, D=128, dt="f16", seed=s) for s in (1, 2)]
+    ops, outs = [], []
+    for b in bs:
+        outs.append(torch.zeros_like(b.q).cuda())
+        ops.append(serving.KV8Attention(serving.KV8Cache(*dev(*b.cache())), b.q.cuda(), outs[-1], *dev(*b.where()), **b.most))
+        assert ops[-1].workspace_bytes > 0
+    want = [S.attention(b.q, *b.cache(), *b.where(), scale=b.D ** -0.5) for b in bs]
+    streams = [torch.cuda.Stream() for _ in bs]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for op, s in zip(ops, streams):
+            op.run(s)
+    sync()
+    for o, w in zip(outs, want):
+        S.close(o, w[0], w[2], "f16")
+        o.zero_()
+    ws = torch.empty(ops[0].workspace_bytes, dtype=torch.uint8, device="cuda")
+    shared = [serving.KV8Attention(serving.KV8Cache(*dev(*b.cache())), b.q.cuda(), o, *dev(*b.where()), workspace=ws, **b.most)
+              for b, o in zip(bs, outs)]
+    for _ in range(5):
+        for op in shared:
+            op.run()
+    sync()
+    for o, w in zip(outs, want):
+        S.close(o, w[0], w[2], "f16")
+
+
+def test_results_repeat(serving):
+    """The same bits on every run: no order of arrival in any sum."""
+    for lens, hk, grp in (([(1, 30000)], 8, 4), ([(1, 3000 + 17 * i) for i in range(30)], 8, 4), ([(700, 900), (300, 2000)], 16, 4)):
+        b = S.Batch(lens, hk=hk, grp=grp, D=128, dt="f16", seed=3)
+        first = attend(serving, b)
+        for _ in range(4):
+            again = attend(serving, b)
+            assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
 
 
 def test_attention_not_causal(serving):

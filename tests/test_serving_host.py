@@ -240,7 +240,7 @@ def test_append_refused():
 
 def test_attention_refused():
     for kw in (dict(q=far(22, (7, 4, 32), "<f2")), dict(out=far(23, (7, 3, 64), "<f2")), dict(out=far(23, (7, 4, 64), "<u2")),
-               dict(heads=3), dict(window=-1), dict(window=3, causal=False), dict(scale=math.nan), dict(max_q=-1),
+               dict(heads=3), dict(window=-1), dict(window=1 << 31), dict(window=3, causal=False), dict(scale=math.nan), dict(max_q=-1), dict(max_q=1 << 31),
                dict(max_k=-1), dict(lse=far(25, (7, 3), "<f4")), dict(lse=far(25, (7, 4), "<f2")),
                dict(max_k=1 << 31)):
         with pytest.raises(ValueError):
@@ -264,6 +264,22 @@ def test_attention_refused():
         refused(op, code)
     assert rt.opened().ktir_launch_kv8_attention(None) == rt.K["KTIR_E_ARG"]
     assert rt.opened().ktir_kv8_attention_plan(None) == rt.K["KTIR_E_ARG"]
+
+
+@no_gpu
+def test_plans_are_in_bounds():
+    """Splits and workspace of every shape of launch: at most 256 splits, none for launches of many rows."""
+    for columns in (16, 64, 80, 128, 192, 256):
+        for heads, grp in ((1, 1), (2, 7), (8, 4), (4, 16), (3, 40)):
+            for tokens, seqs, max_q, max_k in ((1, 1, 1, 1), (1, 1, 1, 1 << 30), (64, 64, 1, 8192), (7, 3, 0, 64), (7, 3, 3, 0),
+                                               (8192, 1, 8192, 8192), (500, 12, 400, 4000), (300, 300, 1, 100)):
+                for window in (0, 1, 1000):
+                    c = cache(heads=heads, columns=columns)
+                    op = attention(c, tokens=tokens, heads=heads * grp, seqs=seqs, max_q=max_q, max_k=max_k, window=window,
+                                   out=Fake((tokens, heads * grp, columns), "<f2", ptr=1 << 40), workspace=Fake((1 << 36,), "|u1", ptr=1 << 41))
+                    assert 1 <= op.desc.splits <= 256
+                    assert (op.workspace_bytes > 0) == (op.desc.splits > 1) and op.workspace_bytes < 1 << 30
+                    passes(op)
 
 
 def test_tensors_of_two_devices_are_refused():
