@@ -33,6 +33,8 @@ def launch(op):
 
 
 def passes(op):
+    if rt._lib is not None:
+        pytest.skip("a device is in use by this process: a good descriptor would launch on made-up addresses")
     rc, msg = launch(op)
     assert rc == rt.K["KTIR_E_ARG"] and "ktir_init has not run" in msg, msg
 
@@ -40,9 +42,6 @@ def passes(op):
 def refused(op, code="KTIR_E_ARG", match=""):
     rc, msg = launch(op)
     assert rc == rt.K[code] and match in msg and "ktir_init" not in msg, msg
-
-
-no_gpu = pytest.mark.skipif(rt._lib is not None, reason="a device is in use: a good descriptor would launch")
 
 
 # ---- frequencies ---------------------------------------------------------------------
@@ -98,7 +97,6 @@ def rope(shape=(5, 4, 64), rot=64, **kw):
                   kw.pop("out", far(3, shape, "<f2")), **kw)
 
 
-@no_gpu
 def test_rope_accepted():
     passes(rope())
     passes(rope(out=None))
@@ -174,7 +172,6 @@ def attention(c=None, tokens=7, heads=4, dt="<f2", **kw):
     return S.KV8Attention(c, q, out, *where(**w), **more)
 
 
-@no_gpu
 def test_cache_operators_accepted():
     for page in (16, 32, 64, 128, 256):
         for columns in (16, 80, 128, 256):
@@ -211,8 +208,7 @@ def test_cache_refused():
     refused(append(same), match="overlap")
     refused(append(cache(v_scale=far(13, (9, 2), "<f4", strides=(0, 4)))), match="share a scale")
     refused(append(cache(v_scale=far(13, (9, 2), "<f4", strides=(8, 0)))), match="share a scale")
-    if rt._lib is None:
-        passes(attention(same))
+    passes(attention(same))
 
 
 def test_append_refused():
@@ -266,7 +262,6 @@ def test_attention_refused():
     assert rt.opened().ktir_kv8_attention_plan(None) == rt.K["KTIR_E_ARG"]
 
 
-@no_gpu
 def test_plans_are_in_bounds():
     """Splits and workspace of every shape of launch: at most 256 splits, none for launches of many rows."""
     for columns in (16, 64, 80, 128, 192, 256):
