@@ -105,14 +105,11 @@ __global__ __launch_bounds__(64 * W, W / 4) void kv8_attn_tile(const ktir_kv8_at
 
   // a thread's share of a step: units of 16 codes of a key, and of 4 columns of 4 keys of V
   const int steps = t.hi > from ? (t.hi - from + TILE_KEYS - 1) / TILE_KEYS : 0;
-  KV8Groups g = {0, 0.f, 0.f, L_UNIT}, before = g, next = g;    // the groups of the 16 steps that keys are fetched of, and the 16s around
-  int g_from = 0;                                               // the first of g's steps
+  // the groups of the 16 steps that the computed one is of, of those that keys are fetched of (three steps on), and the next
+  KV8Groups cur = {0, 0.f, 0.f, L_UNIT}, g = cur, next = cur;
   u32x4_t kraw[KP];
   uint32_t vraw[VP][4];
-  auto page_of = [&](int j, int group) {         // of step j, in the groups of the step or of the 16 before
-    const int at = 4 * (j & 15) + (group & 3), now = __builtin_amdgcn_readlane(g.page, at), old = __builtin_amdgcn_readlane(before.page, at);
-    return (int64_t)(j < g_from ? old : now);
-  };
+  auto page_of = [&](int pages, int j, int group) { return (int64_t)__builtin_amdgcn_readlane(pages, 4 * (j & 15) + (group & 3)); };
   // key of a K unit, first key of a V unit: one group of 16 a wavefront
   auto k_key = [&](int p) { return (tid + NT * p) / (4 * J); };
   // (a V unit is half a chunk of 4 columns: 8 column fours, both halves, the other fours, the chunks)
@@ -126,17 +123,17 @@ __global__ __launch_bounds__(64 * W, W / 4) void kv8_attn_tile(const ktir_kv8_at
     for (int p = 0; p < KP; ++p) {
       // (columns behind D: the first ones again, times zeros in Q)
       const int r = k_key(p), at = (tid + NT * p) % (4 * J) * 16, col = at < D ? at : 0;
-      const int64_t page = page_of(j, uni(r >> 4)), row = (key + r) & (c.page - 1);
+      const int64_t page = page_of(g.page, j, uni(r >> 4)), row = (key + r) & (c.page - 1);
       if (KU % NT == 0 || tid < KU) kraw[p] = *(const KTIR_G(u32x4_t)*)(c.k + page * c.k_page + row * c.k_tok + head * c.k_head + col);
     }
   };
-  auto fetch_v = [&](int j) {
+  auto fetch_v = [&](int j, int pages) {
     const int key = from + TILE_KEYS * j;
 #pragma unroll
     for (int p = 0; p < VP; ++p) {
       // (columns behind D: the first ones again, not stored)
       const int first = v_key(p), x = v_col(p), col = x < D ? x : 0;
-      const int64_t page = page_of(j, uni(first >> 4)), row = (key + first) & (c.page - 1);
+      const int64_t page = page_of(pages, j, uni(first >> 4)), row = (key + first) & (c.page - 1);
       if (VU % NT == 0 || tid < VU) {
         const uint64_t at = c.v + page * c.v_page + row * c.v_tok + head * c.v_head + col;
 #pragma unroll
@@ -205,14 +202,15 @@ __global__ __launch_bounds__(64 * W, W / 4) void kv8_attn_tile(const ktir_kv8_at
     const bool there = from + 16 * l < t.hi;
     g = kv8_groups(d, head, kv8_pages(d, t, from + 16 * l, t.hi, shift), there, err);
     kv8_scales(g, there);
+    cur = g;
     fetch_k(0);
-    fetch_v(0);
+    fetch_v(0, g.page);
     put_k(0);
     put_v(0);
-    fetch_k(steps > 1 ? 1 : 0);
+    fetch_k(1);                        // (steps past the last: page 0)
     put_k(1);
-    fetch_v(steps > 1 ? 1 : 0);
-    fetch_k(steps > 2 ? 2 : 0);
+    fetch_v(1, g.page);
+    fetch_k(2);
     __syncthreads();
     clear();
     scores(0, 0, 4 * J);
@@ -222,21 +220,21 @@ __global__ __launch_bounds__(64 * W, W / 4) void kv8_attn_tile(const ktir_kv8_at
   for (int j = 0; j < steps; ++j) {
     // the next 16 steps' groups: their pages four steps ahead of the first fetch, then the scales
     const int f = j + 3, key = from + TILE_KEYS * j;
-    if ((f & 15) == 12 && f + 4 < steps + 3) next.page = kv8_pages(d, t, from + TILE_KEYS * (f + 4) + 16 * l, t.hi, shift);
-    if ((f & 15) == 14 && f + 2 < steps + 3) next = kv8_groups(d, head, next.page, from + TILE_KEYS * (f + 2) + 16 * l < t.hi, err);
-    if (!(f & 15) && f < steps + 3) {
-      before = g;
+    if ((f & 15) == 12) next.page = kv8_pages(d, t, from + TILE_KEYS * (f + 4) + 16 * l, t.hi, shift);
+    if ((f & 15) == 14) next = kv8_groups(d, head, next.page, from + TILE_KEYS * (f + 2) + 16 * l < t.hi, err);
+    const int vpages = (f & 15) == 0 ? cur.page : g.page;          // of step j + 2, in the 16 before g's next ones then
+    if ((f & 15) == 0) {
       g = next;
-      g_from = f;
       kv8_scales(g, from + TILE_KEYS * f + 16 * l < t.hi);
     }
+    if ((j & 15) == 0) cur = g;
     float gks[4], glv[4], giv[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int at = 4 * (j & 15) + i;
-      gks[i] = j < g_from ? lane_of(before.ks, at) : lane_of(g.ks, at);
-      glv[i] = j < g_from ? lane_of(before.lv, at) : lane_of(g.lv, at);
-      giv[i] = j < g_from ? lane_of(before.iv, at) : lane_of(g.iv, at);
+      gks[i] = lane_of(cur.ks, at);
+      glv[i] = lane_of(cur.lv, at);
+      giv[i] = lane_of(cur.iv, at);
     }
     // exponents of the weights, less b
     const bool cut = key < lo_most || key + TILE_KEYS > hi_least;
@@ -305,8 +303,8 @@ __global__ __launch_bounds__(64 * W, W / 4) void kv8_attn_tile(const ktir_kv8_at
       if (p == 0 || p == 2 || p == 4) __builtin_amdgcn_sched_barrier(0);
       if (p == 0) put_k(j + 2);
       if (p == 1) put_v(j + 1);
-      if (p == 2) fetch_k(j + 3 < steps ? j + 3 : steps - 1);
-      if (p == 3) fetch_v(j + 2 < steps ? j + 2 : steps - 1);
+      if (p == 2) fetch_k(j + 3);
+      if (p == 3) fetch_v(j + 2, vpages);
       if (p < 4) scores(j + 1, p * J, J);
       if (p < 4) {
 #pragma unroll
