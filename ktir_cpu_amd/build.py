@@ -26,7 +26,7 @@ HIPCC_FLAGS = ["-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}", "-ffp-con
 # per-source additions: the paged attention MFMA kernels keep their
 # accumulators in VGPRs (MFMA C/D operands in the VGPR form), since they
 # rescale them with VALU multiplies between products
-FILE_FLAGS = {f: ["-mllvm", "-amdgpu-mfma-vgpr-form"] for f in ("ktir_pattn.hip", "ktir_kv8_rows.hip")}
+FILE_FLAGS = {f: ["-mllvm", "-amdgpu-mfma-vgpr-form"] for f in ("ktir_pattn.hip", "ktir_kv8_rows.hip", "ktir_kv8_tile.hip")}
 
 
 def _hipcc() -> str:

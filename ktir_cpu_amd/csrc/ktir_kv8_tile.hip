@@ -14,6 +14,8 @@
 // One f16 term: w is at most 2^15 and normal down to 2^-14, so a key keeps 11 bits
 // (the result's own, in f16) unless the row's heaviest one outweighs it 2^25 to 2^29
 // times; less is added with the step of 2^-24, which is 2^-35 to 2^-39 of the heaviest.
+#include <type_traits>
+
 #include "ktir_kv8_dev.h"
 
 namespace ktir {
@@ -141,8 +143,8 @@ __global__ __launch_bounds__(64 * W, W / 4) void kv8_attn_tile(const ktir_kv8_at
       }
     }
   };
-  auto put_k = [&](int j) {
-    uint16_t* kb = ks[j & 1];
+  auto put_k = [&](int buf) {
+    uint16_t* kb = ks[buf];
 #pragma unroll
     for (int p = 0; p < KP; ++p) {
       if (KU % NT && tid >= KU) break;
@@ -151,8 +153,8 @@ __global__ __launch_bounds__(64 * W, W / 4) void kv8_attn_tile(const ktir_kv8_at
       *(uint4*)(kb + r * DP + 8 * k_slot(r, chunk + 1)) = row_half8<CODE>(kraw[p].z, kraw[p].w);
     }
   };
-  auto put_v = [&](int j) {
-    uint16_t* vb = vs[j & 1];
+  auto put_v = [&](int j, int buf) {
+    uint16_t* vb = vs[buf];
 #pragma unroll
     for (int p = 0; p < VP; ++p) {
       if (VU % NT && tid >= VU) break;
@@ -170,24 +172,17 @@ __global__ __launch_bounds__(64 * W, W / 4) void kv8_attn_tile(const ktir_kv8_at
         *(uint2*)(vb + (col + n) * TILE_KEYS + 8 * v_slot(col + n, chunk) + 4 * v_half) = make_uint2(a[n], b[n]);
     }
   };
-  f32x16_t s[RB][2];                              // scores of a step: K rows times Q
-  auto clear = [&]() {
-#pragma unroll
-    for (int b = 0; b < RB; ++b)
-#pragma unroll
-      for (int k = 0; k < 2; ++k)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s[b][k][i] = 0.f;
-  };
-  auto scores = [&](int j, int first, int n) {    // of columns 16 first .. 16 (first + n)
-    const uint16_t* kb = ks[j & 1];
+  const f32x16_t zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  // scores of a step, K rows times Q, of columns 16 first .. 16 (first + n)
+  auto scores = [&](f32x16_t (&s)[RB][2], int buf, int first, int n) {
+    const uint16_t* kb = ks[buf];
 #pragma unroll
     for (int x = first; x < first + n; ++x)
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         const uint4 a = *(const uint4*)(kb + (32 * k + r32) * DP + 8 * k_slot(32 * k + r32, 2 * x + h));
 #pragma unroll
-        for (int b = 0; b < RB; ++b) s[b][k] = mfma_at<false>(a, qf[b][x], s[b][k]);
+        for (int b = 0; b < RB; ++b) s[b][k] = mfma_at<false>(a, qf[b][x], x ? s[b][k] : zero);
       }
   };
   auto top_of = [&](const f32x16_t (&x)[2]) {
@@ -198,6 +193,7 @@ __global__ __launch_bounds__(64 * W, W / 4) void kv8_attn_tile(const ktir_kv8_at
       for (int i = 0; i < 16; ++i) top = __builtin_fmaxf(top, x[k][i]);
     return top;
   };
+  f32x16_t s0[RB][2], s1[RB][2];                 // scores of even and odd steps
   if (steps) {
     const bool there = from + 16 * l < t.hi;
     g = kv8_groups(d, head, kv8_pages(d, t, from + 16 * l, t.hi, shift), there, err);
@@ -206,18 +202,20 @@ __global__ __launch_bounds__(64 * W, W / 4) void kv8_attn_tile(const ktir_kv8_at
     fetch_k(0);
     fetch_v(0, g.page);
     put_k(0);
-    put_v(0);
+    put_v(0, 0);
     fetch_k(1);                        // (steps past the last: page 0)
     put_k(1);
     fetch_v(1, g.page);
     fetch_k(2);
     __syncthreads();
-    clear();
-    scores(0, 0, 4 * J);
+    scores(s0, 0, 0, 4 * J);
     __syncthreads();
   }
 
-  for (int j = 0; j < steps; ++j) {
+  // Step j: its scores are in s, those of step j + 1 go to s_next; PAR is j's parity, so that the
+  // buffers' addresses do not change.
+  auto step = [&](int j, auto parity, f32x16_t (&s)[RB][2], f32x16_t (&s_next)[RB][2]) {
+    constexpr int PAR = decltype(parity)::value;
     // the next 16 steps' groups: their pages four steps ahead of the first fetch, then the scales
     const int f = j + 3, key = from + TILE_KEYS * j;
     if ((f & 15) == 12) next.page = kv8_pages(d, t, from + TILE_KEYS * (f + 4) + 16 * l, t.hi, shift);
@@ -289,23 +287,17 @@ __global__ __launch_bounds__(64 * W, W / 4) void kv8_attn_tile(const ktir_kv8_at
       }
     }
     // the codes of steps j + 2 (K) and j + 1 (V) into LDS, those of j + 3 and j + 2 on their way, the scores of j + 1:
-    // beside W V of step j.  (Past the last step: what was fetched last, again.)
-    f32x16_t u[RB][2];
-#pragma unroll
-    for (int b = 0; b < RB; ++b)
-#pragma unroll
-      for (int k = 0; k < 2; ++k) u[b][k] = s[b][k];
-    clear();
-    const uint16_t* vb = vs[j & 1];
+    // beside W V of step j.  (Past the last step: of page 0, unused.)
+    const uint16_t* vb = vs[PAR];
     uint4 w[RB], old[RB];
 #pragma unroll
     for (int p = 0; p < 5; ++p) {
-      if (p == 0 || p == 2 || p == 4) __builtin_amdgcn_sched_barrier(0);
-      if (p == 0) put_k(j + 2);
-      if (p == 1) put_v(j + 1);
+      if (J == 4 || p == 0 || p == 2 || p == 4) __builtin_amdgcn_sched_barrier(0);
+      if (p == 0) put_k(PAR);
+      if (p == 1) put_v(j + 1, 1 - PAR);
       if (p == 2) fetch_k(j + 3);
       if (p == 3) fetch_v(j + 2, vpages);
-      if (p < 4) scores(j + 1, p * J, J);
+      if (p < 4) scores(s_next, 1 - PAR, p * J, J);
       if (p < 4) {
 #pragma unroll
         for (int b = 0; b < RB; ++b) {
@@ -313,7 +305,7 @@ __global__ __launch_bounds__(64 * W, W / 4) void kv8_attn_tile(const ktir_kv8_at
           old[b] = w[b];
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            e[i] = __builtin_amdgcn_exp2f(u[b][p >> 1][8 * (p & 1) + i]);
+            e[i] = __builtin_amdgcn_exp2f(s[b][p >> 1][8 * (p & 1) + i]);
             sum[b] = __builtin_fmaf(e[i], giv[p], sum[b]);
           }
           w[b] = make_uint4(cvt2<false>(e[0], e[1]), cvt2<false>(e[2], e[3]), cvt2<false>(e[4], e[5]), cvt2<false>(e[6], e[7]));
@@ -332,6 +324,10 @@ __global__ __launch_bounds__(64 * W, W / 4) void kv8_attn_tile(const ktir_kv8_at
       }
     }
     __syncthreads();
+  };
+  for (int j = 0; j < steps; j += 2) {
+    step(j, std::integral_constant<int, 0>(), s0, s1);
+    if (j + 1 < steps) step(j + 1, std::integral_constant<int, 1>(), s1, s0);
   }
 
   // O^T: a lane has columns 32 n + 8 g + 4 h + 0..3 of its row
