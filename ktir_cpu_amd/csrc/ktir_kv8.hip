@@ -195,11 +195,10 @@ __global__ __launch_bounds__(256) void kv8_append(const ktir_kv8_append_t d, int
   if (hv >= 2 * c.heads) return;
   const int64_t head = hv >> 1;
   const bool is_v = hv & 1;
-  int64_t nth;
+  int64_t s, nth;
   const int shift = __builtin_ctz((uint32_t)c.page);
-  const int64_t s = seq_of_slot(d.batch, 1, shift, 2, blockIdx.x, &nth);
+  const Seq q = seq_of_slot(d.batch, c.page, 1, shift, 2, blockIdx.x, &s, &nth, err);
   if (nth < 0) return;
-  const Seq q = seq_of(d.batch, c.page, s, err);
   const int64_t pos0 = (int64_t)q.n_kv - q.n_new, from = pos0 < 0 ? 0 : pos0;      // the first position that is stored
   const int64_t p = (from >> shift) + nth;                                       // the page's number in the sequence
   const int64_t lo = p << shift < from ? from : p << shift, hi = (p + 1) << shift < q.n_held ? (p + 1) << shift : q.n_held;

@@ -98,10 +98,6 @@ struct KV8Groups {
   float ks, lv, iv;     // kscale, log2 vscale, 2^-16 / vscale
 };
 
-__device__ __forceinline__ float lane_of(float x, int i) {
-  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), i));
-}
-
 // The rows of one tile of a launch: query head h * grp + r % grp of token
 // i = r / grp of sequence s, r from row0 on; what they see of the keys.
 struct Tile {
@@ -122,11 +118,11 @@ __device__ __forceinline__ void seen(const ktir_kv8_attn_t& d, const Tile& t, in
   token_sees(d, t, (int)((uint32_t)r / (uint32_t)grp), lo, hi);
 }
 
-// tile `nth` (of TM rows) of sequence s
-__device__ __forceinline__ Tile tile_at(const ktir_kv8_attn_t& d, int64_t s, int64_t nth, int TM, int grp, int* err) {
+// tile `nth` (of TM rows) of sequence s, which is q
+__device__ __forceinline__ Tile tile_at(const ktir_kv8_attn_t& d, int64_t s, const Seq& q, int64_t nth, int TM, int grp, int* err) {
   Tile t = {};
   t.s = s;
-  t.q = seq_of(d.batch, d.cache.page, s, err);
+  t.q = q;
   t.keys = t.q.n_held;
   if (t.keys > d.max_k || t.q.n_new > d.max_q) *err = OUT_OF_RANGE;
   if (t.keys > d.max_k) t.keys = (int)d.max_k;
@@ -150,10 +146,10 @@ __host__ __device__ inline bool one_tile(const ktir_kv8_attn_t& d, int TM, int g
 
 // tile `slot` of a launch: a sequence each, or found by the batch's offsets
 __device__ __forceinline__ Tile tile_of(const ktir_kv8_attn_t& d, int64_t slot, int TM, int grp, int* err) {
-  if (one_tile(d, TM, grp)) return tile_at(d, slot, 0, TM, grp, err);
-  int64_t nth;
-  const int64_t s = seq_of_slot(d.batch, grp, __builtin_ctz(TM), 1, slot, &nth);
-  return nth < 0 ? Tile{} : tile_at(d, s, nth, TM, grp, err);
+  if (one_tile(d, TM, grp)) return tile_at(d, slot, seq_of(d.batch, d.cache.page, slot, err), 0, TM, grp, err);
+  int64_t s, nth;
+  const Seq q = seq_of_slot(d.batch, d.cache.page, grp, __builtin_ctz(TM), 1, slot, &s, &nth, err);
+  return nth < 0 ? Tile{} : tile_at(d, s, q, nth, TM, grp, err);
 }
 
 // a tile's fields in scalar registers: they are the same in every lane, or lane i's
@@ -169,11 +165,6 @@ __device__ __forceinline__ Tile uni(Tile t) {
   t.hi = uni(t.hi);
   return t;
 }
-__device__ __forceinline__ int64_t lane_of(int64_t x, int i) {
-  const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)x, i), hi = __builtin_amdgcn_readlane((uint32_t)((uint64_t)x >> 32), i);
-  return (int64_t)((uint64_t)hi << 32 | lo);
-}
-__device__ __forceinline__ int lane_of(int x, int i) { return __builtin_amdgcn_readlane(x, i); }
 __device__ __forceinline__ Tile lane_of(Tile t, int i) {
   t.s = lane_of(t.s, i);
   t.q.start = lane_of(t.q.start, i);

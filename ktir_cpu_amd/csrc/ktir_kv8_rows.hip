@@ -104,7 +104,7 @@ __global__ __launch_bounds__(64 * ROWS_WAVES, MT == 1 ? 2 : 1) void kv8_attn_row
   if (d.batch.seqs == 1 && one_tile(d, TM, grp)) {
     slot = 0;
     split = (int)u;
-    t = uni(tile_at(d, 0, 0, TM, grp, err));
+    t = uni(tile_at(d, 0, seq_of(d.batch, c.page, 0, err), 0, TM, grp, err));
     if (!t.rows) return;
     active = tile_parts(t, part);
     if (split >= active) return;
@@ -114,7 +114,7 @@ __global__ __launch_bounds__(64 * ROWS_WAVES, MT == 1 ? 2 : 1) void kv8_attn_row
     uint32_t before = 0;
     for (int64_t base = 0; base < d.batch.seqs; base += 64) {
       Tile x = {};
-      if (base + l < d.batch.seqs) x = tile_at(d, base + l, 0, TM, grp, err);
+      if (base + l < d.batch.seqs) x = tile_at(d, base + l, seq_of(d.batch, c.page, base + l, err), 0, TM, grp, err);
       int n = x.rows ? tile_parts(x, part) : 0;
       n = n < splits ? n : splits;
       int upto = n;                                          // parts of the sequences up to this lane's

@@ -69,29 +69,44 @@ __device__ __forceinline__ Seq seq_of(const ktir_kv8_batch_t& b, int64_t page, i
   return {start, (int32_t)(end - start), (int32_t)kv, (int32_t)held};
 }
 
+// lane i's value in every lane
+__device__ __forceinline__ float lane_of(float x, int i) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), i)); }
+__device__ __forceinline__ int lane_of(int x, int i) { return __builtin_amdgcn_readlane(x, i); }
+__device__ __forceinline__ int64_t lane_of(int64_t x, int i) {
+  const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)x, i), hi = __builtin_amdgcn_readlane((uint32_t)((uint64_t)x >> 32), i);
+  return (int64_t)((uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ Seq lane_of(const Seq& q, int i) {
+  return {lane_of(q.start, i), lane_of(q.n_new, i), lane_of(q.n_kv, i), lane_of(q.n_held, i)};
+}
+
 // The sequence that slot `w` of a launch belongs to, and its number in it, where
 // sequence s has the slots from floor(q_start[s] * mul / 2^shift) + extra * s on (so
 // one of n tokens has at least floor(n * mul / 2^shift) + extra): the last s whose first
 // slot is not after w, with nth < 0 if there is none.  All lanes of a wavefront
 // search together, 64 sequences a step.
-__device__ __forceinline__ int64_t seq_of_slot(const ktir_kv8_batch_t& b, int64_t mul, int shift, int64_t extra, int64_t w, int64_t* nth) {
+__device__ __forceinline__ Seq seq_of_slot(const ktir_kv8_batch_t& b, int64_t page, int64_t mul, int shift, int64_t extra, int64_t w,
+                                           int64_t* s, int64_t* nth, int* err) {
   const int l = threadIdx.x & 63;
-  int64_t s = 0, first = INT64_MAX;
+  Seq found = {0, 0, 0, 0};
+  *s = 0;
+  *nth = -1;
   for (int64_t base = 0; base < b.seqs; base += 64) {
     int64_t at = INT64_MAX;
+    Seq q = {0, 0, 0, 0};
     if (base + l < b.seqs) {
-      const int64_t q = ints(b.q_start)[base + l];
-      at = ((q < 0 ? 0 : q) * mul >> shift) + extra * (base + l);
+      q = seq_of(b, page, base + l, err);
+      at = (q.start * mul >> shift) + extra * (base + l);
     }
     const uint64_t below = __ballot(at <= w);
     if (!below) break;
     const int last = 63 - __builtin_clzll(below);
-    s = base + last;
-    first = (int64_t)__shfl((long long)at, last);
+    found = lane_of(q, last);
+    *s = base + last;
+    *nth = w - lane_of(at, last);
     if (last < 63) break;
   }
-  *nth = w - first;
-  return s;
+  return found;
 }
 
 }  // namespace ktir
