@@ -2,7 +2,8 @@
 //
 // Keys' codes become f16 operands, which hold both code types exactly, and so do
 // queries of either type, each row times a power of two; so every product of a
-// score is exact and their sum is the matrix instruction's f32.
+// score is exact (but for elements below 2^-28 of a bf16 row's largest) and their
+// sum is the matrix instruction's f32.
 //
 // The scales stay out of the operands: with t_j = log2(e) scale kscale q . k_j and
 // page scales kscale, vscale,

@@ -16,8 +16,14 @@
 //                 exchange between lanes; a lane's load of 4 J codes of eight
 //                 keys is transposed by the byte selects of the conversion
 // Pages, scales and addresses of 64 groups of 16 keys are fetched at once, one per
-// lane, so no step waits for the chain table -> page -> key; the codes of the next
-// step are in flight while this one is computed.
+// lane, so no step waits for the chain table -> page -> key; K's codes of the next
+// step are in flight while this one is computed (V's too: no faster, 35 registers more).
+//
+// Bound: bytes where the cache is long.  131072 tokens of 8 heads of 128, 269 MB of e4m3
+// codes: 53.5 us = 5.0 TB/s and 4 to 7 us to join 128 parts; reads alone in this pattern
+// make 5.6 TB/s.  More workgroups than two a CU lose DRAM locality (64 of 2460 tokens:
+// 68.6 us with 512 workgroups, 81 with 1280).  Short ones are latency: one token after
+// 1000 takes 7.0 us (launch, offsets -> table -> codes, two barriers) and 3.6 to join.
 #include "ktir_kv8_dev.h"
 
 namespace ktir {

@@ -1,15 +1,23 @@
 // Attention over the 8-bit cache for many rows: prompts and chunks of them.
 //
-// A workgroup has 128 RB rows (tokens x the query heads of one KV head) of one
-// sequence, 32 RB of them in each of its four wavefronts, and runs over the keys that
-// they see, 64 at a time.  The codes of a step are made f16 once for all rows and
-// laid into LDS (two buffers): K as [key][column], V as [column][key], with the keys
-// of each 16 in the order that the scores' layout leaves them in:
+// A workgroup has 256 rows (128 for more than 128 columns; tokens x the query heads of
+// one KV head) of one sequence, 32 in each wavefront, and runs over the keys that they
+// see, 64 at a time.  The codes of a step are made f16 once for all rows and laid into
+// LDS (two buffers): K as [key][column], V as [column][key], with the keys of each 16 in
+// the order that the scores' layout leaves them in:
 //   S^T = K Q^T     32 x 32 x 16 MFMA, one row a lane (the two halves share it)
 //   w, b, l         as ktir_kv8_dev.h says; w enters the product as one f16 term
 //   O^T += V^T W^T  no exchange between lanes
-// With RB = 2 a fragment read from LDS serves two products; one wavefront a SIMD
-// then has its 512 registers.
+// The scores of the next step, the conversion of the one after and W V of this step
+// stand side by side, a quarter of each at a time.
+//
+// Bound: issue.  8192 tokens, 32 / 8 heads of 128 columns, causal, i8 codes, 550 GFLOP:
+// 600 to 630 us on three cards = 870 to 920 TFLOP/s (e4m3 590); 39 % of the time the matrix
+// pipe is busy, 58 % the vector pipe (320 instructions a step and wavefront: 48 convert, 128
+// make the weights, 32 of them exponentials), 17 % both; LDS 40 %.  64 columns take 402 us,
+// half the products at the same weights.  Before: 1193 us in ktir_kv8_rows.hip, 906 with
+// four wavefronts of 64 rows, 677 without the next scores beside; matrix instructions
+// pinned between vector ones, seven to one, took 660 to 700.
 //
 // One f16 term: w is at most 2^15 and normal down to 2^-14, so a key keeps 11 bits
 // (the result's own, in f16) unless the row's heaviest one outweighs it 2^25 to 2^29
