@@ -509,8 +509,9 @@ typedef struct ktir_rows3 {
  * the products are f32, and the result is rounded once.  `inverse` is the rotation
  * back: the gradient's way through the operator.  Rows of tokens with
  * pos < 0 are left as they were.  Two tensors (queries and keys) share one
- * launch; heads2 = 0: one.  An output may be its input itself, and must
- * otherwise not overlap it.  dtype: KTIR_F16, KTIR_BF16 or KTIR_F32. */
+ * launch; heads2 = 0: one.  An output may be its input itself and must share
+ * no element with the other tensors (parts of one projection's rows, side by
+ * side, do not).  dtype: KTIR_F16, KTIR_BF16 or KTIR_F32. */
 typedef struct ktir_rope {
   int64_t tokens, heads, heads2, columns, rot;
   ktir_rows3_t in, out, in2, out2;
@@ -576,11 +577,12 @@ int ktir_launch_kv8_append(const ktir_kv8_append_t* d);
  *   out = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m),  lse = m + ln sum_j exp(s_j - m)
  * A row that no token is left for gets 0 and -inf; padding rows are left as
  * they were.  Products of q and codes are exact, sums f32, probabilities enter
- * the second product as ktir_kv8_attn.hip says; the result is rounded once to dtype
+ * the second product as ktir_kv8_rows.hip and ktir_kv8_tile.hip say; the result is rounded once to dtype
  * (KTIR_F16 or KTIR_BF16, of q and out).  Codes of tokens past kv_len are not
  * looked at; an e4m3 NaN code of a value makes the rows of its sequence NaN.
- * max_q and max_k bound the new and the cached tokens of every sequence: what
- * a sequence has beyond is left out, with the device error word set.
+ * max_q and max_k (2^30 at most) bound the new and the cached tokens of every
+ * sequence: what a sequence has beyond is left out, with the device error word set.
+ * out may be q itself; it and lse overlap nothing else that the launch reads.
  * `splits` workgroups share a sequence's cached tokens.  ktir_kv8_attention_plan
  * sets it and ws_bytes (host only), the bytes of workspace that `ws` must then
  * have, on a 16-byte bound; launches that may run at the same time need a

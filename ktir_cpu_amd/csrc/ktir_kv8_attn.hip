@@ -45,10 +45,15 @@ extern "C" int ktir_launch_kv8_attention(const ktir_kv8_attn_t* d) {
   rc = check_rows3(ME, d->q, d->batch.tokens, d->q_heads, d->cache.columns, false);
   if (rc == KTIR_OK) rc = check_rows3(ME, d->out, d->batch.tokens, d->q_heads, d->cache.columns, true);
   if (rc == KTIR_OK && d->lse) {
-    const ktir_rows3_t lse = {d->lse, d->lse_tok, d->lse_head};
-    rc = d->lse & 3 ? set_error(KTIR_E_ARG, "%s: lse off 4-byte bounds", ME) : check_rows3(ME, lse, d->batch.tokens, d->q_heads, 1, true);
+    rc = d->lse & 3 ? set_error(KTIR_E_ARG, "%s: lse off 4-byte bounds", ME)
+                    : check_rows3(ME, {d->lse, d->lse_tok, d->lse_head}, d->batch.tokens, d->q_heads, 1, true);
   }
   if (rc != KTIR_OK) return rc;
+  auto rows = [&](const ktir_rows3_t& r, int64_t columns, int64_t bytes) { return rows_of(r, d->batch.tokens, d->q_heads, columns, bytes); };
+  const Strided q = rows(d->q, d->cache.columns, 2), out = rows(d->out, d->cache.columns, 2);
+  const Strided lse = rows({d->lse, d->lse_tok, d->lse_head}, 1, 4);
+  if (!(same(q, out) || apart(q, out)) || (d->lse && !(apart(lse, out) && apart(lse, q))))
+    return set_error(KTIR_E_ARG, "%s: an output overlaps a tensor that it is not", ME);
   KV8Shape s;
   kv8_rows_shape(*d, &s);
   const int64_t splits = d->splits < 1 ? 1 : d->splits, tiles = s.slots * d->cache.heads;

@@ -1,5 +1,13 @@
 // Rotary positions: pairs of a head's columns rotated by an angle that grows
 // with the token's position, y = (x0 c - x1 s, x1 c + x0 s).
+//
+// Bound: bytes, in and out once.  The angles of a token are made once for all its
+// heads (64-bit remainder, one sine and cosine: about 60 instructions), in LDS, and
+// every vector of 16 bytes is loaded and stored once, two rows of loads ahead.
+// Measured, f16 / bf16: 8192 tokens of 32 + 8 heads of 128, 168 MB, 37.9 us = 4.4 TB/s
+// (a copy of 256 MiB makes 5.4 here); 40 + 40 heads with 64 interleaved columns of
+// 128, 168 MB, 39.4 us, 55.8 with the columns behind rot as units of their own size;
+// one thread per pair over all heads took 97 and 212 us.  One token: a launch, 4.1 us.
 #include "ktir_serve.h"
 
 namespace ktir {
@@ -228,15 +236,18 @@ static void rope_go(const ktir_rope_t& d, hipStream_t st) {
   else hipLaunchKernelGGL((rope_turn<DT, false, V, R>), grid, dim3(256), 0, st, d, (int)per);
 }
 
-static int check_pair(const ktir_rope_t& d, const ktir_rows3_t& in, const ktir_rows3_t& out, int64_t heads) {
-  int rc = check_rows3("ktir_launch_rope", in, d.tokens, heads, d.columns, false);
-  if (rc == KTIR_OK) rc = check_rows3("ktir_launch_rope", out, d.tokens, heads, d.columns, true);
+static int check_tensors(const ktir_rope_t& d) {
+  constexpr const char* ME = "ktir_launch_rope";
+  int rc = check_rows3(ME, d.in, d.tokens, d.heads, d.columns, false);
+  if (rc == KTIR_OK) rc = check_rows3(ME, d.out, d.tokens, d.heads, d.columns, true);
+  if (rc == KTIR_OK && d.heads2) rc = check_rows3(ME, d.in2, d.tokens, d.heads2, d.columns, false);
+  if (rc == KTIR_OK && d.heads2) rc = check_rows3(ME, d.out2, d.tokens, d.heads2, d.columns, true);
   if (rc != KTIR_OK) return rc;
-  if (in.ptr == out.ptr && (in.tok == out.tok || d.tokens == 1) && (in.head == out.head || heads == 1)) return KTIR_OK;
-  const int e = d.dtype == KTIR_F32 ? 4 : 2;
-  if (in.ptr < end_of(out, d.tokens, heads, d.columns, e) && out.ptr < end_of(in, d.tokens, heads, d.columns, e))
-    return set_error(KTIR_E_ARG, "ktir_launch_rope: an output overlaps its input without being it");
-  return KTIR_OK;
+  auto rows = [&](const ktir_rows3_t& r, int64_t heads) { return rows_of(r, d.tokens, heads, d.columns, d.dtype == KTIR_F32 ? 4 : 2); };
+  const Strided in = rows(d.in, d.heads), out = rows(d.out, d.heads), in2 = rows(d.in2, d.heads2), out2 = rows(d.out2, d.heads2);
+  bool good = same(in, out) || apart(in, out);
+  if (d.heads2) good = good && (same(in2, out2) || apart(in2, out2)) && apart(out, in2) && apart(out2, in) && apart(out, out2);
+  return good ? KTIR_OK : set_error(KTIR_E_ARG, "%s: an output overlaps a tensor that it is not", ME);
 }
 
 }  // namespace ktir
@@ -258,8 +269,7 @@ extern "C" int ktir_launch_rope(const ktir_rope_t* d) {
   if (!(d->amplitude - d->amplitude == 0.0)) return set_error(KTIR_E_ARG, "ktir_launch_rope: amplitude is not finite");
   if (d->tokens == 0) return KTIR_OK;
   if (!d->pos || !d->freq || (d->freq & 7)) return set_error(KTIR_E_ARG, "ktir_launch_rope: positions or frequencies missing");
-  int rc = check_pair(*d, d->in, d->out, d->heads);
-  if (rc == KTIR_OK && d->heads2) rc = check_pair(*d, d->in2, d->out2, d->heads2);
+  int rc = check_tensors(*d);
   if (rc == KTIR_OK) rc = ready("ktir_launch_rope");
   if (rc != KTIR_OK) return rc;
   OnDevice on;

@@ -46,10 +46,16 @@ int check_batch(const char* what, const ktir_kv8_batch_t& b, const ktir_kv8_t& c
 int check_rows3(const char* what, const ktir_rows3_t& r, int64_t tokens, int64_t heads, int64_t columns, bool written);
 int ready(const char* what);         // whether ktir_init has run
 
-// the first byte behind a [tokens, heads, columns] tensor of `bytes` an element
-inline uint64_t end_of(const ktir_rows3_t& r, int64_t tokens, int64_t heads, int64_t columns, int bytes) {
-  return r.ptr + ((uint64_t)(tokens - 1) * r.tok + (uint64_t)(heads - 1) * r.head + columns) * bytes;
+// Rows of `width` bytes, counts by counts at steps of so many bytes.
+struct Strided {
+  uint64_t ptr;
+  int64_t width, count[3], step[3];
+};
+inline Strided rows_of(const ktir_rows3_t& r, int64_t tokens, int64_t heads, int64_t columns, int64_t bytes) {
+  return {r.ptr, columns * bytes, {tokens, heads, 1}, {r.tok * bytes, r.head * bytes, 0}};
 }
+bool apart(const Strided& a, const Strided& b);      // whether they share no byte; one of them is an output, whose rows do not overlap
+bool same(const Strided& a, const Strided& b);       // whether they are one tensor
 
 __device__ __forceinline__ const KTIR_G(int32_t)* ints(uint64_t p) { return (const KTIR_G(int32_t)*)p; }
 

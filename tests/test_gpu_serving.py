@@ -333,6 +333,17 @@ def test_results_repeat(serving):
             assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
 
 
+@pytest.mark.parametrize("lens,hk,grp", [([(1, 5000), (1, 70)], 2, 4), ([(300, 400), (200, 900)], 16, 4)])
+def test_attention_into_the_queries(serving, lens, hk, grp):
+    b = S.Batch(lens, hk=hk, grp=grp, D=64, dt="bf16")
+    q = b.q.cuda()
+    serving.KV8Attention(serving.KV8Cache(*dev(*b.cache())), q, q, *dev(*b.where()), **b.most).run()
+    sync()
+    heads = [0, hk * grp - 1]
+    want, _, bound, _ = S.attention(b.q, *b.cache(), *b.where(), scale=b.D ** -0.5, heads=heads)
+    S.close(q[:, heads], want[:, heads], bound[:, heads], "bf16")
+
+
 def test_attention_not_causal(serving):
     b = S.Batch([(5, 40), (70, 33), (2, 0)], hk=2, grp=3, D=96, page=32)
     check(b, *attend(serving, b, causal=False, scale=0.3), causal=False, scale=0.3)

@@ -107,6 +107,32 @@ def test_rope_accepted():
     assert launch(rope(shape=(0, 4, 64)))[0] == 0       # nothing to do
 
 
+@pytest.mark.parametrize("seed", range(40))
+def test_rope_in_place_side_by_side_or_not(seed):
+    # two tensors of equal steps in one allocation, against the set of their elements' addresses
+    rng = np.random.default_rng(seed)
+    tokens, heads, heads2 = (int(rng.integers(1, 5)) for _ in range(3))
+    cols, most = 4, max(heads, heads2)
+    head = int(rng.choice([cols, 2 * cols, 3 * cols, 3 * cols + 2]))
+    tok = int(rng.choice([most * head, 2 * most * head, most * head + 6]))
+    if rng.integers(2):                                # heads apart, their tokens inside
+        head, tok = int(rng.choice([1, 2])) * tokens * 3 * cols, int(rng.choice([cols, 2 * cols, 3 * cols]))
+
+    def elements(at, n):
+        return {at + i * tok + j * head + c for i in range(tokens) for j in range(n) for c in range(cols)}
+
+    def tensor(at, n):
+        return Fake((tokens, n, cols), "<f2", ptr=(8 << 30) + 2 * at, strides=(2 * tok, 2 * head, 2))
+
+    for _ in range(30):
+        at = int(rng.integers(-2 * most * head, 2 * most * head + tok))
+        op = S.Rope(tensor(0, heads), far(1, (tokens,), "<i8"), far(2, (cols // 2,), "<f8"), k=tensor(at, heads2))
+        if elements(0, heads) & elements(at, heads2):
+            refused(op, match="overlaps")
+        else:
+            passes(op)
+
+
 def test_rope_refused_in_python():
     import torch
     with pytest.raises(ValueError, match="on the GPU"):
@@ -127,6 +153,14 @@ def test_rope_refused_in_python():
 def test_rope_refused_in_c():
     refused(rope(out=Fake((5, 4, 64), "<f2", ptr=(4 << 30) + 128)), match="overlaps")
     refused(rope(out=far(3, (5, 4, 64), "<f2", strides=(0, 128, 2))), match="overlap")
+    # queries into the keys' place, both outputs in one place, an output over half of the keys
+    k = far(5, (5, 4, 64), "<f2")
+    refused(rope(out=k, k=k, k_out=far(6, (5, 4, 64), "<f2")), match="overlaps")
+    refused(rope(k=k, k_out=far(3, (5, 4, 64), "<f2")), match="overlaps")
+    refused(rope(out=None, k=far(0, (5, 2, 64), "<f2")), match="overlaps")
+    row = dict(strides=(12 * 128, 128, 2))
+    refused(rope(x=far(0, (5, 8, 64), "<f2", **row), shape=(5, 8, 64), out=None, k=Fake((5, 2, 64), "<f2", ptr=(4 << 30) + 7 * 128, **row)),
+            match="overlaps")
     refused(rope(out=far(3, (5, 4, 64), "<f2", strides=(512, 64, 2))), match="overlap")
     refused(rope(shape=(5, 0, 64)))
     refused(rope(amplitude=math.inf), match="amplitude")
@@ -209,6 +243,15 @@ def test_cache_refused():
     refused(append(cache(v_scale=far(13, (9, 2), "<f4", strides=(0, 4)))), match="share a scale")
     refused(append(cache(v_scale=far(13, (9, 2), "<f4", strides=(8, 0)))), match="share a scale")
     passes(attention(same))
+    # keys and values in one allocation: one page behind the other, heads in turn, or on one another
+    for strides, v in (((4096, 128, 64, 1), 2048), ((4096, 256, 128, 1), 64), ((4096, 256, 64, 1), 128)):
+        one = cache(k=far(10, (9, 16, 2, 64), "|i1", strides=strides),
+                    v=Fake((9, 16, 2, 64), "|i1", ptr=(14 << 30) + v, strides=strides))
+        passes(append(one))
+    k, s = far(10, (9, 16, 2, 64), "|i1"), far(12, (9, 2), "<f4")
+    for c in (cache(k=k, v=k), cache(k=k, v=Fake((9, 16, 2, 64), "|i1", ptr=(14 << 30) + 2048)), cache(k_scale=s, v_scale=s)):
+        refused(append(c), match="overlap")
+        passes(attention(c))
 
 
 def test_append_refused():
@@ -243,6 +286,12 @@ def test_attention_refused():
             attention(**kw)
     refused(attention(out=far(23, (7, 4, 64), "<f2", strides=(512, 64, 2))), match="overlap")
     refused(attention(lse=far(25, (7, 4), "<f4", strides=(4, 4))), match="overlap")
+    q = far(22, (7, 4, 64), "<f2")
+    passes(attention(out=q))
+    refused(attention(out=Fake((7, 4, 64), "<f2", ptr=(26 << 30) + 512)), match="overlaps")
+    refused(attention(out=far(22, (7, 4, 64), "<f2", strides=(1024, 128, 2))), match="overlaps")
+    refused(attention(lse=far(22, (7, 4), "<f4")), match="overlaps")
+    refused(attention(lse=far(23, (7, 4), "<f4")), match="overlaps")
     with pytest.raises(ValueError, match="workspace"):
         attention(max_k=1 << 16, workspace=far(24, (8,), "|u1"))
     with pytest.raises(ValueError, match="workspace"):
