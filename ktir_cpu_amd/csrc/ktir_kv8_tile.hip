@@ -8,16 +8,21 @@
 //   S^T = K Q^T     32 x 32 x 16 MFMA, one row a lane (the two halves share it)
 //   w, b, l         as ktir_kv8_dev.h says; w enters the product as one f16 term
 //   O^T += V^T W^T  no exchange between lanes
-// The scores of the next step, the conversion of the one after and W V of this step
-// stand side by side, a quarter of each at a time.
+// With 65 to 128 columns the two wavefronts of a SIMD take turns, half a step apart: one
+// makes the weights of its step (vector instructions alone), the other multiplies (the
+// scores of its next step and W V of this one) and converts the codes of the step after;
+// a barrier ends each half.  Else scores, conversion, weights and W V stand side by side,
+// a quarter of each at a time: 64 columns 398 us so and 422 in turns, below.  A wavefront
+// alone on its SIMD (more than 128 columns) has no one to take turns with.
 //
 // Bound: issue.  8192 tokens, 32 / 8 heads of 128 columns, causal, i8 codes, 550 GFLOP:
-// 600 to 630 us on three cards = 870 to 920 TFLOP/s (e4m3 590); 39 % of the time the matrix
-// pipe is busy, 58 % the vector pipe (320 instructions a step and wavefront: 48 convert, 128
-// make the weights, 32 of them exponentials), 17 % both; LDS 40 %.  64 columns take 402 us,
-// half the products at the same weights.  Before: 1193 us in ktir_kv8_rows.hip, 906 with
-// four wavefronts of 64 rows, 677 without the next scores beside; matrix instructions
-// pinned between vector ones, seven to one, took 660 to 700.
+// 564 to 607 us on four cards = 905 to 974 TFLOP/s (e4m3 555 to 575); the matrix pipe is busy 44 % of the
+// time, the vector pipe 58 % (128 instructions a step and wavefront make the weights, 32
+// of them exponentials of four times the others' time), LDS 38 %.  Of 602 us the operands'
+// reads from LDS cost 85, codes and their conversion 65, exponentials 30.  Before: 1193 us in
+// ktir_kv8_rows.hip, 906 with four wavefronts of 64 rows, 677 without the next scores beside,
+// 630 side by side (634 on the card of 592 now); not faster: matrix instructions pinned
+// between vector ones, seven to one (660 to 700), operands read six products ahead (604).
 //
 // One f16 term: w is at most 2^15 and normal down to 2^-14, so a key keeps 11 bits
 // (the result's own, in f16) unless the row's heaviest one outweighs it 2^25 to 2^29
@@ -41,7 +46,9 @@ template <int CODE, int J, int RB, int W>
 __global__ __launch_bounds__(64 * W, W / 4) void kv8_attn_tile(const ktir_kv8_attn_t d, uint32_t slots, int* err) {
   constexpr int TM = 32 * RB * W, DP = 64 * J, NT = 64 * W;
   constexpr int KU = TILE_KEYS * 4 * J, VU = 16 * 16 * J, KP = (KU + NT - 1) / NT, VP = (VU + NT - 1) / NT;   // units of a step, a thread's
+  constexpr bool TURNS = J == 2;                 // the two wavefronts of a SIMD take turns
   static_assert(J == 1 || J == 2 || J == 4, "columns in 64s");
+  static_assert(!TURNS || W == 8, "two wavefronts of a SIMD: i and i + 4");
   __shared__ __attribute__((aligned(16))) uint16_t ks[2][TILE_KEYS * DP], vs[2][DP * TILE_KEYS];
   const ktir_kv8_t& c = d.cache;
   const int tid = threadIdx.x, l = tid & 63, wave = uni(tid >> 6), h = l >> 5, r32 = l & 31;
@@ -55,7 +62,8 @@ __global__ __launch_bounds__(64 * W, W / 4) void kv8_attn_tile(const ktir_kv8_at
 
   // this lane's rows; the wavefront's bounds of keys
   const int w0 = t.row0 + wave * 32 * RB, wn = t.rows - wave * 32 * RB < 32 * RB ? t.rows - wave * 32 * RB : 32 * RB;
-  int see_lo[RB], see_hi[RB], lo_most = 0, hi_least = 0, other;
+  int see_lo[RB], lo_most = 0, hi_least = 0, other;
+  uint32_t see[RB];                                  // how many keys a row sees, from see_lo on
   uint4 qf[RB][4 * J];
   float rs[RB];
   const bool whole = !((d.q.ptr | (uint64_t)d.q.tok * 2 | (uint64_t)d.q.head * 2) & 15);
@@ -63,7 +71,9 @@ __global__ __launch_bounds__(64 * W, W / 4) void kv8_attn_tile(const ktir_kv8_at
   for (int b = 0; b < RB; ++b) {
     int r = w0 + 32 * b + r32;
     if (r >= t.row0 + t.rows) r = t.row0 + t.rows - 1;            // a row that is not stored
-    seen(d, t, r, grp, &see_lo[b], &see_hi[b]);
+    int see_hi;
+    seen(d, t, r, grp, &see_lo[b], &see_hi);
+    see[b] = see_hi > see_lo[b] ? see_hi - see_lo[b] : 0;
     const int64_t e = (t.q.start + r / grp) * d.q.tok + (head * grp + r % grp) * d.q.head;
     uint32_t raw[4 * J][4], top = 0;
 #pragma unroll
@@ -115,10 +125,10 @@ __global__ __launch_bounds__(64 * W, W / 4) void kv8_attn_tile(const ktir_kv8_at
 
   // a thread's share of a step: units of 16 codes of a key, and of 4 columns of 4 keys of V
   const int steps = t.hi > from ? (t.hi - from + TILE_KEYS - 1) / TILE_KEYS : 0;
-  // the groups of the 16 steps that the computed one is of, of those that keys are fetched of (three steps on), and the next
+  // the groups of the 16 steps that the computed one is of, of those that keys are fetched of (four steps on), and the next
   KV8Groups cur = {0, 0.f, 0.f, L_UNIT}, g = cur, next = cur;
-  u32x4_t kraw[KP];
-  uint32_t vraw[VP][4];
+  u32x4_t k_raw[2][KP];                               // of even and odd steps
+  uint32_t v_raw[2][VP][4];
   auto page_of = [&](int pages, int j, int group) { return (int64_t)__builtin_amdgcn_readlane(pages, 4 * (j & 15) + (group & 3)); };
   // key of a K unit, first key of a V unit: one group of 16 a wavefront
   auto k_key = [&](int p) { return (tid + NT * p) / (4 * J); };
@@ -127,31 +137,32 @@ __global__ __launch_bounds__(64 * W, W / 4) void kv8_attn_tile(const ktir_kv8_at
   const int v_half = tid >> 3 & 1;
   auto v_col = [&](int p) { return ((tid & 7) + 8 * ((tid + NT * p) / 16 % (2 * J))) * 4; };
   auto v_key = [&](int p) { return 16 * (v_chunk(p) >> 1) + 4 * (v_chunk(p) & 1) + 8 * v_half; };
-  auto fetch_k = [&](int j) {
+  auto fetch_k = [&](int j, u32x4_t (&kraw)[KP]) {
     const int key = from + TILE_KEYS * j;
 #pragma unroll
     for (int p = 0; p < KP; ++p) {
       // (columns behind D: the first ones again, times zeros in Q)
       const int r = k_key(p), at = (tid + NT * p) % (4 * J) * 16, col = at < D ? at : 0;
-      const int64_t page = page_of(g.page, j, uni(r >> 4)), row = (key + r) & (c.page - 1);
-      if (KU % NT == 0 || tid < KU) kraw[p] = *(const KTIR_G(u32x4_t)*)(c.k + page * c.k_page + row * c.k_tok + head * c.k_head + col);
+      const uint64_t page = c.k + page_of(g.page, j, uni(r >> 4)) * c.k_page + head * c.k_head;
+      const uint32_t at32 = (uint32_t)((key + r) & (int)(c.page - 1)) * (uint32_t)c.k_tok + col;    // (tokens of a page lie 2^22 bytes apart at most)
+      if (KU % NT == 0 || tid < KU) kraw[p] = *(const KTIR_G(u32x4_t)*)((const KTIR_G(char)*)page + at32);
     }
   };
-  auto fetch_v = [&](int j, int pages) {
+  auto fetch_v = [&](int j, int pages, uint32_t (&vraw)[VP][4]) {
     const int key = from + TILE_KEYS * j;
 #pragma unroll
     for (int p = 0; p < VP; ++p) {
       // (columns behind D: the first ones again, not stored)
       const int first = v_key(p), x = v_col(p), col = x < D ? x : 0;
-      const int64_t page = page_of(pages, j, uni(first >> 4)), row = (key + first) & (c.page - 1);
+      const uint64_t page = c.v + page_of(pages, j, uni(first >> 4)) * c.v_page + head * c.v_head;
+      const uint32_t at32 = (uint32_t)((key + first) & (int)(c.page - 1)) * (uint32_t)c.v_tok + col;
       if (VU % NT == 0 || tid < VU) {
-        const uint64_t at = c.v + page * c.v_page + row * c.v_tok + head * c.v_head + col;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) vraw[p][i] = *(const KTIR_G(uint32_t)*)(at + i * c.v_tok);
+        for (int i = 0; i < 4; ++i) vraw[p][i] = *(const KTIR_G(uint32_t)*)((const KTIR_G(char)*)(page + i * c.v_tok) + at32);
       }
     }
   };
-  auto put_k = [&](int buf) {
+  auto put_k = [&](int buf, const u32x4_t (&kraw)[KP]) {
     uint16_t* kb = ks[buf];
 #pragma unroll
     for (int p = 0; p < KP; ++p) {
@@ -161,7 +172,7 @@ __global__ __launch_bounds__(64 * W, W / 4) void kv8_attn_tile(const ktir_kv8_at
       *(uint4*)(kb + r * DP + 8 * k_slot(r, chunk + 1)) = row_half8<CODE>(kraw[p].z, kraw[p].w);
     }
   };
-  auto put_v = [&](int j, int buf) {
+  auto put_v = [&](int j, int buf, uint32_t (&vraw)[VP][4]) {
     uint16_t* vb = vs[buf];
 #pragma unroll
     for (int p = 0; p < VP; ++p) {
@@ -207,14 +218,16 @@ __global__ __launch_bounds__(64 * W, W / 4) void kv8_attn_tile(const ktir_kv8_at
     g = kv8_groups(d, head, kv8_pages(d, t, from + 16 * l, t.hi, shift), there, err);
     kv8_scales(g, there);
     cur = g;
-    fetch_k(0);
-    fetch_v(0, g.page);
-    put_k(0);
-    put_v(0, 0);
-    fetch_k(1);                        // (steps past the last: page 0)
-    put_k(1);
-    fetch_v(1, g.page);
-    fetch_k(2);
+    fetch_k(0, k_raw[0]);
+    fetch_v(0, g.page, v_raw[0]);
+    fetch_k(1, k_raw[1]);              // (steps past the last: page 0)
+    fetch_v(1, g.page, v_raw[1]);
+    put_k(0, k_raw[0]);
+    put_v(0, 0, v_raw[0]);
+    put_k(1, k_raw[1]);
+    fetch_k(2, k_raw[0]);
+    fetch_v(2, g.page, v_raw[0]);
+    fetch_k(3, k_raw[1]);
     __syncthreads();
     scores(s0, 0, 0, 4 * J);
     __syncthreads();
@@ -225,10 +238,10 @@ __global__ __launch_bounds__(64 * W, W / 4) void kv8_attn_tile(const ktir_kv8_at
   auto step = [&](int j, auto parity, f32x16_t (&s)[RB][2], f32x16_t (&s_next)[RB][2]) {
     constexpr int PAR = decltype(parity)::value;
     // the next 16 steps' groups: their pages four steps ahead of the first fetch, then the scales
-    const int f = j + 3, key = from + TILE_KEYS * j;
+    const int f = j + 4, key = from + TILE_KEYS * j;
     if ((f & 15) == 12) next.page = kv8_pages(d, t, from + TILE_KEYS * (f + 4) + 16 * l, t.hi, shift);
     if ((f & 15) == 14) next = kv8_groups(d, head, next.page, from + TILE_KEYS * (f + 2) + 16 * l < t.hi, err);
-    const int vpages = (f & 15) == 0 ? cur.page : g.page;          // of step j + 2, in the 16 before g's next ones then
+    const int vpages = (f & 15) == 0 ? cur.page : g.page;          // of step j + 3, in the 16 before g's next ones then
     if ((f & 15) == 0) {
       g = next;
       kv8_scales(g, from + TILE_KEYS * f + 16 * l < t.hi);
@@ -246,17 +259,21 @@ __global__ __launch_bounds__(64 * W, W / 4) void kv8_attn_tile(const ktir_kv8_at
     const bool cut = key < lo_most || key + TILE_KEYS > hi_least;
 #pragma unroll
     for (int b = 0; b < RB; ++b) {
-      auto hidden = [&](int k, int i) {
-        const int at = key + 32 * k + 8 * (i >> 2) + 4 * h + (i & 3);
-        return at < see_lo[b] || at >= see_hi[b];
+      // (made anew in each of the two rare parts: kept, the 32 places take as many registers)
+      auto places = [&]() {
+        int first = key + 4 * h - see_lo[b];
+        asm volatile("" : "+v"(first));
+        return first;
       };
+      auto hidden = [&](int first, int k, int i) { return (uint32_t)(first + 32 * k + 8 * (i >> 2) + (i & 3)) >= see[b]; };
       if (__any(base[b] == B_NONE)) {              // rows that have seen no key: b from this step's, their sums are 0
         float top = -__builtin_inff();
+        const int first = places();
 #pragma unroll
         for (int k = 0; k < 2; ++k)
 #pragma unroll
           for (int i = 0; i < 16; ++i)
-            top = __builtin_fmaxf(top, mask_ninf(__builtin_fmaf(s[b][k][i], gks[2 * k + (i >> 3)] * rs[b], glv[2 * k + (i >> 3)]), hidden(k, i)));
+            top = __builtin_fmaxf(top, mask_ninf(__builtin_fmaf(s[b][k][i], gks[2 * k + (i >> 3)] * rs[b], glv[2 * k + (i >> 3)]), hidden(first, k, i)));
         top = __builtin_fmaxf(top, other_half(top));
         base[b] = base[b] == B_NONE && top > -__builtin_inff() ? top - TILE_TOP : base[b];
       }
@@ -265,10 +282,11 @@ __global__ __launch_bounds__(64 * W, W / 4) void kv8_attn_tile(const ktir_kv8_at
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[b][k][i] = __builtin_fmaf(s[b][k][i], gks[2 * k + (i >> 3)] * rs[b], glv[2 * k + (i >> 3)] - base[b]);
       if (cut) {
+        const int first = places();
 #pragma unroll
         for (int k = 0; k < 2; ++k)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) s[b][k][i] = mask_ninf(s[b][k][i], hidden(k, i));
+          for (int i = 0; i < 16; ++i) s[b][k][i] = mask_ninf(s[b][k][i], hidden(first, k, i));
       }
     }
     float top[RB], most = -__builtin_inff();
@@ -294,49 +312,75 @@ __global__ __launch_bounds__(64 * W, W / 4) void kv8_attn_tile(const ktir_kv8_at
           for (int i = 0; i < 16; ++i) s[b][k][i] -= by;
       }
     }
-    // the codes of steps j + 2 (K) and j + 1 (V) into LDS, those of j + 3 and j + 2 on their way, the scores of j + 1:
+    // the codes of steps j + 2 (K) and j + 1 (V) into LDS, those of the next two steps on their way, the scores of j + 1,
     // beside W V of step j.  (Past the last step: of page 0, unused.)
     const uint16_t* vb = vs[PAR];
-    uint4 w[RB], old[RB];
+    auto move = [&](int p) {
+      if (p == 0) put_k(PAR, k_raw[PAR]);
+      if (p == 1) put_v(j + 1, 1 - PAR, v_raw[1 - PAR]);
+      if (p == 2) fetch_k(j + 4, k_raw[PAR]);
+      if (p == 3) fetch_v(j + 3, vpages, v_raw[1 - PAR]);
+    };
+    auto weights = [&](int p, uint4 (&w)[RB]) {
 #pragma unroll
-    for (int p = 0; p < 5; ++p) {
-      if (J == 4 || p == 0 || p == 2 || p == 4) __builtin_amdgcn_sched_barrier(0);
-      if (p == 0) put_k(PAR);
-      if (p == 1) put_v(j + 1, 1 - PAR);
-      if (p == 2) fetch_k(j + 3);
-      if (p == 3) fetch_v(j + 2, vpages);
-      if (p < 4) scores(s_next, 1 - PAR, p * J, J);
-      if (p < 4) {
+      for (int b = 0; b < RB; ++b) {
+        float e[8];
 #pragma unroll
-        for (int b = 0; b < RB; ++b) {
-          float e[8];
-          old[b] = w[b];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            e[i] = __builtin_amdgcn_exp2f(s[b][p >> 1][8 * (p & 1) + i]);
-            sum[b] = __builtin_fmaf(e[i], giv[p], sum[b]);
-          }
-          w[b] = make_uint4(cvt2<false>(e[0], e[1]), cvt2<false>(e[2], e[3]), cvt2<false>(e[4], e[5]), cvt2<false>(e[6], e[7]));
+        for (int i = 0; i < 8; ++i) {
+          e[i] = __builtin_amdgcn_exp2f(s[b][p >> 1][8 * (p & 1) + i]);
+          sum[b] = __builtin_fmaf(e[i], giv[p], sum[b]);
         }
-      } else {
+        w[b] = make_uint4(cvt2<false>(e[0], e[1]), cvt2<false>(e[2], e[3]), cvt2<false>(e[4], e[5]), cvt2<false>(e[6], e[7]));
+      }
+    };
+    auto weigh = [&](int p, const uint4 (&w)[RB]) {
+#pragma unroll
+      for (int n = 0; n < 2 * J; ++n) {
+        const uint4 a = *(const uint4*)(vb + (32 * n + r32) * TILE_KEYS + 8 * v_slot(32 * n + r32, 2 * p + h));
+#pragma unroll
+        for (int b = 0; b < RB; ++b) acc[b][n] = mfma_at<false>(a, w[b], acc[b][n]);
+      }
+    };
+    if constexpr (TURNS) {
+      uint4 w[4][RB];
+#pragma unroll
+      for (int p = 0; p < 4; ++p) weights(p, w[p]);
+      __builtin_amdgcn_sched_barrier(0);
+      __syncthreads();
+      __builtin_amdgcn_sched_barrier(0);
+      __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+      for (int p = 0; p < 4; ++p) {
+        move(p);
+        scores(s_next, 1 - PAR, p * J, J);
+        weigh(p, w[p]);
+      }
+      __builtin_amdgcn_s_setprio(0);
+      __builtin_amdgcn_sched_barrier(0);
+    } else {
+      uint4 w[RB], old[RB];
+#pragma unroll
+      for (int p = 0; p < 5; ++p) {
+        if (J == 4 || p == 0 || p == 2 || p == 4) __builtin_amdgcn_sched_barrier(0);
+        move(p);
+        if (p < 4) scores(s_next, 1 - PAR, p * J, J);
 #pragma unroll
         for (int b = 0; b < RB; ++b) old[b] = w[b];
-      }
-      if (p > 0) {
-#pragma unroll
-        for (int n = 0; n < 2 * J; ++n) {
-          const uint4 a = *(const uint4*)(vb + (32 * n + r32) * TILE_KEYS + 8 * v_slot(32 * n + r32, 2 * (p - 1) + h));
-#pragma unroll
-          for (int b = 0; b < RB; ++b) acc[b][n] = mfma_at<false>(a, old[b], acc[b][n]);
-        }
+        if (p < 4) weights(p, w);
+        if (p > 0) weigh(p - 1, old);
       }
     }
     __syncthreads();
   };
+  // In turns the later half of the wavefronts, one of each SIMD, is a barrier behind the others, which reach as many in the
+  // end.  A buffer is last read in a half that precedes the first in which any wavefront writes it again, and is whole a
+  // half before it is read.
+  if (TURNS && wave >= W / 2) __syncthreads();
   for (int j = 0; j < steps; j += 2) {
-    step(j, std::integral_constant<int, 0>(), s0, s1);
-    if (j + 1 < steps) step(j + 1, std::integral_constant<int, 1>(), s1, s0);
+    step(j, std::integral_constant<int, 0>(), s0, TURNS ? s0 : s1);
+    if (j + 1 < steps) step(j + 1, std::integral_constant<int, 1>(), TURNS ? s0 : s1, s0);
   }
+  if (TURNS && wave < W / 2) __syncthreads();
 
   // O^T: a lane has columns 32 n + 8 g + 4 h + 0..3 of its row
   const bool packed = !((d.out.ptr | (uint64_t)d.out.tok * 2 | (uint64_t)d.out.head * 2) & 7);
@@ -345,7 +389,7 @@ __global__ __launch_bounds__(64 * W, W / 4) void kv8_attn_tile(const ktir_kv8_at
     const int r = w0 + 32 * b + r32;
     sum[b] += other_half(sum[b]);
     if (r >= t.row0 + t.rows) continue;
-    const bool none = see_lo[b] >= see_hi[b];
+    const bool none = !see[b];
     const float inv = none ? 0.f : L_UNIT / sum[b];
     const int64_t tok = t.q.start + r / grp, hq = head * grp + r % grp, e = tok * d.out.tok + hq * d.out.head;
 #pragma unroll
@@ -383,8 +427,8 @@ static void tile_go(const ktir_kv8_attn_t& d, int64_t slots, hipStream_t st) {
 
 // Whether a launch takes this kernel, and its tiles of rows for each KV head.  With fewer
 // than 128 workgroups the kernel of few rows, which spreads the keys as well, is faster:
-// 512 tokens after 3584 (72 tiles) 89 us there and 149 here, 1024 after 3072 (136) 154
-// and 152, 2048 alone (264) 124 and 87, 16 sequences of 64 after 1984 (128) 105 and 88.
+// the last 512 of 4096 tokens (72 tiles) 89 us there and 149 here, the last 1024 (136)
+// 154 and 152, 2048 alone (264) 124 and 87, 16 sequences of 64 after 1984 (128) 105 and 88.
 bool kv8_tile_takes(const ktir_kv8_attn_t& d, int64_t* slots) {
   const int64_t grp = d.q_heads / d.cache.heads, TM = d.cache.columns <= 128 ? 256 : 128;
   if (d.max_q * grp <= TM / 2) return false;
