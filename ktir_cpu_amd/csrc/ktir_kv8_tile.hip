@@ -427,8 +427,10 @@ static void tile_go(const ktir_kv8_attn_t& d, int64_t slots, hipStream_t st) {
 
 // Whether a launch takes this kernel, and its tiles of rows for each KV head.  With fewer
 // than 128 workgroups the kernel of few rows, which spreads the keys as well, is faster:
-// the last 512 of 4096 tokens (72 tiles) 89 us there and 149 here, the last 1024 (136)
-// 154 and 152, 2048 alone (264) 124 and 87, 16 sequences of 64 after 1984 (128) 105 and 88.
+// the last 512 of 4096 tokens (72 tiles) 86 us there and 123 here, the last 700 (88) 121 and
+// 123, the last 1024 (136) 151 and 125, 2048 alone (264) 124 and 75, 16 sequences of 64
+// after 1984 (128) 103 and 75.  So it is where no tile is more than half full: 16 sequences of 20
+// (80 rows of 256) 52 and 73.
 bool kv8_tile_takes(const ktir_kv8_attn_t& d, int64_t* slots) {
   const int64_t grp = d.q_heads / d.cache.heads, TM = d.cache.columns <= 128 ? 256 : 128;
   if (d.max_q * grp <= TM / 2) return false;
