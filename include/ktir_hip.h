@@ -555,10 +555,11 @@ typedef struct ktir_kv8_batch {
  *            tokens of the sequence lie in the page, where that is more
  *   code   = rint(x * (1 / scale')) or the nearest e4m3 value, within +- top
  * and where scale' is more than the scale before, the older tokens' codes are
- * rounded again: code * (scale before * (1 / scale')).  Every operation is one in f32.  A page that receives a
- * value that is not finite reads as NaN from then on (scale' = NaN, new codes 0).
+ * rounded again: code * (scale before * (1 / scale')).  Every operation is one in f32.
+ * A page that receives a value that is not finite reads as NaN from then on
+ * (scale' = NaN, new codes 0).
  * Tokens at negative positions are not stored.  A page that two sequences of a
- * call both write keeps the codes and the scale of either.
+ * call, or two places of one's table, both write keeps the codes and the scale of either.
  * k, v: [tokens, heads, columns], KTIR_F16 or KTIR_BF16. */
 typedef struct ktir_kv8_append {
   ktir_kv8_t cache;
@@ -577,8 +578,8 @@ int ktir_launch_kv8_append(const ktir_kv8_append_t* d);
  *   out = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m),  lse = m + ln sum_j exp(s_j - m)
  * A row that no token is left for gets 0 and -inf; padding rows are left as
  * they were.  Products of q and codes are exact, sums f32, probabilities enter
- * the second product as ktir_kv8_rows.hip and ktir_kv8_tile.hip say; the result is rounded once to dtype
- * (KTIR_F16 or KTIR_BF16, of q and out).  Codes of tokens past kv_len are not
+ * the second product as ktir_kv8_rows.hip and ktir_kv8_tile.hip say; the result is
+ * rounded once to dtype (KTIR_F16 or KTIR_BF16, of q and out).  Codes of tokens past kv_len are not
  * looked at; an e4m3 NaN code of a value makes the rows of its sequence NaN.
  * max_q and max_k (2^30 at most) bound the new and the cached tokens of every
  * sequence: what a sequence has beyond is left out, with the device error word set.

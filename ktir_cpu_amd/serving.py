@@ -23,7 +23,9 @@ stream, so it is ordered with the torch operations around it and can be captured
 into a graph; a launch on other arrays goes to the library's stream, as all else
 here.  Nothing waits: ``runtime.sync()`` waits for the library's stream, and
 reports lengths and tables that were out of range (IndexError) whatever stream
-found them, once that stream is done.  One handle is run by one thread at a time.
+found them, once that stream is done.  One handle is run by one thread at a time,
+and its runs do not overlap on the device; it and its arrays live until the last of
+them, or the last replay of a graph that holds one, is done.
 """
 
 from __future__ import annotations
@@ -137,6 +139,7 @@ class _Launch:
         self._keep = keep               # what the descriptor's addresses belong to
         self._ref = C.byref(desc)
         self._call = None
+        self._own, self._streams = None, None       # own workspace; where it is a torch tensor, the streams that it was used on
         devices = {v.device for v in views if v.device is not None}
         if len(devices) > 1:
             raise ValueError(f"{self.entry}: tensors on devices {sorted(devices)}")
@@ -165,6 +168,17 @@ class _Launch:
         rc = self._call(self._ref)
         if rc:
             rt.check(rc)
+        if self._streams is not None and self.desc.stream not in self._streams:
+            self._used_on(stream)
+
+    def _used_on(self, stream):
+        """The own workspace came from torch: it goes to no other tensor before this stream is done with it."""
+        torch = sys.modules["torch"]
+        if torch.cuda.is_current_stream_capturing():
+            return                                  # (a replay's stream is not known here)
+        if stream is None or hasattr(stream, "cuda_stream"):
+            self._own.record_stream(torch.cuda.current_stream(self._torch_device) if stream is None else stream)
+        self._streams.add(self.desc.stream)
 
 
 # ---- rotary positions --------------------------------------------------------
@@ -259,7 +273,7 @@ class KV8Cache:
     """A paged key / value cache in 8 bits.
 
     `k`, `v` [pages, page, heads, columns] int8 or float8 (e4m3) codes, `k_scale`,
-    `v_scale` [pages, heads] float32: a code stands for code * scale.  The page
+    `v_scale` [pages, heads] float32, not negative: a code stands for code * scale.  The page
     is a power of two from 16 to 256 tokens, columns a multiple of 16 up to 256.
     Neither needs initial values: a page's scale counts once tokens are in it.
     """
@@ -293,6 +307,7 @@ class KV8Append(_Launch):
     Sequence s brings the tokens q_start[s] .. q_start[s + 1], the last of its
     kv_len[s] (int32, all on the device, read when the launch runs); its token t
     lies in page table[s, t // page].  Tokens outside every sequence pad the batch.
+    No page is written for two places of the batch's tables at once.
     """
 
     entry = "ktir_launch_kv8_append"
@@ -355,6 +370,7 @@ class KV8Attention(_Launch):
                 torch = sys.modules["torch"]
                 self._own = torch.empty(self.workspace_bytes, dtype=torch.uint8, device=f"cuda:{self._torch_device}")
                 d.ws = self._own.data_ptr()
+                self._streams = {torch.cuda.current_stream(self._torch_device).cuda_stream or _NULL_STREAM}
             else:
                 self._own = rt.DeviceBuffer(self.workspace_bytes)
                 d.ws = self._own.ptr

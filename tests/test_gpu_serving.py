@@ -344,6 +344,31 @@ def test_attention_into_the_queries(serving, lens, hk, grp):
     S.close(q[:, heads], want[:, heads], bound[:, heads], "bf16")
 
 
+def test_own_workspace_is_held_for_every_stream(serving):
+    b = S.Batch([(1, 5000), (1, 70)], hk=2, grp=4, D=64, dt="bf16")
+    q = b.q.cuda()
+    op = serving.KV8Attention(serving.KV8Cache(*dev(*b.cache())), q, torch.empty_like(q), *dev(*b.where()), **b.most)
+    assert op.workspace_bytes > 0 and op._own.data_ptr() == op.desc.ws
+    keep, held = op._own, []
+
+    class Own:
+        def record_stream(self, stream):
+            held.append(stream.cuda_stream)
+
+    op._own = Own()
+    op.run()
+    side, other = torch.cuda.Stream(), torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    op.run(side)
+    op.run(side)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(other):
+        op.run()
+    torch.cuda.synchronize()
+    assert held == [side.cuda_stream, other.cuda_stream]
+    del keep
+
+
 def test_attention_not_causal(serving):
     b = S.Batch([(5, 40), (70, 33), (2, 0)], hk=2, grp=3, D=96, page=32)
     check(b, *attend(serving, b, causal=False, scale=0.3), causal=False, scale=0.3)
