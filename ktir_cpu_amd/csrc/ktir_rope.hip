@@ -4,9 +4,9 @@
 // Bound: bytes, in and out once.  The angles of a token are made once for all its
 // heads (64-bit remainder, one sine and cosine: about 60 instructions), in LDS, and
 // every vector of 16 bytes is loaded and stored once, two rows of loads ahead.
-// Measured, f16 / bf16: 8192 tokens of 32 + 8 heads of 128, 168 MB, 37.9 us = 4.4 TB/s
+// Measured, f16 / bf16: 8192 tokens of 32 + 8 heads of 128, 168 MB, 31.6 us = 5.3 TB/s
 // (a copy of 256 MiB makes 5.4 here); 40 + 40 heads with 64 interleaved columns of
-// 128, 168 MB, 39.4 us, 55.8 with the columns behind rot as units of their own size;
+// 128, 168 MB, 36.2 us, 55.8 (of 39.4) with the columns behind rot as units of their own size;
 // one thread per pair over all heads took 97 and 212 us.  One token: a launch, 4.1 us.
 #include "ktir_serve.h"
 
@@ -39,7 +39,7 @@ struct RopeRaw {
   uint32_t w[2][DT == KTIR_F32 ? V : (V + 1) / 2];
 };
 
-template <int DT, int V>
+template <int DT, int V, bool PAST>
 __device__ __forceinline__ void rope_load(uint64_t ptr, int64_t a, int64_t b, RopeRaw<DT, V>& r) {
   const int64_t e[2] = {a, b};
 #pragma unroll
@@ -48,7 +48,8 @@ __device__ __forceinline__ void rope_load(uint64_t ptr, int64_t a, int64_t b, Ro
       if constexpr (DT == KTIR_F32) r.w[i][0] = ((const KTIR_G(uint32_t)*)ptr)[e[i]];
       else r.w[i][0] = ((const KTIR_G(uint16_t)*)ptr)[e[i]];
     } else {
-      const u4_t x = *(const KTIR_G(u4_t)*)(ptr + e[i] * (DT == KTIR_F32 ? 4 : 2));
+      const KTIR_G(u4_t)* p = (const KTIR_G(u4_t)*)(ptr + e[i] * (DT == KTIR_F32 ? 4 : 2));
+      const u4_t x = PAST ? __builtin_nontemporal_load(p) : *p;
 #pragma unroll
       for (int k = 0; k < 4; ++k) r.w[i][k] = x[k];
     }
@@ -138,7 +139,7 @@ __device__ __forceinline__ void rope_columns(int u, int pairs, int half, int rot
 // A workgroup has `per` tokens and, with several in y, a part of the heads.  Its
 // threads first make the angles of the tokens together, then each takes one unit of
 // columns over rows (token, head), R rows' loads ahead of the first's stores.
-template <int DT, bool INTER, int V, int R>
+template <int DT, bool INTER, int V, int R, bool PAST>
 __global__ __launch_bounds__(256) void rope_turn(const ktir_rope_t d, int per) {
   __shared__ __attribute__((aligned(16))) float cs[ROPE_PAIRS], sn[ROPE_PAIRS];
   __shared__ int live[ROPE_TOKENS];
@@ -183,7 +184,7 @@ __global__ __launch_bounds__(256) void rope_turn(const ktir_rope_t d, int per) {
         at[k] = t * half + u * V;
         if (ptr[k]) {
           const int64_t e = (t0 + t) * in.tok + hh * in.head;
-          rope_load<DT, V>(in.ptr, e + a, e + b, r[k]);
+          rope_load<DT, V, PAST>(in.ptr, e + a, e + b, r[k]);
         }
         row += stride;
         h += stride;
@@ -232,8 +233,21 @@ static void rope_go(const ktir_rope_t& d, hipStream_t st) {
     y = y > most ? most : y;
   }
   const dim3 grid((unsigned)blocks, (unsigned)y);
-  if (d.interleaved) hipLaunchKernelGGL((rope_turn<DT, true, V, R>), grid, dim3(256), 0, st, d, (int)per);
-  else hipLaunchKernelGGL((rope_turn<DT, false, V, R>), grid, dim3(256), 0, st, d, (int)per);
+  // Inputs and outputs past 64 MB, twice what the L2s hold: the inputs, which are done with, are read
+  // past the caches and leave them to the outputs.  Turned, appended and attended to by 32 / 8 heads of 128:
+  // 8192 tokens (168 MB) 53.2 -> 49.5 us and 611 -> 610 with attention, 5120 35.3 -> 31.3 and 290.8 -> 289.0,
+  // 3584 (73 MB) 24.1 -> 23.8 and 149.9 -> 148.5, but 2048 (42 MB) 16.1 -> 17.9 and 83.1 -> 84.9.  Outputs stored
+  // past the caches make the turn as fast, but attention then reads them from HBM: 615.7 with 8192 tokens.
+  // In place the lines are written again at once: 4096 tokens 15.8 as they are, 19.0 past the caches.
+  constexpr bool WIDE = V > 1;
+  const bool past = WIDE && d.in.ptr != d.out.ptr && (!d.heads2 || d.in2.ptr != d.out2.ptr) && 2 * d.tokens * heads * d.columns * (DT == KTIR_F32 ? 4 : 2) > (int64_t)64 << 20;
+  if (d.interleaved) {
+    if (past) hipLaunchKernelGGL((rope_turn<DT, true, V, R, WIDE>), grid, dim3(256), 0, st, d, (int)per);
+    else hipLaunchKernelGGL((rope_turn<DT, true, V, R, false>), grid, dim3(256), 0, st, d, (int)per);
+  } else {
+    if (past) hipLaunchKernelGGL((rope_turn<DT, false, V, R, WIDE>), grid, dim3(256), 0, st, d, (int)per);
+    else hipLaunchKernelGGL((rope_turn<DT, false, V, R, false>), grid, dim3(256), 0, st, d, (int)per);
+  }
 }
 
 static int check_tensors(const ktir_rope_t& d) {

@@ -110,6 +110,28 @@ def test_rope_long(serving, tokens, heads, D, rot, dt, inter):
     S.close(out, want, bound, dt)
 
 
+@pytest.mark.parametrize("tokens,heads,kheads,D,rot,dt,inter", [(3501, 32, 8, 128, 96, "bf16", False), (2051, 13, 3, 260, 256, "f32", True)])
+def test_rope_larger_than_the_caches(serving, tokens, heads, kheads, D, rot, dt, inter):
+    g = torch.Generator().manual_seed(D)
+    qkv = torch.randn((tokens, heads + kheads + 1, D), generator=g).to(S.DT[dt])
+    assert 2 * tokens * (heads + kheads) * D * qkv.element_size() > 64 << 20
+    pos = torch.randint(-3, 1 << 17, (tokens,), generator=g)
+    freq, _ = serving.rope_frequencies(rot)
+    d = qkv.cuda()
+    out, k_out = torch.full((tokens, heads, D), 5.0).to(S.DT[dt]).cuda(), torch.full((tokens, kheads, D), 5.0).to(S.DT[dt]).cuda()
+    op = serving.Rope(d[:, :heads], pos.cuda(), torch.from_numpy(freq).cuda(), out, k=d[:, heads:heads + kheads], k_out=k_out,
+                      interleaved=inter)
+    for _ in range(2):                               # the second on values written by the stream just before
+        op.run()
+        sync()
+        want, bound = S.rope(qkv[:, :heads + kheads], pos, freq, interleaved=inter)
+        want[pos < 0] = 5.0
+        S.close(out, want[:, :heads], bound[:, :heads], dt)
+        S.close(k_out, want[:, heads:], bound[:, heads:], dt)
+        qkv = qkv.flip(0).contiguous()
+        d.copy_(qkv)
+
+
 # ---- append ----------------------------------------------------------------------
 
 LENS = {
