@@ -6,7 +6,7 @@
 // LDS (two buffers): K as [key][column], V as [column][key], with the keys of each 16 in
 // the order that the scores' layout leaves them in:
 //   S^T = K Q^T     32 x 32 x 16 MFMA, one row a lane (the two halves share it)
-//   w, b, l         as ktir_kv8_dev.h says; w enters the product as one f16 term
+//   w, b, l         as ktir_kv8_dev.h says; w enters the product as two f16 terms
 //   O^T += V^T W^T  no exchange between lanes
 // With 65 to 128 columns the two wavefronts of a SIMD take turns, half a step apart: one
 // makes the weights of its step (vector instructions alone), the other multiplies (the
@@ -15,18 +15,20 @@
 // a quarter of each at a time: 64 columns 398 us so and 422 in turns, below.  A wavefront
 // alone on its SIMD (more than 128 columns) has no one to take turns with.
 //
-// Bound: issue.  8192 tokens, 32 / 8 heads of 128 columns, causal, i8 codes, 550 GFLOP:
-// 564 to 607 us on four cards = 905 to 974 TFLOP/s (e4m3 555 to 575); the matrix pipe is busy 44 % of the
-// time, the vector pipe 58 % (128 instructions a step and wavefront make the weights, 32
-// of them exponentials of four times the others' time), LDS 38 %.  Of 602 us the operands'
-// reads from LDS cost 85, codes and their conversion 65, exponentials 30.  Before: 1193 us in
-// ktir_kv8_rows.hip, 906 with four wavefronts of 64 rows, 677 without the next scores beside,
-// 630 side by side (634 on the card of 592 now); not faster: matrix instructions pinned
-// between vector ones, seven to one (660 to 700), operands read six products ahead (604).
+// Bound: the instructions of a wavefront one after another, vector and matrix ones.  8192
+// tokens, 32 / 8 heads of 128 columns, causal, i8 codes, 550 GFLOP and half as many for the
+// second terms: 778 to 818 us on two cards (e4m3 747 to 781); 64 columns 525, 16 / 4 heads of 256 1087.
+// With one term of w 628 to 634, 598 to 605, 410 and 963 on the second of the cards: there the matrix pipe is
+// busy 44 % of the time, the vector pipe 58 %, LDS 38 %, so that the two wavefronts of a SIMD hardly
+// cover each other.
+// Before, with one term: 1193 us in ktir_kv8_rows.hip, 906 with four wavefronts of 64 rows, 677 without the
+// next scores beside, 630 side by side (634 on a card that takes 592 in turns); not faster: matrix instructions pinned
+// between vector ones, seven to one (660 to 700), operands read six products ahead (604).  With two
+// terms side by side takes 905 (e4m3 797), where turns take 778 (747).
 //
-// One f16 term: w is at most 2^15 and normal down to 2^-14, so a key keeps 11 bits
-// (the result's own, in f16) unless the row's heaviest one outweighs it 2^25 to 2^29
-// times; less is added with the step of 2^-24, which is 2^-35 to 2^-39 of the heaviest.
+// Two f16 terms, the weight rounded and what that leaves of it rounded again: w is at most 2^15, so
+// down to 2^-3 a weight keeps 22 bits, and below that what is left is held in steps of
+// 2^-24, which is 2^-35 to 2^-39 of the row's heaviest.  One term keeps 11 bits, which f16 results show.
 #include <type_traits>
 
 #include "ktir_kv8_dev.h"
@@ -321,28 +323,39 @@ __global__ __launch_bounds__(64 * W, W / 4) void kv8_attn_tile(const ktir_kv8_at
       if (p == 2) fetch_k(j + 4, k_raw[PAR]);
       if (p == 3) fetch_v(j + 3, vpages, v_raw[1 - PAR]);
     };
-    auto weights = [&](int p, uint4 (&w)[RB]) {
+    // w: the weights rounded, and what that leaves of them
+    auto weights = [&](int p, uint4 (&w)[RB][2]) {
 #pragma unroll
       for (int b = 0; b < RB; ++b) {
-        float e[8];
+        uint32_t t[2][4];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          e[i] = __builtin_amdgcn_exp2f(s[b][p >> 1][8 * (p & 1) + i]);
-          sum[b] = __builtin_fmaf(e[i], giv[p], sum[b]);
+        for (int i = 0; i < 4; ++i) {
+          float e[2];
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            e[k] = __builtin_amdgcn_exp2f(s[b][p >> 1][8 * (p & 1) + 2 * i + k]);
+            sum[b] = __builtin_fmaf(e[k], giv[p], sum[b]);
+          }
+          t[0][i] = cvt2<false>(e[0], e[1]);
+          const f16x2_t top = __builtin_bit_cast(f16x2_t, t[0][i]);
+          t[1][i] = cvt2<false>(__builtin_fmaf((float)top.x, -1.f, e[0]), __builtin_fmaf((float)top.y, -1.f, e[1]));      // (one mixed fma each)
         }
-        w[b] = make_uint4(cvt2<false>(e[0], e[1]), cvt2<false>(e[2], e[3]), cvt2<false>(e[4], e[5]), cvt2<false>(e[6], e[7]));
+#pragma unroll
+        for (int k = 0; k < 2; ++k) w[b][k] = make_uint4(t[k][0], t[k][1], t[k][2], t[k][3]);
       }
     };
-    auto weigh = [&](int p, const uint4 (&w)[RB]) {
+    auto weigh = [&](int p, const uint4 (&w)[RB][2]) {
 #pragma unroll
       for (int n = 0; n < 2 * J; ++n) {
         const uint4 a = *(const uint4*)(vb + (32 * n + r32) * TILE_KEYS + 8 * v_slot(32 * n + r32, 2 * p + h));
 #pragma unroll
-        for (int b = 0; b < RB; ++b) acc[b][n] = mfma_at<false>(a, w[b], acc[b][n]);
+        for (int x = 1; x >= 0; --x)
+#pragma unroll
+          for (int b = 0; b < RB; ++b) acc[b][n] = mfma_at<false>(a, w[b][x], acc[b][n]);
       }
     };
     if constexpr (TURNS) {
-      uint4 w[4][RB];
+      uint4 w[4][RB][2];
 #pragma unroll
       for (int p = 0; p < 4; ++p) weights(p, w[p]);
       __builtin_amdgcn_sched_barrier(0);
@@ -358,14 +371,14 @@ __global__ __launch_bounds__(64 * W, W / 4) void kv8_attn_tile(const ktir_kv8_at
       __builtin_amdgcn_s_setprio(0);
       __builtin_amdgcn_sched_barrier(0);
     } else {
-      uint4 w[RB], old[RB];
+      uint4 w[RB][2], old[RB][2];
 #pragma unroll
       for (int p = 0; p < 5; ++p) {
         if (J == 4 || p == 0 || p == 2 || p == 4) __builtin_amdgcn_sched_barrier(0);
         move(p);
         if (p < 4) scores(s_next, 1 - PAR, p * J, J);
 #pragma unroll
-        for (int b = 0; b < RB; ++b) old[b] = w[b];
+        for (int b = 0; b < RB; ++b) old[b][0] = w[b][0], old[b][1] = w[b][1];
         if (p < 4) weights(p, w);
         if (p > 0) weigh(p - 1, old);
       }
@@ -426,11 +439,13 @@ static void tile_go(const ktir_kv8_attn_t& d, int64_t slots, hipStream_t st) {
 }
 
 // Whether a launch takes this kernel, and its tiles of rows for each KV head.  With fewer
-// than 128 workgroups the kernel of few rows, which spreads the keys as well, is faster:
-// the last 512 of 4096 tokens (72 tiles) 86 us there and 123 here, the last 700 (88) 121 and
-// 123, the last 1024 (136) 151 and 125, 2048 alone (264) 124 and 75, 16 sequences of 64
-// after 1984 (128) 103 and 75.  So it is where no tile is more than half full: 16 sequences of 20
-// (80 rows of 256) 52 and 73.
+// than 128 workgroups the kernel of few rows, which spreads the keys as well, is faster (128
+// columns): the last 512 of 4096 tokens (72 tiles) 86 us there and 156 here, the last 700 (88) 120
+// and 157, the last 1024 (136) 148 and 157, the last 1400 (176) 202 and 164, 2048 alone (264) 120 and 93,
+// 16 sequences of 64 after 1984 (128) 103 and 92, 20 (160) 125 and 90.  With 64 columns 16 sequences (128)
+// take 75 and 73, the last 1024 (136) 114 and 123; with 256 this kernel gains later: the last 512 (136)
+// 176 and 273, 8 sequences of 300 after 1700 (332) 249 and 275, 32 of 40 after 960 (576) 216 and 171.  And the
+// kernel of few rows is where no tile is more than half full: 16 sequences of 20 (80 rows of 256) 50 and 87.
 bool kv8_tile_takes(const ktir_kv8_attn_t& d, int64_t* slots) {
   const int64_t grp = d.q_heads / d.cache.heads, TM = d.cache.columns <= 128 ? 256 : 128;
   if (d.max_q * grp <= TM / 2) return false;
