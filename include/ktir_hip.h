@@ -580,7 +580,9 @@ int ktir_launch_kv8_append(const ktir_kv8_append_t* d);
  * they were.  Products of q and codes are exact, sums f32, probabilities enter
  * the second product as ktir_kv8_rows.hip and ktir_kv8_tile.hip say; the result is
  * rounded once to dtype (KTIR_F16 or KTIR_BF16, of q and out).  Codes of tokens past kv_len are not
- * looked at; an e4m3 NaN code of a value makes the rows of its sequence NaN.
+ * looked at, nor those before the window of a sequence's first new token, where pages that
+ * end before it need no table entry; an e4m3 NaN code of a value may make any row of its
+ * sequence NaN.
  * max_q and max_k (2^30 at most) bound the new and the cached tokens of every
  * sequence: what a sequence has beyond is left out, with the device error word set.
  * out may be q itself; it and lse overlap nothing else that the launch reads.

@@ -179,9 +179,13 @@ __device__ __forceinline__ Tile lane_of(Tile t, int i) {
   return t;
 }
 
-// the page of the group that starts at `key`; from `end` on: page 0, which weighs nothing
-__device__ __forceinline__ int kv8_pages(const ktir_kv8_attn_t& d, const Tile& t, int key, int end, int shift) {
-  return key < end ? ints(d.batch.table)[t.s * d.batch.table_row + (key >> shift)] : 0;
+// whether some row of the tile sees a key of the group that starts at `key`
+__device__ __forceinline__ bool kv8_there(const Tile& t, int64_t key) { return key < t.hi && key + 16 > t.lo; }
+
+// the page of the group that starts at `key`; of one that no row sees: page 0, which weighs
+// nothing (before a window the table's entries may be those of pages that are gone)
+__device__ __forceinline__ int kv8_pages(const ktir_kv8_attn_t& d, const Tile& t, int key, int shift) {
+  return kv8_there(t, key) ? ints(d.batch.table)[t.s * d.batch.table_row + (key >> shift)] : 0;
 }
 
 __device__ __forceinline__ KV8Groups kv8_groups(const ktir_kv8_attn_t& d, int64_t head, int page, bool there, int* err) {

@@ -154,7 +154,7 @@ __global__ __launch_bounds__(64 * ROWS_WAVES, MT == 1 ? 2 : 1) void kv8_attn_row
   const int64_t item = (int64_t)slot * heads + head;
   // (steps of 32 keys go to the splits' wavefronts in turn, so what all read at one time lies close together)
   const int stride = ROWS_STEP * TW * active, lo = from + (split * TW + turn) * ROWS_STEP, mine = (l >> 1) * stride + 16 * (l & 1);
-  const int page0 = kv8_pages(d, t, lo + mine, t.hi, shift);
+  const int page0 = kv8_pages(d, t, lo + mine, shift);
 
   // Q: this lane's row of each 16, pieces g4 J .. g4 J + J of 16 columns (so a load of K touches whole 128-byte lines); times 2^k, so that the row's largest value has exponent 14
   uint4 qf[MT][J][2];
@@ -180,7 +180,7 @@ __global__ __launch_bounds__(64 * ROWS_WAVES, MT == 1 ? 2 : 1) void kv8_attn_row
   }
   const int koff = c16 * (int)c.k_tok, vcol = c16 * 4 * J + 4 * J <= D ? c16 * 4 * J : 0, voff = 4 * g4 * (int)c.v_tok + vcol;
   // the first keys' pages, scales and codes are on their way while Q is made ready
-  KV8Groups g = kv8_groups(d, head, page0, lo + mine < t.hi, err);
+  KV8Groups g = kv8_groups(d, head, page0, kv8_there(t, lo + mine), err);
   KV8Keys<J> k[2];
   if (lo < t.hi) kv8_keys<J>(c, g, 0, lo, head, koff, kpiece, k[0]);
 #pragma unroll
@@ -279,11 +279,13 @@ __global__ __launch_bounds__(64 * ROWS_WAVES, MT == 1 ? 2 : 1) void kv8_attn_row
       wh[m] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
       wl[m] = make_uint4(lo_[0], lo_[1], lo_[2], lo_[3]);
     }
-    if (CODE == KTIR_E4M3 && key + ROWS_STEP > t.hi) {     // NaN codes of tokens that no row sees
+    if (CODE == KTIR_E4M3 && (key < t.lo || key + ROWS_STEP > t.hi)) {     // NaN codes of tokens that no row sees
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
+      for (int i = 0; i < 8; ++i) {
+        const int at = key + 16 * (i >> 2) + 4 * g4 + (i & 3);
 #pragma unroll
-        for (int j = 0; j < J; ++j) ov.v[i][j] = key + 16 * (i >> 2) + 4 * g4 + (i & 3) >= t.hi ? 0u : ov.v[i][j];
+        for (int j = 0; j < J; ++j) ov.v[i][j] = at < t.lo || at >= t.hi ? 0u : ov.v[i][j];
+      }
     }
 #pragma unroll
     for (int j = 0; j < J; ++j) {
@@ -304,9 +306,9 @@ __global__ __launch_bounds__(64 * ROWS_WAVES, MT == 1 ? 2 : 1) void kv8_attn_row
 
   for (int64_t first = lo; first < t.hi; first += (int64_t)stride * (ROWS_GROUPS / 2)) {
     const int base = (int)first;
-    const bool there = first + mine < t.hi;
+    const bool there = kv8_there(t, first + mine);
     if (base != lo) {
-      g = kv8_groups(d, head, there ? kv8_pages(d, t, base + mine, t.hi, shift) : 0, there, err);
+      g = kv8_groups(d, head, there ? kv8_pages(d, t, base + mine, shift) : 0, there, err);
       kv8_keys<J>(c, g, 0, base, head, koff, kpiece, k[0]);
     }
     const int n = (t.hi - base + stride - 1) / stride, steps = n < ROWS_GROUPS / 2 ? n : ROWS_GROUPS / 2;

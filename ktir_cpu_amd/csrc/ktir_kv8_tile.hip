@@ -126,6 +126,7 @@ __global__ __launch_bounds__(64 * W, W / 4) void kv8_attn_tile(const ktir_kv8_at
   }
 
   // a thread's share of a step: units of 16 codes of a key, and of 4 columns of 4 keys of V
+  const uint32_t seen_by_some = t.hi > t.lo ? t.hi - t.lo : 0;      // keys, from t.lo on
   const int steps = t.hi > from ? (t.hi - from + TILE_KEYS - 1) / TILE_KEYS : 0;
   // the groups of the 16 steps that the computed one is of, of those that keys are fetched of (four steps on), and the next
   KV8Groups cur = {0, 0.f, 0.f, L_UNIT}, g = cur, next = cur;
@@ -181,9 +182,9 @@ __global__ __launch_bounds__(64 * W, W / 4) void kv8_attn_tile(const ktir_kv8_at
       if (VU % NT && tid >= VU) break;
       const int chunk = v_chunk(p), col = v_col(p);
       if (CODE == KTIR_E4M3) {                    // NaN codes of tokens that no row sees
-        const int first = from + TILE_KEYS * j + v_key(p);
+        const int first = from + TILE_KEYS * j + v_key(p) - t.lo;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) vraw[p][i] = first + i < t.hi ? vraw[p][i] : 0u;
+        for (int i = 0; i < 4; ++i) vraw[p][i] = (uint32_t)(first + i) < seen_by_some ? vraw[p][i] : 0u;
       }
       uint32_t a[4], b[4];
       cross_half2<CODE>(vraw[p][0], vraw[p][1], a);
@@ -216,8 +217,8 @@ __global__ __launch_bounds__(64 * W, W / 4) void kv8_attn_tile(const ktir_kv8_at
   };
   f32x16_t s0[RB][2], s1[RB][2];                 // scores of even and odd steps
   if (steps) {
-    const bool there = from + 16 * l < t.hi;
-    g = kv8_groups(d, head, kv8_pages(d, t, from + 16 * l, t.hi, shift), there, err);
+    const bool there = kv8_there(t, from + 16 * l);
+    g = kv8_groups(d, head, kv8_pages(d, t, from + 16 * l, shift), there, err);
     kv8_scales(g, there);
     cur = g;
     fetch_k(0, k_raw[0]);
@@ -241,12 +242,12 @@ __global__ __launch_bounds__(64 * W, W / 4) void kv8_attn_tile(const ktir_kv8_at
     constexpr int PAR = decltype(parity)::value;
     // the next 16 steps' groups: their pages four steps ahead of the first fetch, then the scales
     const int f = j + 4, key = from + TILE_KEYS * j;
-    if ((f & 15) == 12) next.page = kv8_pages(d, t, from + TILE_KEYS * (f + 4) + 16 * l, t.hi, shift);
-    if ((f & 15) == 14) next = kv8_groups(d, head, next.page, from + TILE_KEYS * (f + 2) + 16 * l < t.hi, err);
+    if ((f & 15) == 12) next.page = kv8_pages(d, t, from + TILE_KEYS * (f + 4) + 16 * l, shift);
+    if ((f & 15) == 14) next = kv8_groups(d, head, next.page, kv8_there(t, from + TILE_KEYS * (f + 2) + 16 * l), err);
     const int vpages = (f & 15) == 0 ? cur.page : g.page;          // of step j + 3, in the 16 before g's next ones then
     if ((f & 15) == 0) {
       g = next;
-      kv8_scales(g, from + TILE_KEYS * f + 16 * l < t.hi);
+      kv8_scales(g, kv8_there(t, from + TILE_KEYS * f + 16 * l));
     }
     if ((j & 15) == 0) cur = g;
     float gks[4], glv[4], giv[4];

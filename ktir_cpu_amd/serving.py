@@ -329,7 +329,8 @@ class KV8Attention(_Launch):
     `q`, `out` [tokens, query heads, columns]; consecutive query heads share a KV
     head.  `max_q`, `max_k`: the most new and cached tokens that a sequence of the
     batch has, over all runs.  `scale`: of the scores (columns^-1/2 if None).
-    `window` > 0: a token sees that many tokens up to itself.  `causal` False:
+    `window` > 0: a token sees that many tokens up to itself, and pages that end before
+    the window of a sequence's first new token need no table entry.  `causal` False:
     every new token sees all cached ones.  `lse` [tokens, query heads] float32:
     the rows' log-sum-exp.  `workspace`: a device array of at least
     `workspace_bytes` bytes to use instead of an own one, which launches that

@@ -1,9 +1,12 @@
-"""Edges of the serving operators, on the GPU: how many bits results keep."""
+"""Edges of the serving operators, on the GPU: both attention kernels (few rows, many
+rows) at pages and codes that neither may look at, and how many bits results keep."""
+import math
+
 import pytest
 import torch
 
 from tests import _serving as S
-from tests.test_gpu_serving import attend, serving   # noqa: F401 (a fixture)
+from tests.test_gpu_serving import attend, check, serving   # noqa: F401 (a fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -30,3 +33,41 @@ def test_weights_of_prompts(serving, hk, grp, D, page, code):  # noqa: F811
     # `bound` has 2^-11 of every weight; two f16 terms leave 2^-11 of 2^-11
     bound = bound - size * (2.0 ** -11 - 2.0 ** -22)
     S.close(out[:, heads], want[:, heads], bound[:, heads], "f16")
+
+
+# ---- what lies before a window ---------------------------------------------------------
+
+WINDOWS = [
+    # few rows: one sequence, several, in splits, more than one tile a sequence
+    ([(1, 333)], 2, 3, 64, 16), ([(1, 333), (2, 90), (5, 700), (1, 16), (3, 3)], 2, 3, 64, 16),
+    ([(1, 20000), (2, 9000), (1, 5)], 4, 2, 128, 16), ([(37, 600), (1, 70), (20, 300)], 2, 3, 80, 16),
+    # many rows
+    ([(130, 700), (90, 300), (64, 1900), (128, 129), (1, 500)], 16, 4, 128, 16),
+    ([(130, 700), (90, 300), (64, 1900), (128, 129), (1, 500)], 16, 4, 64, 32),
+    ([(70, 700), (90, 300), (64, 1500), (128, 129), (1, 500)], 16, 2, 192, 16),
+]
+
+
+@pytest.mark.parametrize("code", ["i8", "e4m3"])
+@pytest.mark.parametrize("window", [1, 37, 100])
+@pytest.mark.parametrize("lens,hk,grp,D,page", WINDOWS)
+def test_pages_before_the_window_are_not_looked_at(serving, lens, hk, grp, D, page, window, code):  # noqa: F811
+    """Their table entries are gone, and what the first page of the window holds before it is
+    NaN codes, as the memory of a page that was given away may hold."""
+    b = S.Batch(lens, hk=hk, grp=grp, D=D, page=page, code=code, seed=window)
+    clean = [x.clone() for x in (*b.cache(), b.table)]
+    for s, (n, kv) in enumerate(lens):
+        first = max(kv - n - window + 1, 0)                   # what the sequence's first new token sees from on
+        gone = first // page
+        for p in range(gone):
+            at = int(b.table[s, p])
+            for x in (b.k, b.v):
+                x.view(torch.uint8)[at] = 0x7f
+            b.k_scale[at] = b.v_scale[at] = math.nan
+        if first % page:
+            for x in (b.k, b.v):
+                x.view(torch.uint8)[int(b.table[s, gone]), :first % page] = 0x7f
+        b.table[s, :gone] = -1
+    out, lse = attend(serving, b, window=window)              # (and no IndexError)
+    b.k, b.v, b.k_scale, b.v_scale, b.table = clean
+    check(b, out, lse, window=window, heads=(0, hk * grp - 1))
