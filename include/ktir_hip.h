@@ -556,8 +556,8 @@ typedef struct ktir_kv8_batch {
  *   code   = rint(x * (1 / scale')) or the nearest e4m3 value, within +- top
  * and where scale' is more than the scale before, the older tokens' codes are
  * rounded again: code * (scale before * (1 / scale')).  Every operation is one in f32.
- * A page that receives a value that is not finite reads as NaN from then on
- * (scale' = NaN, new codes 0).
+ * An older e4m3 code that is NaN stays NaN.  A page that receives a value that is
+ * not finite reads as NaN from then on (scale' = NaN, new codes 0).
  * Tokens at negative positions are not stored.  A page that two sequences of a
  * call, or two places of one's table, both write keeps the codes and the scale of either.
  * k, v: [tokens, heads, columns], KTIR_F16 or KTIR_BF16. */

@@ -151,8 +151,8 @@ typedef uint32_t u4_t __attribute__((ext_vector_type(4)));
 template <int CODE>
 constexpr float PER_TOP = 1.f / (CODE == KTIR_I8 ? 127.f : 448.f);
 
-// four values over their scale as codes
-template <int CODE>
+// four values over their scale as codes; NAN_TOO: some may be NaN, and stay so (the clamp makes a bound of one)
+template <int CODE, bool NAN_TOO = false>
 __device__ __forceinline__ uint32_t codes4(const float* x) {
   if constexpr (CODE == KTIR_I8) {
     uint32_t w = 0;
@@ -165,7 +165,10 @@ __device__ __forceinline__ uint32_t codes4(const float* x) {
   } else {
     float y[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) y[i] = __builtin_amdgcn_fmed3f(x[i], -448.f, 448.f);
+    for (int i = 0; i < 4; ++i) {
+      y[i] = __builtin_amdgcn_fmed3f(x[i], -448.f, 448.f);
+      if (NAN_TOO) y[i] = x[i] != x[i] ? x[i] : y[i];
+    }
     int w = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
     return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], w, true);
   }
@@ -312,7 +315,7 @@ __global__ __launch_bounds__(256) void kv8_append(const ktir_kv8_append_t d, int
         values4<CODE>(y[i], v);
 #pragma unroll
         for (int k = 0; k < 4; ++k) v[k] *= ratio;
-        y[i] = codes4<CODE>(v);
+        y[i] = codes4<CODE, CODE == KTIR_E4M3>(v);
       }
       *w = y;
     }

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from tests import _serving as S
-from tests.test_gpu_serving import attend, check, serving   # noqa: F401 (a fixture)
+from tests.test_gpu_serving import attend, check, dev, serving, sync   # noqa: F401 (a fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -71,3 +71,25 @@ def test_pages_before_the_window_are_not_looked_at(serving, lens, hk, grp, D, pa
     out, lse = attend(serving, b, window=window)              # (and no IndexError)
     b.k, b.v, b.k_scale, b.v_scale, b.table = clean
     check(b, out, lse, window=window, heads=(0, hk * grp - 1))
+
+
+# ---- codes that are NaN ------------------------------------------------------------------
+
+@pytest.mark.parametrize("hk,D,page", [(2, 64, 16), (1, 256, 64)])
+def test_append_keeps_nan_codes(serving, hk, D, page):  # noqa: F811
+    """A page that was filled elsewhere holds NaN codes: they stay NaN when the page's scale grows."""
+    b = S.Batch([(3, 13)], hk=hk, D=D, page=page, code="e4m3")
+    at = int(b.table[0, 0])
+    b.new_k *= 40
+    b.new_v *= 40                                              # the scales grow
+    for x in (b.k, b.v):
+        x.view(torch.uint8)[at, 4, 0, 5], x.view(torch.uint8)[at, 9, hk - 1, D - 1] = 0x7f, 0xff
+    d = dev(*b.cache())
+    serving.KV8Append(serving.KV8Cache(*d), *dev(b.new_k, b.new_v), *dev(*b.where())).run()
+    sync()
+    for x, codes, scale, c2, s2 in ((b.new_k, b.k, b.k_scale, d[0], d[2]), (b.new_v, b.v, b.v_scale, d[1], d[3])):
+        want, wscale = S.append(x, codes, scale, "e4m3", page, *b.where())
+        assert torch.equal(s2.cpu(), wscale) and bool((wscale[at] > scale[at]).all())
+        nan = torch.isnan(want.float())
+        assert int(nan.sum()) == 2 and torch.equal(torch.isnan(c2.cpu().float()), nan)
+        assert torch.equal(c2.cpu().view(torch.uint8)[~nan], want.view(torch.uint8)[~nan])
