@@ -165,6 +165,8 @@ class _Launch:
             self.desc.stream = int(getattr(stream, "cuda_stream", stream)) or _NULL_STREAM
         elif self._torch_device is not None:
             self.desc.stream = self._current(self._torch_device) or _NULL_STREAM
+        else:
+            self.desc.stream = 0
         rc = self._call(self._ref)
         if rc:
             rt.check(rc)
