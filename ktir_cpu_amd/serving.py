@@ -43,8 +43,6 @@ _TORCH = {"torch.float16": "f16", "torch.bfloat16": "bf16", "torch.float32": "f3
           "torch.uint8": "u8"}
 _TYPESTR = {"<f2": "f16", "<u2": "bf16", "<f4": "f32", "<f8": "f64", "|i1": "i8", "|u1": "e4m3", "<i4": "i32",
             "<i8": "i64"}
-_NUMPY = {"f16": "<f2", "bf16": "<u2", "f32": "<f4", "f64": "<f8", "i8": "|i1", "e4m3": "|u1", "i32": "<i4",
-          "i64": "<i8", "u8": "|u1"}
 
 
 _NULL_STREAM = rt.K["KTIR_STREAM_NULL"]
@@ -174,12 +172,14 @@ class _Launch:
             self._used_on(stream)
 
     def _used_on(self, stream):
-        """The own workspace came from torch: it goes to no other tensor before this stream is done with it."""
+        """The own workspace came from torch: it goes to no other tensor before this stream is done with it.
+        A raw handle is not recorded (its stream may end before the workspace does): its caller waits."""
+        if stream is not None and not hasattr(stream, "cuda_stream"):
+            return
         torch = sys.modules["torch"]
         if torch.cuda.is_current_stream_capturing():
             return                                  # (a replay's stream is not known here)
-        if stream is None or hasattr(stream, "cuda_stream"):
-            self._own.record_stream(torch.cuda.current_stream(self._torch_device) if stream is None else stream)
+        self._own.record_stream(torch.cuda.current_stream(self._torch_device) if stream is None else stream)
         self._streams.add(self.desc.stream)
 
 

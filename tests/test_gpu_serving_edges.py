@@ -93,3 +93,30 @@ def test_append_keeps_nan_codes(serving, hk, D, page):  # noqa: F811
         nan = torch.isnan(want.float())
         assert int(nan.sum()) == 2 and torch.equal(torch.isnan(c2.cpu().float()), nan)
         assert torch.equal(c2.cpu().view(torch.uint8)[~nan], want.view(torch.uint8)[~nan])
+
+
+# ---- the own workspace ---------------------------------------------------------------------
+
+def test_own_workspace_after_a_raw_handle(serving):  # noqa: F811
+    """A run on a raw handle is the caller's to wait for; the same stream as an object is recorded all the same."""
+    b = S.Batch([(1, 5000), (1, 70)], hk=2, grp=4, D=64, dt="bf16")
+    q = b.q.cuda()
+    op = serving.KV8Attention(serving.KV8Cache(*dev(*b.cache())), q, torch.empty_like(q), *dev(*b.where()), **b.most)
+    keep, held = op._own, []
+
+    class Own:
+        def record_stream(self, stream):
+            held.append(stream.cuda_stream)
+
+    op._own = Own()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    op.run(side.cuda_stream)
+    op.run(side)
+    torch.cuda.synchronize()
+    op.run(side.cuda_stream)
+    with torch.cuda.stream(side):
+        op.run()
+    torch.cuda.synchronize()
+    assert held == [side.cuda_stream]
+    del keep
