@@ -491,7 +491,10 @@ int ktir_launch_paged_attention(const ktir_pattn_t* d);
  * from device memory (positions, lengths, tables) it reads when it runs.
  * Lengths, tables and offsets in device memory that are out of range are not
  * followed: the launch stays inside the arrays that its descriptor names and
- * sets the device error word (ktir_check_error_flag: KTIR_E_INDEX). */
+ * sets the device error word (ktir_check_error_flag: KTIR_E_INDEX).  What a launch
+ * writes may share no byte with anything else that its descriptor names, but for what
+ * each says below; it is refused (KTIR_E_ARG), but arrays side by side in one allocation
+ * whose dimensions step alike are told apart. */
 #define KTIR_STREAM_NULL 1
 
 /* A tensor [tokens, heads, columns], column stride 1; strides in elements. */
@@ -509,9 +512,8 @@ typedef struct ktir_rows3 {
  * the products are f32, and the result is rounded once.  `inverse` is the rotation
  * back: the gradient's way through the operator.  Rows of tokens with
  * pos < 0 are left as they were.  Two tensors (queries and keys) share one
- * launch; heads2 = 0: one.  An output may be its input itself and must share
- * no element with the other tensors (parts of one projection's rows, side by
- * side, do not).  dtype: KTIR_F16, KTIR_BF16 or KTIR_F32. */
+ * launch; heads2 = 0: one.  An output may be its input itself (and the
+ * two tensors parts of one projection's rows, side by side).  dtype: KTIR_F16, KTIR_BF16 or KTIR_F32. */
 typedef struct ktir_rope {
   int64_t tokens, heads, heads2, columns, rot;
   ktir_rows3_t in, out, in2, out2;
@@ -585,7 +587,7 @@ int ktir_launch_kv8_append(const ktir_kv8_append_t* d);
  * sequence NaN.
  * max_q and max_k (2^30 at most) bound the new and the cached tokens of every
  * sequence: what a sequence has beyond is left out, with the device error word set.
- * out may be q itself; it and lse overlap nothing else that the launch reads.
+ * out may be q itself.
  * `splits` workgroups share a sequence's cached tokens.  ktir_kv8_attention_plan
  * sets it and ws_bytes (host only), the bytes of workspace that `ws` must then
  * have, on a 16-byte bound; launches that may run at the same time need a

@@ -44,8 +44,8 @@ bool same(const Strided& a, const Strided& b) {
 }
 
 // Whether `off` + sum_i d_i step_i lies between lo and hi for some d_i of first_i to
-// last_i; steps in falling order, and none below the reach of those after it, so that
-// few d_i can do.
+// last_i; steps in falling order, so that few d_i can do (the rows of an output do not
+// overlap: a step is no less than the reach of those after it).
 static bool reaches(int64_t off, int64_t lo, int64_t hi, int dims, const int64_t* step, const int64_t* first, const int64_t* last) {
   if (dims == 0) return lo <= off && off <= hi;
   int64_t down = 0, up = 0;
@@ -59,22 +59,19 @@ static bool reaches(int64_t off, int64_t lo, int64_t hi, int dims, const int64_t
   return false;
 }
 
-// Tensors whose ranges meet share nothing if they step alike over rows side by side (parts
-// of one projection, K and V of one allocation); with other steps they count as shared.
-bool apart(const Strided& a, const Strided& b) {
-  auto end = [](const Strided& x) {
-    uint64_t e = x.ptr + x.width;
-    for (int i = 0; i < 3; ++i) e += (uint64_t)(x.count[i] - 1) * x.step[i];
-    return e;
-  };
-  if (a.ptr >= end(b) || b.ptr >= end(a)) return true;
+// Dimensions that both step alike are followed (parts of one projection, K and V of one
+// allocation, scales behind the codes of their page); in others a tensor counts as
+// all that lies between its first and last byte.
+bool apart_within(Strided a, Strided b) {
   int dims = 0;
   int64_t step[3], first[3], last[3];
   for (int i = 0; i < 3; ++i) {
-    if (a.count[i] == 1 && b.count[i] == 1) continue;
-    if (a.count[i] > 1 && b.count[i] > 1 && a.step[i] != b.step[i]) return false;
+    if (a.count[i] > 1 && b.count[i] > 1 && a.step[i] != b.step[i]) {
+      for (Strided* x : {&a, &b}) x->width += (x->count[i] - 1) * x->step[i], x->count[i] = 1;
+      continue;
+    }
     const int64_t s = a.count[i] > 1 ? a.step[i] : b.step[i];
-    if (s == 0) continue;
+    if (s == 0 || (a.count[i] == 1 && b.count[i] == 1)) continue;
     int at = dims++;
     for (; at > 0 && step[at - 1] < s; --at) step[at] = step[at - 1], first[at] = first[at - 1], last[at] = last[at - 1];
     step[at] = s, first[at] = 1 - a.count[i], last[at] = b.count[i] - 1;
@@ -125,11 +122,11 @@ int check_kv8(const char* what, const ktir_kv8_t& c, bool written) {
   if (!c.k_scale || !c.v_scale || ((c.k_scale | c.v_scale) & 3)) return set_error(KTIR_E_ARG, "%s: scales missing or off 4-byte bounds", what);
   if (written && ((c.pages > 1 && (!c.ks_page || !c.vs_page)) || (c.heads > 1 && (!c.ks_head || !c.vs_head))))
     return set_error(KTIR_E_ARG, "%s: pages or heads share a scale", what);
-  if (written && (!apart({c.k, c.columns, {c.pages, c.page, c.heads}, {c.k_page, c.k_tok, c.k_head}},
-                         {c.v, c.columns, {c.pages, c.page, c.heads}, {c.v_page, c.v_tok, c.v_head}}) ||
-                  !apart({c.k_scale, 4, {c.pages, c.heads, 1}, {c.ks_page * 4, c.ks_head * 4, 0}},
-                         {c.v_scale, 4, {c.pages, c.heads, 1}, {c.vs_page * 4, c.vs_head * 4, 0}})))
-    return set_error(KTIR_E_ARG, "%s: the caches of keys and values overlap", what);
+  if (!written) return KTIR_OK;
+  const CacheParts parts(c);
+  for (int i = 0; i < 4; ++i)
+    for (int j = 0; j < i; ++j)
+      if (!apart(parts.x[i], parts.x[j])) return set_error(KTIR_E_ARG, "%s: the caches or scales of keys and values overlap", what);
   return KTIR_OK;
 }
 
@@ -352,7 +349,14 @@ extern "C" int ktir_launch_kv8_append(const ktir_kv8_append_t* d) {
   if (rc != KTIR_OK || d->batch.seqs == 0 || d->batch.tokens == 0) return rc;
   rc = check_rows3(ME, d->k, d->batch.tokens, d->cache.heads, d->cache.columns, false);
   if (rc == KTIR_OK) rc = check_rows3(ME, d->v, d->batch.tokens, d->cache.heads, d->cache.columns, false);
-  if (rc == KTIR_OK) rc = ready(ME);
+  if (rc != KTIR_OK) return rc;
+  const BatchParts batch(d->batch);
+  const Strided k = rows_of(d->k, d->batch.tokens, d->cache.heads, d->cache.columns, 2), v = rows_of(d->v, d->batch.tokens, d->cache.heads, d->cache.columns, 2);
+  for (const Strided& out : CacheParts(d->cache).x) {
+    if (!apart(out, k) || !apart(out, v)) return set_error(KTIR_E_ARG, "%s: the cache overlaps the new keys or values", ME);
+    if (!batch.clear_of(out)) return set_error(KTIR_E_ARG, "%s: the cache overlaps the table, offsets or lengths", ME);
+  }
+  rc = ready(ME);
   if (rc != KTIR_OK) return rc;
   OnDevice on;
   if (!on.ok()) return set_error(KTIR_E_HIP, "%s: no device", ME);

@@ -54,6 +54,15 @@ extern "C" int ktir_launch_kv8_attention(const ktir_kv8_attn_t* d) {
   const Strided lse = rows({d->lse, d->lse_tok, d->lse_head}, 1, 4);
   if (!(same(q, out) || apart(q, out)) || (d->lse && !(apart(lse, out) && apart(lse, q))))
     return set_error(KTIR_E_ARG, "%s: an output overlaps a tensor that it is not", ME);
+  const CacheParts cache(d->cache);
+  const BatchParts batch(d->batch);
+  auto clear = [&](const Strided& x) { return apart(x, cache.x[0]) && apart(x, cache.x[1]) && apart(x, cache.x[2]) && apart(x, cache.x[3]) && batch.clear_of(x); };
+  if (!clear(out) || (d->lse && !clear(lse))) return set_error(KTIR_E_ARG, "%s: an output overlaps the cache, table, offsets or lengths", ME);
+  if (d->splits > 1 && d->ws && d->ws_bytes > 0) {
+    const Strided ws(d->ws, d->ws_bytes);
+    if (!clear(ws) || !apart(out, ws) || !apart(q, ws) || (d->lse && !apart(lse, ws)))
+      return set_error(KTIR_E_ARG, "%s: the workspace overlaps a tensor", ME);
+  }
   KV8Shape s;
   kv8_rows_shape(*d, &s);
   const int64_t splits = d->splits < 1 ? 1 : d->splits, tiles = s.slots * d->cache.heads;

@@ -261,7 +261,10 @@ static int check_tensors(const ktir_rope_t& d) {
   const Strided in = rows(d.in, d.heads), out = rows(d.out, d.heads), in2 = rows(d.in2, d.heads2), out2 = rows(d.out2, d.heads2);
   bool good = same(in, out) || apart(in, out);
   if (d.heads2) good = good && (same(in2, out2) || apart(in2, out2)) && apart(out, in2) && apart(out2, in) && apart(out, out2);
-  return good ? KTIR_OK : set_error(KTIR_E_ARG, "%s: an output overlaps a tensor that it is not", ME);
+  if (!good) return set_error(KTIR_E_ARG, "%s: an output overlaps a tensor that it is not", ME);
+  const Strided pos(d.pos, d.tokens * (d.pos_dtype == KTIR_I64 ? 8 : 4)), freq(d.freq, d.rot / 2 * 8);
+  good = apart(out, pos) && apart(out, freq) && (!d.heads2 || (apart(out2, pos) && apart(out2, freq)));
+  return good ? KTIR_OK : set_error(KTIR_E_ARG, "%s: an output overlaps the positions or frequencies", ME);
 }
 
 }  // namespace ktir

@@ -48,13 +48,36 @@ int ready(const char* what);         // whether ktir_init has run
 
 // Rows of `width` bytes, counts by counts at steps of so many bytes.
 struct Strided {
-  uint64_t ptr;
-  int64_t width, count[3], step[3];
+  uint64_t ptr = 0;
+  int64_t width = 0, count[3] = {1, 1, 1}, step[3] = {0, 0, 0};
+  uint64_t end = 0;                    // behind the last byte
+  Strided() = default;
+  Strided(uint64_t p, int64_t w, int64_t n0 = 1, int64_t s0 = 0, int64_t n1 = 1, int64_t s1 = 0, int64_t n2 = 1, int64_t s2 = 0)
+      : ptr(p), width(w), count{n0, n1, n2}, step{s0, s1, s2}, end(p + w + (uint64_t)(n0 - 1) * s0 + (uint64_t)(n1 - 1) * s1 + (uint64_t)(n2 - 1) * s2) {}
 };
 inline Strided rows_of(const ktir_rows3_t& r, int64_t tokens, int64_t heads, int64_t columns, int64_t bytes) {
-  return {r.ptr, columns * bytes, {tokens, heads, 1}, {r.tok * bytes, r.head * bytes, 0}};
+  return {r.ptr, columns * bytes, tokens, r.tok * bytes, heads, r.head * bytes};
 }
-bool apart(const Strided& a, const Strided& b);      // whether they share no byte; one of them is an output, whose rows do not overlap
+bool apart_within(Strided a, Strided b);             // for ranges that meet
+// whether they share no byte; one of them is an output, whose rows do not overlap
+inline bool apart(const Strided& a, const Strided& b) { return a.ptr >= b.end || b.ptr >= a.end || apart_within(a, b); }
+
+// what a launch on the cache reads or writes of it: codes of K and V, scales of K and V
+struct CacheParts {
+  Strided x[4];
+  explicit CacheParts(const ktir_kv8_t& c)
+      : x{{c.k, c.columns, c.pages, c.k_page, c.page, c.k_tok, c.heads, c.k_head}, {c.v, c.columns, c.pages, c.v_page, c.page, c.v_tok, c.heads, c.v_head},
+          {c.k_scale, 4, c.pages, c.ks_page * 4, 1, 0, c.heads, c.ks_head * 4}, {c.v_scale, 4, c.pages, c.vs_page * 4, 1, 0, c.heads, c.vs_head * 4}} {}
+};
+// the table (of at least one page a sequence), offsets and lengths
+struct BatchParts {
+  Strided x[3];
+  explicit BatchParts(const ktir_kv8_batch_t& b)
+      : x{{b.table, b.width * 4, b.seqs, b.table_row * 4}, {b.q_start, (b.seqs + 1) * 4}, {b.kv_len, b.seqs * 4}} {
+    if (!b.width) x[0] = x[1];
+  }
+  bool clear_of(const Strided& out) const { return apart(out, x[0]) && apart(out, x[1]) && apart(out, x[2]); }
+};
 bool same(const Strided& a, const Strided& b);       // whether they are one tensor
 
 __device__ __forceinline__ const KTIR_G(int32_t)* ints(uint64_t p) { return (const KTIR_G(int32_t)*)p; }
