@@ -508,8 +508,8 @@ typedef struct ktir_rows3 {
  *   a = inverse ? -pos[t] freq[i] : pos[t] freq[i],  c = amplitude cos a,  s = amplitude sin a
  *   (x, y) = the pair's values: columns i and i + rot / 2, or 2 i and 2 i + 1 (interleaved)
  *   out = (x c - y s, y c + x s)
- * and columns from rot on are copied.  The angle is reduced in 64 bits, c, s and
- * the products are f32, and the result is rounded once.  `inverse` is the rotation
+ * and columns from rot on are copied.  a, c and s are made in 64 bits, c and s rounded
+ * to f32, the products are f32, and the result is rounded once.  `inverse` is the rotation
  * back: the gradient's way through the operator.  Rows of tokens with
  * pos < 0 are left as they were.  Two tensors (queries and keys) share one
  * launch; heads2 = 0: one.  An output may be its input itself (and the

@@ -2,9 +2,9 @@
 // with the token's position, y = (x0 c - x1 s, x1 c + x0 s).
 //
 // Bound: bytes, in and out once.  The angles of a token are made once for all its
-// heads (64-bit remainder, one sine and cosine: about 60 instructions), in LDS, and
+// heads (remainder, sine and cosine in 64 bits), in LDS, and
 // every vector of 16 bytes is loaded and stored once, two rows of loads ahead.
-// Measured, f16 / bf16: 8192 tokens of 32 + 8 heads of 128, 168 MB, 31.6 us = 5.3 TB/s
+// Measured, f16 / bf16: 8192 tokens of 32 + 8 heads of 128, 168 MB, 31.9 us = 5.3 TB/s (31.7 with sine and cosine in 32 bits)
 // (a copy of 256 MiB makes 5.4 here); 40 + 40 heads with 64 interleaved columns of
 // 128, 168 MB, 36.2 us, 55.8 (of 39.4) with the columns behind rot as units of their own size;
 // one thread per pair over all heads took 97 and 212 us.  One token: a launch, 4.1 us.
@@ -15,17 +15,16 @@ namespace ktir {
 typedef uint32_t u4_t __attribute__((ext_vector_type(4)));
 typedef float f4_t __attribute__((ext_vector_type(4)));
 
-// cosine and sine of token t's pair i, times the amplitude.  The angle passes
-// 2^20 radians at far positions, where f32 holds it to a sixteenth: the product
-// and its remainder of whole turns are f64, what is left is f32 (2^-25 turns).
+// cosine and sine of token t's pair i, times the amplitude, rounded once.  The angle passes
+// 2^20 radians at far positions, where f32 holds it to a sixteenth: all of it is f64
+// (the vector pipe's f64 and f32 instructions take as long).
 __device__ __forceinline__ void rope_angle(const ktir_rope_t& d, int64_t pos, int i, float* c, float* s) {
   double turns = (double)pos * ((const KTIR_G(double)*)d.freq)[i] * 0.15915494309189533577;
   turns -= rint(turns);
-  float sn, cs;
-  sincospif((float)(2.0 * turns), &sn, &cs);
-  const float amp = (float)d.amplitude;
-  *c = cs * amp;
-  *s = d.inverse ? -(sn * amp) : sn * amp;
+  double sn, cs;
+  sincospi(2.0 * turns, &sn, &cs);
+  *c = (float)(cs * d.amplitude);
+  *s = (float)(d.inverse ? -(sn * d.amplitude) : sn * d.amplitude);
 }
 
 __device__ __forceinline__ int64_t rope_pos(const ktir_rope_t& d, int64_t t) {

@@ -95,6 +95,32 @@ def test_append_keeps_nan_codes(serving, hk, D, page):  # noqa: F811
         assert torch.equal(c2.cpu().view(torch.uint8)[~nan], want.view(torch.uint8)[~nan])
 
 
+# ---- the angle's sine and cosine ----------------------------------------------------------
+
+@pytest.mark.parametrize("inter", [False, True])
+@pytest.mark.parametrize("amplitude", [1.0, 1.2079441541679836])
+def test_rope_sine_and_cosine_are_rounded_once(serving, amplitude, inter):  # noqa: F811
+    g = torch.Generator().manual_seed(7)
+    x = torch.randn((700, 2, 128), generator=g)
+    pos = torch.randint(0, 1 << 20, (700,), generator=g)
+    freq, _ = serving.rope_frequencies(128)
+    out = torch.zeros_like(x).cuda()
+    serving.Rope(x.cuda(), pos.cuda(), torch.from_numpy(freq).cuda(), out, interleaved=inter, amplitude=amplitude).run()
+    sync()
+    ang = torch.outer(pos.double(), torch.from_numpy(freq))
+    c, s = (ang.cos() * amplitude)[:, None], (ang.sin() * amplitude)[:, None]
+    a, b = (x[..., 0::2], x[..., 1::2]) if inter else (x[..., :64], x[..., 64:])
+    a, b = a.double(), b.double()
+    y, o = (a * c - b * s, b * c + a * s), out.cpu().double()
+    o = (o[..., 0::2], o[..., 1::2]) if inter else (o[..., :64], o[..., 64:])
+    # c and s rounded once, each product once, their sum once (2^-24 each, the first two on each of the
+    # products); the angle in 64 bits: 2^20 radians hold it, in either order of operations, as
+    # far as four roundings of 2^-53 and the amplitude go: 2^-30 of the pair's size
+    for got, want, size in ((o[0], y[0], (a * c).abs() + (b * s).abs()), (o[1], y[1], (b * c).abs() + (a * s).abs())):
+        bound = size * 2 * 2.0 ** -24 * (1 + 2.0 ** -20) + want.abs() * 2.0 ** -24 + (a.abs() + b.abs()) * 2.0 ** -30 + 2.0 ** -126
+        assert bool(((got - want).abs() <= bound).all()), float(((got - want).abs() / bound).max())
+
+
 # ---- the own workspace ---------------------------------------------------------------------
 
 def test_own_workspace_after_a_raw_handle(serving):  # noqa: F811
