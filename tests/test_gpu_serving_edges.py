@@ -1,5 +1,5 @@
 """Edges of the serving operators, on the GPU: both attention kernels (few rows, many
-rows) at pages and codes that neither may look at, and how many bits results keep."""
+rows) at masks, pages and codes that neither may look at, and how many bits results keep."""
 import math
 
 import pytest
@@ -71,6 +71,147 @@ def test_pages_before_the_window_are_not_looked_at(serving, lens, hk, grp, D, pa
     out, lse = attend(serving, b, window=window)              # (and no IndexError)
     b.k, b.v, b.k_scale, b.v_scale, b.table = clean
     check(b, out, lse, window=window, heads=(0, hk * grp - 1))
+
+
+# ---- the kernel of many rows, where the one of few rows has been tested ----------------
+
+MANY = dict(hk=16, grp=4)                          # with these, 8 tiles of more than half their rows
+COLUMNS = [64, 80, 128, 192]
+
+
+@pytest.mark.parametrize("D", COLUMNS)
+def test_many_rows_not_causal(serving, D):  # noqa: F811
+    b = S.Batch([(130, 200), (70, 33), (90, 90), (2, 0)], D=D, page=32, **MANY)
+    check(b, *attend(serving, b, causal=False, scale=0.3), causal=False, scale=0.3, heads=(0, 63))
+
+
+@pytest.mark.parametrize("D", COLUMNS)
+@pytest.mark.parametrize("code", ["i8", "e4m3"])
+def test_many_rows_do_not_look_behind_the_last_token(serving, code, D):  # noqa: F811
+    b = S.Batch([(130, 133), (90, 300), (33, 64), (70, 1100), (1, 129)], D=D, code=code, seed=5, **MANY)
+    clean = [x.clone() for x in b.cache()]
+    used = set()
+    for s, (_, n) in enumerate(b.lens):
+        for p in range(-(-n // b.page)):
+            at = int(b.table[s, p])
+            used.add(at)
+            for x in (b.k, b.v):
+                x.view(torch.uint8)[at, min(n - p * b.page, b.page):] = 0x7f
+    for at in set(range(b.pages)) - used:
+        b.k_scale[at] = b.v_scale[at] = math.nan
+    out, lse = attend(serving, b)
+    b.k, b.v, b.k_scale, b.v_scale = clean
+    check(b, out, lse, heads=(0, 63))
+
+
+@pytest.mark.parametrize("D", COLUMNS)
+@pytest.mark.parametrize("first_page", [0, 1, 5])
+def test_many_rows_of_a_page_that_is_nan(serving, first_page, D):  # noqa: F811
+    """Rows that see a token of the page are NaN, others are as without it."""
+    b = S.Batch([(130, 130)] * 4, D=D, **MANY)
+    start = 16 * first_page
+    for name in ("k_scale", "v_scale"):
+        keep = getattr(b, name)
+        setattr(b, name, keep.clone())
+        getattr(b, name)[int(b.table[1, first_page])] = math.nan
+        out, lse = attend(serving, b)
+        bad = torch.isnan(out.cpu()).all(-1).all(-1)
+        assert bad[130 + start:260].all() and not torch.isnan(out.cpu()[~bad]).any() and int(bad.sum()) == 130 - start, name
+        setattr(b, name, keep)
+        want, wl, bound, lb = S.attention(b.q, *b.cache(), *b.where(), scale=D ** -0.5, heads=(0, 63))
+        for h in (0, 63):
+            S.close(out[:, h][~bad.cuda()], want[:, h][~bad], bound[:, h][~bad], b.dt)
+            S.close(lse[:, h][~bad.cuda()], wl[:, h][~bad], lb[:, h][~bad], "f32")
+
+
+@pytest.mark.parametrize("dt", ["f16", "bf16"])
+@pytest.mark.parametrize("D", COLUMNS)
+def test_many_rows_of_uneven_weights(serving, dt, D):  # noqa: F811
+    """One key holds nearly all the weight and has zeros as its value, so the others
+    make the result; pages' scales lie far apart, some of values that are all 0."""
+    b = S.Batch([(40, 700)] * 8, D=D, dt=dt, seed=9, spread=2.0, **MANY)
+    b.q = (torch.ones_like(b.q) + 0.25 * b.q).to(b.q.dtype)
+    for s in range(8):
+        first = int(b.table[s, 0])
+        b.k[first, 0] = 127
+        b.k_scale[first] = 12.0 / (D ** 0.5 * 127)        # its score: about 12 above the others
+        for p in range(1, b.width):
+            b.k_scale[int(b.table[s, p])] = 0.1 / 127
+        b.v[first, 0] = 0
+        b.v_scale[int(b.table[s, 2])] = 2.0 ** -100
+        b.v[int(b.table[s, 2])] = 0
+        b.v_scale[int(b.table[s, 3])] = 0.0
+        b.v[int(b.table[s, 3])] = 0
+    check(b, *attend(serving, b), heads=(0, 63))
+
+
+def test_many_rows_of_an_empty_v(serving):  # noqa: F811
+    for scale in (2.0 ** -100, 0.0):
+        b = S.Batch([(40, 200)] * 8, D=64, dt="bf16", **MANY)
+        b.v[:] = 0
+        b.v_scale[:] = scale
+        check(b, *attend(serving, b), heads=(0, 63))
+
+
+@pytest.mark.parametrize("D", [48, 128, 208])
+def test_many_rows_strides_and_odd_bases(serving, D):  # noqa: F811
+    """Queries cut from a projection's rows and from a 2-byte bound on, an output with heads
+    outside tokens, a cache with both halves in one allocation."""
+    b = S.Batch([(40, 90), (130, 177), (90, 90)], D=D, page=32, dt="bf16", **MANY)
+    qkv = torch.randn((b.tokens, 70, D)).to(torch.bfloat16)
+    qkv[:, 3:67] = b.q
+    flat = torch.zeros(qkv.numel() + 9, dtype=torch.bfloat16)
+    flat[3:3 + qkv.numel()] = qkv.flatten()
+    odd = flat.cuda()[3:3 + qkv.numel()].view(qkv.shape)
+    both = torch.stack([b.k.transpose(1, 2), b.v.transpose(1, 2)], 1).contiguous().cuda()
+    sc = torch.stack([b.k_scale, b.v_scale], 1).cuda()
+    cache = serving.KV8Cache(both[:, 0].transpose(1, 2), both[:, 1].transpose(1, 2), sc[:, 0], sc[:, 1])
+    want, _, bound, _ = S.attention(b.q, *b.cache(), *b.where(), scale=D ** -0.5, heads=(0, 63))
+    for q in (qkv.cuda()[:, 3:67], odd[:, 3:67]):
+        out = torch.zeros((64, b.tokens, D), dtype=torch.bfloat16, device="cuda")
+        shifted = torch.zeros(out.numel() + 9, dtype=torch.bfloat16, device="cuda")[5:5 + out.numel()].view(b.tokens, 64, D)
+        for o in (out.transpose(0, 1), shifted):
+            serving.KV8Attention(cache, q, o, *dev(*b.where()), **b.most).run()
+            sync()
+            for h in (0, 63):
+                S.close(o[:, h], want[:, h], bound[:, h], "bf16")
+
+
+@pytest.mark.parametrize("code", ["i8", "e4m3"])
+@pytest.mark.parametrize("D,page", [(64, 16), (128, 16), (96, 256), (256, 64)])
+def test_many_rows_behind_long_contexts(serving, D, page, code):  # noqa: F811
+    """Pages and scales are fetched for 16 steps at once: several such fetches, of odd and even numbers."""
+    b = S.Batch([(40, 2100), (33, 3333), (40, 4160), (36, 1024), (40, 2048), (40, 1025), (35, 5000), (40, 64)], D=D, page=page, code=code,
+                dt="bf16", seed=D, **MANY)
+    check(b, *attend(serving, b), heads=(0, 63))
+
+
+def test_many_rows_out_of_range_is_reported_and_stays_inside(serving):  # noqa: F811
+    from ktir_cpu_amd import runtime as rt
+    for what in ("page past the cache", "negative page", "length past the table", "tokens past the batch", "max_k", "max_q"):
+        b = S.Batch([(130, 140), (90, 1160), (70, 70)], D=64, pad=1, **MANY)
+        table, q_start, kv_len = [x.clone() for x in b.where()]
+        most = dict(b.most)
+        if what == "page past the cache":
+            table[1, 3] = b.pages
+        elif what == "negative page":
+            table[1, 71] = -5
+        elif what == "length past the table":
+            kv_len[1] = 16 * b.width + 9
+            most["max_k"] = 1 << 20
+        elif what == "tokens past the batch":
+            q_start[3] = 100000
+        elif what == "max_k":
+            most["max_k"] = 1150
+        else:
+            most["max_q"] = 100
+        print(what, flush=True)
+        serving.KV8Attention(serving.KV8Cache(*dev(*b.cache())), b.q.cuda(), torch.zeros_like(b.q).cuda(), *dev(table, q_start, kv_len),
+                             **most).run()
+        torch.cuda.synchronize()
+        with pytest.raises(IndexError, match="outside"):
+            rt.sync()
+    rt.sync()
 
 
 # ---- codes that are NaN ------------------------------------------------------------------
