@@ -509,8 +509,8 @@ typedef struct ktir_rows3 {
  *   (x, y) = the pair's values: columns i and i + rot / 2, or 2 i and 2 i + 1 (interleaved)
  *   out = (x c - y s, y c + x s)
  * and columns from rot on are copied.  a, c and s are made in 64 bits, c and s rounded
- * to f32, the products are f32, and the result is rounded once.  `inverse` is the rotation
- * back: the gradient's way through the operator.  Rows of tokens with
+ * to f32, the products are f32, and the result is rounded once.  `inverse` is the
+ * transposed map, the gradient's way through the operator (and the way back where amplitude is 1).  Rows of tokens with
  * pos < 0 are left as they were.  Two tensors (queries and keys) share one
  * launch; heads2 = 0: one.  An output may be its input itself (and the
  * two tensors parts of one projection's rows, side by side).  dtype: KTIR_F16, KTIR_BF16 or KTIR_F32. */
@@ -581,7 +581,7 @@ int ktir_launch_kv8_append(const ktir_kv8_append_t* d);
  * A row that no token is left for gets 0 and -inf; padding rows are left as
  * they were.  Products of q and codes are exact, sums f32, probabilities enter
  * the second product as ktir_kv8_rows.hip and ktir_kv8_tile.hip say; the result is
- * rounded once to dtype (KTIR_F16 or KTIR_BF16, of q and out).  Codes of tokens past kv_len are not
+ * rounded once to dtype (KTIR_F16 or KTIR_BF16, of q and out).  Value scales below 2^-100 count as that.  Codes of tokens past kv_len are not
  * looked at, nor those before the window of a sequence's first new token, where pages that
  * end before it need no table entry; an e4m3 NaN code of a value may make any row of its
  * sequence NaN.

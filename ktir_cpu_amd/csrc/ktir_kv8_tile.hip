@@ -17,10 +17,11 @@
 //
 // Bound: the instructions of a wavefront one after another, vector and matrix ones.  8192
 // tokens, 32 / 8 heads of 128 columns, causal, i8 codes, 550 GFLOP and half as many for the
-// second terms: 778 to 818 us on two cards (e4m3 747 to 781); 64 columns 525, 16 / 4 heads of 256 1087.
-// With one term of w 628 to 634, 598 to 605, 410 and 963 on the second of the cards: there the matrix pipe is
-// busy 44 % of the time, the vector pipe 58 %, LDS 38 %, so that the two wavefronts of a SIMD hardly
-// cover each other.
+// second terms: 743 to 818 us on five cards (e4m3 739 to 781); 64 columns 504 to 525, 16 / 4 heads of
+// 256 columns 1087 to 1098.  The matrix pipe is busy 51 % of the time, the vector pipe 58 %, LDS 30 %: the two
+// wavefronts of a SIMD hardly cover each other.  A wavefront issues 41 % of its time and waits
+// for data and barriers 32 %, for a pipe 27 %.  With one term of w 628 to 634, 598 to 605, 410 and 963 on the
+// card of 815, the matrix pipe busy 44 %.
 // Before, with one term: 1193 us in ktir_kv8_rows.hip, 906 with four wavefronts of 64 rows, 677 without the
 // next scores beside, 630 side by side (634 on a card that takes 592 in turns); not faster: matrix instructions pinned
 // between vector ones, seven to one (660 to 700), operands read six products ahead (604).  With two

@@ -17,8 +17,8 @@ object with ``__cuda_array_interface__`` (bf16 as uint16, e4m3 codes as uint8, a
 arrays travel elsewhere in this package).  The last dimension is contiguous;
 other strides are free within the limits that the header names.
 
-Streams: ``run(stream)`` launches on a torch stream or a raw handle (0 is the
-null stream).  Without one, a launch on torch tensors goes to torch's current
+Streams: ``run(stream)`` launches on a torch stream of the library's device or a raw
+handle (0 is the null stream).  Without one, a launch on torch tensors goes to torch's current
 stream, so it is ordered with the torch operations around it and can be captured
 into a graph; a launch on other arrays goes to the library's stream, as all else
 here.  Nothing waits: ``runtime.sync()`` waits for the library's stream, and
@@ -236,8 +236,9 @@ class Rope(_Launch):
 
     `positions` [tokens] int32 or int64, tokens at negative ones are skipped;
     `freq` [rot / 2] float64, radians per position: the first rot columns turn, the
-    others are copied.  `out` / `k_out` None: in place.  `inverse` turns back,
-    which is also how a gradient of the output becomes one of the input.
+    others are copied.  `out` / `k_out` None: in place.  `inverse` turns by the opposite
+    angles, `amplitude` as it is: how a gradient of the output becomes one of the input,
+    and the way back where the amplitude is 1.
     """
 
     entry = "ktir_launch_rope"
