@@ -607,6 +607,85 @@ typedef struct ktir_kv8_attn {
 int ktir_kv8_attention_plan(ktir_kv8_attn_t* d);      /* sets splits and ws_bytes */
 int ktir_launch_kv8_attention(const ktir_kv8_attn_t* d);
 
+/* ---- drafted tokens ----
+ * New tokens of a sequence may be a tree instead of a line: token i's parent is an
+ * earlier new token of the sequence, parents[q_start[s] + i] < i, or -1, the tokens
+ * cached before the new ones.  Its depth is the number of new tokens above it, its
+ * position kv_len[s] - (q_start[s + 1] - q_start[s]) + depth; in the cache it has the
+ * place of any new token, kv_len[s] - (q_start[s + 1] - q_start[s]) + i. */
+
+/* Positions and masks from the parents: for every token i of a sequence
+ *   positions[t] = its position
+ *   bit j % 32 of mask[t * mask_row + j / 32] = whether j is i, or an ancestor of i at a
+ *     position > i's - window (window 0: any), j < 32 * words
+ * which KV heads and layers have in common.  words: 32 at most.  A sequence of more than
+ * 32 * words new tokens is left out, a parent that is none counts as -1, both with the
+ * device error word set.  Rows of tokens outside every sequence are left as they were. */
+typedef struct ktir_draft_tree {
+  uint64_t parents, q_start, kv_len;   /* const int32_t* [tokens], [seqs + 1], [seqs] */
+  uint64_t mask, positions;            /* uint32_t* [tokens, words], int32_t* [tokens] */
+  int64_t seqs, tokens, words, mask_row, window;
+  uint64_t stream;
+} ktir_draft_tree_t;
+int ktir_launch_draft_tree(const ktir_draft_tree_t* d);
+
+/* Rotary positions and append in one: every new token's queries are turned as
+ * ktir_launch_rope does it (q to q_out, rounded once), its keys are turned likewise and
+ * go to the cache with its values, as ktir_launch_kv8_append does it, without being
+ * rounded to 16 bits on the way.  pos: the tokens' positions for the rotation (KTIR_I32 or
+ * KTIR_I64, a negative one counts as 0 with the device error word set), or 0: their places in the cache.
+ * Tokens that the append does not store (outside every sequence, at negative places,
+ * past the table's pages) are left as they were in q_out.  q_out may be q itself. */
+typedef struct ktir_kv8_rope_append {
+  ktir_kv8_t cache;
+  ktir_kv8_batch_t batch;
+  ktir_rows3_t q, q_out, k, v;         /* [tokens, q_heads, columns] and [tokens, heads, columns] */
+  int64_t q_heads, rot;
+  uint64_t pos;                        /* [tokens] or 0 */
+  uint64_t freq;                       /* const double* [rot / 2], radians per position */
+  uint64_t stream;
+  double amplitude;
+  int32_t pos_dtype, dtype, interleaved, pad;
+} ktir_kv8_rope_append_t;
+int ktir_launch_kv8_rope_append(const ktir_kv8_rope_append_t* d);
+
+/* Attention of new tokens that are a tree: as ktir_launch_kv8_attention, but token i of
+ * a sequence sees the tokens cached before the new ones and of the new ones those j
+ * whose bit is set in its row of `mask` (as ktir_launch_draft_tree leaves it; any
+ * other mask does as well, and a row may be 0).  With window > 0 it sees of the tokens
+ * before those at places > pos[t] - window (pos: int32, of each token; 0 if there is no window;
+ * a position before the first new token's place counts as that); the mask says itself what of
+ * the new tokens is in the window.  attn.causal has no effect.  max_q is at most 32 * words. */
+typedef struct ktir_kv8_tree_attn {
+  ktir_kv8_attn_t attn;
+  uint64_t mask, pos;                  /* const uint32_t* [tokens, words], const int32_t* [tokens] or 0 */
+  int64_t mask_row, words;
+} ktir_kv8_tree_attn_t;
+int ktir_kv8_tree_attention_plan(ktir_kv8_tree_attn_t* d);      /* sets attn.splits and attn.ws_bytes */
+int ktir_launch_kv8_tree_attention(const ktir_kv8_tree_attn_t* d);
+
+/* The entries of an accepted path: new token path[s * path_row + i] of sequence s moves
+ * in the cache to the place of new token i, for i < kept[s] (`depth` at most); the
+ * path rises strictly.  Lengths are the caller's: after this the sequence has
+ * kv_len[s] - (new tokens) + kept[s] tokens, and the entries behind them are undefined.  In its
+ * page an entry's codes move as they are.  For a page, a head, and K or V, that entries come to from others:
+ *   scale' = max(max |code| scale_from * (1 / top), 2^-100), and the page's scale before,
+ *            if a token of before or of the path keeps its place in that page, where that is more
+ *   code'  = code * (scale_from * (1 / scale')), rounded
+ * and where scale' is more than the scale before, the codes that stayed are rounded again.  A code that
+ * is NaN stays NaN; entries from a page whose scale is not finite make the page's NaN and their own codes 0.
+ * A path that is too long, leaves its sequence, does not rise, or reaches pages that there
+ * are not is cut before the first such token, with the device error word set.  Sequences share
+ * no page that is written. */
+typedef struct ktir_kv8_keep {
+  ktir_kv8_t cache;
+  ktir_kv8_batch_t batch;
+  uint64_t path, kept;                 /* const int32_t* [seqs, depth], [seqs] */
+  int64_t path_row, depth;
+  uint64_t stream;
+} ktir_kv8_keep_t;
+int ktir_launch_kv8_keep(const ktir_kv8_keep_t* d);
+
 #ifdef __cplusplus
 }
 #endif

@@ -6,6 +6,8 @@
 
 namespace ktir {
 
+typedef uint32_t u4_t __attribute__((ext_vector_type(4)));
+
 constexpr int OUT_OF_RANGE = 2;      // what a kernel leaves in the device error word
 
 // the library's device is current while this lives
@@ -44,6 +46,8 @@ inline hipStream_t stream_of(uint64_t s) {
 int check_kv8(const char* what, const ktir_kv8_t& c, bool written);
 int check_batch(const char* what, const ktir_kv8_batch_t& b, const ktir_kv8_t& c);
 int check_rows3(const char* what, const ktir_rows3_t& r, int64_t tokens, int64_t heads, int64_t columns, bool written);
+int check_kv8_attn(const char* what, const ktir_kv8_attn_t& d, bool tree);      // those of ktir_kv8_attn.hip: the descriptor alone,
+int check_kv8_attn_tensors(const char* what, const ktir_kv8_attn_t& d);         // and its tensors
 int ready(const char* what);         // whether ktir_init has run
 
 // Rows of `width` bytes, counts by counts at steps of so many bytes.

@@ -175,6 +175,28 @@ class KV8Attn(C.Structure):
                 ("dtype", C.c_int32), ("causal", C.c_int32), ("splits", C.c_int32)]
 
 
+class DraftTree(C.Structure):
+    _fields_ = [(n, C.c_uint64) for n in ("parents", "q_start", "kv_len", "mask", "positions")] + \
+               [(n, C.c_int64) for n in ("seqs", "tokens", "words", "mask_row", "window")] + [("stream", C.c_uint64)]
+
+
+class KV8RopeAppend(C.Structure):
+    _fields_ = [("cache", KV8), ("batch", KV8Batch), ("q", Rows3), ("q_out", Rows3), ("k", Rows3), ("v", Rows3),
+                ("q_heads", C.c_int64), ("rot", C.c_int64), ("pos", C.c_uint64), ("freq", C.c_uint64),
+                ("stream", C.c_uint64), ("amplitude", C.c_double), ("pos_dtype", C.c_int32), ("dtype", C.c_int32),
+                ("interleaved", C.c_int32), ("pad", C.c_int32)]
+
+
+class KV8TreeAttn(C.Structure):
+    _fields_ = [("attn", KV8Attn), ("mask", C.c_uint64), ("pos", C.c_uint64), ("mask_row", C.c_int64),
+                ("words", C.c_int64)]
+
+
+class KV8Keep(C.Structure):
+    _fields_ = [("cache", KV8), ("batch", KV8Batch), ("path", C.c_uint64), ("kept", C.c_uint64),
+                ("path_row", C.c_int64), ("depth", C.c_int64), ("stream", C.c_uint64)]
+
+
 class KTIRDeviceError(RuntimeError):
     pass
 
@@ -227,7 +249,9 @@ def _open():
                  "ktir_launch_row_rmw", "ktir_launch_attention", "ktir_rmw_variant", "ktir_shutdown", "ktir_set_row_grid_limit",
                  "ktir_launch_row_rmw_noalloc", "ktir_launch_paged_attention",
                  "ktir_upload_list", "ktir_download_list", "ktir_launch_rope", "ktir_launch_kv8_append",
-                 "ktir_kv8_attention_plan", "ktir_launch_kv8_attention"):
+                 "ktir_kv8_attention_plan", "ktir_launch_kv8_attention", "ktir_launch_draft_tree",
+                 "ktir_launch_kv8_rope_append", "ktir_kv8_tree_attention_plan", "ktir_launch_kv8_tree_attention",
+                 "ktir_launch_kv8_keep"):
         getattr(L, name).restype = C.c_int
     L.ktir_malloc.argtypes = [C.c_uint64, C.POINTER(C.c_uint64)]
     L.ktir_free.argtypes = [C.c_uint64]
@@ -258,6 +282,11 @@ def _open():
     L.ktir_launch_kv8_append.argtypes = [C.POINTER(KV8Append)]
     L.ktir_kv8_attention_plan.argtypes = [C.POINTER(KV8Attn)]
     L.ktir_launch_kv8_attention.argtypes = [C.POINTER(KV8Attn)]
+    L.ktir_launch_draft_tree.argtypes = [C.POINTER(DraftTree)]
+    L.ktir_launch_kv8_rope_append.argtypes = [C.POINTER(KV8RopeAppend)]
+    L.ktir_kv8_tree_attention_plan.argtypes = [C.POINTER(KV8TreeAttn)]
+    L.ktir_launch_kv8_tree_attention.argtypes = [C.POINTER(KV8TreeAttn)]
+    L.ktir_launch_kv8_keep.argtypes = [C.POINTER(KV8Keep)]
     return L
 
 

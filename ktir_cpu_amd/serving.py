@@ -1,5 +1,6 @@
 """Operators of a served model's layer on device arrays: rotary positions, a
-key / value cache in 8 bits, and attention over it.
+key / value cache in 8 bits, attention over it, and the same for drafted tokens that
+are a tree.
 
 They stand next to the launches that KTIR functions become, for programs that
 keep their tensors on the device: each class checks its arrays once, builds the
@@ -11,6 +12,15 @@ descriptor of its entry point in ``include/ktir_hip.h`` and launches it with
     keep = KV8Append(cache, k_rot, v, table, q_start, kv_len)
     attend = KV8Attention(cache, q_rot, out, table, q_start, kv_len, max_q=1, max_k=8192)
     for each step: ...; turn.run(); keep.run(); attend.run()
+
+or, with rotation and append in one launch and new tokens that a draft proposed as a tree:
+
+    tree = DraftTree(parents, q_start, kv_len, mask, positions)
+    store = KV8RopeAppend(cache, q, k, v, freq, table, q_start, kv_len, positions=positions)
+    attend = KV8TreeAttention(cache, q, out, table, q_start, kv_len, mask, max_q=64, max_k=8192)
+    keep = KV8Keep(cache, table, q_start, kv_len, path, kept)
+    for each step: ...; tree.run(); for each layer: store.run(); attend.run(); ...
+                   path, kept = the accepted tokens; for each layer: keep.run()
 
 Arrays are torch tensors on the library's device, :class:`DeviceArray`, or any
 object with ``__cuda_array_interface__`` (bf16 as uint16, e4m3 codes as uint8, as
@@ -132,8 +142,9 @@ class _Launch:
 
     entry = ""
 
-    def __init__(self, desc, views, keep):
+    def __init__(self, desc, views, keep, inner=None):
         self.desc = desc
+        self._inner = desc if inner is None else inner       # what holds the stream and the workspace
         self._keep = keep               # what the descriptor's addresses belong to
         self._ref = C.byref(desc)
         self._call = None
@@ -160,16 +171,31 @@ class _Launch:
         if self._call is None:
             self._first()
         if stream is not None:
-            self.desc.stream = int(getattr(stream, "cuda_stream", stream)) or _NULL_STREAM
+            self._inner.stream = int(getattr(stream, "cuda_stream", stream)) or _NULL_STREAM
         elif self._torch_device is not None:
-            self.desc.stream = self._current(self._torch_device) or _NULL_STREAM
+            self._inner.stream = self._current(self._torch_device) or _NULL_STREAM
         else:
-            self.desc.stream = 0
+            self._inner.stream = 0
         rc = self._call(self._ref)
         if rc:
             rt.check(rc)
-        if self._streams is not None and self.desc.stream not in self._streams:
+        if self._streams is not None and self._inner.stream not in self._streams:
             self._used_on(stream)
+
+    def _own_workspace(self, workspace):
+        """What a planned descriptor needs and the caller did not give."""
+        d = self._inner
+        self.workspace_bytes = int(d.ws_bytes)
+        if not self.workspace_bytes or workspace is not None:
+            return
+        if self._torch_device is not None:
+            torch = sys.modules["torch"]
+            self._own = torch.empty(self.workspace_bytes, dtype=torch.uint8, device=f"cuda:{self._torch_device}")
+            d.ws = self._own.data_ptr()
+            self._streams = {torch.cuda.current_stream(self._torch_device).cuda_stream or _NULL_STREAM}
+        else:
+            self._own = rt.DeviceBuffer(self.workspace_bytes)
+            d.ws = self._own.ptr
 
     def _used_on(self, stream):
         """The own workspace came from torch: it goes to no other tensor before this stream is done with it.
@@ -180,7 +206,7 @@ class _Launch:
         if torch.cuda.is_current_stream_capturing():
             return                                  # (a replay's stream is not known here)
         self._own.record_stream(torch.cuda.current_stream(self._torch_device) if stream is None else stream)
-        self._streams.add(self.desc.stream)
+        self._streams.add(self._inner.stream)
 
 
 # ---- rotary positions --------------------------------------------------------
@@ -325,6 +351,38 @@ class KV8Append(_Launch):
         super().__init__(d, [a, b, *views, *cache.views], (cache, k, v, table, q_start, kv_len))
 
 
+def _attention(cache, q, out, table, q_start, kv_len, max_q, max_k, scale, window, lse):
+    """The descriptor of attention over the cache and its views, before it is planned."""
+    a = _view(q, "q", 3, ("f16", "bf16"))
+    b = _view(out, "out", 3, (a.dtype,))
+    _same("out", b.shape, a.shape)
+    if a.shape[2] != cache.desc.columns:
+        raise ValueError(f"q: {a.shape[2]} columns, the cache has {cache.desc.columns}")
+    batch, views = _batch(table, q_start, kv_len, a.shape[0])
+    d = rt.KV8Attn(cache=cache.desc, batch=batch, q=_rows3(a), out=_rows3(b), q_heads=a.shape[1], max_q=int(max_q),
+                   max_k=int(max_k), window=int(window), scale=a.shape[2] ** -0.5 if scale is None else float(scale),
+                   dtype=rt.SERVING_CODE[a.dtype])
+    views += [a, b, *cache.views]
+    if lse is not None:
+        c = _view(lse, "lse", 2, ("f32",), False)
+        _same("lse", c.shape, a.shape[:2])
+        d.lse, d.lse_tok, d.lse_head = c.ptr, *c.strides
+        views.append(c)
+    return d, views
+
+
+def _given_workspace(d, workspace):
+    """The caller's workspace in a planned descriptor: its views (none without one)."""
+    if workspace is None:
+        return []
+    w = _view(workspace, "workspace", 1, ("u8", "e4m3", "i8", "f32"))
+    size = w.shape[0] * (4 if w.dtype == "f32" else 1)
+    if size < d.ws_bytes or w.ptr % 16:
+        raise ValueError(f"workspace: {size} bytes at {w.ptr:#x}; it takes {d.ws_bytes} on a 16-byte bound")
+    d.ws = w.ptr
+    return [w]
+
+
 class KV8Attention(_Launch):
     """Attention of the batch's new tokens over the cache, the tokens themselves
     (appended before) among it.
@@ -344,37 +402,124 @@ class KV8Attention(_Launch):
 
     def __init__(self, cache: KV8Cache, q, out, table, q_start, kv_len, *, max_q: int, max_k: int,
                  scale: Optional[float] = None, causal: bool = True, window: int = 0, lse=None, workspace=None):
+        d, views = _attention(cache, q, out, table, q_start, kv_len, max_q, max_k, scale, window, lse)
+        d.causal = int(bool(causal))
+        rt.check(rt.opened().ktir_kv8_attention_plan(C.byref(d)))
+        views += _given_workspace(d, workspace)
+        super().__init__(d, views, (cache, q, out, table, q_start, kv_len, lse, workspace))
+        self._own_workspace(workspace)
+
+
+# ---- drafted tokens ----------------------------------------------------------------
+
+class DraftTree(_Launch):
+    """Positions and ancestor masks of a batch whose new tokens are trees.
+
+    `parents` [tokens] int32: of new token i of a sequence (i from 0 in each) an earlier new
+    token of it, or -1 for one that follows the cached tokens; a line (i - 1 for each) is
+    an ordinary sequence.  Writes `positions` [tokens] int32, the cached tokens plus the
+    depth, and `mask` [tokens, words] int32 (words up to 32): bit j % 32 of word j // 32 says whether new
+    token j is the token or an ancestor of it.  `window` > 0: of those the ones at positions
+    > the token's - window.  A sequence has 32 * words new tokens at most.  Heads and layers share the result.
+    """
+
+    entry = "ktir_launch_draft_tree"
+
+    def __init__(self, parents, q_start, kv_len, mask, positions, *, window: int = 0):
+        p, q, n = (_view(x, name, 1, ("i32",)) for x, name in ((parents, "parents"), (q_start, "q_start"), (kv_len, "kv_len")))
+        m, o = _view(mask, "mask", 2, ("i32",)), _view(positions, "positions", 1, ("i32",))
+        _same("q_start", q.shape, (n.shape[0] + 1,))
+        _same("mask", m.shape[:1], p.shape)
+        _same("positions", o.shape, p.shape)
+        d = rt.DraftTree(p.ptr, q.ptr, n.ptr, m.ptr, o.ptr, n.shape[0], p.shape[0], m.shape[1], m.strides[0], int(window), 0)
+        super().__init__(d, [p, q, n, m, o], (parents, q_start, kv_len, mask, positions))
+
+
+class KV8RopeAppend(_Launch):
+    """Rotary positions and append in one launch: `q` [tokens, query heads, columns] is turned into
+    `q_out` (None: in place), `k` [tokens, heads, columns] is turned and goes to the cache with `v`.
+
+    The batch is KV8Append's, the rotation Rope's.  The keys are not rounded to 16 bits between the
+    two, so their codes may differ from those of Rope and KV8Append by the rounding of values half way between codes.
+    `positions` [tokens] int32 or int64: the rotation's positions (DraftTree's for a tree);
+    None: the tokens' places in the cache.  Rows of q_out whose tokens are not stored stay as they were.
+    """
+
+    entry = "ktir_launch_kv8_rope_append"
+
+    def __init__(self, cache: KV8Cache, q, k, v, freq, table, q_start, kv_len, q_out=None, *, positions=None,
+                 interleaved: bool = False, amplitude: float = 1.0):
         a = _view(q, "q", 3, ("f16", "bf16"))
-        b = _view(out, "out", 3, (a.dtype,))
-        _same("out", b.shape, a.shape)
+        o = a if q_out is None else _view(q_out, "q_out", 3, (a.dtype,))
+        b, c, f = _view(k, "k", 3, (a.dtype,)), _view(v, "v", 3, (a.dtype,)), _view(freq, "freq", 1, ("f64",))
+        _same("q_out", o.shape, a.shape)
+        _same("k", b.shape, (a.shape[0], cache.desc.heads, cache.desc.columns))
+        _same("v", c.shape, b.shape)
         if a.shape[2] != cache.desc.columns:
             raise ValueError(f"q: {a.shape[2]} columns, the cache has {cache.desc.columns}")
+        if 2 * f.shape[0] > a.shape[2]:
+            raise ValueError(f"freq: {2 * f.shape[0]} columns to rotate of {a.shape[2]}")
         batch, views = _batch(table, q_start, kv_len, a.shape[0])
-        d = rt.KV8Attn(cache=cache.desc, batch=batch, q=_rows3(a), out=_rows3(b), q_heads=a.shape[1], max_q=int(max_q),
-                       max_k=int(max_k), window=int(window), scale=a.shape[2] ** -0.5 if scale is None else float(scale),
-                       dtype=rt.SERVING_CODE[a.dtype], causal=int(bool(causal)))
-        views += [a, b, *cache.views]
-        if lse is not None:
-            c = _view(lse, "lse", 2, ("f32",), False)
-            _same("lse", c.shape, a.shape[:2])
-            d.lse, d.lse_tok, d.lse_head = c.ptr, *c.strides
-            views.append(c)
-        rt.check(rt.opened().ktir_kv8_attention_plan(C.byref(d)))
-        self.workspace_bytes = int(d.ws_bytes)
-        if workspace is not None:
-            w = _view(workspace, "workspace", 1, ("u8", "e4m3", "i8", "f32"))
-            size = w.shape[0] * (4 if w.dtype == "f32" else 1)
-            if size < self.workspace_bytes or w.ptr % 16:
-                raise ValueError(f"workspace: {size} bytes at {w.ptr:#x}; it takes {self.workspace_bytes} on a 16-byte bound")
-            d.ws = w.ptr
-            views.append(w)
-        super().__init__(d, views, (cache, q, out, table, q_start, kv_len, lse, workspace))
-        if self.workspace_bytes and workspace is None:
-            if self._torch_device is not None:
-                torch = sys.modules["torch"]
-                self._own = torch.empty(self.workspace_bytes, dtype=torch.uint8, device=f"cuda:{self._torch_device}")
-                d.ws = self._own.data_ptr()
-                self._streams = {torch.cuda.current_stream(self._torch_device).cuda_stream or _NULL_STREAM}
-            else:
-                self._own = rt.DeviceBuffer(self.workspace_bytes)
-                d.ws = self._own.ptr
+        d = rt.KV8RopeAppend(cache=cache.desc, batch=batch, q=_rows3(a), q_out=_rows3(o), k=_rows3(b), v=_rows3(c),
+                             q_heads=a.shape[1], rot=2 * f.shape[0], freq=f.ptr, amplitude=float(amplitude),
+                             dtype=rt.SERVING_CODE[a.dtype], interleaved=int(bool(interleaved)))
+        views += [a, o, b, c, f, *cache.views]
+        if positions is not None:
+            p = _view(positions, "positions", 1, ("i32", "i64"))
+            _same("positions", p.shape, a.shape[:1])
+            d.pos, d.pos_dtype = p.ptr, rt.SERVING_CODE[p.dtype]
+            views.append(p)
+        super().__init__(d, views, (cache, q, k, v, freq, table, q_start, kv_len, q_out, positions))
+
+
+class KV8TreeAttention(_Launch):
+    """Attention of drafted tokens over the cache: each sees the tokens cached before the new
+    ones, and of the new ones of its sequence (appended before) those that its row of `mask` names.
+
+    `mask` [tokens, words] int32, words up to 32, as DraftTree writes it: bit j % 32 of word j // 32 is new
+    token j; any other mask does as well, and a row that sees nothing gives 0.  `window` > 0: of the tokens before, those
+    at places > positions[t] - window (`positions` [tokens] int32, DraftTree's); the mask says itself
+    which of the new ones are in the window.  `max_q` is 32 * words at most; the rest as for KV8Attention.
+    """
+
+    entry = "ktir_launch_kv8_tree_attention"
+
+    def __init__(self, cache: KV8Cache, q, out, table, q_start, kv_len, mask, *, max_q: int, max_k: int,
+                 scale: Optional[float] = None, window: int = 0, positions=None, lse=None, workspace=None):
+        inner, views = _attention(cache, q, out, table, q_start, kv_len, max_q, max_k, scale, window, lse)
+        m = _view(mask, "mask", 2, ("i32",))
+        _same("mask", m.shape[:1], (inner.batch.tokens,))
+        if window and positions is None:
+            raise ValueError("positions: a window needs them")
+        d = rt.KV8TreeAttn(attn=inner, mask=m.ptr, mask_row=m.strides[0], words=m.shape[1])
+        views.append(m)
+        if positions is not None:
+            p = _view(positions, "positions", 1, ("i32",))
+            _same("positions", p.shape, m.shape[:1])
+            d.pos = p.ptr
+            views.append(p)
+        rt.check(rt.opened().ktir_kv8_tree_attention_plan(C.byref(d)))
+        views += _given_workspace(d.attn, workspace)
+        super().__init__(d, views, (cache, q, out, table, q_start, kv_len, mask, positions, lse, workspace), d.attn)
+        self._own_workspace(workspace)
+
+
+class KV8Keep(_Launch):
+    """The accepted path of each sequence's new tokens moves to where it belongs in the cache.
+
+    `path` [seqs, depth] int32, `kept` [seqs] int32: new tokens path[s, 0] < path[s, 1] < ... of
+    sequence s, kept[s] of them, take the places of the first kept[s] new ones; `kv_len` still
+    counts all new tokens, and is the caller's to cut afterwards (to kv_len - new + kept).  Entries that stay in their
+    page keep their codes; those that come from another are rounded to that page's scale, which grows where it has to.
+    Run once for each step: a second run would move entries again.
+    """
+
+    entry = "ktir_launch_kv8_keep"
+
+    def __init__(self, cache: KV8Cache, table, q_start, kv_len, path, kept):
+        p, n = _view(path, "path", 2, ("i32",)), _view(kept, "kept", 1, ("i32",))
+        batch, views = _batch(table, q_start, kv_len, (1 << 31) - 1)       # (the tokens themselves are not looked at)
+        _same("path", p.shape[:1], (batch.seqs,))
+        _same("kept", n.shape, p.shape[:1])
+        d = rt.KV8Keep(cache.desc, batch, p.ptr, n.ptr, p.strides[0], p.shape[1], 0)
+        super().__init__(d, [p, n, *views, *cache.views], (cache, table, q_start, kv_len, path, kept))
