@@ -119,7 +119,42 @@ __device__ __forceinline__ void seen(const ktir_kv8_attn_t& d, const Tile& t, in
   token_sees(d, t, (int)((uint32_t)r / (uint32_t)grp), lo, hi);
 }
 
+// What rows see where the new tokens are a tree: of the tokens before them an
+// end, [lo, hi) with one hi for the sequence, and of the new ones the bits of a mask.
+struct KV8Mask {
+  uint64_t mask, pos;    // const uint32_t* [tokens, words], const int32_t* [tokens]
+  int64_t row;
+  int32_t words, pad;
+};
+
+__device__ __forceinline__ int tree_before(const Tile& t) {
+  const int before = t.q.n_kv - t.q.n_new;
+  return before < 0 ? 0 : before < t.keys ? before : t.keys;
+}
+__device__ __forceinline__ int tree_first(const ktir_kv8_attn_t& d, const KV8Mask& m, const Tile& t, int r, int grp) {
+  if (!d.window) return 0;
+  const int before = t.q.n_kv - t.q.n_new, hi = tree_before(t);
+  int pos = ints(m.pos)[t.q.start + (int)((uint32_t)r / (uint32_t)grp)];
+  pos = pos < before ? before : pos;
+  const int64_t lo = (int64_t)pos - d.window + 1;
+  return lo < 0 ? 0 : lo < hi ? (int)lo : hi;
+}
+
+// which of the 32 keys from `key` on a row sees, the first in bit 0; at: its mask's first word, first: its first key of those before
+__device__ __forceinline__ uint32_t tree_bits(const KV8Mask& m, const Tile& t, int64_t at, int first, int key) {
+  const int off = key - (t.q.n_kv - t.q.n_new);
+  auto word = [&](int i) { return i < m.words ? ((const KTIR_G(uint32_t)*)m.mask)[at + i] : 0u; };
+  uint32_t w;
+  if (off <= -32) w = ~0u;
+  else if (off < 0) w = word(0) << -off | ((1u << -off) - 1u);
+  else w = (uint32_t)(((uint64_t)word((off >> 5) + 1) << 32 | word(off >> 5)) >> (off & 31));
+  if (key < first) w &= first - key < 32 ? ~0u << (first - key) : 0u;
+  const int left = t.keys - key;
+  return left >= 32 ? w : left > 0 ? w & ~(~0u << left) : 0u;
+}
+
 // tile `nth` (of TM rows) of sequence s, which is q
+template <bool TREE = false>
 __device__ __forceinline__ Tile tile_at(const ktir_kv8_attn_t& d, int64_t s, const Seq& q, int64_t nth, int TM, int grp, int* err) {
   Tile t = {};
   t.s = s;
@@ -131,6 +166,13 @@ __device__ __forceinline__ Tile tile_at(const ktir_kv8_attn_t& d, int64_t s, con
   if (left <= 0) return t;
   t.row0 = (int)(nth * TM);
   t.rows = left < TM ? (int)left : TM;
+  if constexpr (TREE) {                      // from the first new token's window to the last new token that counts: max_q + window - 1 keys at most
+    const int64_t before = (int64_t)q.n_kv - q.n_new, lo = d.window ? before - d.window + 1 : 0;
+    if (before + d.max_q < t.keys) t.keys = before + d.max_q < 0 ? 0 : (int)(before + d.max_q);
+    t.lo = lo < 0 ? 0 : lo < t.keys ? (int)lo : t.keys;
+    t.hi = t.keys;
+    return t;
+  }
   int x;
   if (nth == 0 && left <= TM) {              // the whole sequence: its first and last token
     token_sees(d, t, 0, &t.lo, &x);
@@ -146,11 +188,12 @@ __device__ __forceinline__ Tile tile_at(const ktir_kv8_attn_t& d, int64_t s, con
 __host__ __device__ inline bool one_tile(const ktir_kv8_attn_t& d, int TM, int grp) { return d.max_q * grp <= TM; }
 
 // tile `slot` of a launch: a sequence each, or found by the batch's offsets
+template <bool TREE = false>
 __device__ __forceinline__ Tile tile_of(const ktir_kv8_attn_t& d, int64_t slot, int TM, int grp, int* err) {
-  if (one_tile(d, TM, grp)) return tile_at(d, slot, seq_of(d.batch, d.cache.page, slot, err), 0, TM, grp, err);
+  if (one_tile(d, TM, grp)) return tile_at<TREE>(d, slot, seq_of(d.batch, d.cache.page, slot, err), 0, TM, grp, err);
   int64_t s, nth;
   const Seq q = seq_of_slot(d.batch, d.cache.page, grp, __builtin_ctz(TM), 1, slot, &s, &nth, err);
-  return nth < 0 ? Tile{} : tile_at(d, s, q, nth, TM, grp, err);
+  return nth < 0 ? Tile{} : tile_at<TREE>(d, s, q, nth, TM, grp, err);
 }
 
 // a tile's fields in scalar registers: they are the same in every lane, or lane i's
@@ -177,6 +220,13 @@ __device__ __forceinline__ Tile lane_of(Tile t, int i) {
   t.lo = lane_of(t.lo, i);
   t.hi = lane_of(t.hi, i);
   return t;
+}
+
+// the parts of a tile's keys, of `part` each from a step's bound on
+template <int STEP>
+__device__ __forceinline__ int tile_parts(const Tile& t, int part) {
+  const int from = t.lo & ~(STEP - 1);
+  return t.hi > from ? (int)((uint32_t)(t.hi - from + part - 1) / (uint32_t)part) : 1;
 }
 
 // whether some row of the tile sees a key of the group that starts at `key`

@@ -1,0 +1,32 @@
+// Attention of drafted tokens over the 8-bit cache: the kernels for many rows.
+#include "ktir_kv8_tile_dev.h"
+#include "ktir_kv8_tree.h"
+
+namespace ktir {
+
+template <int CODE, int J, int W>
+static void tree_tile_go(const ktir_kv8_attn_t& d, const KV8Mask& mask, const TreeTiles& s) {
+  const int part = (int)(((s.span + s.splits - 1) / s.splits + TILE_KEYS - 1) / TILE_KEYS * TILE_KEYS);
+  const unsigned items = (unsigned)(s.slots * d.cache.heads);
+  const hipStream_t st = stream_of(d.stream);
+  hipLaunchKernelGGL((kv8_attn_tile<CODE, J, 1, W, true>), dim3(items * s.splits), dim3(64 * W), 0, st, d, mask, (uint32_t)s.slots, s.splits, part, s.waves, device_error_flag());
+  if (s.splits > 1)
+    hipLaunchKernelGGL((kv8_tile_join<J>), dim3(items, s.waves, 2 * J), dim3(256), 0, st, d, mask, s.splits, part, s.waves, s.TM, device_error_flag());
+}
+
+template <int CODE>
+static void tree_tile_code(const ktir_kv8_attn_t& d, const KV8Mask& mask, const TreeTiles& s) {
+  switch (s.J) {
+    case 1: return tree_tile_go<CODE, 1, 8>(d, mask, s);
+    case 2: return tree_tile_go<CODE, 2, 8>(d, mask, s);
+    default: return tree_tile_go<CODE, 4, 4>(d, mask, s);
+  }
+}
+
+int tree_tile_launch(const ktir_kv8_attn_t& d, const KV8Mask& mask, const TreeTiles& s) {
+  d.cache.dtype == KTIR_I8 ? tree_tile_code<KTIR_I8>(d, mask, s) : tree_tile_code<KTIR_E4M3>(d, mask, s);
+  KTIR_HIP_CHECK(hipGetLastError());
+  return KTIR_OK;
+}
+
+}  // namespace ktir
