@@ -32,10 +32,10 @@ __global__ __launch_bounds__(256) void rope_turn(const ktir_rope_t d, int per) {
 
   for (int i = tid; i < tokens * half; i += 256) {
     const int t = i / half;
-    const int64_t pos = rope_pos(d.pos, d.pos_dtype, t0 + t);
-    rope_angle(d.freq, d.amplitude, d.inverse, pos < 0 ? 0 : pos, i - t * half, &cs[i], &sn[i]);
+    const int64_t pos = rope_pos(d, t0 + t);
+    rope_angle(d, pos < 0 ? 0 : pos, i - t * half, &cs[i], &sn[i]);
   }
-  for (int t = tid; t < tokens; t += 256) live[t] = rope_pos(d.pos, d.pos_dtype, t0 + t) >= 0;
+  for (int t = tid; t < tokens; t += 256) live[t] = rope_pos(d, t0 + t) >= 0;
   __syncthreads();
   if (tid >= wide * step) return;
   for (int u = u0; u < units; u += wide) {

@@ -6,20 +6,22 @@ namespace ktir {
 
 typedef float f4_t __attribute__((ext_vector_type(4)));
 
-// cosine and sine of pair i at a position, times the amplitude, rounded once.  The angle passes
+// cosine and sine of pair i at a position (d: freq, amplitude, inverse), times the amplitude, rounded once.  The angle passes
 // 2^20 radians at far positions, where f32 holds it to a sixteenth: all of it is f64
 // (the vector pipe's f64 and f32 instructions take as long).
-__device__ __forceinline__ void rope_angle(uint64_t freq, double amplitude, bool inverse, int64_t pos, int i, float* c, float* s) {
-  double turns = (double)pos * ((const KTIR_G(double)*)freq)[i] * 0.15915494309189533577;
+template <class D>
+__device__ __forceinline__ void rope_angle(const D& d, int64_t pos, int i, float* c, float* s) {
+  double turns = (double)pos * ((const KTIR_G(double)*)d.freq)[i] * 0.15915494309189533577;
   turns -= rint(turns);
   double sn, cs;
   sincospi(2.0 * turns, &sn, &cs);
-  *c = (float)(cs * amplitude);
-  *s = (float)(inverse ? -(sn * amplitude) : sn * amplitude);
+  *c = (float)(cs * d.amplitude);
+  *s = (float)(d.inverse ? -(sn * d.amplitude) : sn * d.amplitude);
 }
 
-__device__ __forceinline__ int64_t rope_pos(uint64_t pos, int dtype, int64_t t) {
-  return dtype == KTIR_I64 ? ((const KTIR_G(int64_t)*)pos)[t] : (int64_t)ints(pos)[t];
+template <class D>
+__device__ __forceinline__ int64_t rope_pos(const D& d, int64_t t) {
+  return d.pos_dtype == KTIR_I64 ? ((const KTIR_G(int64_t)*)d.pos)[t] : (int64_t)ints(d.pos)[t];
 }
 
 // V pairs: 2 V values as f32, and back.  Half layout: V values at `a` and their V
