@@ -7,41 +7,76 @@ namespace ktir {
 constexpr int64_t TREE_WORDS = 32;           // of a token's mask
 
 // ---- the tree ----------------------------------------------------------------
+//
+// Tokens come after their parents, so 32 of them (a word of the masks) have all other ancestors among
+// the tokens before.  One thread a token: first up the line within its word, at most 32 steps; where that leaves
+// it, the row of the ancestor it comes to has the other words, which are copied word by word of
+// the sequence.  Bound: latency, 32 + 32 steps of LDS for the largest tree, where a walk up the whole line
+// takes as many as the tree is deep.
 
-// One thread a token: up its line of parents, bits from the highest word down.
-__global__ __launch_bounds__(256) void draft_tree(const ktir_draft_tree_t d, int* err) {
+template <int WORDS>
+__global__ __launch_bounds__(32 * WORDS) void draft_tree(const ktir_draft_tree_t d, int* err) {
+  constexpr int N = 32 * WORDS, PITCH = WORDS + 1;
+  __shared__ uint32_t rows[N * PITCH];
+  __shared__ int line[N], depths[N];                // parents, then the first ancestor before a token's word; how many ancestors
+  const int i = threadIdx.x, word = i >> 5;
   const int64_t s = blockIdx.x;
   const int64_t a = ints(d.q_start)[s], e = ints(d.q_start)[s + 1];
+  const int kv = ints(d.kv_len)[s];
   const int64_t start = a < 0 ? 0 : a < d.tokens ? a : d.tokens, end = e < start ? start : e < d.tokens ? e : d.tokens;
-  const int n = (int)(end - start), kv = ints(d.kv_len)[s], before = (kv < 0 ? 0 : kv) - n;
-  if (start != a || end != e || kv < 0 || n > 32 * d.words) {
+  if (start != a || end != e || kv < 0 || end - start > 32 * d.words) {
     *err = OUT_OF_RANGE;
-    if (n > 32 * d.words) return;
+    if (end - start > 32 * d.words) return;
   }
-  const KTIR_G(int32_t)* parents = ints(d.parents) + start;
-  for (int i = (int)(blockIdx.y * 256 + threadIdx.x); i < n; i += 256 * gridDim.y) {
-    KTIR_G(uint32_t)* row = (KTIR_G(uint32_t)*)d.mask + (start + i) * d.mask_row;
-    int j = i, depth = 0;
-    for (int w = (int)d.words - 1; w >= 0; --w) {
-      uint32_t bits = 0;
-      while (j >= 32 * w) {
-        if (!d.window || depth < d.window) bits |= 1u << (j & 31);
-        const int p = parents[j];
-        if (p < -1 || p >= j) *err = OUT_OF_RANGE;
-        j = p < -1 || p >= j ? -1 : p;
-        ++depth;
-      }
-      row[w] = bits;
+  const int n = (int)(end - start);                 // N at most
+  int p = -1;
+  if (i < n) {
+    p = ints(d.parents)[start + i];
+    if (p < -1 || p >= i) *err = OUT_OF_RANGE, p = -1;
+  }
+  line[i] = p;
+  __syncthreads();
+  uint32_t bits = 1u << (i & 31);
+  int steps = 0;
+  while (p >= word * 32) {
+    bits |= 1u << (p & 31);
+    p = line[p];
+    ++steps;
+  }
+  for (int w = word; w < WORDS; ++w) rows[i * PITCH + w] = w == word ? bits : 0u;
+  __syncthreads();
+  line[i] = p;
+  if (p < 0) depths[i] = steps;
+  __syncthreads();
+  for (int b = 0; 32 * b < n; ++b) {                // one thread a word of a row, and one a row for its depth
+    const int t = 32 * b + (i & 31), w = i >> 5, up = line[t];
+    if (w < b) rows[t * PITCH + w] = up < 0 ? 0u : rows[up * PITCH + w];
+    if (word == b && p >= 0) depths[i] = steps + 1 + depths[p];
+    __syncthreads();
+  }
+  if (i < n) ((KTIR_G(int32_t)*)d.positions)[start + i] = (kv < 0 ? 0 : kv) - n + depths[i];
+  const int words = (int)d.words;
+  for (int x = i; x < n * words; x += N) {
+    const int t = x / words, w = x - t * words;
+    uint32_t y = rows[t * PITCH + w];
+    if (d.window && depths[t] >= d.window) {        // the highest `window` bits of the row
+      int left = (int)d.window;
+      for (int k = t >> 5; k > w; --k) left -= __builtin_popcount(rows[t * PITCH + k]);
+      for (int drop = __builtin_popcount(y) - (left > 0 ? left : 0); drop > 0; --drop) y &= y - 1;
     }
-    ((KTIR_G(int32_t)*)d.positions)[start + i] = before + depth - 1;
+    ((KTIR_G(uint32_t)*)d.mask)[(start + t) * d.mask_row + w] = y;
   }
 }
 
 // ---- the kept path -----------------------------------------------------------
-
+//
 // One wavefront for a sequence, a KV head, and K or V.  Entries only move down and in order, so what a
 // page gets is read before its place is written: pages in order, and in a page the rows of
-// one pass of the wavefront (64 units of 16 columns), all read, then written.
+// one pass of the wavefront (64 units of 16 columns), all read, then written.  Bound: latency, offsets and path ->
+// table -> scales and codes; a lane has the place, page and scale that one entry of 64 comes from.
+
+constexpr int KEEP_KEPT = 2;         // passes of rows that stay in registers between the maximum and the codes
+
 template <int CODE>
 __global__ __launch_bounds__(256) void kv8_keep(const ktir_kv8_keep_t d, int* err) {
   const ktir_kv8_t& c = d.cache;
@@ -49,11 +84,13 @@ __global__ __launch_bounds__(256) void kv8_keep(const ktir_kv8_keep_t d, int* er
   if (hv >= 2 * c.heads) return;
   const int64_t head = hv >> 1, s = blockIdx.x;
   const bool is_v = hv & 1;
-  const Seq q = seq_of(d.batch, c.page, s, err);
   const KTIR_G(int32_t)*path = ints(d.path) + s * d.path_row, *table = ints(d.batch.table) + s * d.batch.table_row;
-  const int before = uni(q.n_kv - q.n_new), shift = __builtin_ctz((uint32_t)c.page), rows = (int)c.page;
-  int n = ints(d.kept)[s];
-  if (n < 0 || n > d.depth || n > q.n_new) {
+  // (the first entries and their count on their way with the offsets)
+  int mine = l < d.depth ? path[l] : 0, n = ints(d.kept)[s];
+  const Seq q = seq_of(d.batch, c.page, s, err);
+  const int before = uni(q.n_kv - q.n_new), held = uni(q.n_held), fresh = uni(q.n_new), shift = __builtin_ctz((uint32_t)c.page), rows = (int)c.page;
+  n = uni(n);
+  if (n < 0 || n > d.depth || n > fresh) {
     *err = OUT_OF_RANGE;
     n = n < 0 ? 0 : n > d.depth ? (int)d.depth : n;
   }
@@ -61,75 +98,124 @@ __global__ __launch_bounds__(256) void kv8_keep(const ktir_kv8_keep_t d, int* er
     if (n > 0) *err = OUT_OF_RANGE;
     return;
   }
+  const uint64_t codes = is_v ? c.v + head * c.v_head : c.k + head * c.k_head, scales = is_v ? c.v_scale + head * c.vs_head * 4 : c.k_scale + head * c.ks_head * 4;
+  const int64_t code_page = is_v ? c.v_page : c.k_page, tok = is_v ? c.v_tok : c.k_tok, scale_page = is_v ? c.vs_page : c.ks_page;
+  auto scale_of = [&](int64_t page) { return (KTIR_G(float)*)scales + page * scale_page; };
+  auto row_at = [&](int64_t page, int row) { return (KTIR_G(uint8_t)*)codes + page * code_page + row * tok; };
+
+  // entries base .. base + 63, one a lane: the place in the cache that each comes from, its page and scale, and its new page
+  int base = 0, src = 0, from_page = 0, to_page = 0;
+  float from_scale = 0.f;
   // the first entry that is none, and the first that moves
   int good = n, from = n;
-  for (int base = 0; base < n; base += 64) {
+  for (base = 0; base < n; base += 64) {
     const int i = base + l;
-    bool bad = false, moves = false;
-    if (i < n) {
-      const int p = path[i], last = i ? path[i - 1] : -1;
-      bad = p <= last || p >= q.n_new || before + p >= q.n_held;
-      moves = p != i;
-      if (!bad) {
-        const int a = table[(before + i) >> shift], b = table[(before + p) >> shift];
-        bad = (uint32_t)a >= (uint64_t)c.pages || (uint32_t)b >= (uint64_t)c.pages;
-      }
+    if (base) mine = i < n ? path[i] : 0;
+    int last = __shfl_up(mine, 1);
+    if (l == 0) last = base ? path[base - 1] : -1;
+    src = before + mine;
+    bool bad = i < n && (mine <= last || mine >= fresh || src >= held);
+    if (i < n && !bad) {
+      to_page = table[(before + i) >> shift];
+      from_page = table[src >> shift];
+      bad = (uint32_t)to_page >= (uint64_t)c.pages || (uint32_t)from_page >= (uint64_t)c.pages;
     }
-    const uint64_t stop = __ballot(bad), go = __ballot(moves);
+    const uint64_t stop = __ballot(bad), go = __ballot(i < n && mine != i);
     if (from == n && go) from = base + __builtin_ctzll(go);
     if (stop) {
       good = base + __builtin_ctzll(stop);
       *err = OUT_OF_RANGE;
       break;
     }
+    if (n <= 64) break;
   }
-  n = uni(good);
-  from = uni(from);
+  n = good;
   if (from >= n) return;
-
-  const uint64_t codes = is_v ? c.v + head * c.v_head : c.k + head * c.k_head, scales = is_v ? c.v_scale + head * c.vs_head * 4 : c.k_scale + head * c.ks_head * 4;
-  const int64_t code_page = is_v ? c.v_page : c.k_page, tok = is_v ? c.v_tok : c.k_tok, scale_page = is_v ? c.vs_page : c.ks_page;
-  auto scale_of = [&](int64_t page) { return (KTIR_G(float)*)scales + page * scale_page; };
-  auto row_at = [&](int64_t page, int row) { return (KTIR_G(uint8_t)*)codes + page * code_page + row * tok; };
+  if (base + l < n) from_scale = *scale_of(from_page);
+  auto fetch = [&](int at) {                 // entries from `at` on, where the ones at hand are others
+    base = at;
+    if (at + l >= n) return;
+    src = before + path[at + l];
+    to_page = table[(before + at + l) >> shift];
+    from_page = table[src >> shift];
+    from_scale = *scale_of(from_page);
+  };
   const int G = (int)c.columns >> 4, per = 64 / G, r = l / G, col = (l - r * G) * 16;
-  const bool mine = r < per;
+  auto need = [&](int at, int end) {         // entries [at, end), 64 at most, at hand
+    if (at < base || end > base + 64) fetch(at);
+  };
+  auto rounded = [&](u4_t w, float ratio) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      float x[4];
+      values4<CODE>(w[k], x);
+#pragma unroll
+      for (int y = 0; y < 4; ++y) x[y] *= ratio;
+      w[k] = codes4<CODE, CODE == KTIR_E4M3>(x);
+    }
+    return w;
+  };
 
   for (int p = (before + from) >> shift; p <= (before + n - 1) >> shift; ++p) {
     const int first = p << shift, lo = first > before ? first - before : 0;              // the path's entries of this page: from lo
     const int hi = (int64_t)first + rows - before < n ? first - before + rows : n;       // to hi
-    const int64_t page = table[p];
+    // a unit of each row: where it comes from, whether from this page, its scale and codes
+    struct Unit {
+      int64_t page;
+      float scale;
+      bool on, here;
+      u4_t w;
+    };
+    auto load = [&](int i, Unit& u) {
+      need(i, i + per < hi ? i + per : hi);
+      const int k = i + r - base;
+      u.on = r < per && i + r < hi;
+      const int place = __shfl(src, k & 63);
+      u.page = __shfl(from_page, k & 63);
+      u.scale = __shfl(from_scale, k & 63);
+      u.here = place >> shift == p;
+      u.w = u4_t{0, 0, 0, 0};
+      if (u.on) u.w = *(const KTIR_G(u4_t)*)(row_at(u.page, place & (rows - 1)) + col);
+    };
+    need(lo, lo + 64 < hi ? lo + 64 : hi);
+    const int64_t page = __shfl(to_page, lo - base);
+    const float scale = *scale_of(page);
     // entries of other pages: the largest value; whether something stays
     float top = 0.f;
-    bool finite = true, stays = first < before;
-    int came = 0;
-    for (int i = lo; i < hi; i += per) {
-      const int at = i + r;
-      if (!mine || at >= hi) continue;
-      const int src = before + path[at];
-      if (src >> shift == p) {
-        stays = true;
-        continue;
-      }
-      came = 1;
-      const int64_t sp = table[src >> shift];
-      const float sc = *scale_of(sp);
-      finite = finite && sc < __builtin_inff();
-      const u4_t w = *(const KTIR_G(u4_t)*)(row_at(sp, src & (rows - 1)) + col);
+    bool finite = true, stays = first < before, came = false;
+    auto look = [&](const Unit& u) {
+      if (!u.on) return;
+      stays = stays || u.here;
+      came = came || !u.here;
+      if (u.here) return;
+      finite = finite && u.scale < __builtin_inff();
       float most = 0.f;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         float x[4];
-        values4<CODE>(w[k], x);
+        values4<CODE>(u.w[k], x);
 #pragma unroll
         for (int y = 0; y < 4; ++y) most = __builtin_fmaxf(most, __builtin_fabsf(x[y]));
       }
-      top = __builtin_fmaxf(top, most * sc);
+      top = __builtin_fmaxf(top, most * u.scale);
+    };
+    Unit unit[KEEP_KEPT];
+#pragma unroll
+    for (int k = 0; k < KEEP_KEPT; ++k) {
+      unit[k].on = false;
+      if (lo + k * per < hi) load(lo + k * per, unit[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < KEEP_KEPT; ++k) look(unit[k]);
+    for (int i = lo + KEEP_KEPT * per; i < hi; i += per) {
+      Unit u;
+      load(i, u);
+      look(u);
     }
     for (int o = 32; o; o >>= 1) top = __builtin_fmaxf(top, __shfl_xor(top, o));
     finite = __all(finite);
     stays = __any(stays);
     came = __any(came);
-    const float scale = *scale_of(page);
     float now = scale;
     if (came) {
       now = __builtin_fmaxf(top * PER_TOP<CODE>, LEAST_SCALE);
@@ -138,36 +224,27 @@ __global__ __launch_bounds__(256) void kv8_keep(const ktir_kv8_keep_t d, int* er
     }
     const bool nan = !(now < __builtin_inff()), grown = came && stays && now > scale;
     const float inv = 1.f / now, again = scale * inv;
-    auto rounded = [&](u4_t w, float ratio) {
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        float x[4];
-        values4<CODE>(w[k], x);
-#pragma unroll
-        for (int y = 0; y < 4; ++y) x[y] *= ratio;
-        w[k] = codes4<CODE, CODE == KTIR_E4M3>(x);
-      }
-      return w;
-    };
     if (grown)
-      for (int row = r; mine && row < before - first; row += per) {
+      for (int row = r; r < per && row < before - first; row += per) {
         KTIR_G(u4_t)* w = (KTIR_G(u4_t)*)(row_at(page, row) + col);
         *w = rounded(*w, again);
       }
-    for (int i = lo; i < hi; i += per) {
-      const int at = i + r;
-      const bool on = mine && at < hi;
-      const int src = before + (on ? path[at] : 0), row = (before + at) & (rows - 1);
-      const bool here = src >> shift == p;
-      const int64_t sp = table[src >> shift];
-      u4_t w = {0, 0, 0, 0};
-      if (on) w = *(const KTIR_G(u4_t)*)(row_at(sp, src & (rows - 1)) + col);
-      if (!here) w = nan ? u4_t{0, 0, 0, 0} : rounded(w, *scale_of(sp) * inv);
+    auto put = [&](int i, const Unit& u) {
+      u4_t w = u.w;
+      if (!u.here) w = nan ? u4_t{0, 0, 0, 0} : rounded(w, u.scale * inv);
       else if (grown) w = rounded(w, again);
       // (a lane's place may be another's source: no lane stores before all have loaded)
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       __builtin_amdgcn_wave_barrier();
-      if (on) *(KTIR_G(u4_t)*)(row_at(page, row) + col) = w;
+      if (u.on) *(KTIR_G(u4_t)*)(row_at(page, (before + i + r) & (rows - 1)) + col) = w;
+    };
+#pragma unroll
+    for (int k = 0; k < KEEP_KEPT; ++k)
+      if (lo + k * per < hi) put(lo + k * per, unit[k]);
+    for (int i = lo + KEEP_KEPT * per; i < hi; i += per) {
+      Unit u;
+      load(i, u);
+      put(i, u);
     }
     if (came && l == 0) *scale_of(page) = now;
   }
@@ -199,7 +276,11 @@ extern "C" int ktir_launch_draft_tree(const ktir_draft_tree_t* d) {
   if (rc != KTIR_OK) return rc;
   OnDevice on;
   if (!on.ok()) return set_error(KTIR_E_HIP, "%s: no device", ME);
-  hipLaunchKernelGGL(draft_tree, dim3((unsigned)d->seqs, (unsigned)((d->words + 7) / 8)), dim3(256), 0, stream_of(d->stream), *d, device_error_flag());
+  const dim3 grid((unsigned)d->seqs);
+  const hipStream_t st = stream_of(d->stream);
+  if (d->words <= 4) hipLaunchKernelGGL(draft_tree<4>, grid, dim3(128), 0, st, *d, device_error_flag());
+  else if (d->words <= 16) hipLaunchKernelGGL(draft_tree<16>, grid, dim3(512), 0, st, *d, device_error_flag());
+  else hipLaunchKernelGGL(draft_tree<32>, grid, dim3(1024), 0, st, *d, device_error_flag());
   KTIR_HIP_CHECK(hipGetLastError());
   return KTIR_OK;
 }

@@ -2,30 +2,134 @@
 //
 // Two kinds of workgroups.  One turns queries: a few tokens, whose angles it makes once (in 64
 // bits) for all heads, two rows of 16-byte loads a thread ahead of the stores.  The other has a page that new
-// tokens fall in, and K or V: a wavefront a head (four where a page's part of a head is more
-// than 256 units of 16 columns), its turned values in f32 registers from the maximum to the
+// tokens fall in, and K or V: one, two or four wavefronts a head, its turned values in f32 registers from the maximum to the
 // codes.  A unit of K loads its 16 columns and those that they are turned with, which a neighbour
 // has just loaded: all layouts of pairs then store 16 codes at once.
+//
+// Bound: bytes, queries in and out and keys and values in once, codes out.  8192 tokens of 32 / 8 heads of 128 columns, 185
+// MB: 40.8 us = 4.5 TB/s (a copy of 256 MiB makes 5.4; the rotation and the append by themselves take 31.8 and 12.5).
+// 182 us with an element a thread, 52 with four units a thread (fewer wavefronts a CU), 47.6 with the loads behind the
+// angles, 43 with eight tokens a workgroup of queries.  The two kinds in turn take 63 to 70: in one launch their
+// streams do not go together.  Queries first 44.4, four rows of loads ahead 43.7.
+// Few tokens are latency, and have kernels of their own below.
+#include <type_traits>
+
 #include "ktir_kv8_codes.h"
 #include "ktir_rope_dev.h"
 
 namespace ktir {
 
-constexpr int TURN_PAIRS = 2048;     // angles in LDS
 constexpr int TURN_TOKENS = 8;       // of a workgroup that turns queries
-constexpr int TURN_KEPT = 4;         // units of 16 columns that a thread keeps
-
-struct Angles {
-  uint64_t freq;
-  double amplitude;
-  bool inverse;
-};
+constexpr int TURN_KEPT = 2;         // units of 16 columns that a thread keeps
+// angles in LDS: eight tokens' queries, or the keys of the rows that W wavefronts keep (64 W units each, half of 16 columns a unit)
+constexpr int turn_pairs(int W) { return 1024 * W; }
 
 // how a launch is cut: workgroups of keys and values first, then those of queries
 struct TurnGrid {
-  int kv;              // workgroups for a page: of keys, then as many of values
-  int slots;           // pages
+  int kv, slots;       // workgroups for a page, of keys, then as many of values; pages
   int per, parts;      // tokens of a workgroup of queries, workgroups that share their heads
+};
+
+__device__ __forceinline__ double frequency(const ktir_kv8_rope_append_t& d, int i) { return ((const KTIR_G(double)*)d.freq)[i]; }
+// The angles of `rows` rows into cs and sn, by all threads; `first`: the frequency of a thread's first
+// pair, loaded before anything else is known; pos(row): a row's position, below 0 for one without
+template <class Pos>
+__device__ __forceinline__ void turn_angles(const ktir_kv8_rope_append_t& d, int rows, double first, float* cs, float* sn, Pos pos) {
+  const int half = (int)d.rot / 2, total = rows * half;
+  const bool same = 256 % half == 0;                 // a thread's pairs are one
+  double f = first;
+  for (int i = threadIdx.x; i < total;) {
+    const int row = i / half;
+    const int64_t p = pos(row);
+    if (p >= 0) rope_angle_of(p, f, d.amplitude, false, &cs[i], &sn[i]);
+    i += 256;
+    if (!same && i < total) f = frequency(d, i % half);
+  }
+}
+
+// The position of a token's rotation; false where the token is not stored.
+__device__ __forceinline__ bool token_position(const ktir_kv8_rope_append_t& d, int64_t token, int64_t* pos, int* err) {
+  int64_t s, nth;
+  const int64_t given = d.pos ? rope_pos(d, token) : 0;
+  const Seq q = seq_of_slot(d.batch, d.cache.page, 1, 0, 0, token, &s, &nth, err);
+  const int64_t place = (int64_t)q.n_kv - q.n_new + nth;
+  if (nth < 0 || nth >= q.n_new || place < 0 || place >= q.n_held) return false;
+  if (given < 0) *err = OUT_OF_RANGE;
+  *pos = !d.pos ? place : given < 0 ? 0 : given;
+  return true;
+}
+
+// What of a page's slot of a launch is new: n rows from row r0 on, tokens from t0 on, whose places are from lo on.
+struct PagePart {
+  int64_t page, t0, lo;
+  int n, r0;
+  bool there;          // whether the table's page is one of the cache's
+};
+__device__ __forceinline__ bool page_part(const ktir_kv8_rope_append_t& d, int slot, PagePart* part, int* err) {
+  const ktir_kv8_t& c = d.cache;
+  const int shift = __builtin_ctz((uint32_t)c.page);
+  int64_t s, nth;
+  const Seq q = seq_of_slot(d.batch, c.page, 1, shift, 2, slot, &s, &nth, err);
+  if (nth < 0) return false;
+  const int64_t pos0 = (int64_t)q.n_kv - q.n_new, from = pos0 < 0 ? 0 : pos0;      // the first position that is stored
+  const int64_t p = (from >> shift) + nth;                                       // the page's number in the sequence
+  const int64_t lo = p << shift < from ? from : p << shift, hi = (p + 1) << shift < q.n_held ? (p + 1) << shift : q.n_held;
+  if (lo >= hi) return false;
+  const int64_t page = ints(d.batch.table)[s * d.batch.table_row + p];
+  *part = {page, q.start + lo - pos0, lo, (int)(hi - lo), (int)(lo & (c.page - 1)), page >= 0 && page < c.pages};
+  return true;
+}
+__device__ __forceinline__ int64_t row_position(const ktir_kv8_rope_append_t& d, const PagePart& part, int row, int* err) {
+  const int64_t pos = d.pos ? rope_pos(d, part.t0 + row) : part.lo + row;
+  if (pos < 0) *err = OUT_OF_RANGE;
+  return pos < 0 ? 0 : pos;
+}
+
+// Where a page's part of a head lies.
+template <bool IS_K>
+struct PageHead {
+  KTIR_G(uint8_t)* codes;
+  KTIR_G(float)* scale;
+  int64_t tok;
+  __device__ __forceinline__ PageHead(const ktir_kv8_rope_append_t& d, const PagePart& part, int64_t head) {
+    const ktir_kv8_t& c = d.cache;
+    codes = (KTIR_G(uint8_t)*)(IS_K ? c.k + part.page * c.k_page + head * c.k_head : c.v + part.page * c.v_page + head * c.v_head);
+    scale = IS_K ? (KTIR_G(float)*)c.k_scale + part.page * c.ks_page + head * c.ks_head : (KTIR_G(float)*)c.v_scale + part.page * c.vs_page + head * c.vs_head;
+    tok = IS_K ? c.k_tok : c.v_tok;
+  }
+};
+
+// A page's scale with new values, of absolute bits `top` at most (they grow with the value, and past infinity's for NaN).
+struct NewScale {
+  float scale, inv, ratio;
+  bool nan;
+  __device__ __forceinline__ NewScale(int code, uint32_t top, float before) {
+    const float most = __uint_as_float(top);
+    scale = __builtin_fmaxf(most * (code == KTIR_I8 ? PER_TOP<KTIR_I8> : PER_TOP<KTIR_E4M3>), LEAST_SCALE);
+    if (!(scale >= before)) scale = before;                     // a page that was NaN stays so
+    if (!(most < __builtin_inff())) scale = __builtin_nanf("");
+    nan = !(scale < __builtin_inff());
+    inv = 1.f / scale;
+    ratio = before * inv;
+  }
+  // the page's older rows, up to `end`, rounded to it by `threads` threads
+  __device__ __forceinline__ void again(const ktir_kv8_t& c, KTIR_G(uint8_t)* codes, int64_t tok, int end, int tid, int threads) const {
+    const int G = (int)c.columns >> 4;
+    for (int i = tid; i < end * G; i += threads) {
+      KTIR_G(u4_t)* w = (KTIR_G(u4_t)*)(codes + i / G * tok + i % G * 16);
+      u4_t y = *w;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        float v[4];
+        if (c.dtype == KTIR_I8) values4<KTIR_I8>(y[k], v);
+        else values4<KTIR_E4M3>(y[k], v);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) v[x] *= ratio;
+        y[k] = c.dtype == KTIR_I8 ? codes4<KTIR_I8>(v) : codes4<KTIR_E4M3, true>(v);
+      }
+      *w = y;
+    }
+  }
 };
 
 // ---- queries -----------------------------------------------------------------
@@ -33,79 +137,92 @@ struct TurnGrid {
 template <int DT, bool INTER, int V, bool PAST>
 __device__ __forceinline__ void turn_queries(const ktir_kv8_rope_append_t& d, int block, const TurnGrid& g, float* cs, float* sn, int64_t* place, int* err) {
   constexpr int R = 2;
+  const double f0 = frequency(d, threadIdx.x % (uint32_t)(d.rot / 2));
   const int tid = threadIdx.x, half = (int)d.rot / 2, rot = (int)d.rot, columns = (int)d.cache.columns, pairs = half / V;
   const int64_t t0 = (int64_t)(block / g.parts) * g.per;
   const int tokens = (int)(d.batch.tokens - t0 < g.per ? d.batch.tokens - t0 : g.per), heads = (int)d.q_heads;
-  // a token's position, or -1 where it is not stored
-  for (int t = uni((int)(tid >> 6)); t < tokens; t += 4) {
-    int64_t s, nth;
-    const Seq q = seq_of_slot(d.batch, d.cache.page, 1, 0, 0, t0 + t, &s, &nth, err);
-    int64_t pos = (int64_t)q.n_kv - q.n_new + nth;
-    if (nth < 0 || nth >= q.n_new || pos < 0 || pos >= q.n_held) {
-      pos = -1;
-    } else if (d.pos) {
-      pos = rope_pos(d, t0 + t);
-      if (pos < 0) *err = OUT_OF_RANGE, pos = 0;
-    }
-    if ((tid & 63) == 0) place[t] = pos;
-  }
-  __syncthreads();
-  for (int i = tid; i < tokens * half; i += 256) {
-    const int t = i / half;
-    if (place[t] >= 0) rope_angle(Angles{d.freq, d.amplitude, false}, place[t], i - t * half, &cs[i], &sn[i]);
-  }
-  __syncthreads();
   const bool tail = d.q.ptr != d.q_out.ptr;
   const int units = pairs + (tail ? (columns - rot + 2 * V - 1) / (2 * V) : 0);
   const int wide = units < 256 ? units : 256, step = 256 / wide, stride = step * g.parts, total = tokens * heads;
-  if (tid >= wide * step) return;
-  for (int u = tid % wide; u < units; u += wide) {
-    int a, b;
+  // R rows of a unit at a time; the first ones' loads are ahead of the angles
+  struct Rows {
+    RopeRaw<DT, V> r[R];
+    int t[R], h[R];
+  };
+  int u = tid % wide, a, b;
+  bool two;
+  auto columns_of = [&]() {
     rope_columns<INTER, V>(u, pairs, half, rot, &a, &b);
-    const bool two = b < columns;
+    two = b < columns;                       // the last unit behind rot may be half one
     if (!two) b = a;
-    int row = block % g.parts * step + tid / wide, t = 0, h = row;
-    while (row < total) {
-      RopeRaw<DT, V> r[R];
-      int at[R];
-      int64_t to[R];
-      bool on[R];
+  };
+  auto fetch = [&](int row, Rows& x) {
 #pragma unroll
-      for (int k = 0; k < R; ++k) {
-        while (h >= heads) {
-          h -= heads;
-          ++t;
-        }
-        on[k] = row < total && place[t < tokens ? t : 0] >= 0;
-        to[k] = (t0 + t) * d.q_out.tok + h * d.q_out.head;
-        at[k] = t * half + u * V;
-        if (on[k]) {
-          const int64_t e = (t0 + t) * d.q.tok + h * d.q.head;
-          rope_load<DT, V, PAST>(d.q.ptr, e + a, e + b, r[k]);
-        }
-        row += stride;
-        h += stride;
+    for (int k = 0; k < R; ++k, row += stride) {
+      x.t[k] = (int)((uint32_t)row / (uint32_t)heads);
+      x.h[k] = row - x.t[k] * heads;
+      if (row < total) {
+        const int64_t e = (t0 + x.t[k]) * d.q.tok + x.h[k] * d.q.head;
+        rope_load<DT, V, PAST>(d.q.ptr, e + a, e + b, x.r[k]);
+      } else {
+        x.t[k] = -1;
       }
+    }
+  };
+  const int row0 = block % g.parts * step + tid / wide;
+  const bool mine = tid < wide * step;
+  Rows now;
+  columns_of();
+  if (mine) fetch(row0, now);
+  // a token's position, or -1 where it is not stored
+  auto position = [&](int64_t token) {
+    int64_t pos;
+    return token_position(d, token, &pos, err) ? pos : (int64_t)-1;
+  };
+  int64_t one = -1;
+  if (g.per == 1) {                          // every wavefront by itself: a barrier less
+    one = position(t0);
+    turn_angles(d, 1, f0, cs, sn, [&](int) { return one; });
+  } else {
+    for (int t = uni((int)(tid >> 6)); t < tokens; t += 4) {
+      const int64_t pos = position(t0 + t);
+      if ((tid & 63) == 0) place[t] = pos;
+    }
+    __syncthreads();
+    turn_angles(d, tokens, f0, cs, sn, [&](int t) { return place[t]; });
+  }
+  __syncthreads();
+  auto live = [&](int t) { return (g.per == 1 ? one : place[t]) >= 0; };
+  if (!mine) return;
+  for (;;) {
+    for (int row = row0; row < total; row += R * stride) {
+      if (row != row0) fetch(row, now);
 #pragma unroll
       for (int k = 0; k < R; ++k) {
-        if (!on[k]) continue;
+        if (now.t[k] < 0 || !live(now.t[k])) continue;
         if (u < pairs) {
           __attribute__((aligned(16))) float c[V], s[V];
+          const int at = now.t[k] * half + u * V;
           if constexpr (V > 1) {                             // half and so every unit's angles: multiples of 4
 #pragma unroll
             for (int i = 0; i < V; i += 4) {
-              *(f4_t*)(c + i) = *(const f4_t*)&cs[at[k] + i];
-              *(f4_t*)(s + i) = *(const f4_t*)&sn[at[k] + i];
+              *(f4_t*)(c + i) = *(const f4_t*)&cs[at + i];
+              *(f4_t*)(s + i) = *(const f4_t*)&sn[at + i];
             }
           } else {
-            c[0] = cs[at[k]];
-            s[0] = sn[at[k]];
+            c[0] = cs[at];
+            s[0] = sn[at];
           }
-          rope_turn_raw<DT, INTER, V>(r[k], c, s);
+          rope_turn_raw<DT, INTER, V>(now.r[k], c, s);
         }
-        rope_store<DT, V>(d.q_out.ptr, to[k] + a, to[k] + b, r[k], two);
+        const int64_t to = (t0 + now.t[k]) * d.q_out.tok + now.h[k] * d.q_out.head;
+        rope_store<DT, V>(d.q_out.ptr, to + a, to + b, now.r[k], two);
       }
     }
+    u += wide;
+    if (u >= units) return;
+    columns_of();
+    fetch(row0, now);
   }
 }
 
@@ -118,14 +235,42 @@ __device__ __forceinline__ float of16(const New16& x, int i) {
   else return (float)__builtin_bit_cast(_Float16, (uint16_t)(i & 1 ? w >> 16 : w));
 }
 
-// 16 columns from `col` on of a row at element e, turned by the angles of its row at cs, sn
+// 16 columns of a row, and those that they are turned with
+struct Raw16 {
+  New16 own, other;
+};
+
+// `vectors`: half is a multiple of 8, so eight columns have their partners side by side on a 16-byte bound
 template <int DT, bool INTER>
-__device__ __forceinline__ void turned16(const ktir_kv8_rope_append_t& d, uint64_t ptr, int64_t e, int col, bool wide, bool vectors, const float* cs, const float* sn, float* x) {
+__device__ __forceinline__ void load16(const ktir_kv8_rope_append_t& d, uint64_t ptr, int64_t e, int col, bool wide, bool vectors, Raw16& x) {
   const int half = (int)d.rot / 2, rot = (int)d.rot;
-  const New16 own = new16(ptr, e + col, wide);
+  x.own = new16(ptr, e + col, wide);
+  if constexpr (!INTER) {
+    auto partner = [&](int c0) { return e + (c0 < half ? c0 + half : c0 - half); };
 #pragma unroll
-  for (int i = 0; i < 16; ++i) x[i] = of16<DT>(own, i);
-  if (col >= rot) return;
+    for (int v = 0; v < 16; v += 8) {
+      if (col + v >= rot) break;
+      if (vectors) {
+        const u4_t w = *(const KTIR_G(u4_t)*)(ptr + 2 * partner(col + v));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x.other.w[v / 2 + i] = w[i];
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          uint32_t w = col + v + i < rot ? ((const KTIR_G(uint16_t)*)ptr)[partner(col + v + i)] : 0u;
+          x.other.w[(v + i) / 2] = i & 1 ? x.other.w[(v + i) / 2] | w << 16 : w;
+        }
+      }
+    }
+  }
+}
+
+// turned by the angles of their row at cs, sn
+template <int DT, bool INTER>
+__device__ __forceinline__ void turn16(const ktir_kv8_rope_append_t& d, const Raw16& raw, int col, bool vectors, const float* cs, const float* sn, float* x) {
+  const int half = (int)d.rot / 2, rot = (int)d.rot;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) x[i] = of16<DT>(raw.own, i);
   if constexpr (INTER) {
 #pragma unroll
     for (int i = 0; i < 16; i += 2) {
@@ -134,30 +279,31 @@ __device__ __forceinline__ void turned16(const ktir_kv8_rope_append_t& d, uint64
       x[i] = __fsub_rn(__fmul_rn(a, c), __fmul_rn(b, s));
       x[i + 1] = __fadd_rn(__fmul_rn(b, c), __fmul_rn(a, s));
     }
-  } else if (vectors) {                        // half a multiple of 8: eight columns have their partners side by side
-#pragma unroll
-    for (int v = 0; v < 16; v += 8) {
-      const int c0 = col + v;
-      if (c0 >= rot) break;
-      const bool first = c0 < half;
-      const int at = first ? c0 : c0 - half;
-      const u4_t w = *((const KTIR_G(u4_t)*)(ptr + 2 * (e + (first ? c0 + half : c0 - half))));
-      const New16 other = {{w.x, w.y, w.z, w.w, 0, 0, 0, 0}};
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float p = of16<DT>(other, i), t = __fmul_rn(p, sn[at + i]), y = __fmul_rn(x[v + i], cs[at + i]);
-        x[v + i] = first ? __fsub_rn(y, t) : __fadd_rn(y, t);
-      }
-    }
   } else {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int c0 = col + i;
-      if (c0 >= rot) break;
-      const bool first = c0 < half;
-      const int at = first ? c0 : c0 - half;
-      const float p = load_elem(ptr, e + (first ? c0 + half : c0 - half), DT), t = __fmul_rn(p, sn[at]), y = __fmul_rn(x[i], cs[at]);
-      x[i] = first ? __fsub_rn(y, t) : __fadd_rn(y, t);
+    for (int v = 0; v < 16; v += 8) {
+      if (col + v >= rot) break;
+      __attribute__((aligned(16))) float c[8], s[8];
+      if (vectors) {
+        const int at = col + v < half ? col + v : col + v - half;
+#pragma unroll
+        for (int i = 0; i < 8; i += 4) {
+          *(f4_t*)(c + i) = *(const f4_t*)&cs[at + i];
+          *(f4_t*)(s + i) = *(const f4_t*)&sn[at + i];
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int c0 = col + v + i, at = c0 < half ? c0 : c0 < rot ? c0 - half : 0;
+          c[i] = cs[at], s[i] = sn[at];
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (col + v + i >= rot) break;
+        const float t = __fmul_rn(of16<DT>(raw.other, v + i), s[i]), y = __fmul_rn(x[v + i], c[i]);
+        x[v + i] = col + v + i < half ? __fsub_rn(y, t) : __fadd_rn(y, t);
+      }
     }
   }
 }
@@ -172,106 +318,79 @@ __device__ __forceinline__ u4_t codes_of16(const float* x, float f, int code) {
   return o;
 }
 
-// W wavefronts have a page's part of a head (of K: IS_K, else of V).
-template <int DT, bool INTER, int W, bool IS_K>
+// W wavefronts have a page's part of a head (of K: IS_K, else of V); MORE: it may have rows past those that they keep.
+template <int DT, bool INTER, int W, bool MORE, bool IS_K>
 __device__ __forceinline__ void turn_kv(const ktir_kv8_rope_append_t& d, int slot, int group, float* cs, float* sn, uint32_t* tops, int* err) {
   const ktir_kv8_t& c = d.cache;
-  const int wave = uni((int)(threadIdx.x >> 6)), tid = W == 1 ? (int)(threadIdx.x & 63) : (int)threadIdx.x;
-  const int64_t head = W == 1 ? group * 4 + wave : group;
-  int64_t s, nth;
-  const int shift = __builtin_ctz((uint32_t)c.page);
-  const Seq q = seq_of_slot(d.batch, c.page, 1, shift, 2, slot, &s, &nth, err);
-  if (nth < 0) return;
-  const int64_t pos0 = (int64_t)q.n_kv - q.n_new, from = pos0 < 0 ? 0 : pos0;      // the first position that is stored
-  const int64_t p = (from >> shift) + nth;                                       // the page's number in the sequence
-  const int64_t lo = p << shift < from ? from : p << shift, hi = (p + 1) << shift < q.n_held ? (p + 1) << shift : q.n_held;
-  if (lo >= hi) return;
-  const int64_t at = ints(d.batch.table)[s * d.batch.table_row + p];
-  const int n = (int)(hi - lo), r0 = (int)(lo & (c.page - 1)), half = (int)d.rot / 2;
-  const int64_t t0 = q.start + lo - pos0;
+  const int wave = uni((int)(threadIdx.x >> 6)), tid = (int)threadIdx.x & (64 * W - 1);
+  const int64_t head = group * (4 / W) + wave / W;
+  const double f0 = IS_K ? frequency(d, threadIdx.x % (uint32_t)(d.rot / 2)) : 0.0;
+  PagePart part;
+  if (!page_part(d, slot, &part, err)) return;
+  const int n = part.n, r0 = part.r0, half = (int)d.rot / 2;
   const ktir_rows3_t& in = IS_K ? d.k : d.v;
   const int G = (int)c.columns >> 4, per = 64 * W / G, r = tid / G, col = (tid - r * G) * 16;     // rows a pass; this thread's
   const bool wide = !((in.ptr | (uint64_t)in.tok * 2 | (uint64_t)in.head * 2) & 15), mine = r < per && head < c.heads;
-  const int64_t e0 = t0 * in.tok + head * in.head;
-
-  // the angles of the rows from `first` on, as many as there are up to `most`
-  auto angles = [&](int first, int most) {
-    const int rows = n - first < most ? n - first : most;
-    for (int i = threadIdx.x; i < rows * half; i += 256) {
-      const int row = i / half;
-      int64_t pos = d.pos ? rope_pos(d, t0 + first + row) : lo + first + row;
-      if (pos < 0) *err = OUT_OF_RANGE, pos = 0;
-      rope_angle(Angles{d.freq, d.amplitude, false}, pos, i - row * half, &cs[i], &sn[i]);
-    }
-  };
-  // row `row`'s columns, its angles those of row `of` in LDS
-  auto load = [&](int row, int of, float* x) {
-    if constexpr (IS_K) {
-      turned16<DT, INTER>(d, in.ptr, e0 + row * in.tok, col, wide, wide && half % 8 == 0, cs + of * half, sn + of * half, x);
-    } else {
-      const New16 own = new16(in.ptr, e0 + row * in.tok + col, wide);
+  const int64_t e0 = part.t0 * in.tok + head * in.head;
+  const PageHead<IS_K> to(d, part, head);
+  float before = 0.f;
+  // the unit of 16 columns of the rows first + r, first + per + r, ...: loads, then (K) the angles of these rows into LDS, then the values
+  const bool vectors = wide && half % 8 == 0;
+  auto values = [&](int first, float (&x)[TURN_KEPT][16]) {
+    Raw16 raw[TURN_KEPT];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) x[i] = of16<DT>(own, i);
+    for (int i = 0; i < TURN_KEPT; ++i) {
+      const int row = first + i * per + r;
+      if (!mine || row >= n) continue;
+      if constexpr (IS_K) load16<DT, INTER>(d, in.ptr, e0 + row * in.tok, col, wide, vectors, raw[i]);
+      else raw[i].own = new16(in.ptr, e0 + row * in.tok + col, wide);
     }
-  };
-  // absolute bits: they grow with the value, and past infinity's for NaN
-  auto most_of = [&](const float* x, uint32_t top) {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const uint32_t b = __float_as_uint(x[i]) & 0x7fffffffu;
-      top = top > b ? top : b;
-    }
-    return top;
-  };
-  float x[TURN_KEPT][16];
-  uint32_t top = 0;
-  if constexpr (W == 1) {                    // a page has TURN_KEPT passes of rows at most: all its angles at once
+    if (first == 0 && r0 && part.there && head < c.heads) before = *to.scale;
     if constexpr (IS_K) {
-      angles(0, n);
+      if (first) __syncthreads();
+      const int rows = n - first < TURN_KEPT * per ? n - first : TURN_KEPT * per;
+      turn_angles(d, rows, f0, cs, sn, [&](int row) { return row_position(d, part, first + row, err); });
       __syncthreads();
     }
 #pragma unroll
-    for (int i = 0; i < TURN_KEPT; ++i)
-      if (mine && i * per + r < n) load(i * per + r, i * per + r, x[i]);
+    for (int i = 0; i < TURN_KEPT; ++i) {
+      if (!mine || first + i * per + r >= n) continue;
+      if constexpr (IS_K) {
+        turn16<DT, INTER>(d, raw[i], col, vectors, cs + (i * per + r) * half, sn + (i * per + r) * half, x[i]);
+      } else {
 #pragma unroll
-    for (int i = 0; i < TURN_KEPT; ++i)
-      if (mine && i * per + r < n) top = most_of(x[i], top);
-  } else {
+        for (int k = 0; k < 16; ++k) x[i][k] = of16<DT>(raw[i].own, k);
+      }
+    }
+  };
+  uint32_t top = 0;
+  auto look = [&](int first, const float (&x)[TURN_KEPT][16]) {
 #pragma unroll
     for (int i = 0; i < TURN_KEPT; ++i) {
-      if (i * per >= n) break;
-      if constexpr (IS_K) {
-        __syncthreads();
-        angles(i * per, per);
-        __syncthreads();
-      }
-      if (mine && i * per + r < n) {
-        load(i * per + r, r, x[i]);
-        top = most_of(x[i], top);
+      if (!mine || first + i * per + r >= n) continue;
+#pragma unroll
+      for (int k = 0; k < 16; ++k) {
+        const uint32_t y = __float_as_uint(x[i][k]) & 0x7fffffffu;
+        top = top > y ? top : y;
       }
     }
-    for (int row = TURN_KEPT * per; row < n; row += per) {
-      float y[16];
-      if constexpr (IS_K) {
-        __syncthreads();
-        angles(row, per);
-        __syncthreads();
-      }
-      if (mine && row + r < n) {
-        load(row + r, r, y);
-        top = most_of(y, top);
-      }
+  };
+  // rows past those that are kept are read again, from the cache
+  float x[TURN_KEPT][16];
+  values(0, x);
+  look(0, x);
+  if constexpr (MORE) {
+#pragma unroll 1
+    for (int first = TURN_KEPT * per; first < n; first += TURN_KEPT * per) {
+      float y[TURN_KEPT][16];
+      values(first, y);
+      look(first, y);
     }
   }
-  if (at < 0 || at >= c.pages) {
+  if (!part.there) {
     *err = OUT_OF_RANGE;
     return;
   }
-  KTIR_G(uint8_t)* codes = (KTIR_G(uint8_t)*)(IS_K ? c.k + at * c.k_page + head * c.k_head : c.v + at * c.v_page + head * c.v_head) + col;
-  const int64_t tok = IS_K ? c.k_tok : c.v_tok;
-  KTIR_G(float)* scale = IS_K ? (KTIR_G(float)*)c.k_scale + at * c.ks_page + head * c.ks_head
-                              : (KTIR_G(float)*)c.v_scale + at * c.vs_page + head * c.vs_head;
-  const float before = r0 && head < c.heads ? *scale : 0.f;
 #pragma unroll
   for (int o = 32; o; o >>= 1) {
     const uint32_t y = __shfl_xor(top, o);
@@ -281,62 +400,220 @@ __device__ __forceinline__ void turn_kv(const ktir_kv8_rope_append_t& d, int slo
     if ((threadIdx.x & 63) == 0) tops[wave] = top;
     __syncthreads();                       // also: every wavefront has read the scale before it changes
 #pragma unroll
-    for (int i = 0; i < W; ++i) top = top > tops[i] ? top : tops[i];
+    for (int i = 0; i < W; ++i) top = top > tops[wave / W * W + i] ? top : tops[wave / W * W + i];
   }
-  const float most = __uint_as_float(top), per_top = c.dtype == KTIR_I8 ? PER_TOP<KTIR_I8> : PER_TOP<KTIR_E4M3>;
-  float now = __builtin_fmaxf(most * per_top, LEAST_SCALE);
-  if (!(now >= before)) now = before;                     // a page that was NaN stays so
-  if (!(most < __builtin_inff())) now = __builtin_nanf("");
-  const bool nan = !(now < __builtin_inff());
-  const float inv = 1.f / now;
-  if (now > before && mine) {              // older rows rounded to the new scale
-    const float ratio = before * inv;
-    for (int row = r; row < r0; row += per) {
-      KTIR_G(u4_t)* w = (KTIR_G(u4_t)*)(codes + row * tok);
-      u4_t y = *w;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float v[4];
-        if (c.dtype == KTIR_I8) values4<KTIR_I8>(y[i], v);
-        else values4<KTIR_E4M3>(y[i], v);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] *= ratio;
-        y[i] = c.dtype == KTIR_I8 ? codes4<KTIR_I8>(v) : codes4<KTIR_E4M3, true>(v);
-      }
-      *w = y;
-    }
-  }
+  const NewScale now(c.dtype, top, before);
+  if (now.scale > before && r0 && head < c.heads) now.again(c, to.codes, to.tok, r0, tid, 64 * W);
   const u4_t none = {0, 0, 0, 0};
+  auto store = [&](int first, const float (&x)[TURN_KEPT][16]) {
 #pragma unroll
-  for (int i = 0; i < TURN_KEPT; ++i)
-    if (mine && i * per + r < n) *(KTIR_G(u4_t)*)(codes + (r0 + i * per + r) * tok) = nan ? none : codes_of16(x[i], inv, c.dtype);
-  if constexpr (W > 1) {
-    for (int row = TURN_KEPT * per; row < n; row += per) {
-      float y[16];
-      if constexpr (IS_K) {
-        __syncthreads();
-        angles(row, per);
-        __syncthreads();
-      }
-      if (mine && row + r < n) {
-        load(row + r, r, y);
-        *(KTIR_G(u4_t)*)(codes + (r0 + row + r) * tok) = nan ? none : codes_of16(y, inv, c.dtype);
-      }
+    for (int i = 0; i < TURN_KEPT; ++i) {
+      const int row = first + i * per + r;
+      if (mine && row < n) *(KTIR_G(u4_t)*)(to.codes + (r0 + row) * to.tok + col) = now.nan ? none : codes_of16(x[i], now.inv, c.dtype);
+    }
+  };
+  store(0, x);
+  if constexpr (MORE) {
+#pragma unroll 1
+    for (int first = TURN_KEPT * per; first < n; first += TURN_KEPT * per) {
+      float y[TURN_KEPT][16];
+      values(first, y);
+      store(first, y);
     }
   }
-  if (tid == 0 && head < c.heads) *scale = now;
+  if (tid == 0 && head < c.heads) *to.scale = now.scale;
 }
 
-template <int DT, bool INTER, int V, bool PAST, int W>
-__global__ __launch_bounds__(256) void kv8_turn(const ktir_kv8_rope_append_t d, const TurnGrid g, int* err) {
-  __shared__ __attribute__((aligned(16))) float cs[TURN_PAIRS], sn[TURN_PAIRS];
+template <int DT, bool INTER, int V, bool PAST, int W, bool MORE>
+__global__ __launch_bounds__(256, MORE ? 1 : 4) void kv8_turn(const ktir_kv8_rope_append_t d, const TurnGrid g, int* err) {
+  __shared__ __attribute__((aligned(16))) float cs[turn_pairs(W)], sn[turn_pairs(W)];
   __shared__ int64_t place[TURN_TOKENS];
   __shared__ uint32_t tops[4];
-  const int block = blockIdx.x, kv = 2 * g.kv * g.slots;
+  const int kv = 2 * g.kv * g.slots, block = blockIdx.x;
   if (block >= kv) return turn_queries<DT, INTER, V, PAST>(d, block - kv, g, cs, sn, place, err);
   const int slot = block / (2 * g.kv), group = block - slot * 2 * g.kv;
-  if (group < g.kv) turn_kv<DT, INTER, W, true>(d, slot, group, cs, sn, tops, err);
-  else turn_kv<DT, INTER, W, false>(d, slot, group - g.kv, cs, sn, tops, err);
+  if (group < g.kv) turn_kv<DT, INTER, W, MORE, true>(d, slot, group, cs, sn, tops, err);
+  else turn_kv<DT, INTER, W, MORE, false>(d, slot, group - g.kv, cs, sn, tops, err);
+}
+
+// ---- few tokens ---------------------------------------------------------------------
+//
+// A decode step, or a few drafts of each sequence, is latency: the instructions of one wavefront, one after
+// another, and its loads.  Here a lane has pairs of one row (and columns behind the turned ones), so an angle is made where
+// it is used, without LDS, and what a wavefront does is short.  A workgroup has a page's part of a head of K or
+// V, a row a wavefront, or one token's part of the queries, a head a wavefront at a time.
+
+constexpr int FEW_TOKENS = 8;
+constexpr int FEW_HEADS = 16;        // of the queries, for a workgroup
+constexpr int FEW_KEPT = 2;          // rows that a wavefront keeps
+static_assert(4 * FEW_KEPT >= FEW_TOKENS, "four wavefronts read no row again");
+
+struct FewAngles {
+  float c[2], s[2];                  // of pairs l and l + 64
+};
+struct FewRow {
+  float pair[2][2], rest[4];         // columns rot + l + 64 i
+};
+
+__device__ __forceinline__ FewAngles few_angles(const ktir_kv8_rope_append_t& d, int64_t pos, const double (&f)[2]) {
+  FewAngles a;
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    if ((int)(threadIdx.x & 63) + 64 * i < d.rot / 2) rope_angle_of(pos, f[i], d.amplitude, false, &a.c[i], &a.s[i]);
+  return a;
+}
+
+// where the first column of a lane's pair i lies, and how far the second is from it
+__device__ __forceinline__ int few_first(const ktir_kv8_rope_append_t& d, int i) {
+  const int p = (threadIdx.x & 63) + 64 * i;
+  return d.interleaved ? 2 * p : p;
+}
+__device__ __forceinline__ int few_gap(const ktir_kv8_rope_append_t& d) { return d.interleaved ? 1 : (int)d.rot / 2; }
+
+template <int DT>
+__device__ __forceinline__ void few_load(const ktir_kv8_rope_append_t& d, uint64_t ptr, int64_t e, bool rest, FewRow& x) {
+  const int l = threadIdx.x & 63, half = (int)d.rot / 2;
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    if (l + 64 * i < half) {
+      x.pair[i][0] = load_elem(ptr, e + few_first(d, i), DT);
+      x.pair[i][1] = load_elem(ptr, e + few_first(d, i) + few_gap(d), DT);
+    }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (rest && d.rot + l + 64 * i < d.cache.columns) x.rest[i] = load_elem(ptr, e + d.rot + l + 64 * i, DT);
+}
+
+__device__ __forceinline__ void few_turn(FewRow& x, const FewAngles& a) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const float u = x.pair[i][0], v = x.pair[i][1];
+    x.pair[i][0] = __fsub_rn(__fmul_rn(u, a.c[i]), __fmul_rn(v, a.s[i]));
+    x.pair[i][1] = __fadd_rn(__fmul_rn(v, a.c[i]), __fmul_rn(u, a.s[i]));
+  }
+}
+
+template <int DT>
+__device__ __forceinline__ void few_queries(const ktir_kv8_rope_append_t& d, int block, int parts, const double (&f)[2], int* err) {
+  const int64_t token = block / parts;
+  const int wave = uni((int)(threadIdx.x >> 6)), l = threadIdx.x & 63, half = (int)d.rot / 2;
+  const int h0 = block % parts * FEW_HEADS, end = h0 + FEW_HEADS < d.q_heads ? h0 + FEW_HEADS : (int)d.q_heads;
+  const bool rest = d.q.ptr != d.q_out.ptr;
+  FewRow x;
+  if (h0 + wave < end) few_load<DT>(d, d.q.ptr, token * d.q.tok + (h0 + wave) * d.q.head, rest, x);
+  int64_t pos;
+  if (!token_position(d, token, &pos, err)) return;
+  const FewAngles a = few_angles(d, pos, f);
+  for (int h = h0 + wave; h < end; h += 4) {
+    if (h != h0 + wave) few_load<DT>(d, d.q.ptr, token * d.q.tok + h * d.q.head, rest, x);
+    few_turn(x, a);
+    const int64_t e = token * d.q_out.tok + h * d.q_out.head;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (l + 64 * i < half) {
+        store_elem(d.q_out.ptr, e + few_first(d, i), DT, x.pair[i][0]);
+        store_elem(d.q_out.ptr, e + few_first(d, i) + few_gap(d), DT, x.pair[i][1]);
+      }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (rest && d.rot + l + 64 * i < d.cache.columns) store_elem(d.q_out.ptr, e + d.rot + l + 64 * i, DT, x.rest[i]);
+  }
+}
+
+// W wavefronts (1 or 4) have a page's part of a head.
+template <int DT, bool IS_K, int W>
+__device__ __forceinline__ void few_kv(const ktir_kv8_rope_append_t& d, int slot, int64_t head, const double (&f)[2], uint32_t* tops, int* err) {
+  const ktir_kv8_t& c = d.cache;
+  const int wave = W == 1 ? 0 : uni((int)(threadIdx.x >> 6)), l = threadIdx.x & 63, half = (int)d.rot / 2;
+  PagePart part;
+  if (!page_part(d, slot, &part, err)) return;
+  const ktir_rows3_t& in = IS_K ? d.k : d.v;
+  const int64_t e0 = part.t0 * in.tok + head * in.head;
+  auto values = [&](int row, FewRow& x) {
+    few_load<DT>(d, in.ptr, e0 + row * in.tok, true, x);
+    if constexpr (IS_K) few_turn(x, few_angles(d, row_position(d, part, row, err), f));
+  };
+  uint32_t top = 0;
+  auto look = [&](const FewRow& x) {
+    auto see = [&](float v) {
+      const uint32_t y = __float_as_uint(v) & 0x7fffffffu;
+      top = top > y ? top : y;
+    };
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (l + 64 * i < half) see(x.pair[i][0]), see(x.pair[i][1]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (d.rot + l + 64 * i < c.columns) see(x.rest[i]);
+  };
+  FewRow x[FEW_KEPT];
+  const PageHead<IS_K> to(d, part, head);
+  const float before = part.there && part.r0 ? *to.scale : 0.f;
+#pragma unroll
+  for (int k = 0; k < FEW_KEPT; ++k)
+    if (wave + W * k < part.n) {
+      values(wave + W * k, x[k]);
+      look(x[k]);
+    }
+#pragma unroll 1
+  for (int row = FEW_KEPT; W == 1 && row < part.n; ++row) {          // (four have FEW_TOKENS at most)
+    FewRow y;
+    values(row, y);
+    look(y);
+  }
+  if (!part.there) {
+    *err = OUT_OF_RANGE;
+    return;
+  }
+  for (int o = 32; o; o >>= 1) {
+    const uint32_t y = __shfl_xor(top, o);
+    top = top > y ? top : y;
+  }
+  if constexpr (W > 1) {
+    if (l == 0) tops[wave] = top;
+    __syncthreads();                       // also: every wavefront has read the scale before it changes
+#pragma unroll
+    for (int i = 0; i < W; ++i) top = top > tops[i] ? top : tops[i];
+  }
+  const NewScale now(c.dtype, top, before);
+  if (now.scale > before && part.r0) now.again(c, to.codes, to.tok, part.r0, 64 * wave + l, 64 * W);
+  auto put = [&](int row, const FewRow& x) {
+    KTIR_G(uint8_t)* p = to.codes + (part.r0 + row) * to.tok;
+    float a[4] = {x.pair[0][0] * now.inv, x.pair[0][1] * now.inv, x.pair[1][0] * now.inv, x.pair[1][1] * now.inv};
+    float b[4] = {x.rest[0] * now.inv, x.rest[1] * now.inv, x.rest[2] * now.inv, x.rest[3] * now.inv};
+    uint32_t u = c.dtype == KTIR_I8 ? codes4<KTIR_I8>(a) : codes4<KTIR_E4M3>(a), v = c.dtype == KTIR_I8 ? codes4<KTIR_I8>(b) : codes4<KTIR_E4M3>(b);
+    if (now.nan) u = v = 0;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (l + 64 * i < half) {
+        p[few_first(d, i)] = (uint8_t)(u >> (16 * i));
+        p[few_first(d, i) + few_gap(d)] = (uint8_t)(u >> (16 * i + 8));
+      }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (d.rot + l + 64 * i < c.columns) p[d.rot + l + 64 * i] = (uint8_t)(v >> (8 * i));
+  };
+#pragma unroll
+  for (int k = 0; k < FEW_KEPT; ++k)
+    if (wave + W * k < part.n) put(wave + W * k, x[k]);
+#pragma unroll 1
+  for (int row = FEW_KEPT; W == 1 && row < part.n; ++row) {
+    FewRow y;
+    values(row, y);
+    put(row, y);
+  }
+  if (wave == 0 && l == 0) *to.scale = now.scale;
+}
+
+template <int DT, int W>
+__global__ __launch_bounds__(256) void kv8_turn_few(const ktir_kv8_rope_append_t d, int slots, int groups, int parts, int* err) {
+  __shared__ uint32_t tops[4];
+  const int l = threadIdx.x & 63, half = (int)d.rot / 2, heads = (int)d.cache.heads, kv = groups * slots, block = blockIdx.x;
+  const double f[2] = {frequency(d, l < half ? l : 0), frequency(d, l + 64 < half ? l + 64 : 0)};
+  if (block >= kv) return few_queries<DT>(d, block - kv, parts, f, err);
+  const int slot = block / groups, hv = (block - slot * groups) * (4 / W) + (W == 1 ? uni((int)(threadIdx.x >> 6)) : 0);
+  if (hv < heads) few_kv<DT, true, W>(d, slot, hv, f, tops, err);
+  else if (hv < 2 * heads) few_kv<DT, false, W>(d, slot, hv - heads, f, tops, err);
 }
 
 // whether every vector of 8 values of the queries starts on a 16-byte bound
@@ -344,7 +621,7 @@ static bool wide_rows(const ktir_rows3_t& r, int64_t tokens, int64_t heads) {
   return !(r.ptr & 15) && (tokens == 1 || r.tok % 8 == 0) && (heads == 1 || r.head % 8 == 0);
 }
 
-template <int DT, bool INTER, int W>
+template <int DT, bool INTER, int W, bool MORE>
 static int turn_go(const ktir_kv8_rope_append_t& d, hipStream_t st) {
   constexpr const char* ME = "ktir_launch_kv8_rope_append";
   const int64_t tokens = d.batch.tokens, half = d.rot / 2, columns = d.cache.columns;
@@ -353,12 +630,11 @@ static int turn_go(const ktir_kv8_rope_append_t& d, hipStream_t st) {
   TurnGrid g;
   // a sequence's n new tokens touch at most floor(n / page) + 2 pages
   const int64_t slots = tokens / d.cache.page + 2 * d.batch.seqs;
-  g.kv = (int)(W == 1 ? (d.cache.heads + 3) / 4 : d.cache.heads);
+  g.kv = (int)((d.cache.heads + 4 / W - 1) / (4 / W));
   // the queries: as ktir_rope.hip cuts them
   const int64_t units = half / V + (columns - d.rot + 2 * V - 1) / (2 * V), step = 256 / (units < 256 ? units : 256);
-  int64_t per = tokens / 1024;
+  int64_t per = tokens / 2048;
   per = per > TURN_TOKENS ? TURN_TOKENS : per < 1 ? 1 : per;
-  if (per * half > TURN_PAIRS) per = TURN_PAIRS / half;
   const int64_t blocks = (tokens + per - 1) / per;
   int64_t parts = 1;
   if (blocks < 512) {
@@ -366,24 +642,46 @@ static int turn_go(const ktir_kv8_rope_append_t& d, hipStream_t st) {
     const int64_t most = (1024 + blocks - 1) / blocks;
     parts = parts > most ? most : parts;
   }
-  if (2 * g.kv * slots + blocks * parts > INT32_MAX) return set_error(KTIR_E_UNSUPPORTED, "%s: %lld pages, %lld heads in one launch", ME, (long long)slots, (long long)d.cache.heads);
+  const int64_t kv = 2 * g.kv * slots, queries = blocks * parts;
+  if (kv > (1 << 29) || queries > (1 << 29)) return set_error(KTIR_E_UNSUPPORTED, "%s: %lld pages, %lld heads in one launch", ME, (long long)slots, (long long)d.cache.heads);
   g.slots = (int)slots;
   g.per = (int)per;
   g.parts = (int)parts;
-  const dim3 grid((unsigned)(2 * g.kv * slots + blocks * parts));
+  const dim3 grid((unsigned)(kv + queries));
   const bool past = wide && d.q.ptr != d.q_out.ptr && 2 * tokens * d.q_heads * columns * 2 > (int64_t)64 << 20;      // (as ktir_rope.hip has it)
-  if (past) hipLaunchKernelGGL((kv8_turn<DT, INTER, 8, true, W>), grid, dim3(256), 0, st, d, g, device_error_flag());
-  else if (wide) hipLaunchKernelGGL((kv8_turn<DT, INTER, 8, false, W>), grid, dim3(256), 0, st, d, g, device_error_flag());
-  else hipLaunchKernelGGL((kv8_turn<DT, INTER, 1, false, W>), grid, dim3(256), 0, st, d, g, device_error_flag());
+  if (past) hipLaunchKernelGGL((kv8_turn<DT, INTER, 8, true, W, MORE>), grid, dim3(256), 0, st, d, g, device_error_flag());
+  else if (wide) hipLaunchKernelGGL((kv8_turn<DT, INTER, 8, false, W, MORE>), grid, dim3(256), 0, st, d, g, device_error_flag());
+  else hipLaunchKernelGGL((kv8_turn<DT, INTER, 1, false, W, MORE>), grid, dim3(256), 0, st, d, g, device_error_flag());
   KTIR_HIP_CHECK(hipGetLastError());
   return KTIR_OK;
 }
 
 template <int DT>
 static int turn_type(const ktir_kv8_rope_append_t& d, hipStream_t st) {
-  // a page's units fit into one wavefront's registers: four heads share a workgroup
-  if (d.cache.page * (d.cache.columns / 16) <= 64 * TURN_KEPT) return d.interleaved ? turn_go<DT, true, 1>(d, st) : turn_go<DT, false, 1>(d, st);
-  return d.interleaved ? turn_go<DT, true, 4>(d, st) : turn_go<DT, false, 4>(d, st);
+  // The kernels for few tokens, four wavefronts a head for up to 8 (32 / 8 heads of 128 columns, one sequence of 1 to 4: 4.6 us,
+  // of 8 5.5, the other kernel 6.6 to 7.0; 16 in pages of 64 8.4 and 7.2), one where there are up to two a sequence
+  // (64 sequences of one 6.1, of two 6.5, the other kernel 7.5 and 7.7, with pages of 64 6.3 and 12.8; of four 10.4 and 8.4).
+  const bool few = d.batch.tokens <= FEW_TOKENS;
+  if (few || d.batch.tokens <= 2 * d.batch.seqs) {
+    const int64_t slots = d.batch.tokens / d.cache.page + 2 * d.batch.seqs, parts = (d.q_heads + FEW_HEADS - 1) / FEW_HEADS;
+    const int64_t groups = few ? 2 * d.cache.heads : (2 * d.cache.heads + 3) / 4, blocks = groups * slots + d.batch.tokens * parts;
+    if (blocks <= (1 << 30)) {
+      if (!few) hipLaunchKernelGGL((kv8_turn_few<DT, 1>), dim3((unsigned)blocks), dim3(256), 0, st, d, (int)slots, (int)groups, (int)parts, device_error_flag());
+      else hipLaunchKernelGGL((kv8_turn_few<DT, 4>), dim3((unsigned)blocks), dim3(256), 0, st, d, (int)slots, (int)groups, (int)parts, device_error_flag());
+      KTIR_HIP_CHECK(hipGetLastError());
+      return KTIR_OK;
+    }
+  }
+  // a page's units fit into the registers of one wavefront, or of two: several heads share a workgroup (and their angles).
+  // (64 W / G rows a pass, two passes: whole pages of 16 rows or more for all G up to 8 W)
+  const int64_t G = d.cache.columns / 16, units = d.cache.page * G;
+  const bool whole = TURN_KEPT * (256 / G) >= d.cache.page;
+  auto go = [&](auto inter) {
+    constexpr bool INTER = decltype(inter)::value;
+    return units <= 128 ? turn_go<DT, INTER, 1, false>(d, st) : units <= 256 ? turn_go<DT, INTER, 2, false>(d, st)
+                     : whole ? turn_go<DT, INTER, 4, false>(d, st) : turn_go<DT, INTER, 4, true>(d, st);
+  };
+  return d.interleaved ? go(std::true_type()) : go(std::false_type());
 }
 
 }  // namespace ktir

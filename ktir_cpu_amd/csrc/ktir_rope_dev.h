@@ -6,17 +6,19 @@ namespace ktir {
 
 typedef float f4_t __attribute__((ext_vector_type(4)));
 
-// cosine and sine of pair i at a position (d: freq, amplitude, inverse), times the amplitude, rounded once.  The angle passes
+// cosine and sine of a pair at a position, times the amplitude, rounded once.  The angle passes
 // 2^20 radians at far positions, where f32 holds it to a sixteenth: all of it is f64
 // (the vector pipe's f64 and f32 instructions take as long).
-template <class D>
-__device__ __forceinline__ void rope_angle(const D& d, int64_t pos, int i, float* c, float* s) {
-  double turns = (double)pos * ((const KTIR_G(double)*)d.freq)[i] * 0.15915494309189533577;
+__device__ __forceinline__ void rope_angle_of(int64_t pos, double freq, double amplitude, bool inverse, float* c, float* s) {
+  double turns = (double)pos * freq * 0.15915494309189533577;
   turns -= rint(turns);
   double sn, cs;
   sincospi(2.0 * turns, &sn, &cs);
-  *c = (float)(cs * d.amplitude);
-  *s = (float)(d.inverse ? -(sn * d.amplitude) : sn * d.amplitude);
+  *c = (float)(cs * amplitude);
+  *s = (float)(inverse ? -(sn * amplitude) : sn * amplitude);
+}
+__device__ __forceinline__ void rope_angle(const ktir_rope_t& d, int64_t pos, int i, float* c, float* s) {
+  rope_angle_of(pos, ((const KTIR_G(double)*)d.freq)[i], d.amplitude, d.inverse, c, s);
 }
 
 template <class D>
