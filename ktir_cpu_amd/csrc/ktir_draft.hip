@@ -55,16 +55,23 @@ __global__ __launch_bounds__(32 * WORDS) void draft_tree(const ktir_draft_tree_t
     __syncthreads();
   }
   if (i < n) ((KTIR_G(int32_t)*)d.positions)[start + i] = (kv < 0 ? 0 : kv) - n + depths[i];
+  if (d.window) {                                   // the highest `window` bits of each row
+    if (i < n && depths[i] >= d.window) {
+      int left = (int)d.window;
+      for (int w = word; w >= 0; --w) {
+        uint32_t y = left > 0 ? rows[i * PITCH + w] : 0u;
+        const int some = __builtin_popcount(y);
+        for (int drop = some - left; drop > 0; --drop) y &= y - 1;
+        rows[i * PITCH + w] = y;
+        left = left > some ? left - some : 0;
+      }
+    }
+    __syncthreads();
+  }
   const int words = (int)d.words;
   for (int x = i; x < n * words; x += N) {
     const int t = x / words, w = x - t * words;
-    uint32_t y = rows[t * PITCH + w];
-    if (d.window && depths[t] >= d.window) {        // the highest `window` bits of the row
-      int left = (int)d.window;
-      for (int k = t >> 5; k > w; --k) left -= __builtin_popcount(rows[t * PITCH + k]);
-      for (int drop = __builtin_popcount(y) - (left > 0 ? left : 0); drop > 0; --drop) y &= y - 1;
-    }
-    ((KTIR_G(uint32_t)*)d.mask)[(start + t) * d.mask_row + w] = y;
+    ((KTIR_G(uint32_t)*)d.mask)[(start + t) * d.mask_row + w] = rows[t * PITCH + w];
   }
 }
 

@@ -33,7 +33,7 @@
 #pragma once
 #include <type_traits>
 
-#include "ktir_kv8_dev.h"
+#include "ktir_kv8_tree.h"
 
 namespace ktir {
 
@@ -46,13 +46,101 @@ constexpr float TILE_TOP = 11.f, TILE_LAG = 4.f;       // exponent of the larges
 __device__ __forceinline__ int k_slot(int key, int chunk) { return chunk ^ (key & 7) ^ (chunk >> 3 & 1); }
 __device__ __forceinline__ int v_slot(int col, int chunk) { return chunk ^ (((col >> 2) ^ col) & 7); }
 
-// A tree's keys may be split over `splits` workgroups, `part` (a multiple of 64) each: what each leaves in the
-// workspace lies as the lanes have it, 8 J vectors of 4 columns of each wavefront's 64 lanes, then b and l of 32 rows.
-template <int J>
-__host__ __device__ constexpr int64_t tile_part_size(int waves) { return (int64_t)waves * (32 * 64 * J + 64); }
+// The steps over the keys of all tiles of rows of a head are cut into pieces of `each` steps, a workgroup each and `pieces`
+// at most, whatever the batch: the lengths are on the device, and so is the cut.
+constexpr int TREE_WHOLE = 1 << 25;    // more steps than a tile has
+
+__device__ __forceinline__ int64_t wave_sum(int64_t x) {
+  for (int o = 32; o; o >>= 1) x += __shfl_xor((long long)x, o);
+  return x;
+}
+// tiles of rows of a sequence, whose first one is t, and steps of each
+__device__ __forceinline__ int tree_tiles(const ktir_kv8_attn_t& d, const Tile& t, int grp, int TM) {
+  const int64_t n = t.q.n_new < d.max_q ? t.q.n_new : d.max_q;
+  return t.rows ? (int)((n * grp + TM - 1) / TM) : 0;
+}
+__device__ __forceinline__ int tree_steps(const Tile& t) {
+  const int keys = t.hi - (t.lo & ~(TILE_KEYS - 1));
+  return keys > TILE_KEYS ? (keys + TILE_KEYS - 1) / TILE_KEYS : 1;
+}
+__device__ __forceinline__ int ceil_div(int a, int b) { return (int)((uint32_t)(a + b - 1) / (uint32_t)b); }
+// steps of the pieces of a tile: as many pieces as `each` makes of it, alike
+__device__ __forceinline__ int tree_piece_steps(int steps, int each) { return ceil_div(steps, ceil_div(steps, each)); }
+
+// the first tile of sequence s, no rows where there is none
+__device__ __forceinline__ Tile tree_first_tile(const ktir_kv8_attn_t& d, int64_t s, int grp, int TM, int* err) {
+  return s < d.batch.seqs ? tile_at<true>(d, s, seq_of(d.batch, d.cache.page, s, err), 0, TM, grp, err) : Tile{};
+}
+
+// What all lanes of a wavefront find out together of a head's sequences, 64 at a time.
+struct TreeLook {
+  Tile t;              // the first tile of sequence l of the 64 at hand
+  int tiles, steps;    // of the sequence's rows; of each over its keys
+  __device__ __forceinline__ void at(const ktir_kv8_attn_t& d, int64_t base, int grp, int TM, int* err) {
+    t = tree_first_tile(d, base + (threadIdx.x & 63), grp, TM, err);
+    tiles = tree_tiles(d, t, grp, TM);
+    steps = tree_steps(t);
+  }
+};
+// Most steps of a piece; pieces 0: none is cut.  One sequence of n tiles is cut into floor(pieces / n) for each; of more, n tiles
+// of so many steps together make n pieces more than their steps' share at most.  `look` is at the first 64 sequences.
+__device__ __forceinline__ int tree_each(const ktir_kv8_attn_t& d, int grp, int TM, int pieces, const TreeLook& look, int* err) {
+  if (!pieces) return TREE_WHOLE;
+  int64_t each;
+  if (d.batch.seqs == 1) {
+    const int n = lane_of(look.tiles, 0), parts = n ? pieces / n : 1;
+    each = ceil_div(lane_of(look.steps, 0), parts > 1 ? parts : 1);
+  } else {
+    int64_t tiles = look.tiles, steps = (int64_t)look.tiles * look.steps;
+    for (int64_t base = 64; base < d.batch.seqs; base += 64) {
+      TreeLook x;
+      x.at(d, base, grp, TM, err);
+      tiles += x.tiles;
+      steps += (int64_t)x.tiles * x.steps;
+    }
+    steps = wave_sum(steps);
+    const int64_t spare = pieces - wave_sum(tiles);
+    each = spare > 0 ? (steps + spare - 1) / spare : TREE_WHOLE;
+  }
+  return uni(each < TREE_LEAST ? TREE_LEAST : each < TREE_WHOLE ? (int)each : TREE_WHOLE);
+}
+// The tile that piece `at` of a head is of, its number in the tile and the steps of one.  The pieces of a sequence's tiles that
+// have the same keys follow one another, so that they read them together (eight sequences of 256 drafts after up to
+// 16384: 463 us with a tile's pieces together, 429).
+__device__ __forceinline__ Tile tree_piece(const ktir_kv8_attn_t& d, int grp, int TM, int each, int64_t at, TreeLook& look, int* piece, int* steps, int* err) {
+  const int l = threadIdx.x & 63;
+  for (int64_t base = 0; base < d.batch.seqs; base += 64) {
+    if (base) look.at(d, base, grp, TM, err);
+    const int part = tree_piece_steps(look.steps, each), own = ceil_div(look.steps, part), n = look.tiles * own;
+    int upto = n;
+    for (int o = 1; o < 64; o <<= 1) {
+      const int y = __shfl_up(upto, o);
+      upto += l >= o ? y : 0;
+    }
+    const uint64_t past = __ballot(at < upto);
+    if (past) {
+      const int i = __builtin_ctzll(past), tiles = lane_of(look.tiles, i), rest = (int)at - (lane_of(upto, i) - lane_of(n, i));
+      *piece = rest / tiles;
+      *steps = lane_of(part, i);
+      return tile_at<true>(d, base + i, lane_of(look.t.q, i), rest % tiles, TM, grp, err);
+    }
+    at -= lane_of(upto, 63);
+  }
+  return Tile{};
+}
+// pieces of a head's sequences before sequence s
+__device__ __forceinline__ int64_t tree_before_seq(const ktir_kv8_attn_t& d, int grp, int TM, int each, int64_t s, TreeLook& look, int* err) {
+  const int l = threadIdx.x & 63;
+  int64_t before = 0;
+  for (int64_t base = 0; base < s; base += 64) {
+    if (base) look.at(d, base, grp, TM, err);
+    before += base + l < s ? look.tiles * ceil_div(look.steps, tree_piece_steps(look.steps, each)) : 0;
+  }
+  return wave_sum(before);
+}
 
 template <int CODE, int J, int RB, int W, bool TREE>
-__global__ __launch_bounds__(64 * W, W / 4) void kv8_attn_tile(const ktir_kv8_attn_t d, const KV8Mask mask, uint32_t slots, int splits, int part, int part_waves, int* err) {
+__global__ __launch_bounds__(64 * W, W / 4) void kv8_attn_tile(const ktir_kv8_attn_t d, const KV8Mask mask, uint32_t slots, int pieces, int part_waves, int* err) {
   constexpr int TM = 32 * RB * W, DP = 64 * J, NT = 64 * W;
   constexpr int KU = TILE_KEYS * 4 * J, VU = 16 * 16 * J, KP = (KU + NT - 1) / NT, VP = (VU + NT - 1) / NT;   // units of a step, a thread's
   constexpr bool TURNS = J == 2;                 // the two wavefronts of a SIMD take turns
@@ -64,22 +152,29 @@ __global__ __launch_bounds__(64 * W, W / 4) void kv8_attn_tile(const ktir_kv8_at
   const int grp = (int)((uint32_t)d.q_heads / (uint32_t)c.heads), D = (int)c.columns, shift = __builtin_ctz((uint32_t)c.page);
   // a head's tiles share one XCD's L2 where there are 8 heads; the longest rows (the last tiles) start first
   const uint32_t heads = (uint32_t)c.heads, order = blockIdx.x / heads;
-  uint32_t slot = slots - 1 - order;
+  const uint32_t slot = slots - 1 - order;
   const int64_t head = blockIdx.x - order * heads;
-  int split = 0;
+  Tile t;
+  int from;
+  KTIR_G(float)* ws = nullptr;                       // of a tile of several pieces
   if constexpr (TREE) {
-    slot = order % slots;
-    split = (int)(order / slots);
-  }
-  Tile t = uni(tile_of<TREE>(d, slot, TM, grp, err));
-  if (!t.rows) return;
-  const int from = (t.lo & ~(TILE_KEYS - 1)) + split * part;
-  int active = 1;
-  if constexpr (TREE) {                              // this workgroup's part of the keys
-    active = tile_parts<TILE_KEYS>(t, part);
-    if (split >= active) return;
+    TreeLook look;
+    look.at(d, 0, grp, TM, err);
+    const int each = tree_each(d, grp, TM, pieces > (int)slots ? pieces : 0, look, err);
+    int piece = 0, part = 0;
+    t = uni(tree_piece(d, grp, TM, each, order, look, &piece, &part, err));
+    if (!t.rows) return;
+    piece = uni(piece);
+    part = uni(part);
+    const int steps = tree_steps(t);
+    from = (t.lo & ~(TILE_KEYS - 1)) + TILE_KEYS * part * piece;
     t.lo = t.lo > from ? t.lo : from;
-    t.hi = t.hi - from < part ? t.hi : from + part;
+    t.hi = steps > part * (piece + 1) ? from + TILE_KEYS * part : t.hi;
+    if (steps > part) ws = (KTIR_G(float)*)d.ws + blockIdx.x * tree_part_size(J, part_waves);
+  } else {
+    t = uni(tile_of(d, slot, TM, grp, err));
+    if (!t.rows) return;
+    from = t.lo & ~(TILE_KEYS - 1);
   }
 
   // this lane's rows; the wavefront's bounds of keys
@@ -453,10 +548,9 @@ __global__ __launch_bounds__(64 * W, W / 4) void kv8_attn_tile(const ktir_kv8_at
   for (int b = 0; b < RB; ++b) {
     const int r = w0 + 32 * b + r32;
     sum[b] += other_half(sum[b]);
-    if (TREE && active > 1) {
+    if (TREE && ws) {
       static_assert(!TREE || RB == 1, "a wavefront's rows in the workspace");
-      if (wave >= part_waves) continue;
-      KTIR_G(float)* ws = (KTIR_G(float)*)d.ws + (((int64_t)slot * heads + head) * splits + split) * tile_part_size<J>(part_waves);
+      if (wn <= 0) continue;
 #pragma unroll
       for (int n = 0; n < 2 * J; ++n)
 #pragma unroll
@@ -494,38 +588,69 @@ __global__ __launch_bounds__(64 * W, W / 4) void kv8_attn_tile(const ktir_kv8_at
   }
 }
 
-// The parts of a tile's splits, joined: a wavefront for each vector of 4 columns of 32 rows, four a workgroup.
-template <int J>
-__global__ __launch_bounds__(256) void kv8_tile_join(const ktir_kv8_attn_t d, const KV8Mask mask, int splits, int part, int part_waves, int TM, int* err) {
+// The pieces of a tile, joined: a wavefront has V of the 8 J vectors of 4 columns of 32 rows, EACH pieces of them at once.
+template <int J, int V, int EACH>
+__global__ __launch_bounds__(256) void kv8_tile_join(const ktir_kv8_attn_t d, int pieces, int part_waves, int TM, int* err) {
+  static_assert(8 * J % (4 * V) == 0, "four wavefronts");
   const ktir_kv8_t& c = d.cache;
-  const int l = threadIdx.x & 63, at = (int)blockIdx.z * 4 + uni((int)(threadIdx.x >> 6)), wave = blockIdx.y, h = l >> 5, r32 = l & 31;
+  const int l = threadIdx.x & 63, at = ((int)blockIdx.z * 4 + uni((int)(threadIdx.x >> 6))) * V, wave = blockIdx.y, h = l >> 5, r32 = l & 31;
   const int grp = (int)((uint32_t)d.q_heads / (uint32_t)c.heads), D = (int)c.columns;
   const uint32_t heads = (uint32_t)c.heads, slot = blockIdx.x / heads;
-  const int64_t item = blockIdx.x, head = blockIdx.x - slot * heads, size = tile_part_size<J>(part_waves);
+  const int64_t head = blockIdx.x - slot * heads, size = tree_part_size(J, part_waves);
+  TreeLook look;
+  look.at(d, 0, grp, TM, err);
   const Tile t = uni(tile_of<true>(d, slot, TM, grp, err));
   if (!t.rows || 32 * wave >= t.rows) return;
-  const int parts = tile_parts<TILE_KEYS>(t, part), active = parts < splits ? parts : splits;
-  if (active < 2) return;
-  const KTIR_G(float)*ws = (const KTIR_G(float)*)d.ws + item * splits * size, *bl = ws + (int64_t)part_waves * 2048 * J + 64 * wave + r32;
-  float top = B_NONE;
-  for (int i = 0; i < active; ++i) top = __builtin_fmaxf(top, bl[i * size]);
-  float sum = 0.f;
-  f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
-  const KTIR_G(float)* mine = ws + ((int64_t)wave * 8 * J + at) * 256 + 4 * l;
-#pragma unroll 8
-  for (int i = 0; i < active; ++i) {
-    const float f = __builtin_amdgcn_exp2f(bl[i * size] - top);
-    sum = __builtin_fmaf(bl[i * size + 32], f, sum);
-    acc += *(const KTIR_G(f32x4_t)*)(mine + i * size) * f;
+  const int each = tree_each(d, grp, TM, pieces, look, err), parts = ceil_div(tree_steps(t), tree_piece_steps(tree_steps(t), each));
+  if (parts < 2) return;
+  const int64_t first = tree_before_seq(d, grp, TM, each, t.s, look, err) + t.row0 / TM;
+  const KTIR_G(float)* ws = (const KTIR_G(float)*)d.ws + (first * heads + head) * size;
+  const int64_t next = tree_tiles(d, t, grp, TM) * heads * size, bl = (int64_t)part_waves * 2048 * J + 64 * wave + r32, mine = ((int64_t)wave * 8 * J + at) * 256 + 4 * l;
+  float top = B_NONE, sum = 0.f;
+  f32x4_t acc[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) acc[v] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  for (int i0 = 0; i0 < parts; i0 += EACH) {
+    float b[EACH], w[EACH];
+    f32x4_t x[EACH][V];
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+      if (i0 + i >= parts) continue;
+      const KTIR_G(float)* p = ws + (i0 + i) * next;
+      b[i] = p[bl];
+      w[i] = p[bl + 32];
+#pragma unroll
+      for (int v = 0; v < V; ++v) x[i][v] = *(const KTIR_G(f32x4_t)*)(p + mine + 256 * v);
+    }
+    float now = top;
+#pragma unroll
+    for (int i = 0; i < EACH; ++i)
+      if (i0 + i < parts) now = __builtin_fmaxf(now, b[i]);
+    const float keep = __builtin_amdgcn_exp2f(top - now);
+    top = now;
+    sum *= keep;
+#pragma unroll
+    for (int v = 0; v < V; ++v) acc[v] *= keep;
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+      if (i0 + i >= parts) continue;
+      const float f = __builtin_amdgcn_exp2f(b[i] - top);
+      sum = __builtin_fmaf(w[i], f, sum);
+#pragma unroll
+      for (int v = 0; v < V; ++v) acc[v] += x[i][v] * f;
+    }
   }
-  const int r = t.row0 + 32 * wave + r32, x = 32 * (at >> 2) + 8 * (at & 3) + 4 * h;
+  const int r = t.row0 + 32 * wave + r32;
   if (r >= t.row0 + t.rows) return;
+  const int64_t tok = t.q.start + r / grp, hq = head * grp + r % grp, e = tok * d.out.tok + hq * d.out.head;
   const bool none = top == B_NONE && sum == 0.f;
   const float inv = none ? 0.f : L_UNIT / sum;
-  const int64_t tok = t.q.start + r / grp, hq = head * grp + r % grp, e = tok * d.out.tok + hq * d.out.head;
-  if (x < D) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) store_elem(d.out.ptr, e + x + i, d.dtype, none ? 0.f : acc[i] * inv);
+  for (int v = 0; v < V; ++v) {
+    const int x = 32 * ((at + v) >> 2) + 8 * ((at + v) & 3) + 4 * h;
+    if (x >= D) continue;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) store_elem(d.out.ptr, e + x + i, d.dtype, none ? 0.f : acc[v][i] * inv);
   }
   if (d.lse && at == 0 && h == 0)
     ((KTIR_G(float)*)d.lse)[tok * d.lse_tok + hq * d.lse_head] = none ? -__builtin_inff() : (top + 16.f + __builtin_amdgcn_logf(sum)) * 0.69314718055994530942f;

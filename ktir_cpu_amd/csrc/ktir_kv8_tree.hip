@@ -12,7 +12,7 @@ struct TreePlan {
   bool tile;
   KV8Shape rows;       // tile false
   TreeTiles tiles;     // true
-  int64_t items, floats;        // tiles of rows times KV heads; of a split's part
+  int64_t groups, floats;       // how many share the keys (of a tile, or of a head); of the workspace for each
 };
 
 static TreePlan tree_plan(const ktir_kv8_attn_t& d) {
@@ -20,25 +20,28 @@ static TreePlan tree_plan(const ktir_kv8_attn_t& d) {
   kv8_rows_shape(d, true, &p.rows);
   p.tile = tree_tiles(d, p.rows);
   if (p.tile) {
-    const int64_t grp = d.q_heads / d.cache.heads, most = d.max_q * grp;
+    const int64_t grp = d.q_heads / d.cache.heads, rows = d.max_q * grp;
     TreeTiles& t = p.tiles;
     t.J = d.cache.columns <= 64 ? 1 : d.cache.columns <= 128 ? 2 : 4;
     t.TM = t.J == 4 ? 128 : 256;
-    t.slots = most > t.TM ? d.batch.tokens * grp / t.TM + d.batch.seqs : d.batch.seqs;
-    t.waves = (int)((most < t.TM ? most : t.TM) + 31) / 32;
-    t.span = d.max_k;
-    if (d.window && d.window + d.max_q < t.span) t.span = d.window + d.max_q;
-    t.span += 63;
-    const int64_t sets = t.slots * d.cache.heads;
-    int64_t n = sets ? 256 / sets : 1;
-    const int64_t most_parts = (t.span + 255) / 256;
-    n = n > most_parts ? most_parts : n;
-    t.splits = n < 1 ? 1 : n > 256 ? 256 : (int)n;
-    p.items = sets;
-    p.floats = (int64_t)t.waves * (2048 * t.J + 64);
+    t.slots = rows > t.TM ? d.batch.tokens * grp / t.TM + d.batch.seqs : d.batch.seqs;
+    t.waves = (int)((rows < t.TM ? rows : t.TM) + 31) / 32;
+    // Pieces: one for each CU where that cuts every tile into several; up to 1024 tiles two for each, so that no long
+    // tile is left at the end (more give evener shares, but each costs 12 us and 264 KB to and from the workspace); more tiles
+    // are not cut.  No more than the longest sequence can have.
+    const int64_t heads = d.cache.heads, n = t.slots * heads;
+    int64_t span = d.max_k;
+    if (d.window && d.window + d.max_q < span) span = d.window + d.max_q;
+    const int64_t most = t.slots * ((span / 64 + 1) / TREE_LEAST + 1);
+    int64_t pieces = n <= 1024 ? 2 * t.slots : t.slots;
+    if (n <= 256 && pieces < 256 / heads) pieces = 256 / heads;
+    if (pieces > most) pieces = most;
+    t.pieces = (int)(pieces > t.slots ? pieces : t.slots);
+    p.groups = t.pieces > t.slots ? t.pieces : 1;
+    p.floats = heads * tree_part_size(t.J, t.waves);
   } else {
-    p.items = p.rows.slots * d.cache.heads;
-    p.floats = p.rows.part;
+    p.groups = p.rows.splits;
+    p.floats = p.rows.slots * d.cache.heads * p.rows.part;
   }
   return p;
 }
@@ -62,8 +65,8 @@ extern "C" int ktir_kv8_tree_attention_plan(ktir_kv8_tree_attn_t* d) {
   const int rc = check_tree(ME, *d);
   if (rc != KTIR_OK) return rc;
   const TreePlan p = tree_plan(d->attn);
-  d->attn.splits = p.tile ? p.tiles.splits : p.rows.splits;
-  d->attn.ws_bytes = d->attn.splits > 1 ? p.items * d->attn.splits * p.floats * 4 : 0;
+  d->attn.splits = (int32_t)p.groups;
+  d->attn.ws_bytes = p.groups > 1 ? p.groups * p.floats * 4 : 0;
   return KTIR_OK;
 }
 
@@ -83,9 +86,11 @@ extern "C" int ktir_launch_kv8_tree_attention(const ktir_kv8_tree_attn_t* t) {
     return set_error(KTIR_E_ARG, "%s: an output or the workspace overlaps the mask or positions", ME);
   TreePlan p = tree_plan(*d);
   const int64_t splits = d->splits < 1 ? 1 : d->splits;
-  if (splits > 256) return set_error(KTIR_E_ARG, "%s: %lld splits, 256 at most", ME, (long long)splits);
-  if (p.items > INT32_MAX / splits) return set_error(KTIR_E_UNSUPPORTED, "%s: %lld tiles in %lld splits", ME, (long long)p.items, (long long)splits);
-  if (splits > 1 && (!d->ws || (d->ws & 15) || d->ws_bytes / 4 / p.floats / p.items < splits))
+  if (splits > (p.tile ? 1 << 16 : 256)) return set_error(KTIR_E_ARG, "%s: %lld splits", ME, (long long)splits);
+  const int64_t items = (p.tile ? 1 : p.rows.slots) * d->cache.heads;
+  if (p.tile && splits > 1 && splits <= p.tiles.slots) return set_error(KTIR_E_ARG, "%s: %lld splits of %lld tiles", ME, (long long)splits, (long long)p.tiles.slots);
+  if (items > INT32_MAX / splits || (p.tile && p.tiles.slots * d->cache.heads > INT32_MAX)) return set_error(KTIR_E_UNSUPPORTED, "%s: %lld tiles in %lld splits", ME, (long long)items, (long long)splits);
+  if (splits > 1 && (!d->ws || (d->ws & 15) || d->ws_bytes / 4 / p.floats < splits))
     return set_error(KTIR_E_ARG, "%s: %lld splits with a workspace of %lld bytes at %llx", ME, (long long)splits, (long long)d->ws_bytes, (unsigned long long)d->ws);
   rc = ready(ME);
   if (rc != KTIR_OK) return rc;
@@ -93,6 +98,6 @@ extern "C" int ktir_launch_kv8_tree_attention(const ktir_kv8_tree_attn_t* t) {
   if (!on.ok()) return set_error(KTIR_E_HIP, "%s: no device", ME);
   const KV8Mask m = {t->mask, t->pos, t->mask_row, (int32_t)t->words, 0};
   if (!p.tile) return tree_rows_launch(*d, m, p.rows);
-  p.tiles.splits = (int)splits;
+  p.tiles.pieces = splits > 1 ? (int)splits : (int)p.tiles.slots;
   return tree_tile_launch(*d, m, p.tiles);
 }

@@ -6,12 +6,15 @@ namespace ktir {
 
 template <int CODE, int J, int W>
 static void tree_tile_go(const ktir_kv8_attn_t& d, const KV8Mask& mask, const TreeTiles& s) {
-  const int part = (int)(((s.span + s.splits - 1) / s.splits + TILE_KEYS - 1) / TILE_KEYS * TILE_KEYS);
-  const unsigned items = (unsigned)(s.slots * d.cache.heads);
+  const unsigned heads = (unsigned)d.cache.heads, items = (unsigned)s.slots * heads;
   const hipStream_t st = stream_of(d.stream);
-  hipLaunchKernelGGL((kv8_attn_tile<CODE, J, 1, W, true>), dim3(items * s.splits), dim3(64 * W), 0, st, d, mask, (uint32_t)s.slots, s.splits, part, s.waves, device_error_flag());
-  if (s.splits > 1)
-    hipLaunchKernelGGL((kv8_tile_join<J>), dim3(items, s.waves, 2 * J), dim3(256), 0, st, d, mask, s.splits, part, s.waves, s.TM, device_error_flag());
+  hipLaunchKernelGGL((kv8_attn_tile<CODE, J, 1, W, true>), dim3(s.pieces * heads), dim3(64 * W), 0, st, d, mask, (uint32_t)s.slots, s.pieces, s.waves, device_error_flag());
+  if (s.pieces > s.slots) {
+    // many tiles: more for each wavefront, which has to find its place first
+    constexpr int V = J == 1 ? 2 : 4;
+    if (items <= 16) hipLaunchKernelGGL((kv8_tile_join<J, 1, 16>), dim3(items, s.waves, 2 * J), dim3(256), 0, st, d, s.pieces, s.waves, s.TM, device_error_flag());
+    else hipLaunchKernelGGL((kv8_tile_join<J, V, 8>), dim3(items, s.waves, 2 * J / V), dim3(256), 0, st, d, s.pieces, s.waves, s.TM, device_error_flag());
+  }
 }
 
 template <int CODE>
