@@ -153,6 +153,26 @@ __device__ __forceinline__ uint32_t tree_bits(const KV8Mask& m, const Tile& t, i
   return left >= 32 ? w : left > 0 ? w & ~(~0u << left) : 0u;
 }
 
+// What the kernels for trees leave behind the parts in the workspace for the kernel that joins them: each sequence's
+// first part of a head, and how many each of its tiles has (kernels: all of one head's; 1: nothing to join).
+struct TreeNote {
+  int32_t first, parts;
+};
+__device__ __forceinline__ KTIR_G(int32_t)* tree_note(const ktir_kv8_attn_t& d, int64_t parts, int64_t floats, int64_t s) {
+  return (KTIR_G(int32_t)*)(d.ws + (uint64_t)(parts * d.cache.heads * floats) * 4) + 2 * s;
+}
+__device__ __forceinline__ void note_tree(const ktir_kv8_attn_t& d, int64_t parts, int64_t floats, int64_t s, const TreeNote& n) {
+  KTIR_G(int32_t)* p = tree_note(d, parts, floats, s);
+  p[0] = n.first, p[1] = n.parts;
+}
+// (never past the launch's parts, whatever the note says: offsets that overlap may have more tiles than the launch has parts)
+__device__ __forceinline__ TreeNote tree_noted(const ktir_kv8_attn_t& d, int64_t parts, int64_t floats, int64_t s, int tiles) {
+  const KTIR_G(int32_t)* p = tree_note(d, parts, floats, s);
+  TreeNote n = {p[0], p[1]};
+  if (n.first < 0 || n.parts < 1 || n.first + (int64_t)n.parts * tiles > parts) n.parts = 1;
+  return {uni(n.first), uni(n.parts)};
+}
+
 // tile `nth` (of TM rows) of sequence s, which is q
 template <bool TREE = false>
 __device__ __forceinline__ Tile tile_at(const ktir_kv8_attn_t& d, int64_t s, const Seq& q, int64_t nth, int TM, int grp, int* err) {

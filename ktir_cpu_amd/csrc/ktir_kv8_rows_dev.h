@@ -94,8 +94,68 @@ __device__ __forceinline__ void kv8_values(const ktir_kv8_t& c, const KV8Groups&
   }
 }
 
+// Trees: the parts of a head's sequences are cut on the device, where the lengths are, `parts` of them at most.  All lanes of a
+// wavefront look together, 64 sequences at a time.
+struct RowsLook {
+  Tile t;              // of sequence l of the 64 at hand
+  int units;           // steps of all wavefronts of a part over its keys
+  __device__ __forceinline__ void at(const ktir_kv8_attn_t& d, int64_t base, int grp, int TM, int quant, int* err) {
+    const int64_t s = base + (threadIdx.x & 63);
+    t = s < d.batch.seqs ? tile_at<true>(d, s, seq_of(d.batch, d.cache.page, s, err), 0, TM, grp, err) : Tile{};
+    const int keys = t.hi - (t.lo & ~(ROWS_STEP - 1));
+    units = !t.rows ? 0 : keys > quant ? (int)((uint32_t)(keys + quant - 1) / (uint32_t)quant) : 1;
+  }
+};
+// Most units of a part (at least 128 keys); parts 0: none is cut.  n sequences of so many units together make n parts more
+// than their units' share at most.  `look` is at the first 64 sequences.
+__device__ __forceinline__ int rows_each(const ktir_kv8_attn_t& d, int grp, int TM, int quant, int parts, const RowsLook& look, int* err) {
+  if (!parts) return 1 << 30;
+  int64_t units = look.units, seqs = look.units > 0;
+  for (int64_t base = 64; base < d.batch.seqs; base += 64) {
+    RowsLook x;
+    x.at(d, base, grp, TM, quant, err);
+    units += x.units;
+    seqs += x.units > 0;
+  }
+  for (int o = 32; o; o >>= 1) {
+    units += __shfl_xor((long long)units, o);
+    seqs += __shfl_xor((long long)seqs, o);
+  }
+  const int64_t spare = seqs == 1 ? parts : parts - seqs, each = spare > 0 ? (units + spare - 1) / spare : 1 << 30, least = quant < 128 ? 128 / quant : 1;
+  return uni((int)(each < least ? least : each < 1 << 30 ? each : 1 << 30));
+}
+// one sequence by itself: how many parts it has
+__device__ __forceinline__ int rows_parts_of_one(const Tile& t, int quant, int parts) {
+  const int keys = t.hi - (t.lo & ~(ROWS_STEP - 1)), units = keys > quant ? (int)((uint32_t)(keys + quant - 1) / (uint32_t)quant) : 1;
+  const int least = quant < 128 ? 128 / quant : 1, even = (int)((uint32_t)(units + parts - 1) / (uint32_t)parts), each = even < least ? least : even;
+  return (int)((uint32_t)(units + each - 1) / (uint32_t)each);
+}
+// part `at` of a head: its tile, its number of the tile's parts, and how many they are; no rows where there is none
+__device__ __forceinline__ Tile rows_part(const ktir_kv8_attn_t& d, int grp, int TM, int quant, int each, int64_t at, RowsLook& look, int* split, int* active, int* err) {
+  const int l = threadIdx.x & 63;
+  for (int64_t base = 0; base < d.batch.seqs; base += 64) {
+    if (base) look.at(d, base, grp, TM, quant, err);
+    const int n = (int)((uint32_t)(look.units + each - 1) / (uint32_t)each);
+    int upto = n;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int y = __shfl_up(upto, o);
+      upto += l >= o ? y : 0;
+    }
+    const uint64_t past = __ballot(at < upto);
+    if (past) {
+      const int i = __builtin_ctzll(past);
+      *active = lane_of(n, i);
+      *split = (int)at - (lane_of(upto, i) - *active);
+      return lane_of(look.t, i);
+    }
+    at -= lane_of(upto, 63);
+  }
+  return Tile{};
+}
+
 template <int CODE, int J, int MT, bool TREE>
-__global__ __launch_bounds__(64 * ROWS_WAVES, MT == 1 ? 2 : 1) void kv8_attn_rows(const ktir_kv8_attn_t d, const KV8Mask mask, int splits, int part, int part_rows, uint32_t slots, int hw, int* err) {
+__global__ __launch_bounds__(64 * ROWS_WAVES, MT == 1 || (TREE && J * MT <= 4) ? 2 : 1) void kv8_attn_rows(const ktir_kv8_attn_t d, const KV8Mask mask, int splits, int part, int part_rows, uint32_t slots, int hw, int* err) {
   constexpr int W = ROWS_WAVES, TM = 16 * MT, N = 4 * J, PITCH = 64 * J + 4;
   __shared__ __attribute__((aligned(16))) float o_sum[W][TM * PITCH];
   __shared__ float w_b[W][TM], w_l[W][TM];
@@ -111,7 +171,23 @@ __global__ __launch_bounds__(64 * ROWS_WAVES, MT == 1 ? 2 : 1) void kv8_attn_row
   Tile t;
   int split, active, from;
   uint32_t slot;
-  if (d.batch.seqs == 1 && one_tile(d, TM, grp)) {
+  if (TREE && d.batch.seqs == 1) {
+    slot = u;                                          // (of the part in the workspace)
+    split = (int)u;
+    t = uni(tile_at<TREE>(d, 0, seq_of(d.batch, c.page, 0, err), 0, TM, grp, err));
+    if (!t.rows) return;
+    active = splits ? rows_parts_of_one(t, ROWS_STEP * TW, splits) : 1;
+    if (split >= active) return;
+  } else if constexpr (TREE) {
+    RowsLook look;
+    look.at(d, 0, grp, TM, ROWS_STEP * TW, err);
+    slot = u;
+    t = rows_part(d, grp, TM, ROWS_STEP * TW, rows_each(d, grp, TM, ROWS_STEP * TW, splits, look, err), u, look, &split, &active, err);
+    if (!t.rows) return;
+    t = uni(t);
+    split = uni(split);
+    active = uni(active);
+  } else if (d.batch.seqs == 1 && one_tile(d, TM, grp)) {
     slot = 0;
     split = (int)u;
     t = uni(tile_at<TREE>(d, 0, seq_of(d.batch, c.page, 0, err), 0, TM, grp, err));
@@ -381,8 +457,9 @@ __global__ __launch_bounds__(64 * ROWS_WAVES, MT == 1 ? 2 : 1) void kv8_attn_row
   }
   __syncthreads();
 
+  if (TREE && splits && split == 0 && octet == eighth * sets && threadIdx.x == 0) note_tree(d, splits, part_size<J>(part_rows), t.s, {(int)u, active});
   // alone: the result; otherwise its part for kv8_attn_join
-  KTIR_G(float)* ws = (KTIR_G(float)*)d.ws + (item * splits + split) * part_size<J>(part_rows);
+  KTIR_G(float)* ws = (KTIR_G(float)*)d.ws + (TREE ? item : item * splits + split) * part_size<J>(part_rows);
   for (int at = turn * 64 + l; at < t.rows * 16 * J; at += 64 * TW) {
     const int row = at / (16 * J), x4 = at % (16 * J) * 4;
     f32x4_t o = {0.f, 0.f, 0.f, 0.f};
@@ -419,7 +496,7 @@ __global__ __launch_bounds__(64 * ROWS_WAVES, MT == 1 ? 2 : 1) void kv8_attn_row
 // read at once, before the sequence's length says which of them were written.
 constexpr int JOIN_EACH = 16;
 
-template <int J, int MT, int R, int B, bool TREE>
+template <int J, int MT, int R, int B>
 __global__ __launch_bounds__(64 * R * B) void kv8_attn_join(const ktir_kv8_attn_t d, int splits, int part, int part_rows, int* err) {
   constexpr int TM = 16 * MT, LOOK = B == 1 ? 1 : MOST_SPLITS / 64;
   static_assert(B * JOIN_EACH <= 64 * LOOK, "a lane looks at the b and l of each split");
@@ -446,7 +523,7 @@ __global__ __launch_bounds__(64 * R * B) void kv8_attn_join(const ktir_kv8_attn_
 #pragma unroll
       for (int j = 0; j < J; ++j) x[k][j] = ws[(turn + B * k) * size + row * 64 * J + 64 * j + l];
     }
-  const Tile t = uni(tile_of<TREE>(d, slot, TM, grp, err));
+  const Tile t = uni(tile_of(d, slot, TM, grp, err));
   const int parts = tile_parts<ROWS_STEP>(t, part), active = parts < splits ? parts : splits;
   const bool on = row < t.rows && active > 1;
   float top = B_NONE, lt = 0.f;
@@ -485,7 +562,7 @@ __global__ __launch_bounds__(64 * R * B) void kv8_attn_join(const ktir_kv8_attn_
   }
   if (!on || turn) return;
   const int r = t.row0 + row;
-  const bool none = sees_none<TREE>(d, t, r, grp, top, lt);
+  const bool none = sees_none<false>(d, t, r, grp, top, lt);
   const int64_t tok = t.q.start + r / grp, h = head * grp + r % grp;
   const float inv = L_UNIT / lt;
 #pragma unroll
@@ -496,6 +573,65 @@ __global__ __launch_bounds__(64 * R * B) void kv8_attn_join(const ktir_kv8_attn_
         none ? -__builtin_inff() : (top + 16.f + __builtin_amdgcn_logf(lt)) * 0.69314718055994530942f;
 }
 
+// The parts of a tree's rows, joined: a wavefront for each row, J columns a lane, EACH parts at once.
+template <int J, int MT>
+__global__ __launch_bounds__(256) void kv8_rows_join(const ktir_kv8_attn_t d, int parts, int part_rows, int* err) {
+  constexpr int TM = 16 * MT, EACH = J <= 2 ? 16 : 8;
+  const ktir_kv8_t& c = d.cache;
+  const int l = threadIdx.x & 63, row = (int)blockIdx.y * 4 + uni((int)(threadIdx.x >> 6)), grp = (int)((uint32_t)d.q_heads / (uint32_t)c.heads), D = (int)c.columns;
+  const uint32_t heads = (uint32_t)c.heads, slot = blockIdx.x / heads;
+  const int64_t head = blockIdx.x - slot * heads, size = part_size<J>(part_rows), next = heads * size;
+  const Tile t = uni(tile_at<true>(d, slot, seq_of(d.batch, c.page, slot, err), 0, TM, grp, err));
+  if (row >= t.rows) return;
+  const TreeNote note = tree_noted(d, parts, size, slot, 1);
+  const int active = note.parts;
+  const int64_t first = note.first;
+  if (active < 2) return;
+  const KTIR_G(float)* ws = (const KTIR_G(float)*)d.ws + (first * heads + head) * size;
+  float top = B_NONE, sum = 0.f, acc[J] = {};
+  for (int i0 = 0; i0 < active; i0 += EACH) {
+    float x[EACH][J], b = B_NONE, w = 0.f;
+    if (l < EACH && i0 + l < active) {
+      b = ws[(i0 + l) * next + part_rows * 64 * J + row];
+      w = ws[(i0 + l) * next + part_rows * (64 * J + 1) + row];
+    }
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+      if (i0 + i >= active) break;
+#pragma unroll
+      for (int j = 0; j < J; ++j) x[i][j] = ws[(i0 + i) * next + row * 64 * J + 64 * j + l];
+    }
+    float now = b;
+#pragma unroll
+    for (int o = EACH / 2; o; o >>= 1) now = __builtin_fmaxf(now, __shfl_xor(now, o));
+    now = __builtin_fmaxf(top, lane_of(now, 0));
+    const float keep = __builtin_amdgcn_exp2f(top - now), f = __builtin_amdgcn_exp2f(b - now);
+    top = now;
+    w *= f;
+#pragma unroll
+    for (int o = EACH / 2; o; o >>= 1) w += __shfl_xor(w, o);
+    sum = sum * keep + lane_of(w, 0);
+#pragma unroll
+    for (int j = 0; j < J; ++j) acc[j] *= keep;
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+      if (i0 + i >= active) break;
+      const float fi = lane_of(f, i);
+#pragma unroll
+      for (int j = 0; j < J; ++j) acc[j] = __builtin_fmaf(x[i][j], fi, acc[j]);
+    }
+  }
+  const int r = t.row0 + row;
+  const bool none = top == B_NONE && sum == 0.f;
+  const float inv = L_UNIT / sum;
+  const int64_t tok = t.q.start + r / grp, h = head * grp + r % grp;
+#pragma unroll
+  for (int j = 0; j < J; ++j)
+    if (64 * j + l < D) store_elem(d.out.ptr, tok * d.out.tok + h * d.out.head + 64 * j + l, d.dtype, none ? 0.f : acc[j] * inv);
+  if (d.lse && l == 0)
+    ((KTIR_G(float)*)d.lse)[tok * d.lse_tok + h * d.lse_head] = none ? -__builtin_inff() : (top + 16.f + __builtin_amdgcn_logf(sum)) * 0.69314718055994530942f;
+}
+
 template <int CODE, int J, int MT, bool TREE>
 int kv8_rows_go(const ktir_kv8_attn_t& d, const KV8Mask& mask, const KV8Shape& s) {
   constexpr int W = ROWS_WAVES;
@@ -504,10 +640,12 @@ int kv8_rows_go(const ktir_kv8_attn_t& d, const KV8Mask& mask, const KV8Shape& s
   // two workgroups a CU, evenly: where three fit, some CUs get three and others one (510 parts of 704 keys: 89 and 72 us)
   constexpr int held = (int)(sizeof(float) * W * (16 * MT * (64 * J + 4) + 2 * 16 * MT)), spare = held < 55000 ? 55000 - held : 0;
   const hipStream_t st = stream_of(d.stream);
-  hipLaunchKernelGGL((kv8_attn_rows<CODE, J, MT, TREE>), dim3((unsigned)((s.slots * splits + 7) / 8 * 8 * (d.cache.heads / s.HW))), dim3(64 * W), spare, st, d, mask, (int)splits, part, s.rows, (uint32_t)s.slots, s.HW, device_error_flag());
+  const int64_t groups = !TREE ? s.slots * splits : splits > 1 ? splits : s.slots;
+  hipLaunchKernelGGL((kv8_attn_rows<CODE, J, MT, TREE>), dim3((unsigned)((groups + 7) / 8 * 8 * (d.cache.heads / s.HW))), dim3(64 * W), spare, st, d, mask, TREE && splits == 1 ? 0 : (int)splits, part, s.rows, (uint32_t)s.slots, s.HW, device_error_flag());
   if (splits > 1) {
-    if (splits <= JOIN_EACH) hipLaunchKernelGGL((kv8_attn_join<J, MT, 4, 1, TREE>), dim3((unsigned)items, (unsigned)((s.rows + 3) / 4)), dim3(256), 0, st, d, (int)splits, part, s.rows, device_error_flag());
-    else hipLaunchKernelGGL((kv8_attn_join<J, MT, 1, 16, TREE>), dim3((unsigned)items, (unsigned)s.rows), dim3(1024), 0, st, d, (int)splits, part, s.rows, device_error_flag());
+    if constexpr (TREE) hipLaunchKernelGGL((kv8_rows_join<J, MT>), dim3((unsigned)items, (unsigned)((s.rows + 3) / 4)), dim3(256), 0, st, d, (int)splits, s.rows, device_error_flag());
+    else if (splits <= JOIN_EACH) hipLaunchKernelGGL((kv8_attn_join<J, MT, 4, 1>), dim3((unsigned)items, (unsigned)((s.rows + 3) / 4)), dim3(256), 0, st, d, (int)splits, part, s.rows, device_error_flag());
+    else hipLaunchKernelGGL((kv8_attn_join<J, MT, 1, 16>), dim3((unsigned)items, (unsigned)s.rows), dim3(1024), 0, st, d, (int)splits, part, s.rows, device_error_flag());
   }
   KTIR_HIP_CHECK(hipGetLastError());
   return KTIR_OK;

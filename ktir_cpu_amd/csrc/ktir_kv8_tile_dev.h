@@ -128,17 +128,6 @@ __device__ __forceinline__ Tile tree_piece(const ktir_kv8_attn_t& d, int grp, in
   }
   return Tile{};
 }
-// pieces of a head's sequences before sequence s
-__device__ __forceinline__ int64_t tree_before_seq(const ktir_kv8_attn_t& d, int grp, int TM, int each, int64_t s, TreeLook& look, int* err) {
-  const int l = threadIdx.x & 63;
-  int64_t before = 0;
-  for (int64_t base = 0; base < s; base += 64) {
-    if (base) look.at(d, base, grp, TM, err);
-    before += base + l < s ? look.tiles * ceil_div(look.steps, tree_piece_steps(look.steps, each)) : 0;
-  }
-  return wave_sum(before);
-}
-
 template <int CODE, int J, int RB, int W, bool TREE>
 __global__ __launch_bounds__(64 * W, W / 4) void kv8_attn_tile(const ktir_kv8_attn_t d, const KV8Mask mask, uint32_t slots, int pieces, int part_waves, int* err) {
   constexpr int TM = 32 * RB * W, DP = 64 * J, NT = 64 * W;
@@ -170,6 +159,8 @@ __global__ __launch_bounds__(64 * W, W / 4) void kv8_attn_tile(const ktir_kv8_at
     from = (t.lo & ~(TILE_KEYS - 1)) + TILE_KEYS * part * piece;
     t.lo = t.lo > from ? t.lo : from;
     t.hi = steps > part * (piece + 1) ? from + TILE_KEYS * part : t.hi;
+    if (pieces > (int)slots && piece == 0 && t.row0 == 0 && head == 0 && tid == 0)
+      note_tree(d, pieces, tree_part_size(J, part_waves), t.s, {(int)order, ceil_div(steps, part)});
     if (steps > part) ws = (KTIR_G(float)*)d.ws + blockIdx.x * tree_part_size(J, part_waves);
   } else {
     t = uni(tile_of(d, slot, TM, grp, err));
@@ -597,15 +588,15 @@ __global__ __launch_bounds__(256) void kv8_tile_join(const ktir_kv8_attn_t d, in
   const int grp = (int)((uint32_t)d.q_heads / (uint32_t)c.heads), D = (int)c.columns;
   const uint32_t heads = (uint32_t)c.heads, slot = blockIdx.x / heads;
   const int64_t head = blockIdx.x - slot * heads, size = tree_part_size(J, part_waves);
-  TreeLook look;
-  look.at(d, 0, grp, TM, err);
   const Tile t = uni(tile_of<true>(d, slot, TM, grp, err));
   if (!t.rows || 32 * wave >= t.rows) return;
-  const int each = tree_each(d, grp, TM, pieces, look, err), parts = ceil_div(tree_steps(t), tree_piece_steps(tree_steps(t), each));
+  const int tiles = tree_tiles(d, t, grp, TM);
+  const TreeNote note = tree_noted(d, pieces, size, t.s, tiles);
+  const int parts = note.parts;
   if (parts < 2) return;
-  const int64_t first = tree_before_seq(d, grp, TM, each, t.s, look, err) + t.row0 / TM;
+  const int64_t first = note.first + t.row0 / TM;
   const KTIR_G(float)* ws = (const KTIR_G(float)*)d.ws + (first * heads + head) * size;
-  const int64_t next = tree_tiles(d, t, grp, TM) * heads * size, bl = (int64_t)part_waves * 2048 * J + 64 * wave + r32, mine = ((int64_t)wave * 8 * J + at) * 256 + 4 * l;
+  const int64_t next = tiles * heads * size, bl = (int64_t)part_waves * 2048 * J + 64 * wave + r32, mine = ((int64_t)wave * 8 * J + at) * 256 + 4 * l;
   float top = B_NONE, sum = 0.f;
   f32x4_t acc[V];
 #pragma unroll

@@ -12,7 +12,7 @@ struct TreePlan {
   bool tile;
   KV8Shape rows;       // tile false
   TreeTiles tiles;     // true
-  int64_t groups, floats;       // how many share the keys (of a tile, or of a head); of the workspace for each
+  int64_t groups, floats;       // how many share the keys of a head; of the workspace for each
 };
 
 static TreePlan tree_plan(const ktir_kv8_attn_t& d) {
@@ -40,8 +40,13 @@ static TreePlan tree_plan(const ktir_kv8_attn_t& d) {
     p.groups = t.pieces > t.slots ? t.pieces : 1;
     p.floats = heads * tree_part_size(t.J, t.waves);
   } else {
-    p.groups = p.rows.splits;
-    p.floats = p.rows.slots * d.cache.heads * p.rows.part;
+    // Parts: two workgroups for each CU, and two at least for each sequence; from 2048 on none is cut.  No more than 128 keys each.
+    const KV8Shape& s = p.rows;
+    const int64_t sets = d.cache.heads / s.HW, most = s.slots * ((s.span + 127) / 128);
+    int64_t parts = 512 / sets > 2 * s.slots ? 512 / sets : 2 * s.slots;
+    if (parts > most) parts = most;
+    p.groups = s.slots * sets >= 2048 || parts <= s.slots ? 1 : parts;
+    p.floats = d.cache.heads * s.part;
   }
   return p;
 }
@@ -66,7 +71,7 @@ extern "C" int ktir_kv8_tree_attention_plan(ktir_kv8_tree_attn_t* d) {
   if (rc != KTIR_OK) return rc;
   const TreePlan p = tree_plan(d->attn);
   d->attn.splits = (int32_t)p.groups;
-  d->attn.ws_bytes = p.groups > 1 ? p.groups * p.floats * 4 : 0;
+  d->attn.ws_bytes = p.groups > 1 ? p.groups * p.floats * 4 + d->attn.batch.seqs * (int64_t)sizeof(TreeNote) : 0;
   return KTIR_OK;
 }
 
@@ -86,11 +91,11 @@ extern "C" int ktir_launch_kv8_tree_attention(const ktir_kv8_tree_attn_t* t) {
     return set_error(KTIR_E_ARG, "%s: an output or the workspace overlaps the mask or positions", ME);
   TreePlan p = tree_plan(*d);
   const int64_t splits = d->splits < 1 ? 1 : d->splits;
-  if (splits > (p.tile ? 1 << 16 : 256)) return set_error(KTIR_E_ARG, "%s: %lld splits", ME, (long long)splits);
-  const int64_t items = (p.tile ? 1 : p.rows.slots) * d->cache.heads;
-  if (p.tile && splits > 1 && splits <= p.tiles.slots) return set_error(KTIR_E_ARG, "%s: %lld splits of %lld tiles", ME, (long long)splits, (long long)p.tiles.slots);
-  if (items > INT32_MAX / splits || (p.tile && p.tiles.slots * d->cache.heads > INT32_MAX)) return set_error(KTIR_E_UNSUPPORTED, "%s: %lld tiles in %lld splits", ME, (long long)items, (long long)splits);
-  if (splits > 1 && (!d->ws || (d->ws & 15) || d->ws_bytes / 4 / p.floats < splits))
+  const int64_t slots = p.tile ? p.tiles.slots : p.rows.slots;
+  if (splits > (1 << 16) || (splits > 1 && splits <= slots)) return set_error(KTIR_E_ARG, "%s: %lld splits of %lld tiles", ME, (long long)splits, (long long)slots);
+  if ((slots + 8) * d->cache.heads > INT32_MAX || splits * d->cache.heads > INT32_MAX)
+    return set_error(KTIR_E_UNSUPPORTED, "%s: %lld tiles of %lld heads in %lld splits", ME, (long long)slots, (long long)d->cache.heads, (long long)splits);
+  if (splits > 1 && (!d->ws || (d->ws & 15) || (d->ws_bytes - d->batch.seqs * (int64_t)sizeof(TreeNote)) / 4 / p.floats < splits))
     return set_error(KTIR_E_ARG, "%s: %lld splits with a workspace of %lld bytes at %llx", ME, (long long)splits, (long long)d->ws_bytes, (unsigned long long)d->ws);
   rc = ready(ME);
   if (rc != KTIR_OK) return rc;
