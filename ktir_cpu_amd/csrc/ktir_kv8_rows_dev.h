@@ -94,66 +94,6 @@ __device__ __forceinline__ void kv8_values(const ktir_kv8_t& c, const KV8Groups&
   }
 }
 
-// Trees: the parts of a head's sequences are cut on the device, where the lengths are, `parts` of them at most.  All lanes of a
-// wavefront look together, 64 sequences at a time.
-struct RowsLook {
-  Tile t;              // of sequence l of the 64 at hand
-  int units;           // steps of all wavefronts of a part over its keys
-  __device__ __forceinline__ void at(const ktir_kv8_attn_t& d, int64_t base, int grp, int TM, int quant, int* err) {
-    const int64_t s = base + (threadIdx.x & 63);
-    t = s < d.batch.seqs ? tile_at<true>(d, s, seq_of(d.batch, d.cache.page, s, err), 0, TM, grp, err) : Tile{};
-    const int keys = t.hi - (t.lo & ~(ROWS_STEP - 1));
-    units = !t.rows ? 0 : keys > quant ? (int)((uint32_t)(keys + quant - 1) / (uint32_t)quant) : 1;
-  }
-};
-// Most units of a part (at least 128 keys); parts 0: none is cut.  n sequences of so many units together make n parts more
-// than their units' share at most.  `look` is at the first 64 sequences.
-__device__ __forceinline__ int rows_each(const ktir_kv8_attn_t& d, int grp, int TM, int quant, int parts, const RowsLook& look, int* err) {
-  if (!parts) return 1 << 30;
-  int64_t units = look.units, seqs = look.units > 0;
-  for (int64_t base = 64; base < d.batch.seqs; base += 64) {
-    RowsLook x;
-    x.at(d, base, grp, TM, quant, err);
-    units += x.units;
-    seqs += x.units > 0;
-  }
-  for (int o = 32; o; o >>= 1) {
-    units += __shfl_xor((long long)units, o);
-    seqs += __shfl_xor((long long)seqs, o);
-  }
-  const int64_t spare = seqs == 1 ? parts : parts - seqs, each = spare > 0 ? (units + spare - 1) / spare : 1 << 30, least = quant < 128 ? 128 / quant : 1;
-  return uni((int)(each < least ? least : each < 1 << 30 ? each : 1 << 30));
-}
-// one sequence by itself: how many parts it has
-__device__ __forceinline__ int rows_parts_of_one(const Tile& t, int quant, int parts) {
-  const int keys = t.hi - (t.lo & ~(ROWS_STEP - 1)), units = keys > quant ? (int)((uint32_t)(keys + quant - 1) / (uint32_t)quant) : 1;
-  const int least = quant < 128 ? 128 / quant : 1, even = (int)((uint32_t)(units + parts - 1) / (uint32_t)parts), each = even < least ? least : even;
-  return (int)((uint32_t)(units + each - 1) / (uint32_t)each);
-}
-// part `at` of a head: its tile, its number of the tile's parts, and how many they are; no rows where there is none
-__device__ __forceinline__ Tile rows_part(const ktir_kv8_attn_t& d, int grp, int TM, int quant, int each, int64_t at, RowsLook& look, int* split, int* active, int* err) {
-  const int l = threadIdx.x & 63;
-  for (int64_t base = 0; base < d.batch.seqs; base += 64) {
-    if (base) look.at(d, base, grp, TM, quant, err);
-    const int n = (int)((uint32_t)(look.units + each - 1) / (uint32_t)each);
-    int upto = n;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int y = __shfl_up(upto, o);
-      upto += l >= o ? y : 0;
-    }
-    const uint64_t past = __ballot(at < upto);
-    if (past) {
-      const int i = __builtin_ctzll(past);
-      *active = lane_of(n, i);
-      *split = (int)at - (lane_of(upto, i) - *active);
-      return lane_of(look.t, i);
-    }
-    at -= lane_of(upto, 63);
-  }
-  return Tile{};
-}
-
 template <int CODE, int J, int MT, bool TREE>
 __global__ __launch_bounds__(64 * ROWS_WAVES, MT == 1 || (TREE && J * MT <= 4) ? 2 : 1) void kv8_attn_rows(const ktir_kv8_attn_t d, const KV8Mask mask, int splits, int part, int part_rows, uint32_t slots, int hw, int* err) {
   constexpr int W = ROWS_WAVES, TM = 16 * MT, N = 4 * J, PITCH = 64 * J + 4;
@@ -171,22 +111,14 @@ __global__ __launch_bounds__(64 * ROWS_WAVES, MT == 1 || (TREE && J * MT <= 4) ?
   Tile t;
   int split, active, from;
   uint32_t slot;
-  if (TREE && d.batch.seqs == 1) {
+  if constexpr (TREE) {
+    const int quant = ROWS_STEP * TW;
+    TreePart p;
     slot = u;                                          // (of the part in the workspace)
-    split = (int)u;
-    t = uni(tile_at<TREE>(d, 0, seq_of(d.batch, c.page, 0, err), 0, TM, grp, err));
+    t = uni(tree_part<ROWS_STEP>(d, grp, TM, quant, quant < 128 ? 128 / quant : 1, splits, u, &p, err));
     if (!t.rows) return;
-    active = splits ? rows_parts_of_one(t, ROWS_STEP * TW, splits) : 1;
-    if (split >= active) return;
-  } else if constexpr (TREE) {
-    RowsLook look;
-    look.at(d, 0, grp, TM, ROWS_STEP * TW, err);
-    slot = u;
-    t = rows_part(d, grp, TM, ROWS_STEP * TW, rows_each(d, grp, TM, ROWS_STEP * TW, splits, look, err), u, look, &split, &active, err);
-    if (!t.rows) return;
-    t = uni(t);
-    split = uni(split);
-    active = uni(active);
+    split = uni(p.at);
+    active = uni(p.count);
   } else if (d.batch.seqs == 1 && one_tile(d, TM, grp)) {
     slot = 0;
     split = (int)u;
@@ -457,7 +389,7 @@ __global__ __launch_bounds__(64 * ROWS_WAVES, MT == 1 || (TREE && J * MT <= 4) ?
   }
   __syncthreads();
 
-  if (TREE && splits && split == 0 && octet == eighth * sets && threadIdx.x == 0) note_tree(d, splits, part_size<J>(part_rows), t.s, {(int)u, active});
+  if (TREE && splits && split == 0 && t.row0 == 0 && octet == eighth * sets && threadIdx.x == 0) note_tree(d, splits, part_size<J>(part_rows), t.s, {(int)u, active});
   // alone: the result; otherwise its part for kv8_attn_join
   KTIR_G(float)* ws = (KTIR_G(float)*)d.ws + (TREE ? item : item * splits + split) * part_size<J>(part_rows);
   for (int at = turn * 64 + l; at < t.rows * 16 * J; at += 64 * TW) {
@@ -580,14 +512,15 @@ __global__ __launch_bounds__(256) void kv8_rows_join(const ktir_kv8_attn_t d, in
   const ktir_kv8_t& c = d.cache;
   const int l = threadIdx.x & 63, row = (int)blockIdx.y * 4 + uni((int)(threadIdx.x >> 6)), grp = (int)((uint32_t)d.q_heads / (uint32_t)c.heads), D = (int)c.columns;
   const uint32_t heads = (uint32_t)c.heads, slot = blockIdx.x / heads;
-  const int64_t head = blockIdx.x - slot * heads, size = part_size<J>(part_rows), next = heads * size;
-  const Tile t = uni(tile_at<true>(d, slot, seq_of(d.batch, c.page, slot, err), 0, TM, grp, err));
+  const int64_t head = blockIdx.x - slot * heads, size = part_size<J>(part_rows);
+  const Tile t = uni(tile_of<true>(d, slot, TM, grp, err));
   if (row >= t.rows) return;
-  const TreeNote note = tree_noted(d, parts, size, slot, 1);
+  const int tiles = tree_tiles(d, t.q, grp, TM);
+  const TreeNote note = tree_noted(d, parts, size, t.s, tiles);
   const int active = note.parts;
-  const int64_t first = note.first;
   if (active < 2) return;
-  const KTIR_G(float)* ws = (const KTIR_G(float)*)d.ws + (first * heads + head) * size;
+  const KTIR_G(float)* ws = (const KTIR_G(float)*)d.ws + ((note.first + t.row0 / TM) * (int64_t)heads + head) * size;
+  const int64_t next = tiles * (int64_t)heads * size;
   float top = B_NONE, sum = 0.f, acc[J] = {};
   for (int i0 = 0; i0 < active; i0 += EACH) {
     float x[EACH][J], b = B_NONE, w = 0.f;

@@ -7,9 +7,9 @@ template <int CODE>
 static void tile_go(const ktir_kv8_attn_t& d, int64_t slots, hipStream_t st) {
   const dim3 grid((unsigned)(slots * d.cache.heads));
   const int D = (int)d.cache.columns;
-  if (D <= 64) hipLaunchKernelGGL((kv8_attn_tile<CODE, 1, 1, 8, false>), grid, dim3(512), 0, st, d, KV8Mask{}, (uint32_t)slots, 0, 0, device_error_flag());
-  else if (D <= 128) hipLaunchKernelGGL((kv8_attn_tile<CODE, 2, 1, 8, false>), grid, dim3(512), 0, st, d, KV8Mask{}, (uint32_t)slots, 0, 0, device_error_flag());
-  else hipLaunchKernelGGL((kv8_attn_tile<CODE, 4, 1, 4, false>), grid, dim3(256), 0, st, d, KV8Mask{}, (uint32_t)slots, 0, 0, device_error_flag());
+  if (D <= 64) hipLaunchKernelGGL((kv8_attn_tile<CODE, 1, 1, 8, false, false>), grid, dim3(512), 0, st, d, KV8Mask{}, (uint32_t)slots, 0, 0, device_error_flag());
+  else if (D <= 128) hipLaunchKernelGGL((kv8_attn_tile<CODE, 2, 1, 8, false, false>), grid, dim3(512), 0, st, d, KV8Mask{}, (uint32_t)slots, 0, 0, device_error_flag());
+  else hipLaunchKernelGGL((kv8_attn_tile<CODE, 4, 1, 4, false, false>), grid, dim3(256), 0, st, d, KV8Mask{}, (uint32_t)slots, 0, 0, device_error_flag());
 }
 
 // Whether a launch takes this kernel, and its tiles of rows for each KV head.  With fewer

@@ -46,95 +46,15 @@ constexpr float TILE_TOP = 11.f, TILE_LAG = 4.f;       // exponent of the larges
 __device__ __forceinline__ int k_slot(int key, int chunk) { return chunk ^ (key & 7) ^ (chunk >> 3 & 1); }
 __device__ __forceinline__ int v_slot(int col, int chunk) { return chunk ^ (((col >> 2) ^ col) & 7); }
 
-// The steps over the keys of all tiles of rows of a head are cut into pieces of `each` steps, a workgroup each and `pieces`
-// at most, whatever the batch: the lengths are on the device, and so is the cut.
-constexpr int TREE_WHOLE = 1 << 25;    // more steps than a tile has
-
-__device__ __forceinline__ int64_t wave_sum(int64_t x) {
-  for (int o = 32; o; o >>= 1) x += __shfl_xor((long long)x, o);
-  return x;
-}
-// tiles of rows of a sequence, whose first one is t, and steps of each
-__device__ __forceinline__ int tree_tiles(const ktir_kv8_attn_t& d, const Tile& t, int grp, int TM) {
-  const int64_t n = t.q.n_new < d.max_q ? t.q.n_new : d.max_q;
-  return t.rows ? (int)((n * grp + TM - 1) / TM) : 0;
-}
-__device__ __forceinline__ int tree_steps(const Tile& t) {
-  const int keys = t.hi - (t.lo & ~(TILE_KEYS - 1));
-  return keys > TILE_KEYS ? (keys + TILE_KEYS - 1) / TILE_KEYS : 1;
-}
-__device__ __forceinline__ int ceil_div(int a, int b) { return (int)((uint32_t)(a + b - 1) / (uint32_t)b); }
-// steps of the pieces of a tile: as many pieces as `each` makes of it, alike
-__device__ __forceinline__ int tree_piece_steps(int steps, int each) { return ceil_div(steps, ceil_div(steps, each)); }
-
-// the first tile of sequence s, no rows where there is none
-__device__ __forceinline__ Tile tree_first_tile(const ktir_kv8_attn_t& d, int64_t s, int grp, int TM, int* err) {
-  return s < d.batch.seqs ? tile_at<true>(d, s, seq_of(d.batch, d.cache.page, s, err), 0, TM, grp, err) : Tile{};
-}
-
-// What all lanes of a wavefront find out together of a head's sequences, 64 at a time.
-struct TreeLook {
-  Tile t;              // the first tile of sequence l of the 64 at hand
-  int tiles, steps;    // of the sequence's rows; of each over its keys
-  __device__ __forceinline__ void at(const ktir_kv8_attn_t& d, int64_t base, int grp, int TM, int* err) {
-    t = tree_first_tile(d, base + (threadIdx.x & 63), grp, TM, err);
-    tiles = tree_tiles(d, t, grp, TM);
-    steps = tree_steps(t);
-  }
-};
-// Most steps of a piece; pieces 0: none is cut.  One sequence of n tiles is cut into floor(pieces / n) for each; of more, n tiles
-// of so many steps together make n pieces more than their steps' share at most.  `look` is at the first 64 sequences.
-__device__ __forceinline__ int tree_each(const ktir_kv8_attn_t& d, int grp, int TM, int pieces, const TreeLook& look, int* err) {
-  if (!pieces) return TREE_WHOLE;
-  int64_t each;
-  if (d.batch.seqs == 1) {
-    const int n = lane_of(look.tiles, 0), parts = n ? pieces / n : 1;
-    each = ceil_div(lane_of(look.steps, 0), parts > 1 ? parts : 1);
-  } else {
-    int64_t tiles = look.tiles, steps = (int64_t)look.tiles * look.steps;
-    for (int64_t base = 64; base < d.batch.seqs; base += 64) {
-      TreeLook x;
-      x.at(d, base, grp, TM, err);
-      tiles += x.tiles;
-      steps += (int64_t)x.tiles * x.steps;
-    }
-    steps = wave_sum(steps);
-    const int64_t spare = pieces - wave_sum(tiles);
-    each = spare > 0 ? (steps + spare - 1) / spare : TREE_WHOLE;
-  }
-  return uni(each < TREE_LEAST ? TREE_LEAST : each < TREE_WHOLE ? (int)each : TREE_WHOLE);
-}
-// The tile that piece `at` of a head is of, its number in the tile and the steps of one.  The pieces of a sequence's tiles that
-// have the same keys follow one another, so that they read them together (eight sequences of 256 drafts after up to
-// 16384: 463 us with a tile's pieces together, 429).
-__device__ __forceinline__ Tile tree_piece(const ktir_kv8_attn_t& d, int grp, int TM, int each, int64_t at, TreeLook& look, int* piece, int* steps, int* err) {
-  const int l = threadIdx.x & 63;
-  for (int64_t base = 0; base < d.batch.seqs; base += 64) {
-    if (base) look.at(d, base, grp, TM, err);
-    const int part = tree_piece_steps(look.steps, each), own = ceil_div(look.steps, part), n = look.tiles * own;
-    int upto = n;
-    for (int o = 1; o < 64; o <<= 1) {
-      const int y = __shfl_up(upto, o);
-      upto += l >= o ? y : 0;
-    }
-    const uint64_t past = __ballot(at < upto);
-    if (past) {
-      const int i = __builtin_ctzll(past), tiles = lane_of(look.tiles, i), rest = (int)at - (lane_of(upto, i) - lane_of(n, i));
-      *piece = rest / tiles;
-      *steps = lane_of(part, i);
-      return tile_at<true>(d, base + i, lane_of(look.t.q, i), rest % tiles, TM, grp, err);
-    }
-    at -= lane_of(upto, 63);
-  }
-  return Tile{};
-}
-template <int CODE, int J, int RB, int W, bool TREE>
-__global__ __launch_bounds__(64 * W, W / 4) void kv8_attn_tile(const ktir_kv8_attn_t d, const KV8Mask mask, uint32_t slots, int pieces, int part_waves, int* err) {
+// IDLE: half of the wavefronts have no rows and lay keys into LDS alone, so that the pipes are the others' (128 columns, eight KV heads:
+// 80 rows of one sequence of 16000 tokens 44 -> 39 us, of six 135 -> 118; but full tiles take 2 % longer).
+template <int CODE, int J, int RB, int W, bool TREE, bool IDLE>
+__global__ __launch_bounds__(64 * W, J == 1 ? 2 : W / 4) void kv8_attn_tile(const ktir_kv8_attn_t d, const KV8Mask mask, uint32_t slots, int pieces, int part_waves, int* err) {
   constexpr int TM = 32 * RB * W, DP = 64 * J, NT = 64 * W;
   constexpr int KU = TILE_KEYS * 4 * J, VU = 16 * 16 * J, KP = (KU + NT - 1) / NT, VP = (VU + NT - 1) / NT;   // units of a step, a thread's
   constexpr bool TURNS = J == 2;                 // the two wavefronts of a SIMD take turns
-  static_assert(J == 1 || J == 2 || J == 4, "columns in 64s");
   static_assert(!TURNS || W == 8, "two wavefronts of a SIMD: i and i + 4");
+  static_assert(J == 1 || J == 2 || J == 4, "columns in 64s");
   __shared__ __attribute__((aligned(16))) uint16_t ks[2][TILE_KEYS * DP], vs[2][DP * TILE_KEYS];
   const ktir_kv8_t& c = d.cache;
   const int tid = threadIdx.x, l = tid & 63, wave = uni(tid >> 6), h = l >> 5, r32 = l & 31;
@@ -147,21 +67,16 @@ __global__ __launch_bounds__(64 * W, W / 4) void kv8_attn_tile(const ktir_kv8_at
   int from;
   KTIR_G(float)* ws = nullptr;                       // of a tile of several pieces
   if constexpr (TREE) {
-    TreeLook look;
-    look.at(d, 0, grp, TM, err);
-    const int each = tree_each(d, grp, TM, pieces > (int)slots ? pieces : 0, look, err);
-    int piece = 0, part = 0;
-    t = uni(tree_piece(d, grp, TM, each, order, look, &piece, &part, err));
+    TreePart part;
+    t = uni(tree_part<TILE_KEYS>(d, grp, TM, TILE_KEYS, TREE_LEAST, pieces > (int)slots ? pieces : 0, order, &part, err));
     if (!t.rows) return;
-    piece = uni(piece);
-    part = uni(part);
-    const int steps = tree_steps(t);
-    from = (t.lo & ~(TILE_KEYS - 1)) + TILE_KEYS * part * piece;
+    const int at = uni(part.at), units = uni(part.units), count = uni(part.count);
+    from = (t.lo & ~(TILE_KEYS - 1)) + TILE_KEYS * units * at;
     t.lo = t.lo > from ? t.lo : from;
-    t.hi = steps > part * (piece + 1) ? from + TILE_KEYS * part : t.hi;
-    if (pieces > (int)slots && piece == 0 && t.row0 == 0 && head == 0 && tid == 0)
-      note_tree(d, pieces, tree_part_size(J, part_waves), t.s, {(int)order, ceil_div(steps, part)});
-    if (steps > part) ws = (KTIR_G(float)*)d.ws + blockIdx.x * tree_part_size(J, part_waves);
+    t.hi = at + 1 < count ? from + TILE_KEYS * units : t.hi;
+    if (pieces > (int)slots && at == 0 && t.row0 == 0 && head == 0 && tid == 0)
+      note_tree(d, pieces, tree_part_size(J, part_waves), t.s, {(int)order, count});
+    if (count > 1) ws = (KTIR_G(float)*)d.ws + blockIdx.x * tree_part_size(J, part_waves);
   } else {
     t = uni(tile_of(d, slot, TM, grp, err));
     if (!t.rows) return;
@@ -237,6 +152,7 @@ __global__ __launch_bounds__(64 * W, W / 4) void kv8_attn_tile(const ktir_kv8_at
   }
   lo_most = uni(lo_most), hi_least = uni(hi_least);
 
+  const bool busy = !IDLE || wn > 0;
   f32x16_t acc[RB][2 * J];
   float base[RB], sum[RB];
 #pragma unroll
@@ -356,7 +272,7 @@ __global__ __launch_bounds__(64 * W, W / 4) void kv8_attn_tile(const ktir_kv8_at
     fetch_v(2, g.page, v_raw[0]);
     fetch_k(3, k_raw[1]);
     __syncthreads();
-    scores(s0, 0, 0, 4 * J);
+    if (busy) scores(s0, 0, 0, 4 * J);
     __syncthreads();
   }
 
@@ -384,72 +300,74 @@ __global__ __launch_bounds__(64 * W, W / 4) void kv8_attn_tile(const ktir_kv8_at
     }
     // exponents of the weights, less b
     const bool cut = key < lo_most || key + TILE_KEYS > hi_least;
-#pragma unroll
-    for (int b = 0; b < RB; ++b) {
-      // (made anew in each of the two rare parts: kept, the 32 places take as many registers)
-      struct Places {
-        int first;
-        uint32_t bits[2];
-      };
-      auto places = [&]() {
-        Places at = {};
-        if constexpr (TREE) {
-#pragma unroll
-          for (int k = 0; k < 2; ++k) at.bits[k] = tree_bits(mask, t, see_at[b], see_lo[b], key + 32 * k) >> (4 * h);
-        } else {
-          at.first = key + 4 * h - see_lo[b];
-          asm volatile("" : "+v"(at.first));
-        }
-        return at;
-      };
-      auto hidden = [&](const Places& at, int k, int i) {
-        if constexpr (TREE) return !(at.bits[k] >> (8 * (i >> 2) + (i & 3)) & 1u);
-        else return (uint32_t)(at.first + 32 * k + 8 * (i >> 2) + (i & 3)) >= see[b];
-      };
-      if (__any(base[b] == B_NONE)) {              // rows that have seen no key: b from this step's, their sums are 0
-        float top = -__builtin_inff();
-        const Places first = places();
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            top = __builtin_fmaxf(top, mask_ninf(__builtin_fmaf(s[b][k][i], gks[2 * k + (i >> 3)] * rs[b], glv[2 * k + (i >> 3)]), hidden(first, k, i)));
-        top = __builtin_fmaxf(top, other_half(top));
-        base[b] = base[b] == B_NONE && top > -__builtin_inff() ? top - TILE_TOP : base[b];
-      }
-#pragma unroll
-      for (int k = 0; k < 2; ++k)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s[b][k][i] = __builtin_fmaf(s[b][k][i], gks[2 * k + (i >> 3)] * rs[b], glv[2 * k + (i >> 3)] - base[b]);
-      if (cut) {
-        const Places first = places();
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) s[b][k][i] = mask_ninf(s[b][k][i], hidden(first, k, i));
-      }
-    }
-    float top[RB], most = -__builtin_inff();
-#pragma unroll
-    for (int b = 0; b < RB; ++b) {
-      top[b] = top_of(s[b]);
-      most = __builtin_fmaxf(most, top[b]);
-    }
-    if (__any(most > TILE_TOP + TILE_LAG)) {
+    if (busy) {
 #pragma unroll
       for (int b = 0; b < RB; ++b) {
-        top[b] = __builtin_fmaxf(top[b], other_half(top[b]));
-        const float by = top[b] > TILE_TOP ? top[b] - TILE_TOP : 0.f, keep = __builtin_amdgcn_exp2f(-by);
-        base[b] += by;
-        sum[b] *= keep;
+        // (made anew in each of the two rare parts: kept, the 32 places take as many registers)
+        struct Places {
+          int first;
+          uint32_t bits[2];
+        };
+        auto places = [&]() {
+          Places at = {};
+          if constexpr (TREE) {
 #pragma unroll
-        for (int n = 0; n < 2 * J; ++n)
+            for (int k = 0; k < 2; ++k) at.bits[k] = tree_bits(mask, t, see_at[b], see_lo[b], key + 32 * k) >> (4 * h);
+          } else {
+            at.first = key + 4 * h - see_lo[b];
+            asm volatile("" : "+v"(at.first));
+          }
+          return at;
+        };
+        auto hidden = [&](const Places& at, int k, int i) {
+          if constexpr (TREE) return !(at.bits[k] >> (8 * (i >> 2) + (i & 3)) & 1u);
+          else return (uint32_t)(at.first + 32 * k + 8 * (i >> 2) + (i & 3)) >= see[b];
+        };
+        if (__any(base[b] == B_NONE)) {              // rows that have seen no key: b from this step's, their sums are 0
+          float top = -__builtin_inff();
+          const Places first = places();
 #pragma unroll
-          for (int i = 0; i < 16; ++i) acc[b][n][i] *= keep;
+          for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              top = __builtin_fmaxf(top, mask_ninf(__builtin_fmaf(s[b][k][i], gks[2 * k + (i >> 3)] * rs[b], glv[2 * k + (i >> 3)]), hidden(first, k, i)));
+          top = __builtin_fmaxf(top, other_half(top));
+          base[b] = base[b] == B_NONE && top > -__builtin_inff() ? top - TILE_TOP : base[b];
+        }
 #pragma unroll
         for (int k = 0; k < 2; ++k)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) s[b][k][i] -= by;
+          for (int i = 0; i < 16; ++i) s[b][k][i] = __builtin_fmaf(s[b][k][i], gks[2 * k + (i >> 3)] * rs[b], glv[2 * k + (i >> 3)] - base[b]);
+        if (cut) {
+          const Places first = places();
+#pragma unroll
+          for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[b][k][i] = mask_ninf(s[b][k][i], hidden(first, k, i));
+        }
+      }
+      float top[RB], most = -__builtin_inff();
+#pragma unroll
+      for (int b = 0; b < RB; ++b) {
+        top[b] = top_of(s[b]);
+        most = __builtin_fmaxf(most, top[b]);
+      }
+      if (__any(most > TILE_TOP + TILE_LAG)) {
+#pragma unroll
+        for (int b = 0; b < RB; ++b) {
+          top[b] = __builtin_fmaxf(top[b], other_half(top[b]));
+          const float by = top[b] > TILE_TOP ? top[b] - TILE_TOP : 0.f, keep = __builtin_amdgcn_exp2f(-by);
+          base[b] += by;
+          sum[b] *= keep;
+#pragma unroll
+          for (int n = 0; n < 2 * J; ++n)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[b][n][i] *= keep;
+#pragma unroll
+          for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[b][k][i] -= by;
+        }
       }
     }
     // the codes of steps j + 2 (K) and j + 1 (V) into LDS, those of the next two steps on their way, the scores of j + 1,
@@ -494,8 +412,10 @@ __global__ __launch_bounds__(64 * W, W / 4) void kv8_attn_tile(const ktir_kv8_at
     };
     if constexpr (TURNS) {
       uint4 w[4][RB][2];
+      if (busy) {
 #pragma unroll
-      for (int p = 0; p < 4; ++p) weights(p, w[p]);
+        for (int p = 0; p < 4; ++p) weights(p, w[p]);
+      }
       __builtin_amdgcn_sched_barrier(0);
       __syncthreads();
       __builtin_amdgcn_sched_barrier(0);
@@ -503,8 +423,10 @@ __global__ __launch_bounds__(64 * W, W / 4) void kv8_attn_tile(const ktir_kv8_at
 #pragma unroll
       for (int p = 0; p < 4; ++p) {
         move(p);
-        scores(s_next, 1 - PAR, p * J, J);
-        weigh(p, w[p]);
+        if (busy) {
+          scores(s_next, 1 - PAR, p * J, J);
+          weigh(p, w[p]);
+        }
       }
       __builtin_amdgcn_s_setprio(0);
       __builtin_amdgcn_sched_barrier(0);
@@ -514,6 +436,7 @@ __global__ __launch_bounds__(64 * W, W / 4) void kv8_attn_tile(const ktir_kv8_at
       for (int p = 0; p < 5; ++p) {
         if (J == 4 || p == 0 || p == 2 || p == 4) __builtin_amdgcn_sched_barrier(0);
         move(p);
+        if (!busy) continue;
         if (p < 4) scores(s_next, 1 - PAR, p * J, J);
 #pragma unroll
         for (int b = 0; b < RB; ++b) old[b][0] = w[b][0], old[b][1] = w[b][1];
@@ -590,7 +513,7 @@ __global__ __launch_bounds__(256) void kv8_tile_join(const ktir_kv8_attn_t d, in
   const int64_t head = blockIdx.x - slot * heads, size = tree_part_size(J, part_waves);
   const Tile t = uni(tile_of<true>(d, slot, TM, grp, err));
   if (!t.rows || 32 * wave >= t.rows) return;
-  const int tiles = tree_tiles(d, t, grp, TM);
+  const int tiles = tree_tiles(d, t.q, grp, TM);
   const TreeNote note = tree_noted(d, pieces, size, t.s, tiles);
   const int parts = note.parts;
   if (parts < 2) return;

@@ -5,8 +5,10 @@ namespace ktir {
 
 constexpr int64_t MASK_WORDS = 32;
 
-// Whether a launch's rows of a KV head are more than one tile of the kernels for few rows takes.
-static bool tree_tiles(const ktir_kv8_attn_t& d, const KV8Shape& s) { return d.max_q * (d.q_heads / d.cache.heads) > 16 * s.MT; }
+// Whether a launch's rows of a KV head are more than the kernels for few rows take at best: 64, in one tile of 64 or, with more
+// than 128 columns, two of 32 (eight KV heads of 256 columns: one sequence of 16000 tokens 57 us, 57 here, six 133, 196; 24 of
+// 1500 113, 102.  128 columns: 80 rows 57, 44; 128 rows of six sequences 129, 135; 192 194, 142).
+static bool tree_tiles(const ktir_kv8_attn_t& d) { return d.max_q * (d.q_heads / d.cache.heads) > 64; }
 
 struct TreePlan {
   bool tile;
@@ -18,12 +20,12 @@ struct TreePlan {
 static TreePlan tree_plan(const ktir_kv8_attn_t& d) {
   TreePlan p = {};
   kv8_rows_shape(d, true, &p.rows);
-  p.tile = tree_tiles(d, p.rows);
+  p.tile = tree_tiles(d);
   if (p.tile) {
     const int64_t grp = d.q_heads / d.cache.heads, rows = d.max_q * grp;
     TreeTiles& t = p.tiles;
     t.J = d.cache.columns <= 64 ? 1 : d.cache.columns <= 128 ? 2 : 4;
-    t.TM = t.J == 4 ? 128 : 256;
+    t.TM = t.J == 4 || (t.J == 1 && rows <= 128) ? 128 : 256;
     t.slots = rows > t.TM ? d.batch.tokens * grp / t.TM + d.batch.seqs : d.batch.seqs;
     t.waves = (int)((rows < t.TM ? rows : t.TM) + 31) / 32;
     // Pieces: one for each CU where that cuts every tile into several; up to 1024 tiles two for each, so that no long
