@@ -56,7 +56,7 @@ extern "C" int ktir_kv8_attention_plan(ktir_kv8_attn_t* d) {
   if (rc != KTIR_OK) return rc;
   KV8Shape s;
   int64_t slots;
-  kv8_rows_shape(*d, false, &s);
+  kv8_rows_shape(*d, &s);
   if (kv8_tile_takes(*d, &slots)) s.splits = 1;
   d->splits = s.splits;
   d->ws_bytes = s.splits > 1 ? s.slots * d->cache.heads * s.splits * s.part * 4 : 0;
@@ -71,7 +71,7 @@ extern "C" int ktir_launch_kv8_attention(const ktir_kv8_attn_t* d) {
   rc = check_kv8_attn_tensors(ME, *d);
   if (rc != KTIR_OK) return rc;
   KV8Shape s;
-  kv8_rows_shape(*d, false, &s);
+  kv8_rows_shape(*d, &s);
   const int64_t splits = d->splits < 1 ? 1 : d->splits, tiles = s.slots * d->cache.heads;
   if (splits > 256) return set_error(KTIR_E_ARG, "%s: %lld splits, 256 at most", ME, (long long)splits);
   if (tiles > INT32_MAX / splits)

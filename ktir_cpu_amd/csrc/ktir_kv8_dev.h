@@ -326,6 +326,14 @@ __device__ __forceinline__ void q_scaled(uint32_t (&raw)[N], float up) {
 // The keys of all tiles of rows of a head are cut into parts, a workgroup each and `parts` of them at most, whatever
 // the batch: its lengths are on the device, and so is the cut.  Keys count in units of `quant` from a bound of STEP
 // on; the parts of a tile are alike, of `least` units at least.
+//
+// Tiles stay whole where cutting them does not end the launch sooner.  Whole, it takes the longest tile's keys or, with more tiles than
+// CUs, a CU's share of all and half the longest; cut, an eighth more than a part or a CU's share (which parts lose to each other), and
+// what it costs to launch the join and to write and join the parts.  Eight KV heads of 128 columns, whole and cut: 32 sequences of 8 tokens after
+// 1000 to 2000 34.7 and 45.0 us, after 80 to 4000 53.8, 40.5; 32 of 64 after 2000 to 4000 183, 243, after 80 to 4000 168, 132; four
+// of 8 after 150 to 300 11.5, 14.0.
+
+__host__ __device__ constexpr int64_t tree_cut_cost(int64_t tiles) { return 400 + 304 * (tiles < 256 ? tiles : 256) / 256; }      // of so many tiles, in keys
 
 constexpr int TREE_WHOLE = 1 << 30;    // more units than a tile has
 
@@ -334,10 +342,6 @@ struct TreePart {
 };
 
 __device__ __forceinline__ int ceil_div(int a, int b) { return (int)((uint32_t)(a + b - 1) / (uint32_t)b); }
-__device__ __forceinline__ int64_t wave_sum(int64_t x) {
-  for (int o = 32; o; o >>= 1) x += __shfl_xor((long long)x, o);
-  return x;
-}
 // tiles of rows of a sequence
 __device__ __forceinline__ int tree_tiles(const ktir_kv8_attn_t& d, const Seq& q, int grp, int TM) {
   const int64_t n = q.n_new < d.max_q ? q.n_new : d.max_q;
@@ -351,18 +355,29 @@ __device__ __forceinline__ int tree_units(const Tile& t, int quant) {
 
 // part `at` of a head: its tile, and what of it; no rows where there is none.  parts 0: no tile is cut.  All lanes of a
 // wavefront look together, 64 sequences at a time.
-template <int STEP>
-__device__ __forceinline__ Tile tree_part(const ktir_kv8_attn_t& d, int grp, int TM, int quant, int least, int parts, int64_t at, TreePart* part, int* err) {
+template <int STEP, int TIME>
+__device__ __forceinline__ Tile tree_part(const ktir_kv8_attn_t& d, int grp, int TM, int sets, int quant, int least, int held, int parts, int64_t at, TreePart* part, int* err) {
   auto of_parts = [&](int units, int each) {               // units of a part, where `each` is the most
     return ceil_div(units, ceil_div(units, each < least ? least : each));
+  };
+  // whether `n` parts of `each` units are worth it for so many tiles, of so many units, the longest of so many; n and tiles of all sets
+  auto worth = [&](int64_t tiles, int64_t units, int longest, int64_t n, int each) {
+    const int64_t share = units / 256, rounds = (tiles + 255) / 256 * longest;
+    int64_t whole = share + (held > 256 ? 0 : (int64_t)longest * 5 / 8);
+    whole = whole > rounds ? rounds : whole;
+    whole = whole > longest ? whole : longest;
+    each = each < least ? least : each;
+    const int64_t cut = n <= held ? (each > share ? each : share) * 9 / 8 : share * 9 / 8 + each / 2;
+    return cut + (tree_cut_cost(tiles) + TIME / 2) / TIME < whole;
   };
   if (d.batch.seqs == 1) {                                 // floor(parts / tiles) for each tile
     const Seq q = seq_of(d.batch, d.cache.page, 0, err);
     const int tiles = tree_tiles(d, q, grp, TM);
     if (!tiles) return Tile{};
     const Tile t = tile_at<true>(d, 0, q, at % tiles, TM, grp, err);
-    const int units = tree_units<STEP>(t, quant), cuts = parts / tiles;
-    part->units = of_parts(units, !parts ? TREE_WHOLE : cuts > 1 ? ceil_div(units, cuts) : units);
+    const int units = tree_units<STEP>(t, quant), cuts = parts / tiles, each = cuts > 1 ? ceil_div(units, cuts) : units;
+    const int64_t all = tiles * (int64_t)sets;
+    part->units = of_parts(units, parts && worth(all, all * units, units, cuts * all, each) ? each : TREE_WHOLE);
     part->count = ceil_div(units, part->units);
     part->at = (int)(at / tiles);
     return part->at < part->count ? t : Tile{};
@@ -383,14 +398,44 @@ __device__ __forceinline__ Tile tree_part(const ktir_kv8_attn_t& d, int grp, int
   int each = TREE_WHOLE;
   if (parts) {       // n tiles of so many units together make n parts more than their units' share at most
     int64_t tiles = x.tiles, units = (int64_t)x.tiles * x.units;
+    int longest = x.units;
     for (int64_t base = 64; base < d.batch.seqs; base += 64) {
       const Look y = look(base);
       tiles += y.tiles;
       units += (int64_t)y.tiles * y.units;
+      longest = longest > y.units ? longest : y.units;
     }
-    units = wave_sum(units);
-    const int64_t spare = parts - wave_sum(tiles), share = spare > 0 ? (units + spare - 1) / spare : TREE_WHOLE;
-    each = share < TREE_WHOLE ? (int)share : TREE_WHOLE;
+    for (int o = 32; o; o >>= 1) {
+      tiles += __shfl_xor((long long)tiles, o);
+      units += __shfl_xor((long long)units, o);
+      const int y = __shfl_xor(longest, o);
+      longest = longest > y ? longest : y;
+    }
+    const int64_t limit = tiles * sets * 2 <= held && (int64_t)parts * sets > held ? held / sets : parts;      // no second round where one takes all
+    const int64_t spare = limit - tiles, share = spare > 0 ? (units + spare - 1) / spare : TREE_WHOLE;
+    if (share < TREE_WHOLE && worth(tiles * sets, units * sets, longest, tiles * sets, (int)(units / limit))) {
+      int most = (int)share, below = (int)(units / limit);
+      int64_t n = limit;
+      if (tiles * sets <= held && d.batch.seqs <= 64) {   // fewer units may do, from their even share on
+        for (int i = 0; i < 2 && most - below > 1; ++i) {
+          int at[3], y[3];
+#pragma unroll
+          for (int k = 0; k < 3; ++k) {
+            at[k] = below + (int)((int64_t)(most - below) * (k + 1) / 4);
+            const int64_t mine = (int64_t)x.tiles * ceil_div(x.units, at[k] < least ? least : at[k]);
+            y[k] = mine < 1 << 20 ? (int)mine : 1 << 20;
+          }
+          for (int o = 32; o; o >>= 1)
+#pragma unroll
+            for (int k = 0; k < 3; ++k) y[k] += __shfl_xor(y[k], o);
+          const int ok = y[0] <= limit ? 0 : y[1] <= limit ? 1 : y[2] <= limit ? 2 : 3;
+          below = ok == 0 ? below : ok == 1 ? at[0] : ok == 2 ? at[1] : at[2];
+          most = ok == 0 ? at[0] : ok == 1 ? at[1] : ok == 2 ? at[2] : most;
+          n = ok == 0 ? y[0] : ok == 1 ? y[1] : ok == 2 ? y[2] : n;
+        }
+      }
+      if (worth(tiles * sets, units * sets, longest, n * sets, most)) each = most;
+    }
   }
   // The parts of a sequence's tiles that have the same keys follow one another, so that they read them together (eight
   // sequences of 256 drafts after up to 16384: 463 us with a tile's parts together, 429).

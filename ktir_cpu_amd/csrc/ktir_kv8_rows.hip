@@ -4,11 +4,11 @@
 namespace ktir {
 
 // the launch's shape: columns in 64s (192 alone has its three: other heads' loads of 12 codes would pass their end), rows, splits
-void kv8_rows_shape(const ktir_kv8_attn_t& d, bool tree, KV8Shape* s) {
+void kv8_rows_shape(const ktir_kv8_attn_t& d, KV8Shape* s) {
   const int D = (int)d.cache.columns;
   const int64_t grp = d.q_heads / d.cache.heads;
   s->J = D <= 64 ? 1 : D <= 128 ? 2 : D == 192 ? 3 : 4;
-  s->MT = d.max_q * grp > 32 && tree && s->J <= 2 ? 4 : d.max_q * grp > 16 ? 2 : 1;
+  s->MT = d.max_q * grp > 16 ? 2 : 1;
   const int64_t TM = 16 * s->MT;
   s->slots = d.max_q * grp > TM ? d.batch.tokens * grp / TM + d.batch.seqs : d.batch.seqs;
   s->rows = (int)(d.max_q * grp < TM ? d.max_q * grp : TM);
@@ -16,7 +16,7 @@ void kv8_rows_shape(const ktir_kv8_attn_t& d, bool tree, KV8Shape* s) {
   s->part = s->rows * (64 * s->J + 4);
   // the most tokens that a tile's rows see, from a step's bound on
   s->span = d.max_k;
-  const int64_t near = d.window + (tree ? d.max_q : (TM - 1) / grp + 1);
+  const int64_t near = d.window + (TM - 1) / grp + 1;
   if (d.window && near < s->span) s->span = near;
   s->span += ROWS_STEP - 1;
   // Heads of a workgroup, parts of the keys.  Up to 2^19 keys (times KV heads) a wavefront's

@@ -115,7 +115,7 @@ __global__ __launch_bounds__(64 * ROWS_WAVES, MT == 1 || (TREE && J * MT <= 4) ?
     const int quant = ROWS_STEP * TW;
     TreePart p;
     slot = u;                                          // (of the part in the workspace)
-    t = uni(tree_part<ROWS_STEP>(d, grp, TM, quant, quant < 128 ? 128 / quant : 1, splits, u, &p, err));
+    t = uni(tree_part<ROWS_STEP, ROWS_STEP * W>(d, grp, TM, (int)sets, quant, quant < 128 ? 128 / quant : 1, 512, splits, u, &p, err));
     if (!t.rows) return;
     split = uni(p.at);
     active = uni(p.count);

@@ -68,7 +68,7 @@ __global__ __launch_bounds__(64 * W, J == 1 ? 2 : W / 4) void kv8_attn_tile(cons
   KTIR_G(float)* ws = nullptr;                       // of a tile of several pieces
   if constexpr (TREE) {
     TreePart part;
-    t = uni(tree_part<TILE_KEYS>(d, grp, TM, TILE_KEYS, TREE_LEAST, pieces > (int)slots ? pieces : 0, order, &part, err));
+    t = uni(tree_part<TILE_KEYS, TILE_KEYS>(d, grp, TM, (int)heads, TILE_KEYS, TREE_LEAST, 256, pieces > (int)slots ? pieces : 0, order, &part, err));
     if (!t.rows) return;
     const int at = uni(part.at), units = uni(part.units), count = uni(part.count);
     from = (t.lo & ~(TILE_KEYS - 1)) + TILE_KEYS * units * at;

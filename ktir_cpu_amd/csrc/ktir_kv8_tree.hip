@@ -5,11 +5,6 @@ namespace ktir {
 
 constexpr int64_t MASK_WORDS = 32;
 
-// Whether a launch's rows of a KV head are more than the kernels for few rows take at best: 64, in one tile of 64 or, with more
-// than 128 columns, two of 32 (eight KV heads of 256 columns: one sequence of 16000 tokens 57 us, 57 here, six 133, 196; 24 of
-// 1500 113, 102.  128 columns: 80 rows 57, 44; 128 rows of six sequences 129, 135; 192 194, 142).
-static bool tree_tiles(const ktir_kv8_attn_t& d) { return d.max_q * (d.q_heads / d.cache.heads) > 64; }
-
 struct TreePlan {
   bool tile;
   KV8Shape rows;       // tile false
@@ -17,39 +12,68 @@ struct TreePlan {
   int64_t groups, floats;       // how many share the keys of a head; of the workspace for each
 };
 
+// The kernels for few rows, MT tiles of 16 each.
+static KV8Shape tree_rows(const ktir_kv8_attn_t& d, int MT, int64_t span) {
+  const int64_t grp = d.q_heads / d.cache.heads, rows = d.max_q * grp, TM = 16 * MT;
+  KV8Shape s = {};
+  s.J = d.cache.columns <= 64 ? 1 : d.cache.columns <= 128 ? 2 : d.cache.columns == 192 ? 3 : 4;
+  s.MT = MT;
+  s.HW = 1;
+  s.slots = rows > TM ? d.batch.tokens * grp / TM + d.batch.seqs : d.batch.seqs;
+  s.rows = rows < 1 ? 1 : rows < TM ? (int)rows : (int)TM;
+  s.part = s.rows * (64 * s.J + 4);
+  s.span = span + 31;                    // (from a step's bound on)
+  return s;
+}
+
 static TreePlan tree_plan(const ktir_kv8_attn_t& d) {
   TreePlan p = {};
-  kv8_rows_shape(d, true, &p.rows);
-  p.tile = tree_tiles(d);
-  if (p.tile) {
-    const int64_t grp = d.q_heads / d.cache.heads, rows = d.max_q * grp;
-    TreeTiles& t = p.tiles;
-    t.J = d.cache.columns <= 64 ? 1 : d.cache.columns <= 128 ? 2 : 4;
-    t.TM = t.J == 4 || (t.J == 1 && rows <= 128) ? 128 : 256;
-    t.slots = rows > t.TM ? d.batch.tokens * grp / t.TM + d.batch.seqs : d.batch.seqs;
-    t.waves = (int)((rows < t.TM ? rows : t.TM) + 31) / 32;
-    // Pieces: one for each CU where that cuts every tile into several; up to 1024 tiles two for each, so that no long
-    // tile is left at the end (more give evener shares, but each costs 12 us and 264 KB to and from the workspace); more tiles
-    // are not cut.  No more than the longest sequence can have.
-    const int64_t heads = d.cache.heads, n = t.slots * heads;
-    int64_t span = d.max_k;
-    if (d.window && d.window + d.max_q < span) span = d.window + d.max_q;
-    const int64_t most = t.slots * ((span / 64 + 1) / TREE_LEAST + 1);
-    int64_t pieces = n <= 1024 ? 2 * t.slots : t.slots;
-    if (n <= 256 && pieces < 256 / heads) pieces = 256 / heads;
-    if (pieces > most) pieces = most;
-    t.pieces = (int)(pieces > t.slots ? pieces : t.slots);
-    p.groups = t.pieces > t.slots ? t.pieces : 1;
-    p.floats = heads * tree_part_size(t.J, t.waves);
-  } else {
-    // Parts: two workgroups for each CU, and two at least for each sequence; from 2048 on none is cut.  No more than 128 keys each.
-    const KV8Shape& s = p.rows;
-    const int64_t sets = d.cache.heads / s.HW, most = s.slots * ((s.span + 127) / 128);
+  const int64_t heads = d.cache.heads, grp = d.q_heads / heads, rows = d.max_q * grp;
+  const bool wide = d.cache.columns > 128;
+  int64_t span = d.max_k;                // the most keys that a tile's rows see
+  if (d.window && d.window + d.max_q < span) span = d.window + d.max_q;
+  // Little work takes tiles of 16 rows, however many: more workgroups and shorter ones (eight KV heads of 128 columns, 4 query
+  // heads each, one sequence: 8 tokens after 1000 13.2 us, tiles of 32 rows 15.7; 64 after 1000 19.0, of 256 27.3; 16 after
+  // 16000 34.7, 29.6; sixteen sequences of 16 after 1000 38.6, 32.5).  Tiles of 32 rows read the cache half as often, but with more
+  // than 128 columns leave a SIMD one wavefront, so that they need more work (256 columns, 16 tokens, tiles of 16 rows and
+  // of 32: four sequences of 4000 52.0, 55.7; sixteen 146, 123).  Up to 64 rows two tiles of 32 beat one of 256 (80 rows 57 us, 44;
+  // 192 of six sequences 194, 142) and beat one of 64 by what that spills (64 rows of 16 sequences of up to 16000: 51, 69).
+  const KV8Shape least = tree_rows(d, 1, span);
+  const int64_t work = least.slots * heads * span;
+  const bool little = least.slots * heads <= 512 && work <= 1 << 18;
+  if (rows <= 64 || little) {
+    const bool narrow = little || rows <= 16 || (wide && least.slots * heads <= 2048 && work <= 1 << 20);
+    KV8Shape& s = p.rows = narrow ? least : tree_rows(d, 2, span);
+    const int64_t n = s.slots * heads, most = s.slots * ((s.span + 127) / 128);
+    // Heads of a workgroup: several, a wavefront each, for many tiles of few keys, where nothing is left to join then (200
+    // sequences of 8 tokens after up to 500: 56.7 us, a workgroup for each head 72; up to 2000 156, 151), and for many long ones, whose
+    // rows of several heads are read together (64 sequences of 64 to 8192 keys, cold: 78.7, 85.7; 128 of 1000 to 2000 147, 120).
+    const bool many = n >= 1024 && span <= (wide ? 2048 : 768), far = n >= 512 && n < 2048 && span > 2048;
+    if (many || far) s.HW = heads % 4 == 0 ? 4 : heads % 2 == 0 ? 2 : 1;
+    // Parts that the device may cut: two workgroups for each CU, and two at least for each tile (eight sequences for each CU are not cut).
+    const int64_t sets = heads / s.HW;
     int64_t parts = 512 / sets > 2 * s.slots ? 512 / sets : 2 * s.slots;
     if (parts > most) parts = most;
-    p.groups = s.slots * sets >= 2048 || parts <= s.slots ? 1 : parts;
-    p.floats = d.cache.heads * s.part;
+    p.groups = many || n >= 2048 || span <= tree_cut_cost(n) || parts <= s.slots ? 1 : parts;
+    p.floats = heads * s.part;
+    return p;
   }
+  p.tile = true;
+  TreeTiles& t = p.tiles;
+  t.J = d.cache.columns <= 64 ? 1 : d.cache.columns <= 128 ? 2 : 4;
+  t.TM = t.J == 4 || (t.J == 1 && rows <= 128) ? 128 : 256;
+  t.slots = rows > t.TM ? d.batch.tokens * grp / t.TM + d.batch.seqs : d.batch.seqs;
+  t.waves = (int)((rows < t.TM ? rows : t.TM) + 31) / 32;
+  // Pieces that the device may cut: one for each CU where that cuts every tile into several; up to 1024 tiles two for each, so that no long
+  // tile is left at the end (more give evener shares, but each costs 12 us and 264 KB to and from the workspace); more tiles
+  // are not cut.  No more than the longest sequence can have.
+  const int64_t n = t.slots * heads, most = t.slots * ((span / 64 + 1) / TREE_LEAST + 1);
+  int64_t pieces = n <= 1024 && span > tree_cut_cost(n) ? 2 * t.slots : t.slots;
+  if (n <= 256 && pieces > t.slots && pieces < 256 / heads) pieces = 256 / heads;
+  if (pieces > most) pieces = most;
+  t.pieces = (int)(pieces > t.slots ? pieces : t.slots);
+  p.groups = t.pieces > t.slots ? t.pieces : 1;
+  p.floats = heads * tree_part_size(t.J, t.waves);
   return p;
 }
 

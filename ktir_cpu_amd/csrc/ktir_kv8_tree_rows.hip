@@ -6,8 +6,6 @@ namespace ktir {
 
 template <int CODE, int J>
 static int tree_rows_j(const ktir_kv8_attn_t& d, const KV8Mask& mask, const KV8Shape& s) {
-  if constexpr (J <= 2)
-    if (s.MT == 4) return kv8_rows_go<CODE, J, 4, true>(d, mask, s);
   return s.MT == 2 ? kv8_rows_go<CODE, J, 2, true>(d, mask, s) : kv8_rows_go<CODE, J, 1, true>(d, mask, s);
 }
 

@@ -33,7 +33,7 @@ struct KV8Shape {
   int J, MT, HW, rows, splits;         // columns in 64s, rows in 16s, heads of a workgroup, most rows of a tile
   int64_t slots, part, span;           // tiles of rows for each KV head; floats of a split's part in the workspace; most keys of a tile
 };
-void kv8_rows_shape(const ktir_kv8_attn_t& d, bool tree, KV8Shape* s);
+void kv8_rows_shape(const ktir_kv8_attn_t& d, KV8Shape* s);
 int kv8_rows_launch(const ktir_kv8_attn_t& d, const KV8Shape& s);
 bool kv8_tile_takes(const ktir_kv8_attn_t& d, int64_t* slots);       // whether ktir_kv8_tile.hip takes it instead
 int kv8_tile_launch(const ktir_kv8_attn_t& d, int64_t slots);
