@@ -39,10 +39,10 @@ static TreePlan tree_plan(const ktir_kv8_attn_t& d) {
   // of 32: four sequences of 4000 52.0, 55.7; sixteen 146, 123).  Up to 64 rows two tiles of 32 beat one of 256 (80 rows 57 us, 44;
   // 192 of six sequences 194, 142) and beat one of 64 by what that spills (64 rows of 16 sequences of up to 16000: 51, 69).
   const KV8Shape least = tree_rows(d, 1, span);
-  const int64_t work = least.slots * heads * span;
-  const bool little = least.slots * heads <= 512 && work <= 1 << 18;
+  const int64_t tiles = least.slots * heads;
+  const bool little = tiles <= 512 && tiles * span <= 1 << 18;
   if (rows <= 64 || little) {
-    const bool narrow = little || rows <= 16 || (wide && least.slots * heads <= 2048 && work <= 1 << 20);
+    const bool narrow = little || rows <= 16 || (wide && tiles <= 2048 && tiles * span <= 1 << 20);
     KV8Shape& s = p.rows = narrow ? least : tree_rows(d, 2, span);
     const int64_t n = s.slots * heads, most = s.slots * ((s.span + 127) / 128);
     // Heads of a workgroup: several, a wavefront each, for many tiles of few keys, where nothing is left to join then (200
