@@ -9,16 +9,18 @@ constexpr int64_t TREE_WORDS = 32;           // of a token's mask
 // ---- the tree ----------------------------------------------------------------
 //
 // Tokens come after their parents, so 32 of them (a word of the masks) have all other ancestors among
-// the tokens before.  One thread a token: first up the line within its word, at most 32 steps; where that leaves
-// it, the row of the ancestor it comes to has the other words, which are copied word by word of
-// the sequence.  Bound: latency, 32 + 32 steps of LDS for the largest tree, where a walk up the whole line
-// takes as many as the tree is deep.
+// the tokens before.  One thread a token: first up the line within its word, which half a wavefront holds, in 5
+// doublings; where that leaves the word, the row of the ancestor it comes to has the other words, which are copied word
+// by word of the sequence.  Bound: latency, the chain offsets -> parents, then a step of LDS and a barrier for each word.
+// 64 sequences of up to 64 tokens 3.8 us (2.7 in a graph), 24 of up to 500, with a window, 6.8; 10.7 with the line walked token
+// by token and the window's bits dropped one by one, 41 without the words.  Threads for 4, 16 or 32 words: in a graph
+// 512 sequences of up to 64 tokens take 2.9, 3.7 and 6.8 us, of up to 500 8.1 with 16 words and 13.8 with 32.
 
 template <int WORDS>
 __global__ __launch_bounds__(32 * WORDS) void draft_tree(const ktir_draft_tree_t d, int* err) {
   constexpr int N = 32 * WORDS, PITCH = WORDS + 1;
   __shared__ uint32_t rows[N * PITCH];
-  __shared__ int line[N], depths[N];                // parents, then the first ancestor before a token's word; how many ancestors
+  __shared__ int line[N], depths[N];                // the first ancestor before a token's word; how many ancestors
   const int i = threadIdx.x, word = i >> 5;
   const int64_t s = blockIdx.x;
   const int64_t a = ints(d.q_start)[s], e = ints(d.q_start)[s + 1];
@@ -34,22 +36,26 @@ __global__ __launch_bounds__(32 * WORDS) void draft_tree(const ktir_draft_tree_t
     p = ints(d.parents)[start + i];
     if (p < -1 || p >= i) *err = OUT_OF_RANGE, p = -1;
   }
-  line[i] = p;
-  __syncthreads();
   uint32_t bits = 1u << (i & 31);
-  int steps = 0;
-  while (p >= word * 32) {
-    bits |= 1u << (p & 31);
-    p = line[p];
-    ++steps;
+#pragma unroll
+  for (int o = 0; o < 5; ++o) {                     // (a word is half a wavefront)
+    const bool inside = p >= word * 32;
+    const int at = inside ? p & 31 : i & 31, up = __shfl(p, at, 32);
+    bits |= __shfl(bits, at, 32);
+    p = inside ? up : p;
   }
+  const int steps = __builtin_popcount(bits) - 1;
   for (int w = word; w < WORDS; ++w) rows[i * PITCH + w] = w == word ? bits : 0u;
-  __syncthreads();
   line[i] = p;
   if (p < 0) depths[i] = steps;
   __syncthreads();
-  for (int b = 0; 32 * b < n; ++b) {                // one thread a word of a row, and one a row for its depth
-    const int t = 32 * b + (i & 31), w = i >> 5, up = line[t];
+  int ups[WORDS];
+#pragma unroll
+  for (int b = 0; b < WORDS; ++b) ups[b] = line[32 * b + (i & 31)];
+#pragma unroll
+  for (int b = 0; b < WORDS; ++b) {                 // one thread a word of a row, and one a row for its depth
+    if (32 * b >= n) break;
+    const int t = 32 * b + (i & 31), w = i >> 5, up = ups[b];
     if (w < b) rows[t * PITCH + w] = up < 0 ? 0u : rows[up * PITCH + w];
     if (word == b && p >= 0) depths[i] = steps + 1 + depths[p];
     __syncthreads();
@@ -58,21 +64,28 @@ __global__ __launch_bounds__(32 * WORDS) void draft_tree(const ktir_draft_tree_t
   if (d.window) {                                   // the highest `window` bits of each row
     if (i < n && depths[i] >= d.window) {
       int left = (int)d.window;
-      for (int w = word; w >= 0; --w) {
-        uint32_t y = left > 0 ? rows[i * PITCH + w] : 0u;
-        const int some = __builtin_popcount(y);
-        for (int drop = some - left; drop > 0; --drop) y &= y - 1;
-        rows[i * PITCH + w] = y;
+      uint32_t y[WORDS];
+#pragma unroll
+      for (int w = 0; w < WORDS; ++w) y[w] = rows[i * PITCH + w];
+#pragma unroll
+      for (int w = WORDS - 1; w >= 0; --w) {
+        const int some = __builtin_popcount(y[w]);
+        if (left < some) {                          // the highest `left` of a word's: from the bit on below which it has one more
+          int low = 0;
+#pragma unroll
+          for (int o = 16; o; o >>= 1) low += __builtin_popcount(y[w] >> (low + o)) > left ? o : 0;
+          y[w] = left ? y[w] & ~1u << low : 0u;
+        }
         left = left > some ? left - some : 0;
       }
+#pragma unroll
+      for (int w = 0; w < WORDS; ++w) rows[i * PITCH + w] = y[w];
     }
     __syncthreads();
   }
-  const int words = (int)d.words;
-  for (int x = i; x < n * words; x += N) {
-    const int t = x / words, w = x - t * words;
-    ((KTIR_G(uint32_t)*)d.mask)[(start + t) * d.mask_row + w] = rows[t * PITCH + w];
-  }
+  const int words = (int)d.words, each = N / words, w = i % words;
+  if (i < each * words)
+    for (int t = i / words; t < n; t += each) ((KTIR_G(uint32_t)*)d.mask)[(start + t) * d.mask_row + w] = rows[t * PITCH + w];
 }
 
 // ---- the kept path -----------------------------------------------------------
@@ -80,7 +93,8 @@ __global__ __launch_bounds__(32 * WORDS) void draft_tree(const ktir_draft_tree_t
 // One wavefront for a sequence, a KV head, and K or V.  Entries only move down and in order, so what a
 // page gets is read before its place is written: pages in order, and in a page the rows of
 // one pass of the wavefront (64 units of 16 columns), all read, then written.  Bound: latency, offsets and path ->
-// table -> scales and codes; a lane has the place, page and scale that one entry of 64 comes from.
+// table -> scales and codes, for each page; a lane has the place, page and scale that one entry of 64 comes from.  One sequence of
+// 16 drafts 4.2 us, which is the launch, 256 of up to 64 10.0 (12.7 with each entry's place looked up by every lane).
 
 constexpr int KEEP_KEPT = 2;         // passes of rows that stay in registers between the maximum and the codes
 
