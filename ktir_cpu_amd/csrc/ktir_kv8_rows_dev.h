@@ -505,7 +505,8 @@ __global__ __launch_bounds__(64 * R * B) void kv8_attn_join(const ktir_kv8_attn_
         none ? -__builtin_inff() : (top + 16.f + __builtin_amdgcn_logf(lt)) * 0.69314718055994530942f;
 }
 
-// The parts of a tree's rows, joined: a wavefront for each row, J columns a lane, EACH parts at once.
+// The parts of a tree's rows, joined: a wavefront for each row, J columns a lane, EACH parts at once (16 of more than 128 columns
+// do not fit the registers).  26 parts of 16 rows of 8 heads 4.0 us, of 64 sequences of up to 32 rows, 256 at most, 11.9.
 template <int J, int MT>
 __global__ __launch_bounds__(256) void kv8_rows_join(const ktir_kv8_attn_t d, int parts, int part_rows, int* err) {
   constexpr int TM = 16 * MT, EACH = J <= 2 ? 16 : 8;

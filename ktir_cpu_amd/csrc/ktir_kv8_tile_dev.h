@@ -503,6 +503,7 @@ __global__ __launch_bounds__(64 * W, J == 1 ? 2 : W / 4) void kv8_attn_tile(cons
 }
 
 // The pieces of a tile, joined: a wavefront has V of the 8 J vectors of 4 columns of 32 rows, EACH pieces of them at once.
+// 32 pieces of each of 8 heads' tile, 34 MB, 12.5 us; 60 of 28 tiles of 8 heads, 64 MB, 22.8.
 template <int J, int V, int EACH>
 __global__ __launch_bounds__(256) void kv8_tile_join(const ktir_kv8_attn_t d, int pieces, int part_waves, int TM, int* err) {
   static_assert(8 * J % (4 * V) == 0, "four wavefronts");
