@@ -325,7 +325,8 @@ __device__ __forceinline__ void q_scaled(uint32_t (&raw)[N], float up) {
 //
 // The keys of all tiles of rows of a head are cut into parts, a workgroup each and `parts` of them at most, whatever
 // the batch: its lengths are on the device, and so is the cut.  Keys count in units of `quant` from a bound of STEP
-// on; the parts of a tile are alike, of `least` units at least.
+// on; the parts of a tile are alike, of `least` units at least.  The chip holds `held` workgroups at a time, each of which has
+// one of `sets` sets of heads and takes the time of TIME keys for a unit.
 //
 // Tiles stay whole where cutting them does not end the launch sooner.  Whole, it takes the longest tile's keys or, with more tiles than
 // CUs, a CU's share of all and half the longest; cut, an eighth more than a part or a CU's share (which parts lose to each other), and
