@@ -3,8 +3,9 @@ many heads a workgroup has, and whether keys may be cut; small inputs reach all 
 import pytest
 import torch
 
+from ktir_cpu_amd import serving as S
 from tests._serving import Batch
-from tests.test_gpu_drafts import ATTN, attend, check, done, tree_of
+from tests.test_gpu_drafts import ATTN, attend, cache_of, check, dev, done, tree_of
 
 pytestmark = pytest.mark.gpu
 
@@ -70,3 +71,36 @@ def test_a_nan_page_of_a_cut_tile_is_its_sequences_alone(n, D, most):
     done()
     assert torch.equal(got[:n], out[:n]) and torch.equal(gline[:n], line[:n])
     assert torch.equal(got[n:, :4], out[n:, :4]) and got[n:, 4:].isnan().all()
+
+
+@pytest.mark.parametrize("n,D", [(8, 128), (12, 64), (10, 256), (40, 128)])
+def test_one_graph_whole_and_cut(n, D):
+    # lengths change between the replays of two graphs that share a workspace: tiles are cut, stay whole, and are none
+    b = Batch([(n, 4200), (n, 4000), (3, 3900)], hk=2, grp=4, D=D, page=16, code="i8", dt="bf16", seed=n)
+    most = dict(max_q=n, max_k=4200)
+    cache, _ = cache_of(b)
+    q, table, q_start, kv_len = dev(b.q, *b.where())
+    mask, _ = tree_of(b, 3, 0)
+    at = dev(mask)
+    out = [torch.empty_like(q) for _ in range(2)]
+    line = [torch.empty(q.shape[:2], device="cuda") for _ in range(2)]
+    first = S.KV8TreeAttention(cache, q, out[0], table, q_start, kv_len, at, lse=line[0], **most)
+    space = torch.empty(max(16, first.desc.attn.ws_bytes), dtype=torch.uint8, device="cuda")
+    ops = [S.KV8TreeAttention(cache, q, o, table, q_start, kv_len, at, lse=x, workspace=space, **most) for o, x in zip(out, line)]
+    graphs = []
+    for op in ops:
+        op.run()
+        torch.cuda.synchronize()
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            op.run()
+    for lens in ((4200, 4000, 3900), (n, n, 3), (4200, n, 50), (300, 2000, 3), (n, 4000, 3900), (60, 70, 80), (4200, 4000, 3900)):
+        b.kv_len = torch.tensor(lens, dtype=torch.int32)
+        b.lens = [(a, k) for (a, _), k in zip(b.lens, lens)]
+        kv_len.copy_(b.kv_len)
+        for g, o, x in zip(graphs, out, line):
+            o.fill_(7.0)
+            x.fill_(7.0)
+            g.replay()
+            done()
+            check(b, o, x, mask)
