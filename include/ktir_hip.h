@@ -652,7 +652,7 @@ int ktir_launch_kv8_rope_append(const ktir_kv8_rope_append_t* d);
 /* Attention of new tokens that are a tree: as ktir_launch_kv8_attention, but token i of
  * a sequence sees the tokens cached before the new ones and of the new ones those j
  * whose bit is set in its row of `mask` (as ktir_launch_draft_tree leaves it; any
- * other mask does as well, and a row may be 0).  With window > 0 it sees of the tokens
+ * other mask does as well, and a row may be 0; scores that are all -inf make a row NaN).  With window > 0 it sees of the tokens
  * before those at places > pos[t] - window (pos: int32, of each token; 0 if there is no window;
  * a position before the first new token's place counts as that); the mask says itself what of
  * the new tokens is in the window.  attn.causal has no effect.  max_q is at most 32 * words. */

@@ -36,10 +36,10 @@ constexpr int MOST_SPLITS = 256;      // of a tile's keys
 template <int J>
 __host__ __device__ constexpr int64_t part_size(int rows) { return (int64_t)rows * (64 * J + 4); }
 
-// whether a row of b and l has seen no key
+// whether a row of b has seen no key
 template <bool TREE>
-__device__ __forceinline__ bool sees_none(const ktir_kv8_attn_t& d, const Tile& t, int r, int grp, float b, float l) {
-  if constexpr (TREE) return b == B_NONE && l == 0.f;
+__device__ __forceinline__ bool sees_none(const ktir_kv8_attn_t& d, const Tile& t, int r, int grp, float b) {
+  if constexpr (TREE) return b == B_NONE;
   int lo, hi;
   seen(d, t, r, grp, &lo, &hi);
   return lo >= hi;
@@ -279,9 +279,13 @@ __global__ __launch_bounds__(64 * ROWS_WAVES, MT == 1 || (TREE && J * MT <= 4) ?
         for (int i = 0; i < 4; ++i) u[4 * h + i] = __builtin_fmaf(s[m][h][i], f, lv[h]);
       }
       if (TREE && cut) {
-        const uint32_t bits = tree_bits(mask, t, see_at[m], see_lo[m], key) >> (4 * g4);
+        uint32_t bits = tree_bits(mask, t, see_at[m], see_lo[m], key);
+        if (bits) b[m] = __builtin_fmaxf(b[m], B_SEEN);
+        bits >>= 4 * g4;
 #pragma unroll
         for (int i = 0; i < 8; ++i) u[i] = bits >> (16 * (i >> 2) + (i & 3)) & 1u ? u[i] : -__builtin_inff();
+      } else if (TREE) {
+        b[m] = __builtin_fmaxf(b[m], B_SEEN);
       } else if (cut) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -410,7 +414,7 @@ __global__ __launch_bounds__(64 * ROWS_WAVES, MT == 1 || (TREE && J * MT <= 4) ?
       continue;
     }
     const int r = t.row0 + row;
-    const bool none = sees_none<TREE>(d, t, r, grp, top, lt);
+    const bool none = sees_none<TREE>(d, t, r, grp, top);
     const int64_t tok = t.q.start + r / grp, h = head * grp + r % grp, e = tok * d.out.tok + h * d.out.head + x4;
     const float inv = L_UNIT / lt;
     if (x4 < D) {
@@ -494,7 +498,7 @@ __global__ __launch_bounds__(64 * R * B) void kv8_attn_join(const ktir_kv8_attn_
   }
   if (!on || turn) return;
   const int r = t.row0 + row;
-  const bool none = sees_none<false>(d, t, r, grp, top, lt);
+  const bool none = sees_none<false>(d, t, r, grp, top);
   const int64_t tok = t.q.start + r / grp, h = head * grp + r % grp;
   const float inv = L_UNIT / lt;
 #pragma unroll
@@ -556,7 +560,7 @@ __global__ __launch_bounds__(256) void kv8_rows_join(const ktir_kv8_attn_t d, in
     }
   }
   const int r = t.row0 + row;
-  const bool none = top == B_NONE && sum == 0.f;
+  const bool none = sees_none<true>(d, t, r, grp, top);
   const float inv = L_UNIT / sum;
   const int64_t tok = t.q.start + r / grp, h = head * grp + r % grp;
 #pragma unroll

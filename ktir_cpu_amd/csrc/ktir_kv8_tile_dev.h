@@ -307,12 +307,16 @@ __global__ __launch_bounds__(64 * W, J == 1 ? 2 : W / 4) void kv8_attn_tile(cons
         struct Places {
           int first;
           uint32_t bits[2];
+          bool some;                                 // of a tree: whether the row, both lanes of it, sees one
         };
         auto places = [&]() {
           Places at = {};
           if constexpr (TREE) {
 #pragma unroll
-            for (int k = 0; k < 2; ++k) at.bits[k] = tree_bits(mask, t, see_at[b], see_lo[b], key + 32 * k) >> (4 * h);
+            for (int k = 0; k < 2; ++k) at.bits[k] = tree_bits(mask, t, see_at[b], see_lo[b], key + 32 * k);
+            at.some = (at.bits[0] | at.bits[1]) != 0;
+#pragma unroll
+            for (int k = 0; k < 2; ++k) at.bits[k] >>= 4 * h;
           } else {
             at.first = key + 4 * h - see_lo[b];
             asm volatile("" : "+v"(at.first));
@@ -323,7 +327,8 @@ __global__ __launch_bounds__(64 * W, J == 1 ? 2 : W / 4) void kv8_attn_tile(cons
           if constexpr (TREE) return !(at.bits[k] >> (8 * (i >> 2) + (i & 3)) & 1u);
           else return (uint32_t)(at.first + 32 * k + 8 * (i >> 2) + (i & 3)) >= see[b];
         };
-        if (__any(base[b] == B_NONE)) {              // rows that have seen no key: b from this step's, their sums are 0
+        auto not_yet = [&]() { return base[b] == B_NONE || (TREE && base[b] == B_SEEN); };
+        if (__any(not_yet())) {                      // rows that have seen no key, or none that counts: b from this step's, their sums are 0
           float top = -__builtin_inff();
           const Places first = places();
 #pragma unroll
@@ -332,7 +337,8 @@ __global__ __launch_bounds__(64 * W, J == 1 ? 2 : W / 4) void kv8_attn_tile(cons
             for (int i = 0; i < 16; ++i)
               top = __builtin_fmaxf(top, mask_ninf(__builtin_fmaf(s[b][k][i], gks[2 * k + (i >> 3)] * rs[b], glv[2 * k + (i >> 3)]), hidden(first, k, i)));
           top = __builtin_fmaxf(top, other_half(top));
-          base[b] = base[b] == B_NONE && top > -__builtin_inff() ? top - TILE_TOP : base[b];
+          base[b] = not_yet() && top > -__builtin_inff() ? top - TILE_TOP : base[b];
+          if constexpr (TREE) base[b] = base[b] == B_NONE && first.some ? B_SEEN : base[b];
         }
 #pragma unroll
         for (int k = 0; k < 2; ++k)
@@ -475,7 +481,7 @@ __global__ __launch_bounds__(64 * W, J == 1 ? 2 : W / 4) void kv8_attn_tile(cons
       continue;
     }
     if (r >= t.row0 + t.rows) continue;
-    const bool none = TREE ? base[b] == B_NONE && sum[b] == 0.f : !see[b];
+    const bool none = TREE ? base[b] == B_NONE : !see[b];
     const float inv = none ? 0.f : L_UNIT / sum[b];
     const int64_t tok = t.q.start + r / grp, hq = head * grp + r % grp, e = tok * d.out.tok + hq * d.out.head;
 #pragma unroll
@@ -558,7 +564,7 @@ __global__ __launch_bounds__(256) void kv8_tile_join(const ktir_kv8_attn_t d, in
   const int r = t.row0 + 32 * wave + r32;
   if (r >= t.row0 + t.rows) return;
   const int64_t tok = t.q.start + r / grp, hq = head * grp + r % grp, e = tok * d.out.tok + hq * d.out.head;
-  const bool none = top == B_NONE && sum == 0.f;
+  const bool none = top == B_NONE;
   const float inv = none ? 0.f : L_UNIT / sum;
 #pragma unroll
   for (int v = 0; v < V; ++v) {
