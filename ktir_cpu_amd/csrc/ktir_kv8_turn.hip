@@ -65,19 +65,51 @@ struct PagePart {
   int n, r0;
   bool there;          // whether the table's page is one of the cache's
 };
-__device__ __forceinline__ bool page_part(const ktir_kv8_rope_append_t& d, int slot, PagePart* part, int* err) {
+// page number `p` of sequence s, which is q
+__device__ __forceinline__ bool part_of(const ktir_kv8_rope_append_t& d, const Seq& q, int64_t s, int64_t p, PagePart* part) {
   const ktir_kv8_t& c = d.cache;
   const int shift = __builtin_ctz((uint32_t)c.page);
-  int64_t s, nth;
-  const Seq q = seq_of_slot(d.batch, c.page, 1, shift, 2, slot, &s, &nth, err);
-  if (nth < 0) return false;
   const int64_t pos0 = (int64_t)q.n_kv - q.n_new, from = pos0 < 0 ? 0 : pos0;      // the first position that is stored
-  const int64_t p = (from >> shift) + nth;                                       // the page's number in the sequence
   const int64_t lo = p << shift < from ? from : p << shift, hi = (p + 1) << shift < q.n_held ? (p + 1) << shift : q.n_held;
   if (lo >= hi) return false;
   const int64_t page = ints(d.batch.table)[s * d.batch.table_row + p];
   *part = {page, q.start + lo - pos0, lo, (int)(hi - lo), (int)(lo & (c.page - 1)), page >= 0 && page < c.pages};
   return true;
+}
+__device__ __forceinline__ bool page_part(const ktir_kv8_rope_append_t& d, int slot, PagePart* part, int* err) {
+  const int shift = __builtin_ctz((uint32_t)d.cache.page);
+  int64_t s, nth;
+  const Seq q = seq_of_slot(d.batch, d.cache.page, 1, shift, 2, slot, &s, &nth, err);
+  if (nth < 0) return false;
+  const int64_t pos0 = (int64_t)q.n_kv - q.n_new;
+  return part_of(d, q, s, ((pos0 < 0 ? 0 : pos0) >> shift) + nth, part);
+}
+// Part `at` of those of more than `most` rows (fewer than a page has), of all sequences in order; false where there are not as
+// many.  All lanes of a wavefront search together, 64 sequences a step.
+__device__ __forceinline__ bool long_part(const ktir_kv8_rope_append_t& d, int64_t at, int most, PagePart* part, int* err) {
+  const int64_t page = d.cache.page;
+  const int l = threadIdx.x & 63, shift = __builtin_ctz((uint32_t)page);
+  for (int64_t base = 0; base < d.batch.seqs; base += 64) {
+    Seq q = {0, 0, 0, 0};
+    if (base + l < d.batch.seqs) q = seq_of(d.batch, page, base + l, err);
+    const int64_t from = q.n_kv > q.n_new ? q.n_kv - q.n_new : 0, end = q.n_held;
+    const int64_t first = from >> shift, last = (end - 1) >> shift, head = ((first + 1) << shift < end ? (first + 1) << shift : end) - from;
+    // (all pages between the first and the last are full)
+    const int begins = head > most, n = end <= from ? 0 : first == last ? begins : begins + (int)(last - first - 1) + (end - (last << shift) > most);
+    int upto = n;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int y = __shfl_up(upto, o);
+      upto += l >= o ? y : 0;
+    }
+    const uint64_t past = __ballot(at < upto);
+    if (past) {
+      const int i = __builtin_ctzll(past), nth = (int)at - (lane_of(upto, i) - lane_of(n, i));
+      return part_of(d, lane_of(q, i), base + i, lane_of(first, i) + nth + 1 - lane_of(begins, i), part);
+    }
+    at -= lane_of(upto, 63);
+  }
+  return false;
 }
 __device__ __forceinline__ int64_t row_position(const ktir_kv8_rope_append_t& d, const PagePart& part, int row, int* err) {
   const int64_t pos = d.pos ? rope_pos(d, part.t0 + row) : part.lo + row;
@@ -85,17 +117,16 @@ __device__ __forceinline__ int64_t row_position(const ktir_kv8_rope_append_t& d,
   return pos < 0 ? 0 : pos;
 }
 
-// Where a page's part of a head lies.
-template <bool IS_K>
+// Where a page's part of a head of K or V lies.
 struct PageHead {
   KTIR_G(uint8_t)* codes;
   KTIR_G(float)* scale;
   int64_t tok;
-  __device__ __forceinline__ PageHead(const ktir_kv8_rope_append_t& d, const PagePart& part, int64_t head) {
+  __device__ __forceinline__ PageHead(const ktir_kv8_rope_append_t& d, const PagePart& part, int64_t head, bool is_k) {
     const ktir_kv8_t& c = d.cache;
-    codes = (KTIR_G(uint8_t)*)(IS_K ? c.k + part.page * c.k_page + head * c.k_head : c.v + part.page * c.v_page + head * c.v_head);
-    scale = IS_K ? (KTIR_G(float)*)c.k_scale + part.page * c.ks_page + head * c.ks_head : (KTIR_G(float)*)c.v_scale + part.page * c.vs_page + head * c.vs_head;
-    tok = IS_K ? c.k_tok : c.v_tok;
+    codes = (KTIR_G(uint8_t)*)(is_k ? c.k + part.page * c.k_page + head * c.k_head : c.v + part.page * c.v_page + head * c.v_head);
+    scale = is_k ? (KTIR_G(float)*)c.k_scale + part.page * c.ks_page + head * c.ks_head : (KTIR_G(float)*)c.v_scale + part.page * c.vs_page + head * c.vs_head;
+    tok = is_k ? c.k_tok : c.v_tok;
   }
 };
 
@@ -332,7 +363,7 @@ __device__ __forceinline__ void turn_kv(const ktir_kv8_rope_append_t& d, int slo
   const int G = (int)c.columns >> 4, per = 64 * W / G, r = tid / G, col = (tid - r * G) * 16;     // rows a pass; this thread's
   const bool wide = !((in.ptr | (uint64_t)in.tok * 2 | (uint64_t)in.head * 2) & 15), mine = r < per && head < c.heads;
   const int64_t e0 = part.t0 * in.tok + head * in.head;
-  const PageHead<IS_K> to(d, part, head);
+  const PageHead to(d, part, head, IS_K);
   float before = 0.f;
   // the unit of 16 columns of the rows first + r, first + per + r, ...: loads, then (K) the angles of these rows into LDS, then the values
   const bool vectors = wide && half % 8 == 0;
@@ -441,11 +472,13 @@ __global__ __launch_bounds__(256, MORE ? 1 : 4) void kv8_turn(const ktir_kv8_rop
 // A decode step, or a few drafts of each sequence, is latency: the instructions of one wavefront, one after
 // another, and its loads.  Here a lane has pairs of one row (and columns behind the turned ones), so an angle is made where
 // it is used, without LDS, and what a wavefront does is short.  A workgroup has a page's part of a head of K or
-// V, a row a wavefront, or one token's part of the queries, a head a wavefront at a time.
+// V, a row a wavefront (of four heads, a wavefront each, where most sequences have a token or two), or one token's part of
+// the queries, a head a wavefront at a time.
 
 constexpr int FEW_TOKENS = 8;
 constexpr int FEW_HEADS = 16;        // of the queries, for a workgroup
 constexpr int FEW_KEPT = 2;          // rows that a wavefront keeps
+constexpr int FEW_WIDE = 256;        // workgroups for longer ones
 static_assert(4 * FEW_KEPT >= FEW_TOKENS, "four wavefronts read no row again");
 
 struct FewAngles {
@@ -469,6 +502,27 @@ __device__ __forceinline__ int few_first(const ktir_kv8_rope_append_t& d, int i)
   return d.interleaved ? 2 * p : p;
 }
 __device__ __forceinline__ int few_gap(const ktir_kv8_rope_append_t& d) { return d.interleaved ? 1 : (int)d.rot / 2; }
+
+// The same by a call, for a loop over rows: inline, the constants of sine and cosine stay in registers around the loop, which costs
+// the short parts of the same kernel wavefronts (1024 sequences of one token 60.2 us, 57.8).
+struct OneAngle {
+  float c, s;
+};
+__device__ __attribute__((noinline)) OneAngle one_angle(int64_t pos, double freq, double amplitude) {
+  OneAngle a;
+  rope_angle_of(pos, freq, amplitude, false, &a.c, &a.s);
+  return a;
+}
+__device__ __forceinline__ FewAngles few_angles_again(const ktir_kv8_rope_append_t& d, int64_t pos, const double (&f)[2]) {
+  FewAngles a;
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    if ((int)(threadIdx.x & 63) + 64 * i < d.rot / 2) {
+      const OneAngle x = one_angle(pos, f[i], d.amplitude);
+      a.c[i] = x.c, a.s[i] = x.s;
+    }
+  return a;
+}
 
 template <int DT>
 __device__ __forceinline__ void few_load(const ktir_kv8_rope_append_t& d, uint64_t ptr, int64_t e, bool rest, FewRow& x) {
@@ -520,18 +574,19 @@ __device__ __forceinline__ void few_queries(const ktir_kv8_rope_append_t& d, int
   }
 }
 
-// W wavefronts (1 or 4) have a page's part of a head.
-template <int DT, bool IS_K, int W>
-__device__ __forceinline__ void few_kv(const ktir_kv8_rope_append_t& d, int slot, int64_t head, const double (&f)[2], uint32_t* tops, int* err) {
+// W wavefronts (1 or 4) have a page's part of a head, a row each in turn: rows that they keep between the maximum and
+// the codes, or (MORE) any number, each read twice.
+template <int DT, int W, bool MORE>
+__device__ __forceinline__ void few_kv(const ktir_kv8_rope_append_t& d, const PagePart& part, int64_t head, bool is_k, const double (&f)[2], uint32_t* tops, int* err) {
   const ktir_kv8_t& c = d.cache;
   const int wave = W == 1 ? 0 : uni((int)(threadIdx.x >> 6)), l = threadIdx.x & 63, half = (int)d.rot / 2;
-  PagePart part;
-  if (!page_part(d, slot, &part, err)) return;
-  const ktir_rows3_t& in = IS_K ? d.k : d.v;
+  const ktir_rows3_t in = is_k ? d.k : d.v;
   const int64_t e0 = part.t0 * in.tok + head * in.head;
   auto values = [&](int row, FewRow& x) {
     few_load<DT>(d, in.ptr, e0 + row * in.tok, true, x);
-    if constexpr (IS_K) few_turn(x, few_angles(d, row_position(d, part, row, err), f));
+    if (!is_k) return;
+    const int64_t pos = row_position(d, part, row, err);
+    few_turn(x, MORE ? few_angles_again(d, pos, f) : few_angles(d, pos, f));
   };
   uint32_t top = 0;
   auto look = [&](const FewRow& x) {
@@ -546,20 +601,22 @@ __device__ __forceinline__ void few_kv(const ktir_kv8_rope_append_t& d, int slot
     for (int i = 0; i < 4; ++i)
       if (d.rot + l + 64 * i < c.columns) see(x.rest[i]);
   };
-  FewRow x[FEW_KEPT];
-  const PageHead<IS_K> to(d, part, head);
+  FewRow x[FEW_KEPT];                      // (MORE: unused)
+  const PageHead to(d, part, head, is_k);
   const float before = part.there && part.r0 ? *to.scale : 0.f;
-#pragma unroll
-  for (int k = 0; k < FEW_KEPT; ++k)
-    if (wave + W * k < part.n) {
-      values(wave + W * k, x[k]);
-      look(x[k]);
-    }
+  if constexpr (MORE) {
 #pragma unroll 1
-  for (int row = FEW_KEPT; W == 1 && row < part.n; ++row) {          // (four have FEW_TOKENS at most)
-    FewRow y;
-    values(row, y);
-    look(y);
+    for (int row = wave; row < part.n; row += W) {
+      values(row, x[0]);
+      look(x[0]);
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < FEW_KEPT; ++k)
+      if (wave + W * k < part.n) {
+        values(wave + W * k, x[k]);
+        look(x[k]);
+      }
   }
   if (!part.there) {
     *err = OUT_OF_RANGE;
@@ -593,27 +650,48 @@ __device__ __forceinline__ void few_kv(const ktir_kv8_rope_append_t& d, int slot
     for (int i = 0; i < 4; ++i)
       if (d.rot + l + 64 * i < c.columns) p[d.rot + l + 64 * i] = (uint8_t)(v >> (8 * i));
   };
-#pragma unroll
-  for (int k = 0; k < FEW_KEPT; ++k)
-    if (wave + W * k < part.n) put(wave + W * k, x[k]);
+  if constexpr (MORE) {
 #pragma unroll 1
-  for (int row = FEW_KEPT; W == 1 && row < part.n; ++row) {
-    FewRow y;
-    values(row, y);
-    put(row, y);
+    for (int row = wave; row < part.n; row += W) {
+      values(row, x[0]);
+      put(row, x[0]);
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < FEW_KEPT; ++k)
+      if (wave + W * k < part.n) put(wave + W * k, x[k]);
   }
   if (wave == 0 && l == 0) *to.scale = now.scale;
 }
 
+// `wide` workgroups come first, for parts that are too long for one wavefront: a batch of a token or two a sequence may have
+// most of them in one, which the host does not know.  Each looks for its parts itself and ends where there are no more.  256
+// sequences of one token and one of 200, pages of 16, 64 and 256: 17.3, 34.2 and 58.8 us (28.8, 83.8 and 163.8 with a wavefront for each part,
+// 18.6, 50.9 and 112 in the other kernel); what they cost where there are no long parts: 64 of one token 6.1 -> 6.5, 256 11.6 -> 12.7.
 template <int DT, int W>
-__global__ __launch_bounds__(256) void kv8_turn_few(const ktir_kv8_rope_append_t d, int slots, int groups, int parts, int* err) {
+__global__ __launch_bounds__(256) void kv8_turn_few(const ktir_kv8_rope_append_t d, int slots, int groups, int parts, int wide, int* err) {
   __shared__ uint32_t tops[4];
-  const int l = threadIdx.x & 63, half = (int)d.rot / 2, heads = (int)d.cache.heads, kv = groups * slots, block = blockIdx.x;
+  const int l = threadIdx.x & 63, half = (int)d.rot / 2, heads = (int)d.cache.heads, kv = groups * slots, block = (int)blockIdx.x - wide;
   const double f[2] = {frequency(d, l < half ? l : 0), frequency(d, l + 64 < half ? l + 64 : 0)};
   if (block >= kv) return few_queries<DT>(d, block - kv, parts, f, err);
+  PagePart part;
+  if (W == 1 && block < 0) {
+    // (the descriptor by an address that the compiler does not know: else it is loaded, and spilled, before the branch; 64 of one token 7.4 us)
+    auto* again = (const __attribute__((address_space(4))) ktir_kv8_rope_append_t*)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(again));
+    const ktir_kv8_rope_append_t& d = *(const ktir_kv8_rope_append_t*)again;
+    for (int64_t at = blockIdx.x;; at += wide) {
+      const int64_t nth = at / (2 * heads);
+      const int hv = (int)(at - nth * 2 * heads);
+      if (!long_part(d, nth, FEW_KEPT, &part, err)) return;
+      few_kv<DT, 4, true>(d, part, hv < heads ? hv : hv - heads, hv < heads, f, tops, err);
+      __syncthreads();
+    }
+  }
   const int slot = block / groups, hv = (block - slot * groups) * (4 / W) + (W == 1 ? uni((int)(threadIdx.x >> 6)) : 0);
-  if (hv < heads) few_kv<DT, true, W>(d, slot, hv, f, tops, err);
-  else if (hv < 2 * heads) few_kv<DT, false, W>(d, slot, hv - heads, f, tops, err);
+  if (hv >= 2 * heads || !page_part(d, slot, &part, err) || (W == 1 && part.n > FEW_KEPT)) return;
+  if (hv < heads) few_kv<DT, W, false>(d, part, hv, true, f, tops, err);
+  else few_kv<DT, W, false>(d, part, hv - heads, false, f, tops, err);
 }
 
 // whether every vector of 8 values of the queries starts on a 16-byte bound
@@ -659,15 +737,17 @@ static int turn_go(const ktir_kv8_rope_append_t& d, hipStream_t st) {
 template <int DT>
 static int turn_type(const ktir_kv8_rope_append_t& d, hipStream_t st) {
   // The kernels for few tokens, four wavefronts a head for up to 8 (32 / 8 heads of 128 columns, one sequence of 1 to 4: 4.6 us,
-  // of 8 5.5, the other kernel 6.6 to 7.0; 16 in pages of 64 8.4 and 7.2), one where there are up to two a sequence
-  // (64 sequences of one 6.1, of two 6.5, the other kernel 7.5 and 7.7, with pages of 64 6.3 and 12.8; of four 10.4 and 8.4).
+  // of 8 5.5, the other kernel 6.6 to 7.0; 16 in pages of 64 8.4 and 7.2), one where there are up to two a sequence on average (64
+  // sequences of one 6.5, of two 7.4, the other kernel 7.5 and 7.7, with pages of 64 6.5 and 12.8; 256 of one 12.5 and 15.9) and four
+  // for a part of more (64 of one and 40 of another sequence, pages of 16 and 64, 12.7 and 21.3, the other kernel 10.4 and 18.2).
   const bool few = d.batch.tokens <= FEW_TOKENS;
   if (few || d.batch.tokens <= 2 * d.batch.seqs) {
     const int64_t slots = d.batch.tokens / d.cache.page + 2 * d.batch.seqs, parts = (d.q_heads + FEW_HEADS - 1) / FEW_HEADS;
-    const int64_t groups = few ? 2 * d.cache.heads : (2 * d.cache.heads + 3) / 4, blocks = groups * slots + d.batch.tokens * parts;
+    const int64_t groups = few ? 2 * d.cache.heads : (2 * d.cache.heads + 3) / 4, most = d.batch.tokens / (FEW_KEPT + 1) * 2 * d.cache.heads;
+    const int64_t wide = few ? 0 : most < FEW_WIDE ? most : FEW_WIDE, blocks = wide + groups * slots + d.batch.tokens * parts;
     if (blocks <= (1 << 30)) {
-      if (!few) hipLaunchKernelGGL((kv8_turn_few<DT, 1>), dim3((unsigned)blocks), dim3(256), 0, st, d, (int)slots, (int)groups, (int)parts, device_error_flag());
-      else hipLaunchKernelGGL((kv8_turn_few<DT, 4>), dim3((unsigned)blocks), dim3(256), 0, st, d, (int)slots, (int)groups, (int)parts, device_error_flag());
+      if (!few) hipLaunchKernelGGL((kv8_turn_few<DT, 1>), dim3((unsigned)blocks), dim3(256), 0, st, d, (int)slots, (int)groups, (int)parts, (int)wide, device_error_flag());
+      else hipLaunchKernelGGL((kv8_turn_few<DT, 4>), dim3((unsigned)blocks), dim3(256), 0, st, d, (int)slots, (int)groups, (int)parts, 0, device_error_flag());
       KTIR_HIP_CHECK(hipGetLastError());
       return KTIR_OK;
     }
