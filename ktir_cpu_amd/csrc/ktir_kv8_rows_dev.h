@@ -97,6 +97,7 @@ __device__ __forceinline__ void kv8_values(const ktir_kv8_t& c, const KV8Groups&
 template <int CODE, int J, int MT, bool TREE>
 __global__ __launch_bounds__(64 * ROWS_WAVES, MT == 1 || (TREE && J * MT <= 4) ? 2 : 1) void kv8_attn_rows(const ktir_kv8_attn_t d, const KV8Mask mask, int splits, int part, int part_rows, uint32_t slots, int hw, int* err) {
   constexpr int W = ROWS_WAVES, TM = 16 * MT, N = 4 * J, PITCH = 64 * J + 4;
+  static_assert(kv8_rows_lds(J, MT) == sizeof(float) * W * TM * (PITCH + 2), "what is declared next");
   __shared__ __attribute__((aligned(16))) float o_sum[W][TM * PITCH];
   __shared__ float w_b[W][TM], w_l[W][TM];
   const ktir_kv8_t& c = d.cache;
@@ -115,7 +116,7 @@ __global__ __launch_bounds__(64 * ROWS_WAVES, MT == 1 || (TREE && J * MT <= 4) ?
     const int quant = ROWS_STEP * TW;
     TreePart p;
     slot = u;                                          // (of the part in the workspace)
-    t = uni(tree_part<ROWS_STEP, ROWS_STEP * W>(d, grp, TM, (int)sets, quant, quant < 128 ? 128 / quant : 1, 512, splits, u, &p, err));
+    t = uni(tree_part<ROWS_STEP, ROWS_STEP * W>(d, grp, TM, (int)sets, quant, quant < 128 ? 128 / quant : 1, kv8_rows_held(J, MT), splits, u, &p, err));
     if (!t.rows) return;
     split = uni(p.at);
     active = uni(p.count);
@@ -576,7 +577,7 @@ int kv8_rows_go(const ktir_kv8_attn_t& d, const KV8Mask& mask, const KV8Shape& s
   const int64_t QUANT = ROWS_STEP * W / s.HW, items = s.slots * d.cache.heads, splits = d.splits < 1 ? 1 : d.splits;
   const int part = (int)(((s.span + splits - 1) / splits + QUANT - 1) / QUANT * QUANT);
   // two workgroups a CU, evenly: where three fit, some CUs get three and others one (510 parts of 704 keys: 89 and 72 us)
-  constexpr int held = (int)(sizeof(float) * W * (16 * MT * (64 * J + 4) + 2 * 16 * MT)), spare = held < 55000 ? 55000 - held : 0;
+  constexpr int lds = kv8_rows_lds(J, MT), spare = lds < 55000 ? 55000 - lds : 0;
   const hipStream_t st = stream_of(d.stream);
   const int64_t groups = !TREE ? s.slots * splits : splits > 1 ? splits : s.slots;
   hipLaunchKernelGGL((kv8_attn_rows<CODE, J, MT, TREE>), dim3((unsigned)((groups + 7) / 8 * 8 * (d.cache.heads / s.HW))), dim3(64 * W), spare, st, d, mask, TREE && splits == 1 ? 0 : (int)splits, part, s.rows, (uint32_t)s.slots, s.HW, device_error_flag());

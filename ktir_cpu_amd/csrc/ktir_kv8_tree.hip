@@ -46,14 +46,16 @@ static TreePlan tree_plan(const ktir_kv8_attn_t& d) {
   // Little work takes tiles of 16 rows, however many: more workgroups and shorter ones (eight KV heads of 128 columns, 4 query
   // heads each, one sequence: 8 tokens after 1000 13.2 us, tiles of 32 rows 15.7; 64 after 1000 19.0, of 256 27.3; 16 after
   // 16000 34.7, 29.6; sixteen sequences of 16 after 1000 38.6, 32.5).  Tiles of 32 rows read the cache half as often, but with more
-  // than 128 columns leave a SIMD one wavefront, so that they need more work (256 columns, 16 tokens, tiles of 16 rows and
-  // of 32: four sequences of 4000 52.0, 55.7; sixteen 146, 123).  Up to 64 rows two tiles of 32 beat one of 256 (80 rows 57 us, 44;
+  // than 128 columns leave a SIMD one wavefront, so that they need longer keys, or more work, where lengths are uneven (192 and 256
+  // columns, tiles of 16 rows and of 32: four sequences of 16 tokens after 4000 46.7 and 60.3, 37.4 and 42.6; one after 16000 45.1 and
+  // 58.3, 35.7 and 40.6; 14 after 200 to 1500 42.8 and 54.0, 64.4 and 73.1; 28 of four KV heads after 200 to 2000 39.5 and 49.9, 53.9 and
+  // 59.0, after 1800 to 2000 60.2 and 85.5, 52.3 and 59.8; 20 of two after 300 to 5000 30.5 and 37.3, 33.6 and 37.2).  Up to 64 rows two tiles of 32 beat one of 256 (80 rows 57 us, 44;
   // 192 of six sequences 194, 142) and beat one of 64 by what that spills (64 rows of 16 sequences of up to 16000: 51, 69).
   const KV8Shape least = tree_rows(d, 1, span);
   const int64_t tiles = least.slots * heads;
   const bool little = tiles <= 512 && tiles * span <= 1 << 18;
   if (rows <= 64 || little) {
-    const bool narrow = little || rows <= 16 || (wide && tiles <= 2048 && tiles * span <= 1 << 20);
+    const bool narrow = little || rows <= 16 || (wide && tiles <= 2048 && tiles * span <= 1 << 20 && span < 3500);
     KV8Shape& s = p.rows = narrow ? least : tree_rows(d, 2, span);
     const int64_t n = s.slots * heads, most = s.slots * ((s.span + 127) / 128);
     // Heads of a workgroup: several, a wavefront each, for many tiles of few keys, where nothing is left to join then (200
@@ -61,9 +63,9 @@ static TreePlan tree_plan(const ktir_kv8_attn_t& d) {
     // rows of several heads are read together (64 sequences of 64 to 8192 keys, cold: 78.7, 85.7; 128 of 1000 to 2000 147, 120).
     const bool many = n >= 1024 && span <= (wide ? 2048 : 768), far = n >= 512 && n < 2048 && span > 2048;
     if (many || far) s.HW = heads % 4 == 0 ? 4 : heads % 2 == 0 ? 2 : 1;
-    // Parts that the device may cut: two workgroups for each CU, and two at least for each tile (eight sequences for each CU are not cut).
-    const int64_t sets = heads / s.HW;
-    int64_t parts = 512 / sets > 2 * s.slots ? 512 / sets : 2 * s.slots;
+    // Parts that the device may cut: the workgroups that the chip holds, and two at least for each tile (eight sequences for each CU are not cut).
+    const int64_t sets = heads / s.HW, held = kv8_rows_held(s.J, s.MT);
+    int64_t parts = held / sets > 2 * s.slots ? held / sets : 2 * s.slots;
     if (parts > most) parts = most;
     p.groups = many || n >= 2048 || span <= tree_cut_cost(n) || parts <= s.slots ? 1 : parts;
     p.floats = heads * s.part;

@@ -33,6 +33,10 @@ struct KV8Shape {
   int J, MT, HW, rows, splits;         // columns in 64s, rows in 16s, heads of a workgroup, most rows of a tile
   int64_t slots, part, span;           // tiles of rows for each KV head; floats of a split's part in the workspace; most keys of a tile
 };
+// Bytes of LDS that a workgroup of ktir_kv8_rows_dev.h takes: the sums, b and l of its four wavefronts' 16 MT rows.
+__host__ __device__ constexpr int kv8_rows_lds(int J, int MT) { return 4 * 4 * (16 * MT * (64 * J + 4) + 2 * 16 * MT); }
+// How many of them the 256 CUs, of 160 KB each, hold at a time: two a CU (no more are wanted), or one.
+__host__ __device__ constexpr int kv8_rows_held(int J, int MT) { return 2 * kv8_rows_lds(J, MT) <= 160 * 1024 ? 512 : 256; }
 void kv8_rows_shape(const ktir_kv8_attn_t& d, KV8Shape* s);
 int kv8_rows_launch(const ktir_kv8_attn_t& d, const KV8Shape& s);
 bool kv8_tile_takes(const ktir_kv8_attn_t& d, int64_t* slots);       // whether ktir_kv8_tile.hip takes it instead
