@@ -634,8 +634,9 @@ int ktir_launch_draft_tree(const ktir_draft_tree_t* d);
  * go to the cache with its values, as ktir_launch_kv8_append does it, without being
  * rounded to 16 bits on the way.  pos: the tokens' positions for the rotation (KTIR_I32 or
  * KTIR_I64, a negative one counts as 0 with the device error word set), or 0: their places in the cache.
- * Tokens that the append does not store (outside every sequence, at negative places,
- * past the table's pages) are left as they were in q_out.  q_out may be q itself. */
+ * Tokens that have no place (outside every sequence, at negative places, past the table's pages) are
+ * left as they were in q_out; one whose table entry is no page of the cache is turned there, and its key and value go
+ * nowhere, with the device error word set.  q_out may be q itself. */
 typedef struct ktir_kv8_rope_append {
   ktir_kv8_t cache;
   ktir_kv8_batch_t batch;

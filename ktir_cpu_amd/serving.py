@@ -442,7 +442,7 @@ class KV8RopeAppend(_Launch):
     The batch is KV8Append's, the rotation Rope's.  The keys are not rounded to 16 bits between the
     two, so their codes may differ from those of Rope and KV8Append by the rounding of values half way between codes.
     `positions` [tokens] int32 or int64: the rotation's positions (DraftTree's for a tree);
-    None: the tokens' places in the cache.  Rows of q_out whose tokens are not stored stay as they were.
+    None: the tokens' places in the cache.  Rows of q_out whose tokens have no place in the cache stay as they were.
     """
 
     entry = "ktir_launch_kv8_rope_append"

@@ -130,3 +130,26 @@ def test_turn_of_a_long_run_among_many_sequences(ones, run, page):
         took.append(microseconds(op))
     done()
     assert took[0] <= 4 * took[1], took
+
+
+def test_turn_out_of_range_and_its_queries():
+    """Queries of tokens whose table entry is no page are turned; those of tokens past the table, or before it, stay."""
+    for dt, many in (("f16", False), ("bf16", True)):
+        lens = [(20, 40), (10, 100), (5, 30), (9, 4)] + [(600, 600)] * many
+        b = Batch(lens, hk=1, grp=2, D=32, page=16, dt=dt, seed=5)
+        freq, where = freq_of(32), P.places(b.q_start, b.kv_len, b.tokens)
+        table = b.table[:, :6 if not many else 38].contiguous()          # (the first: sequence 1 ends at 96 of 100)
+        clean = table.clone()
+        table[0, 1] = b.pages                                            # sequence 0's new tokens 0 to 11
+        cache, arrays = cache_of(b)
+        q = dev(b.q)
+        S.KV8RopeAppend(cache, q, *dev(b.new_k, b.new_v, freq, table, b.q_start, b.kv_len)).run()
+        with pytest.raises(IndexError):
+            done()
+        done()
+        placed = (where >= 0) & ~((torch.arange(b.tokens) >= 26) & (torch.arange(b.tokens) < 30) & (not many))
+        want, bound = rope(b.q, where.clamp(min=0), freq)
+        close(q[placed], want[placed], bound[placed], dt)
+        same_bits(q[~placed], b.q[~placed], "queries without a place")
+        at = int(clean[0, 1])
+        same_bits(arrays[0][at], b.k[at], "a page that was not named")
