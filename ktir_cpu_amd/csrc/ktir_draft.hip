@@ -12,7 +12,7 @@ constexpr int64_t TREE_WORDS = 32;           // of a token's mask
 // the tokens before.  One thread a token: first up the line within its word, which half a wavefront holds, in 5
 // doublings; where that leaves the word, the row of the ancestor it comes to has the other words, which are copied word
 // by word of the sequence.  Bound: latency, the chain offsets -> parents, then a step of LDS and a barrier for each word.
-// 64 sequences of up to 64 tokens 3.8 us (2.7 in a graph), 24 of up to 500, with a window, 6.8; 10.7 with the line walked token
+// 64 sequences of up to 64 tokens 3.8 to 4.1 us (2.7 in a graph), 24 of up to 500, with a window, 6.8; 10.7 with the line walked token
 // by token and the window's bits dropped one by one, 41 without the words.  Threads for 4, 16 or 32 words: in a graph
 // 512 sequences of up to 64 tokens take 2.9, 3.7 and 6.8 us, of up to 500 8.1 with 16 words and 13.8 with 32.
 
@@ -94,7 +94,7 @@ __global__ __launch_bounds__(32 * WORDS) void draft_tree(const ktir_draft_tree_t
 // page gets is read before its place is written: pages in order, and in a page the rows of
 // one pass of the wavefront (64 units of 16 columns), all read, then written.  Bound: latency, offsets and path ->
 // table -> scales and codes, for each page; a lane has the place, page and scale that one entry of 64 comes from.  One sequence of
-// 16 drafts 4.2 us, which is the launch, 256 of up to 64 10.0 (12.7 with each entry's place looked up by every lane).
+// 16 drafts 4.3 us, which is the launch, 256 of up to 64 10.2 (12.7 with each entry's place looked up by every lane).
 
 constexpr int KEEP_KEPT = 2;         // passes of rows that stay in registers between the maximum and the codes
 

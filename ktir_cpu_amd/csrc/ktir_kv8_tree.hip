@@ -5,11 +5,11 @@
 // kernels are those of new tokens in a line (ktir_kv8_rows_dev.h, ktir_kv8_tile_dev.h) but for where a step reaches the
 // window's start or the new tokens.  Their tiles' keys are cut by the device (ktir_kv8_dev.h), and a second kernel joins the parts.
 //
-// 32 / 8 heads of 128 columns, cold caches.  8 tokens after 1000: 12.6 us, latency (9.1 and 4.0 for the join).  64 sequences of up to 8
-// after 64 to 8192, 208 MB: 66, 56 at 3.7 TB/s and 12 for the join.  64 after 131072, 137 GFLOP and half as many for
-// the weights' second terms: 208, the products at 1.0 PFLOP/s and 12 for the join.  8 of 128 to 256 after 2048 to 16384, 199 GFLOP and half
-// as many: 382, an even share of the steps is 318.  12 of up to 100 after up to 4000, a window of 1000, 21 / 3 heads of 80: 31.6, the
-// longest piece and a join (26 and 7).
+// 32 / 8 heads of 128 columns, in loops of launches on inputs in turn; kernels under a profiler.  8 tokens after 1000: 12.6 us, latency (8.7 and
+// 4.4 for the join).  64 sequences of up to 8 after 64 to 8192, 208 MB: 66, 55 at 3.8 TB/s and 12 for the join.  64 after 131072, 137
+// GFLOP and half as many for the weights' second terms: 208 to 210, the products at 1.0 PFLOP/s (198) and 11 for the join; 252 for the first launches
+// of an idle card.  8 of 128 to 256 after 2048 to 16384, 199 GFLOP and half as many: 376 to 382 (362 and 22; 443 for the first launches), an even share
+// of the steps is 318.  12 of up to 100 after up to 4000, a window of 1000, 21 / 3 heads of 80: 31.5, the longest piece and a join (24 and 7).
 #include "ktir_kv8_tree.h"
 
 namespace ktir {
@@ -60,7 +60,9 @@ static TreePlan tree_plan(const ktir_kv8_attn_t& d) {
     const int64_t n = s.slots * heads, most = s.slots * ((s.span + 127) / 128);
     // Heads of a workgroup: several, a wavefront each, for many tiles of few keys, where nothing is left to join then (200
     // sequences of 8 tokens after up to 500: 56.7 us, a workgroup for each head 72; up to 2000 156, 151), and for many long ones, whose
-    // rows of several heads are read together (64 sequences of 64 to 8192 keys, cold: 78.7, 85.7; 128 of 1000 to 2000 147, 120).
+    // rows of several heads are read together (one, two and four heads, of eight, 1 to 8 tokens: 64 sequences of 64 to 8192 keys 78.0, 69.1,
+    // 68.9; 100 117.6, 137.3, 108.3; 64 of 64 to 4000 55.6, 48.0, 50.5; 128 116.8, 97.9, 105.4; 128 of four heads, 64 to 8192, 84.0, 85.4, 78.6;
+    // where lengths are alike one or two gain: 128 of 1000 to 2500 123.8, 124.9, 143.3; 64 of 8 tokens after 2500 98.2, 95.2, 100.5).
     const bool many = n >= 1024 && span <= (wide ? 2048 : 768), far = n >= 512 && n < 2048 && span > 2048;
     if (many || far) s.HW = heads % 4 == 0 ? 4 : heads % 2 == 0 ? 2 : 1;
     // Parts that the device may cut: the workgroups that the chip holds, and two at least for each tile (eight sequences for each CU are not cut).

@@ -7,8 +7,8 @@
 // has just loaded: all layouts of pairs then store 16 codes at once.
 //
 // Bound: bytes, queries in and out and keys and values in once, codes out.  8192 tokens of 32 / 8 heads of 128 columns, 185
-// MB: 40.8 us = 4.5 TB/s (a copy of 256 MiB makes 5.4; the rotation and the append by themselves take 31.8 and 12.5).
-// 182 us with an element a thread, 52 with four units a thread (fewer wavefronts a CU), 47.6 with the loads behind the
+// MB: 43.6 us = 4.2 TB/s in a loop of launches, 45.6 (44.7 to 47.3) in a card's first ones (a copy of 256 MiB makes 5.4; the rotation and the
+// append by themselves take 31.8 and 12.5).  On a card where it takes 40.8: 182 us with an element a thread, 52 with four units a thread (fewer wavefronts a CU), 47.6 with the loads behind the
 // angles, 43 with eight tokens a workgroup of queries.  The two kinds in turn take 63 to 70: in one launch their
 // streams do not go together.  Queries first 44.4, four rows of loads ahead 43.7.
 // Few tokens are latency, and have kernels of their own below.

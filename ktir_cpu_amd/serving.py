@@ -479,7 +479,8 @@ class KV8TreeAttention(_Launch):
     `mask` [tokens, words] int32, words up to 32, as DraftTree writes it: bit j % 32 of word j // 32 is new
     token j; any other mask does as well, and a row that sees nothing gives 0.  `window` > 0: of the tokens before, those
     at places > positions[t] - window (`positions` [tokens] int32, DraftTree's); the mask says itself
-    which of the new ones are in the window.  `max_q` is 32 * words at most; the rest as for KV8Attention.
+    which of the new ones are in the window.  `max_q` is 32 * words at most, and best what the drafts are: it is taken as the
+    rows that there are.  The rest as for KV8Attention.
     """
 
     entry = "ktir_launch_kv8_tree_attention"
