@@ -23,7 +23,7 @@ typedef uint32_t u32x3_t __attribute__((ext_vector_type(3), aligned(4)));
 
 constexpr float B_LAG = 8.f;                     // b is changed when an exponent passes it by more
 constexpr float B_NONE = -1e38f;                 // b of a row that has seen no key
-constexpr float B_SEEN = -0.5e38f;               // of a tree: b of one that has seen keys, none of them with a score above -inf
+constexpr float B_SEEN = -0.999e38f;             // of a tree: b of one that has seen keys, none of them with a score above -inf
 constexpr float L_UNIT = 0x1p-16f;
 constexpr float LEAST_V = 0x1p-100f;             // the least vscale that w is computed with (append's least; smaller ones count as this)
 
