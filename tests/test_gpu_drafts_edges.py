@@ -40,6 +40,26 @@ def test_attention_of_rows_whose_scores_are_all_minus_infinity(n, grp, D, most, 
     check(b, out, line, mask)
 
 
+@pytest.mark.parametrize("n,grp,D,most", KERNELS)
+@pytest.mark.parametrize("k", [90, 2600])
+def test_attention_of_rows_whose_scores_are_far_below_zero(n, grp, D, most, k):
+    # finite scores of -4e37 and below: the least of them has all the weight, whole tiles and cut ones
+    b = Batch([(n, k + n)], hk=2, grp=grp, D=D, page=16, dt="bf16", seed=n)
+    b.q.zero_()
+    b.q[..., 0] = -1.25 * 2.0 ** 118
+    b.k.zero_()
+    b.k[..., 0] = 120
+    b.k_scale.fill_(1.0)
+    page, row = int(b.table[0, 37 // 16]), 37 % 16
+    b.k[page, row, :, 0] = 100
+    mask, _ = tree_of(b, 3, 0)
+    _, out, line = attend(b, mask, scale=1.0, **({"max_k": most} if most else {}))
+    done()
+    want = (b.v[page, row].double() * b.v_scale[page].double()[:, None]).repeat_interleave(grp, 0).expand(n, -1, -1)
+    close(out, want, want.abs() * 2.0 ** -20, "bf16")          # (the weight's sum and quotient in f32)
+    assert ((line.double().cpu() / (-125 * 2.0 ** 118) - 1).abs() <= 2.0 ** -20).all()
+
+
 # ---- rotation with append: a long run of tokens among many sequences of one -------------------
 
 UNEVEN = [
